@@ -278,6 +278,104 @@ int kf_decode_argmax_step(const void* logits, int n, void* token, void* pos, voi
 int kf_decode_attention(const void* q, const void* cache_k, const void* cache_v, const void* mask, void* out,
                         int heads, int kv_heads, int head_dim, int max_seq, int mask_stride, void* stream);
 
+/* ---- several requests at once: a paged KV cache ---------------------------------------------------
+ * The cache is two arrays [num_pages, kv_heads, block_size, head_dim], fp16 or bf16, with any strides
+ * (in elements, multiples of 8) of the first three dimensions; block_size is a power of two from 16 up.  A
+ * request's page table row names its pages in order; token i of it lies in slot
+ * row[i / block_size] * block_size + i % block_size.  No counterpart in the reference, which serves one stream.
+ * Every length, offset, position, slot and page that the kernels read is bounded before it is used: wrong
+ * ones give wrong results, never an access outside the arrays.  Pointers 16-byte aligned. */
+
+/* The tables of one step, from the requests' lengths, in one launch.  Request r has context_lens[r] tokens in the
+ * cache and gets new_lens[r] more (negative: 0).  Where they need new pages (up to table_width in all), these are taken
+ * from the top of the stack free_pages[0 .. *free_count), requests in order, and entered into block_table; -1 is
+ * entered when the stack is empty.  Writes cu_new [seqs + 1] (where each request's new tokens begin), seq_lens [seqs]
+ * (context + new), positions and slots int64 [max_tokens] of the new tokens in order (slot -1 where there is no page;
+ * both -1 behind the last token) and *free_left.  free_left must not be free_count. */
+typedef struct {
+  void* block_table;        /* int32 [seqs, table_width], rows table_stride apart */
+  const void* context_lens; /* int32 [seqs] */
+  const void* new_lens;     /* int32 [seqs] */
+  const void* free_pages;   /* int32 [free_capacity] */
+  const void* free_count;   /* int32 [1] */
+  void* cu_new;             /* int32 [seqs + 1] */
+  void* seq_lens;           /* int32 [seqs] */
+  void* positions;          /* int64 [max_tokens] */
+  void* slots;              /* int64 [max_tokens] */
+  void* free_left;          /* int32 [1] */
+  int64_t table_stride;
+  int seqs, table_width, block_size, free_capacity, max_tokens;
+} kf_paged_tables_args;
+int kf_paged_tables(const kf_paged_tables_args* args, void* stream);
+
+/* RoPE on q and k of a q|k|v projection and the cache's update, one launch.  Row t of qkv holds heads q heads, kv_heads
+ * k heads and kv_heads v heads of head_dim (rows qkv_stride apart).  With c, s = rows positions[t] of cos, sin (fp32
+ * [max_pos, head_dim], sin with the rotate-half sign folded in: -sin on the first half), y[j] = x[j] c[j] +
+ * x[(j + head_dim / 2) mod head_dim] s[j], 32 bits inside, one rounding; q and k rotated go to qk [tokens,
+ * heads + kv_heads, head_dim] (contiguous), k and v to slots[t] of the cache.  A slot outside the cache (-1) writes
+ * no cache entry; so does a position outside [0, max_pos), which rotates with row 0.  Slots must be distinct. */
+typedef struct {
+  const void* qkv;
+  const void* cos;
+  const void* sin;
+  const void* positions; /* int64 [tokens] */
+  const void* slots;     /* int64 [tokens] */
+  void* qk;
+  void* cache_k;
+  void* cache_v;
+  int64_t qkv_stride;
+  int64_t k_page, k_head, k_token, v_page, v_head, v_token;
+  int tokens, heads, kv_heads, head_dim, max_pos, num_pages, block_size;
+  int dtype; /* KF_DTYPE_F16 or KF_DTYPE_BF16 */
+} kf_rope_paged_args;
+int kf_rope_paged_cache(const kf_rope_paged_args* args, void* stream);
+
+/* Causal attention of whole prompts, packed: sequence s is the tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1
+ * (ascending, from 0), and token t of it gets
+ *   out[t, h] = sum_{u <= t} softmax_u(scale q[t, h] . k[u, kv]) v[u, kv],  kv = h / (heads / kv_heads),
+ * with 32-bit scores, maxima and sums; probabilities are rounded to the inputs' type for the second product, out
+ * once more.  Keys after a token do not reach it whatever they hold.  Rows in no sequence are zeroed where
+ * zero_rest is set and left as they are otherwise.  Strides in elements, multiples of 8; head_dim a multiple of 8
+ * up to KF_ATTN_MAX_HEAD_DIM; scale positive. */
+typedef struct {
+  const void* q;          /* [tokens, heads, head_dim] */
+  const void* k;          /* [tokens, kv_heads, head_dim] */
+  const void* v;
+  void* out;              /* [tokens, heads, head_dim] */
+  const void* cu_seqlens; /* int32 [seqs + 1] */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+  int tokens, seqs, heads, kv_heads, head_dim, dtype;
+  float scale;
+  int zero_rest;
+} kf_prompt_attention_args;
+int kf_prompt_attention(const kf_prompt_attention_args* args, void* stream);
+
+/* Causal attention of every request's new tokens over its pages of the cache (which hold the new tokens' keys and
+ * values already): request r's new tokens are rows cu_new[r] .. cu_new[r + 1] - 1 of q, the last of its
+ * seq_lens[r] tokens.  Otherwise as kf_prompt_attention.  Tokens whose page is not in [0, num_pages) are not
+ * attended to; a row that is left with no key gets zeros.  max_new: an upper bound of the new tokens of a
+ * request if the caller knows one, else 0; it chooses kernels and splits, results hold for any value.
+ * ws: at least kf_paged_attention_workspace_bytes(args) bytes, 16-byte aligned, not shared with a call that may run
+ * at the same time. */
+typedef struct {
+  const void* q;           /* [tokens, heads, head_dim] */
+  const void* cache_k;
+  const void* cache_v;
+  void* out;               /* [tokens, heads, head_dim] */
+  const void* block_table; /* int32 [seqs, table_width], rows table_stride apart */
+  const void* cu_new;      /* int32 [seqs + 1] */
+  const void* seq_lens;    /* int32 [seqs] */
+  int64_t q_token, q_head, out_token, out_head;
+  int64_t k_page, k_head, k_token, v_page, v_head, v_token;
+  int64_t table_stride;
+  int tokens, seqs, heads, kv_heads, head_dim, dtype;
+  int table_width, num_pages, block_size, max_new;
+  float scale;
+  int zero_rest;
+} kf_paged_attention_args;
+size_t kf_paged_attention_workspace_bytes(const kf_paged_attention_args* args);
+int kf_paged_attention(const kf_paged_attention_args* args, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -167,6 +167,75 @@ int gemm_entry(const void* x, const void* packed, const void* scales, void* y, v
                     "int4_gemm launch");
 }
 
+// ---- paged cache: checks shared by its entry points ------------------------------------------------
+constexpr int kMaxTokenStride = 1 << 26;  // elements: 16 keys' byte offsets fit 32 bits
+constexpr int kFewRows = 64;              // (token, query head of a group) rows of a request up to which the kernel
+                                          // that splits keys over workgroups takes it where both kernels run
+
+int check_block(int block_size, int* log2_block) {
+  if (block_size < 16 || block_size > (1 << 20) || (block_size & (block_size - 1)))
+    return fail(KF_ERR_INVALID_ARG, "block_size must be a power of two from 16 to 2^20, got %d", block_size);
+  *log2_block = __builtin_ctz(block_size);
+  return KF_OK;
+}
+
+int check_heads(int heads, int kv_heads, int head_dim, int dtype) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads)
+    return fail(KF_ERR_INVALID_ARG, "kv_heads=%d must divide heads=%d", kv_heads, heads);
+  if (head_dim < 8 || head_dim % 8 || head_dim > KF_ATTN_MAX_HEAD_DIM)
+    return fail(KF_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 up to %d, got %d", KF_ATTN_MAX_HEAD_DIM, head_dim);
+  if (dtype != KF_DTYPE_F16 && dtype != KF_DTYPE_BF16)
+    return fail(KF_ERR_INVALID_ARG, "dtype must be KF_DTYPE_F16 or KF_DTYPE_BF16, got %d", dtype);
+  return KF_OK;
+}
+
+int check_attention(int tokens, int seqs, int heads, int kv_heads, int head_dim, int dtype, float scale) {
+  if (tokens < 0 || seqs < 1) return fail(KF_ERR_INVALID_ARG, "need tokens >= 0 and seqs >= 1, got %d, %d", tokens, seqs);
+  if (int st = check_heads(heads, kv_heads, head_dim, dtype)) return st;
+  if (!(scale > 0.0f) || scale > 3.0e38f) return fail(KF_ERR_INVALID_ARG, "scale must be positive and finite, got %g", scale);
+  // Row numbers (tokens x query heads of a group), and the grid in work-items, fit 31 bits.
+  const int64_t rep = heads / kv_heads;
+  if (tokens * rep >= (int64_t)1 << 31 || (tokens * rep / 128 + seqs + 1) * kv_heads * 256 >= (int64_t)1 << 31)
+    return fail(KF_ERR_UNSUPPORTED, "%d tokens of %d heads in %d sequences are more than one launch takes", tokens, heads,
+                seqs);
+  return KF_OK;
+}
+
+int check_arrays(const void* const* p, int count) {
+  for (int i = 0; i < count; ++i) {
+    if (!p[i]) return fail(KF_ERR_INVALID_ARG, "every array must be non-null");
+    if (!aligned(p[i], 16)) return fail(KF_ERR_INVALID_ARG, "arrays must be 16-byte aligned");
+  }
+  return KF_OK;
+}
+
+int check_strides(const int64_t* s, int count) {
+  for (int i = 0; i < count; ++i)
+    if (s[i] < 0 || s[i] % 8) return fail(KF_ERR_INVALID_ARG, "strides must be multiples of 8 elements, got %lld", (long long)s[i]);
+  return KF_OK;
+}
+
+// Which kernels a paged_attention call launches.  few: the one that splits the keys; many: the one that splits the rows.
+struct PagedPlan {
+  bool few, many;
+  int row_tiles, grid, log2_block;
+};
+int paged_plan(const kf_paged_attention_args& a, PagedPlan* p) {
+  if (int st = check_attention(a.tokens, a.seqs, a.heads, a.kv_heads, a.head_dim, a.dtype, a.scale)) return st;
+  if (int st = check_block(a.block_size, &p->log2_block)) return st;
+  if (a.table_width < 1 || a.num_pages < 1 || a.max_new < 0)
+    return fail(KF_ERR_INVALID_ARG, "need table_width, num_pages >= 1 and max_new >= 0, got %d, %d, %d", a.table_width,
+                a.num_pages, a.max_new);
+  if ((int64_t)a.table_width << p->log2_block >= (int64_t)1 << 30)
+    return fail(KF_ERR_UNSUPPORTED, "tables of %d pages of %d tokens are too long", a.table_width, a.block_size);
+  const int64_t rows = (int64_t)(a.max_new ? std::min(a.max_new, a.tokens) : a.tokens) * (a.heads / a.kv_heads);
+  p->many = rows > kFewRows;
+  p->few = !p->many || a.seqs > 1;
+  p->row_tiles = kf::few_rows_tiles(a.head_dim, std::min<int64_t>(rows, kFewRows));
+  p->grid = 0;
+  return KF_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -533,6 +602,153 @@ int kf_decode_attention(const void* q, const void* cache_k, const void* cache_v,
                                                 mask_stride, 1.0f / sqrtf((float)head_dim),
                                                 static_cast<hipStream_t>(stream)),
                     "decode_attention launch");
+}
+
+int kf_paged_tables(const kf_paged_tables_args* a, void* stream) {
+  if (!a) return fail(KF_ERR_INVALID_ARG, "args must be non-null");
+  if (a->seqs < 1 || a->table_width < 1 || a->free_capacity < 0 || a->max_tokens < 0)
+    return fail(KF_ERR_INVALID_ARG, "need seqs, table_width >= 1 and free_capacity, max_tokens >= 0, got %d, %d, %d, %d",
+                a->seqs, a->table_width, a->free_capacity, a->max_tokens);
+  int log2_block;
+  if (int st = check_block(a->block_size, &log2_block)) return st;
+  if (!a->block_table || !a->context_lens || !a->new_lens || (!a->free_pages && a->free_capacity) || !a->free_count ||
+      !a->cu_new || !a->seq_lens || (a->max_tokens && (!a->positions || !a->slots)) || !a->free_left)
+    return fail(KF_ERR_INVALID_ARG, "every array must be non-null");
+  if (a->free_left == a->free_count) return fail(KF_ERR_INVALID_ARG, "free_left must not be free_count");
+  if (a->seqs > (1 << 20)) return fail(KF_ERR_UNSUPPORTED, "paged_tables takes up to %d requests, got %d", 1 << 20, a->seqs);
+  kf::TablesArgs t;
+  t.table = static_cast<int*>(a->block_table);
+  t.context_lens = static_cast<const int*>(a->context_lens);
+  t.new_lens = static_cast<const int*>(a->new_lens);
+  t.free_pages = static_cast<const int*>(a->free_pages);
+  t.free_count = static_cast<const int*>(a->free_count);
+  t.cu_new = static_cast<int*>(a->cu_new);
+  t.seq_lens = static_cast<int*>(a->seq_lens);
+  t.positions = static_cast<int64_t*>(a->positions);
+  t.slots = static_cast<int64_t*>(a->slots);
+  t.free_left = static_cast<int*>(a->free_left);
+  t.table_stride = a->table_stride;
+  t.seqs = a->seqs;
+  t.width = a->table_width;
+  t.log2_block = log2_block;
+  t.free_capacity = a->free_capacity;
+  t.max_tokens = a->max_tokens;
+  return hip_status(kf::paged_tables_launch(t, static_cast<hipStream_t>(stream)), "paged_tables launch");
+}
+
+int kf_rope_paged_cache(const kf_rope_paged_args* a, void* stream) {
+  if (!a) return fail(KF_ERR_INVALID_ARG, "args must be non-null");
+  if (a->tokens < 0) return fail(KF_ERR_INVALID_ARG, "tokens must not be negative, got %d", a->tokens);
+  if (int st = check_heads(a->heads, a->kv_heads, a->head_dim, a->dtype)) return st;
+  int log2_block;
+  if (int st = check_block(a->block_size, &log2_block)) return st;
+  if (a->max_pos < 1 || a->num_pages < 1)
+    return fail(KF_ERR_INVALID_ARG, "need max_pos, num_pages >= 1, got %d, %d", a->max_pos, a->num_pages);
+  if (a->tokens == 0) return KF_OK;
+  const void* const p[] = {a->qkv, a->cos, a->sin, a->positions, a->slots, a->qk, a->cache_k, a->cache_v};
+  if (int st = check_arrays(p, 8)) return st;
+  const int64_t strides[] = {a->qkv_stride, a->k_page, a->k_head, a->k_token, a->v_page, a->v_head, a->v_token};
+  if (int st = check_strides(strides, 7)) return st;
+  if ((int64_t)a->tokens * (a->heads + 2 * (int64_t)a->kv_heads) * (a->head_dim / 8) >= (int64_t)1 << 31)
+    return fail(KF_ERR_UNSUPPORTED, "%d tokens of %d + 2 x %d heads are more than one launch takes", a->tokens, a->heads,
+                a->kv_heads);
+  kf::RopePagedArgs r;
+  r.qkv = a->qkv;
+  r.cos = a->cos;
+  r.sin = a->sin;
+  r.positions = static_cast<const int64_t*>(a->positions);
+  r.slots = static_cast<const int64_t*>(a->slots);
+  r.qk = a->qk;
+  r.cache_k = a->cache_k;
+  r.cache_v = a->cache_v;
+  r.qkv_stride = a->qkv_stride;
+  r.k_page = a->k_page, r.k_head = a->k_head, r.k_token = a->k_token;
+  r.v_page = a->v_page, r.v_head = a->v_head, r.v_token = a->v_token;
+  r.num_slots = (int64_t)a->num_pages << log2_block;
+  r.tokens = a->tokens;
+  r.heads = a->heads;
+  r.kv_heads = a->kv_heads;
+  r.head_dim = a->head_dim;
+  r.max_pos = a->max_pos;
+  r.log2_block = log2_block;
+  return hip_status(kf::rope_paged_launch(r, a->dtype == KF_DTYPE_BF16, static_cast<hipStream_t>(stream)),
+                    "rope_paged_cache launch");
+}
+
+int kf_prompt_attention(const kf_prompt_attention_args* a, void* stream) {
+  if (!a) return fail(KF_ERR_INVALID_ARG, "args must be non-null");
+  if (int st = check_attention(a->tokens, a->seqs, a->heads, a->kv_heads, a->head_dim, a->dtype, a->scale)) return st;
+  if (a->tokens == 0) return KF_OK;
+  const void* const p[] = {a->q, a->k, a->v, a->out, a->cu_seqlens};
+  if (int st = check_arrays(p, 4)) return st;
+  if (!a->cu_seqlens) return fail(KF_ERR_INVALID_ARG, "every array must be non-null");
+  const int64_t strides[] = {a->q_token, a->q_head, a->k_token, a->k_head, a->v_token, a->v_head, a->out_token, a->out_head};
+  if (int st = check_strides(strides, 8)) return st;
+  if (a->k_token > kMaxTokenStride || a->v_token > kMaxTokenStride)
+    return fail(KF_ERR_UNSUPPORTED, "token strides of k and v go up to %d elements", kMaxTokenStride);
+  kf::AttnArgs t = {};
+  t.q = a->q, t.k = a->k, t.v = a->v, t.out = a->out;
+  t.cu = static_cast<const int*>(a->cu_seqlens);
+  t.q_token = a->q_token, t.q_head = a->q_head, t.out_token = a->out_token, t.out_head = a->out_head;
+  t.k_token = a->k_token, t.k_head = a->k_head, t.v_token = a->v_token, t.v_head = a->v_head;
+  t.tokens = a->tokens, t.seqs = a->seqs, t.heads = a->heads, t.kv_heads = a->kv_heads, t.head_dim = a->head_dim;
+  t.zero_rest = a->zero_rest;
+  t.scale = a->scale;
+  return hip_status(kf::flash_attention_launch(t, false, a->dtype == KF_DTYPE_BF16, 0, static_cast<hipStream_t>(stream)),
+                    "prompt_attention launch");
+}
+
+size_t kf_paged_attention_workspace_bytes(const kf_paged_attention_args* a) {
+  PagedPlan p;
+  if (!a || paged_plan(*a, &p) || (p.few && cu_count(&p.grid))) return 0;
+  return p.few ? kf::few_rows_workspace_bytes(a->head_dim, p.row_tiles, p.grid) : 0;
+}
+
+int kf_paged_attention(const kf_paged_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
+  if (!a) return fail(KF_ERR_INVALID_ARG, "args must be non-null");
+  PagedPlan p;
+  if (int st = paged_plan(*a, &p)) return st;
+  if (a->tokens == 0) return KF_OK;
+  const void* const arrays[] = {a->q, a->cache_k, a->cache_v, a->out};
+  if (int st = check_arrays(arrays, 4)) return st;
+  if (!a->block_table || !a->cu_new || !a->seq_lens) return fail(KF_ERR_INVALID_ARG, "every array must be non-null");
+  const int64_t strides[] = {a->q_token, a->q_head, a->out_token, a->out_head, a->k_page, a->k_head,
+                             a->k_token, a->v_page, a->v_head, a->v_token};
+  if (int st = check_strides(strides, 10)) return st;
+  if (a->k_token > kMaxTokenStride || a->v_token > kMaxTokenStride)
+    return fail(KF_ERR_UNSUPPORTED, "token strides of the caches go up to %d elements", kMaxTokenStride);
+  kf::AttnArgs t = {};
+  t.q = a->q, t.k = a->cache_k, t.v = a->cache_v, t.out = a->out;
+  t.cu = static_cast<const int*>(a->cu_new);
+  t.seq_lens = static_cast<const int*>(a->seq_lens);
+  t.table = static_cast<const int*>(a->block_table);
+  t.table_stride = a->table_stride;
+  t.q_token = a->q_token, t.q_head = a->q_head, t.out_token = a->out_token, t.out_head = a->out_head;
+  t.k_page = a->k_page, t.k_head = a->k_head, t.k_token = a->k_token;
+  t.v_page = a->v_page, t.v_head = a->v_head, t.v_token = a->v_token;
+  t.tokens = a->tokens, t.seqs = a->seqs, t.heads = a->heads, t.kv_heads = a->kv_heads, t.head_dim = a->head_dim;
+  t.table_width = a->table_width, t.log2_block = p.log2_block, t.num_pages = a->num_pages;
+  t.zero_rest = a->zero_rest;
+  t.scale = a->scale;
+  const bool bf16 = a->dtype == KF_DTYPE_BF16;
+  if (p.few) {
+    if (int st = cu_count(&p.grid)) return st;
+    const size_t need = kf::few_rows_workspace_bytes(a->head_dim, p.row_tiles, p.grid);
+    if (!ws || ws_bytes < need)
+      return fail(KF_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, ws ? ws_bytes : (size_t)0);
+    if (!aligned(ws, 16)) return fail(KF_ERR_WORKSPACE, "the workspace must be 16-byte aligned");
+    if (kf::few_rows_units(t, p.row_tiles) >= (int64_t)1 << 31)
+      return fail(KF_ERR_UNSUPPORTED, "%d tokens over tables of %d pages are more than one launch takes", a->tokens,
+                  a->table_width);
+    const int max_rows = p.many ? kFewRows : 0x7fffffff;
+    if (int st = hip_status(kf::few_rows_launch(t, bf16, p.row_tiles, max_rows, p.grid, ws, static_cast<hipStream_t>(stream)),
+                            "paged_attention launch"))
+      return st;
+  }
+  if (p.many)
+    return hip_status(kf::flash_attention_launch(t, true, bf16, p.few ? kFewRows + 1 : 0, static_cast<hipStream_t>(stream)),
+                      "paged_attention launch");
+  return KF_OK;
 }
 
 }  // extern "C"

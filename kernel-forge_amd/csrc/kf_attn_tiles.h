@@ -1,0 +1,259 @@
+// Pieces shared by the kernels of prompt_attention and paged_attention (kf_flash.hip, kf_paged_attn.hip):
+// element types, the rows a workgroup owns, tiles of K and V in LDS and the products on them.
+//
+// Rows.  A row is (token, query head of the KV head's group), tokens first: row r of a sequence is its token
+// r / rep with query head kv * rep + r % rep.  So the rep heads that read the same keys share every tile
+// of K and V, and a single token of a grouped model already fills rep rows of a matrix instruction.
+//
+// Products.  Scores are computed transposed, S^T = K Q^T, so a lane holds scores of one query only (column
+// lane % 32) and its maximum, its sum and the factor that rescales its outputs are plain per-lane values.
+// The lane's eight scores 8 i .. 8 i + 7 of a 32-key tile are keys 16 kk + {4 h + 0..3, 8 + 4 h + 0..3} (h =
+// lane / 32), which serve as they are as the right operand of O^T += V^T P^T if V^T is read with its keys
+// in that order: probabilities go from one product to the next without leaving their registers.  V^T comes from
+// the row-major tile of V by transposing LDS reads (ds_read_b64_tr_b16: each 16 lanes read a 4 x 16 block
+// of 16-bit values, lane i of them gets column i).
+#pragma once
+
+#include "kf_device.h"
+
+namespace kf {
+
+typedef __bf16 bhalf_t;
+typedef __bf16 bhalf8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bhalf2_t __attribute__((ext_vector_type(2)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
+template <class E>
+struct Elem;
+template <>
+struct Elem<half_t> {
+  static constexpr uint32_t kExp = 0x7C007C00u, kExpLow = 0x04000400u, kOnes = 0x3C003C00u;
+  static __device__ __forceinline__ float16_t mfma32(u32x4 a, u32x4 b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<half8_t>(a), bit_cast<half8_t>(b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float4_t mfma16(u32x4 a, u32x4 b, float4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(bit_cast<half8_t>(a), bit_cast<half8_t>(b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {  // both rounded to nearest even
+    const half2_t v = {(half_t)a, (half_t)b};
+    return bit_cast<uint32_t>(v);
+  }
+  static __device__ __forceinline__ float lo(uint32_t v) { return (float)bit_cast<half2_t>(v)[0]; }
+  static __device__ __forceinline__ float hi(uint32_t v) { return (float)bit_cast<half2_t>(v)[1]; }
+};
+template <>
+struct Elem<bhalf_t> {
+  static constexpr uint32_t kExp = 0x7F807F80u, kExpLow = 0x00800080u, kOnes = 0x3F803F80u;
+  static __device__ __forceinline__ float16_t mfma32(u32x4 a, u32x4 b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bit_cast<bhalf8_t>(a), bit_cast<bhalf8_t>(b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float4_t mfma16(u32x4 a, u32x4 b, float4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bit_cast<bhalf8_t>(a), bit_cast<bhalf8_t>(b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const bhalf2_t v = {(bhalf_t)a, (bhalf_t)b};
+    return bit_cast<uint32_t>(v);
+  }
+  static __device__ __forceinline__ float lo(uint32_t v) { return bit_cast<float>(v << 16); }
+  static __device__ __forceinline__ float hi(uint32_t v) { return bit_cast<float>(v & 0xFFFF0000u); }
+};
+
+// Source of the 16 bytes that stand for what is not there: head sizes below the tile's, keys past the end,
+// pages that are not in the cache.  Zeros keep such places finite, so a product with a zero is zero.
+static __device__ __attribute__((aligned(16))) uint32_t g_attn_zeros[4] = {0, 0, 0, 0};
+
+__device__ __forceinline__ void lds_dma16(uint32_t lds, const void* src) {
+  asm volatile("global_load_lds_dwordx4 %1, off" ::"{m0}"(lds), "v"(src) : "memory");
+}
+__device__ __forceinline__ void lds_dma16(uint32_t lds, const void* base, uint32_t offset) {
+  asm volatile("global_load_lds_dwordx4 %1, %2" ::"{m0}"(lds), "v"(offset), "s"(base) : "memory");
+}
+// All of this wavefront's copies have landed and its reads are done, and every wavefront of the workgroup has come
+// here.
+__device__ __forceinline__ void dma_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The 16-byte pieces of a row of a tile are stored at piece ^ swizzle(row), so that the 16 (K) or 4 (V) rows which
+// one read touches lie in different banks.
+template <int HDP>
+__device__ __forceinline__ constexpr int swizzle_k(int key) {
+  return HDP == 64 ? (key >> 1) & 7 : key & 15;
+}
+template <int HDP>
+__device__ __forceinline__ constexpr int swizzle_v(int key) {
+  return HDP == 64 ? 4 * ((key >> 1) & 1) : 4 * (key & 3);
+}
+
+// V's swizzle for 16-column reads (16 x 16 products): eight rows of one read in different banks.
+template <int HDP>
+__device__ __forceinline__ constexpr int swizzle_v16(int key) {
+  return HDP == 64 ? 2 * ((key >> 1) & 3) : 2 * (key & 7);
+}
+
+// Copies 16 keys of K and of V into tiles, swizzled.  The source offsets of a lane do not change, so a copy of 16 keys
+// that are all there is one instruction per KiB.
+template <class E, int HDP, bool V16>
+struct Copy16 {
+  static constexpr int CPR = HDP / 8;    // 16-byte pieces per row
+  static constexpr int RPI = 64 / CPR;   // rows per copy instruction
+  static constexpr int N = 16 / RPI;     // instructions per tile
+  uint32_t vo_k[N], vo_v[N];
+  int pieces;  // of a row that are there
+
+  __device__ __forceinline__ static int piece_k(int j, int lane) {
+    return (lane % CPR) ^ swizzle_k<HDP>(RPI * j + lane / CPR);
+  }
+  __device__ __forceinline__ static int piece_v(int j, int lane) {
+    const int r = RPI * j + lane / CPR;
+    return (lane % CPR) ^ (V16 ? swizzle_v16<HDP>(r) : swizzle_v<HDP>(r));
+  }
+  // Strides of at most 2^26 elements (checked by the caller), so offsets fit 32 bits.
+  __device__ __forceinline__ Copy16(int64_t k_token, int64_t v_token, int head_dim, int lane) : pieces(head_dim / 8) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const uint32_t r = RPI * j + lane / CPR;
+      vo_k[j] = 2u * (r * (uint32_t)k_token + 8u * piece_k(j, lane));
+      vo_v[j] = 2u * (r * (uint32_t)v_token + 8u * piece_v(j, lane));
+    }
+  }
+  // kb, vb: the first key's values; `rows` of the 16 keys are there (any value), the others and the pieces past
+  // the head size become zeros.
+  __device__ __forceinline__ void operator()(uint32_t dst_k, uint32_t dst_v, const E* kb, const E* vb, int rows,
+                                             int lane) const {
+    if (rows >= 16 && pieces == CPR) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        lds_dma16(dst_k + 1024 * j, kb, vo_k[j]);
+        lds_dma16(dst_v + 1024 * j, vb, vo_v[j]);
+      }
+      return;
+    }
+    int there = pieces, lane_here = lane;
+    asm volatile("" : "+s"(there), "+v"(lane_here));  // the comparisons below are made here, not kept in registers for the whole loop
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const bool row_ok = RPI * j + lane_here / CPR < rows;
+      const char* const sk = reinterpret_cast<const char*>(kb) + vo_k[j];
+      const char* const sv = reinterpret_cast<const char*>(vb) + vo_v[j];
+      lds_dma16(dst_k + 1024 * j, row_ok && piece_k(j, lane_here) < there ? sk : (const char*)g_attn_zeros);
+      lds_dma16(dst_v + 1024 * j, row_ok && piece_v(j, lane_here) < there ? sv : (const char*)g_attn_zeros);
+    }
+  }
+};
+
+// 4 x 16 transposing read of 16-bit values: see the head of this file.
+__device__ __forceinline__ u32x2 lds_read_tr(uint32_t lds) {
+  typedef __attribute__((address_space(3))) short4_t* ptr_t;
+  return bit_cast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr_t)(uintptr_t)lds));
+}
+__device__ __forceinline__ u32x4 lds_read16(uint32_t lds) {
+  typedef const __attribute__((address_space(3))) u32x4* ptr_t;
+  return *(ptr_t)(uintptr_t)lds;
+}
+
+__device__ __forceinline__ float max_halves(float v) {  // of lanes l and l ^ 32
+  const auto s = __builtin_amdgcn_permlane32_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+  return fmaxf(bit_cast<float>((uint32_t)s[0]), bit_cast<float>((uint32_t)s[1]));
+}
+__device__ __forceinline__ float add_halves(float v) {
+  const auto s = __builtin_amdgcn_permlane32_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+  return bit_cast<float>((uint32_t)s[0]) + bit_cast<float>((uint32_t)s[1]);
+}
+
+// Whether any 16-bit value of the four words is infinite or NaN.
+template <class E>
+__device__ __forceinline__ bool any_nonfinite(u32x4 v) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t |= (v[i] & Elem<E>::kExp) + Elem<E>::kExpLow;
+  return (t & 0x80008000u) != 0;
+}
+
+// A piece of V next to masked keys.  A masked key may hold infinities or NaN, which a probability of zero does not
+// cancel.  They are taken out of v, and come back as ones where v had NaN, +inf and -inf: with ones for the
+// probabilities of the keys that a row attends to, a product counts how many of them the row meets.
+template <class E>
+__device__ __forceinline__ void split_nonfinite(u32x4& v, u32x4& nan, u32x4& pos, u32x4& neg) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t wn = 0, wp = 0, wm = 0, keep = 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t x = (v[i] >> (16 * e)) & 0xFFFFu, ex = Elem<E>::kExp & 0xFFFFu;
+      const uint32_t one = (Elem<E>::kOnes & 0xFFFFu) << (16 * e);
+      if ((x & ex) != ex) keep |= 0xFFFFu << (16 * e);
+      else if (x == ex) wp |= one;
+      else if (x == (ex | 0x8000u)) wm |= one;
+      else wn |= one;
+    }
+    nan[i] = wn, pos[i] = wp, neg[i] = wm;
+    v[i] &= keep;
+  }
+}
+__device__ __forceinline__ float with_nonfinite(float o, float nan, float pos, float neg) {
+  if (pos > 0.0f) o += __builtin_inff();
+  if (neg > 0.0f) o -= __builtin_inff();
+  return nan > 0.0f ? __builtin_nanf("") : o;
+}
+
+// Lengths, offsets and pages do not change while a kernel runs: scalar loads where the index is uniform.
+__device__ __forceinline__ int load_const(const int* p, int64_t i) {
+  return ((const __attribute__((address_space(4))) int*)p)[i];
+}
+// 16 bytes of q and stores to out, as global memory (pointers read from memory would be generic ones).
+__device__ __forceinline__ u32x4 load_global16(const void* p) {
+  return *(const __attribute__((address_space(1))) u32x4*)p;
+}
+template <class V>
+__device__ __forceinline__ void store_global(void* p, V v) {
+  *(__attribute__((address_space(1))) V*)p = v;
+}
+
+// The kernel's first argument, read anew: what is made from it inside a loop over items is loaded there by scalar loads
+// instead of being held in scalar registers, which are too few, for the whole kernel.
+__device__ __forceinline__ AttnArgs reload_args() {
+  typedef const __attribute__((address_space(4))) uint64_t* words_t;
+  words_t p = (words_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  static_assert(sizeof(AttnArgs) % 8 == 0, "whole words");
+  struct Words {
+    uint64_t w[sizeof(AttnArgs) / 8];
+  } v;
+#pragma unroll
+  for (size_t i = 0; i < sizeof(AttnArgs) / 8; ++i) v.w[i] = p[i];
+  return bit_cast<AttnArgs>(v);
+}
+
+// Sequences of packed tokens: [offset(s), offset(s + 1)) for s < seqs, then the rows in no sequence as sequence
+// `seqs`.  Offsets outside [0, tokens] are clamped, so no row index made from them leaves the tensors.
+__device__ __forceinline__ int seq_offset(const int* cu, int s, int seqs, int tokens) {
+  return s <= 0 ? 0 : s > seqs ? tokens : min(max(load_const(cu, s), 0), tokens);
+}
+
+// Tiles of BM rows over the packed sequences, numbered so that a tile finds its sequence without a scan: sequence
+// s owns the numbers from offset(s) * rep / BM + s on, enough for its rows, as
+// floor(a + b) + 1 >= floor(a) + ceil(b).  Returns the largest s <= seqs whose first number is at most t.
+// 64 probes a round; all lanes return the same.
+template <int BM>
+__device__ __forceinline__ int find_seq(const int* cu, int seqs, int tokens, int rep, int t, int lane,
+                                        int* first) {
+  int lo = 0, range = seqs + 1;
+  while (range > 1) {
+    const int step = (range + 63) >> 6;
+    const int s = lo + lane * step;
+    const bool in = lane * step < range;
+    const bool at_or_before = in && (lane == 0 || seq_offset(cu, s, seqs, tokens) * rep / BM + s <= t);
+    // The last probe that holds: offsets that do not ascend still give a first number of at most t.
+    const int n = 63 - __clzll((long long)__ballot(at_or_before));
+    lo += n * step;
+    range = min(step, range - n * step);
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  *first = lo == 0 ? 0 : seq_offset(cu, lo, seqs, tokens) * rep / BM + lo;
+  return lo;
+}
+
+}  // namespace kf

@@ -217,6 +217,69 @@ hipError_t decode_attention_launch(const void* q, const void* cache_k, const voi
                                    int heads, int kv_heads, int head_dim, int max_seq, int mask_stride, float scale,
                                    hipStream_t stream);
 
+// ---- attention of packed sequences, many rows per sequence (kf_flash.hip) -------
+// Strides in elements.  Paged: k, v are [pages, kv_heads, block, d] with strides (page, head, slot); otherwise
+// [tokens, kv_heads, d] with strides (unused, head, token).
+struct AttnArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const int* cu;            // [seqs + 1] offsets of the sequences' (new) tokens
+  const int* seq_lens;      // paged: [seqs] keys of each request, its new tokens included
+  const int* table;         // paged: [seqs, table_width] pages
+  int64_t table_stride;
+  int64_t q_token, q_head, out_token, out_head;
+  int64_t k_page, k_head, k_token, v_page, v_head, v_token;
+  int tokens, seqs, heads, kv_heads, head_dim;
+  int table_width, log2_block, num_pages;
+  int zero_rest;            // write zeros to the rows of out that are in no sequence
+  float scale;
+};
+// Requests of fewer than min_rows rows are left to the other kernel.
+hipError_t flash_attention_launch(const AttnArgs& a, bool paged, bool bf16, int min_rows, hipStream_t stream);
+
+// ---- attention of few rows per request over a paged cache (kf_paged_attn.hip) -----
+// row_tiles: 16-row tiles that share a pass over the keys; requests of more than max_rows rows are left to the other
+// kernel.  ws: few_rows_workspace_bytes, 16-byte aligned.
+int few_rows_tiles(int head_dim, int64_t rows);
+size_t few_rows_workspace_bytes(int head_dim, int row_tiles, int grid);
+int64_t few_rows_units(const AttnArgs& a, int row_tiles);  // an upper bound of the kernel's work units
+hipError_t few_rows_launch(const AttnArgs& a, bool bf16, int row_tiles, int max_rows, int grid, void* ws,
+                           hipStream_t stream);
+
+// ---- the paged cache's tables and writer (kf_paged.hip) -----------------------
+struct TablesArgs {
+  int* table;               // [seqs, width], pages of each request in order; new ones are entered
+  const int* context_lens;  // [seqs]
+  const int* new_lens;      // [seqs]
+  const int* free_pages;    // [free_capacity], a stack whose top is free_pages[*free_count - 1]
+  const int* free_count;
+  int* cu_new;              // [seqs + 1]
+  int* seq_lens;            // [seqs]
+  int64_t* positions;       // [max_tokens]
+  int64_t* slots;           // [max_tokens]
+  int* free_left;
+  int64_t table_stride;
+  int seqs, width, log2_block, free_capacity, max_tokens;
+};
+hipError_t paged_tables_launch(const TablesArgs& a, hipStream_t stream);
+
+struct RopePagedArgs {
+  const void* qkv;          // [tokens, (heads + 2 kv_heads) d], rows qkv_stride apart
+  const void* cos;          // fp32 [max_pos, d]
+  const void* sin;          // fp32 [max_pos, d], rotate-half sign folded in
+  const int64_t* positions; // [tokens]
+  const int64_t* slots;     // [tokens]
+  void* qk;                 // [tokens, heads + kv_heads, d]
+  void* cache_k;            // [pages, kv_heads, block, d]: strides (page, head, slot) in elements
+  void* cache_v;
+  int64_t qkv_stride, k_page, k_head, k_token, v_page, v_head, v_token;
+  int64_t num_slots;
+  int tokens, heads, kv_heads, head_dim, max_pos, log2_block;
+};
+hipError_t rope_paged_launch(const RopePagedArgs& a, bool bf16, hipStream_t stream);
+
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 }  // namespace kf

@@ -1,0 +1,443 @@
+// Attention of few rows per request over the pages of a cache: decode steps, short continuations.
+//
+//   out[t, h] = sum_s softmax_s(scale q[t, h] . k[s, kv]) v[s, kv],   s <= position of t,   kv = h / rep
+//
+// What bounds it: the bytes of K and V, read once.  So the work of all requests is laid end to end, in units of 128
+// keys of one (request, row tile, KV head), and cut into one equal stretch per workgroup whatever the lengths
+// are; a workgroup finds its stretch from the lengths by itself (they are read on the device only, so a captured launch
+// follows them).  The wavefronts of a workgroup take 32 keys each and do not wait for each other: each keeps its keys' tiles of K
+// and V coming through LDS buffers of its own by asynchronous copies, and they meet at the end of an item.
+// An item inside one stretch is finished there; the pieces of one that is cut go to the workspace (maximum, sum,
+// unscaled outputs, 32 bits) and a second launch joins them, in the order of the keys: results do not depend on timing.
+#include "kf_attn_tiles.h"
+#include "kf_launch.h"
+
+namespace kf {
+namespace {
+
+template <int HDP, int MT>
+struct FewConfig {
+  static constexpr int WAVES = HDP == 256 ? 2 : 4;
+  static constexpr int THREADS = 64 * WAVES;
+  static constexpr int STAGES = HDP == 64 ? 4 : 2;
+  static constexpr int ROW = HDP * 2;
+  static constexpr int STAGE = 2 * 32 * ROW;         // K and V of 32 keys
+  static constexpr int RING = STAGES * STAGE;        // of one wavefront
+  static constexpr int ROWS = 16 * MT;
+  static constexpr int UNIT = 32 * WAVES;            // keys
+  static constexpr int LDS = WAVES * RING;           // 128 KiB
+  static_assert(WAVES * ROWS * HDP * 4 <= LDS, "the wavefronts' sums meet in the buffers");
+};
+
+// What the second launch needs to know of a cut item, left by the workgroup in whose stretch it begins.
+struct Piece {
+  int seq, row0, kv, last;  // last: the workgroup in whose stretch it ends; seq < 0: nothing begins and goes on here
+};
+
+__device__ __forceinline__ int few_seq_len(const AttnArgs& a, int s) {
+  return min(max(load_const(a.seq_lens, s), 0), a.table_width << a.log2_block);
+}
+// Units of a request: (row tiles) x (KV heads) x (units of keys), one at least where it has rows, so that they are written.
+template <class C>
+__device__ __forceinline__ int few_units(const AttnArgs& a, int s, int rep, int max_rows, int* key_units) {
+  const int rows = max(seq_offset(a.cu, s + 1, a.seqs, a.tokens) - seq_offset(a.cu, s, a.seqs, a.tokens), 0) * rep;
+  const int ku = max((few_seq_len(a, s) + C::UNIT - 1) / C::UNIT, 1);
+  *key_units = ku;
+  return rows > max_rows ? 0 : (rows + C::ROWS - 1) / C::ROWS * a.kv_heads * ku;
+}
+
+__device__ __forceinline__ float max_groups(float v) {  // of lanes l, l ^ 16, l ^ 32, l ^ 48
+  const auto s = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+  return max_halves(fmaxf(bit_cast<float>((uint32_t)s[0]), bit_cast<float>((uint32_t)s[1])));
+}
+__device__ __forceinline__ float add_groups(float v) {
+  const auto s = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+  return add_halves(bit_cast<float>((uint32_t)s[0]) + bit_cast<float>((uint32_t)s[1]));
+}
+
+template <class E, int HDP, int MT>
+__global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel(AttnArgs args, int rep, int max_rows,
+                                                                                 float scale_log2, float* ws,
+                                                                                 Piece* pieces) {
+  using C = FewConfig<HDP, MT>;
+  using Copy = Copy16<E, HDP, true>;
+  constexpr int PER_STAGE = 4 * Copy::N, ROW = C::ROW;  // copy instructions of a stage
+  constexpr int ST = HDP / 32, DT = HDP / 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
+  __shared__ float stat[2][C::WAVES][C::ROWS];
+  __shared__ int64_t scan[C::WAVES];
+  __shared__ int found[2];
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  int begin, end, per;
+  {
+  const AttnArgs& a = args;
+  // This workgroup's stretch.  Every thread sums a run of requests; the one whose run holds the stretch's
+  // first unit says which request that is.
+  const int run = (a.seqs + C::THREADS - 1) / C::THREADS;
+  const int s0 = min(tid * run, a.seqs), s1 = min(s0 + run, a.seqs);
+  int ku;
+  int64_t mine = 0;
+  for (int s = s0; s < s1; ++s) mine += few_units<C>(a, s, rep, max_rows, &ku);
+  int64_t upto = mine;  // inclusive prefix in the wavefront
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t v = __shfl_up(upto, off);
+    if (lane >= off) upto += v;
+  }
+  if (lane == 63) scan[wave] = upto;
+  __syncthreads();
+  int64_t sum_all = 0, before = upto - mine;
+#pragma unroll
+  for (int w = 0; w < C::WAVES; ++w) {
+    if (w < wave) before += scan[w];
+    sum_all += scan[w];
+  }
+  // The launch checks that ascending offsets stay below 2^31 units; with others there is no work.
+  const int total = __builtin_amdgcn_readfirstlane(sum_all < 0x7fffffff ? (int)sum_all : 0);
+  per = total / (int)gridDim.x + (total % (int)gridDim.x ? 1 : 0);
+  // 64 bits: workgroups past the end begin past it.
+  begin = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
+  end = begin + min(per, total - begin);
+  if (begin >= before && begin < before + mine) {
+    int at = (int)before;
+    for (int s = s0; s < s1; ++s) {
+      const int n = few_units<C>(a, s, rep, max_rows, &ku);
+      if (begin < at + n) {
+        found[0] = s;
+        found[1] = at;
+        break;
+      }
+      at += n;
+    }
+  }
+  if (tid == 0) pieces[blockIdx.x].seq = -1;
+  __syncthreads();
+
+  // Rows in no sequence.
+  if (a.zero_rest) {
+    const int t0 = seq_offset(a.cu, a.seqs, a.seqs, a.tokens);
+    const int cpr = a.head_dim / 8, per_row = a.heads * cpr;
+    for (int64_t i = (int64_t)blockIdx.x * C::THREADS + tid; i < (int64_t)(a.tokens - t0) * per_row;
+         i += (int64_t)gridDim.x * C::THREADS) {
+      const int64_t t = i / per_row;
+      const int r = (int)(i - t * per_row), h = r / cpr;
+      *(u32x4*)((E*)a.out + (t0 + t) * a.out_token + h * a.out_head + 8 * (r - h * cpr)) = u32x4{0, 0, 0, 0};
+    }
+  }
+  if (begin >= end) return;
+  }
+
+  int seq = __builtin_amdgcn_readfirstlane(found[0]);
+  int seq_at = __builtin_amdgcn_readfirstlane(found[1]);  // the request's first unit
+  const uint32_t ring = lds + (uint32_t)wave * C::RING;
+  const uint32_t k_at = (uint32_t)l16 * ROW + 16u * (uint32_t)(g ^ swizzle_k<HDP>(l16));
+  const int vrow = 4 * g + (l16 >> 2);
+  const uint32_t v_at = 32u * ROW + (uint32_t)vrow * ROW + 16u * (uint32_t)(((l16 & 3) >> 1) ^ swizzle_v16<HDP>(vrow)) +
+                        8u * (uint32_t)(l16 & 1);
+  const float slack = 8.0f / scale_log2;
+  for (int at = begin; at < end;) {
+    const AttnArgs a = reload_args();
+    const Copy copy(a.k_token, a.v_token, a.head_dim, lane);
+    int n, ku;
+    while ((n = few_units<C>(a, seq, rep, max_rows, &ku)) <= at - seq_at) {  // next request with units
+      seq_at += n;
+      ++seq;
+    }
+    const int item = (at - seq_at) / ku, item_at = seq_at + item * ku;
+    const int u0 = at - item_at, u1 = min(ku, end - item_at);
+    const int kv = item % a.kv_heads, row0 = item / a.kv_heads * C::ROWS;
+    const int tok0 = seq_offset(a.cu, seq, a.seqs, a.tokens);
+    const int len = seq_offset(a.cu, seq + 1, a.seqs, a.tokens) - tok0, rows = len * rep;
+    const int seq_len = few_seq_len(a, seq), shift = seq_len - len;
+    const int64_t table_at = (int64_t)seq * a.table_stride;
+
+    u32x4 qf[MT][ST];
+    int limit[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const int row = min(row0 + 16 * t + l16, rows - 1), tok = row / rep, head = kv * rep + (row - tok * rep);
+      limit[t] = shift + tok;
+      const E* const qp = (const E*)a.q + (size_t)(tok0 + tok) * a.q_token + (size_t)head * a.q_head;
+#pragma unroll
+      for (int s = 0; s < ST; ++s)
+        qf[t][s] = 4 * s + g < a.head_dim / 8 ? load_global16(qp + 32 * s + 8 * g) : u32x4{0, 0, 0, 0};
+    }
+    const int kend = shift + min(row0 + C::ROWS - 1, rows - 1) / rep + 1;  // keys of the tile's last row
+    const int first_limit = shift + row0 / rep;
+
+    auto page_of = [&](int key) {  // uniform; -1: not in the cache
+      if (kend <= 0) return -1;
+      const int p = load_const(a.table, table_at + (min(key, kend - 1) >> a.log2_block));
+      return (unsigned)p < (unsigned)a.num_pages ? p : -1;
+    };
+    auto issue = [&](int i, int p0, int p1) {  // unit u0 + i; pages of its two 16 keys
+      const int key0 = (u0 + i) * C::UNIT + 32 * wave;
+      const uint32_t dst = ring + (uint32_t)(i % C::STAGES) * C::STAGE;
+      const E* const k = (const E*)a.k + kv * a.k_head;
+      const E* const v = (const E*)a.v + kv * a.v_head;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int page = half ? p1 : p0, key = key0 + 16 * half;
+        const int slot = key & ((1 << a.log2_block) - 1);
+        copy(dst + (16 * half) * ROW, dst + (32 + 16 * half) * ROW, k + page * a.k_page + slot * a.k_token,
+             v + page * a.v_page + slot * a.v_token, page >= 0 ? kend - key : 0, lane);
+      }
+    };
+
+    float4_t o[MT][DT];
+    float m[MT], mc[MT], sum[MT], limit_max[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      m[t] = limit_max[t] = -__builtin_inff();
+      mc[t] = sum[t] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < DT; ++c) o[t][c] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    const int n_units = u1 - u0, live_rows = rows - row0;
+    auto key_of = [&](int i) { return (u0 + i) * C::UNIT + 32 * wave; };
+    int next0 = page_of(key_of(0)), next1 = page_of(key_of(0) + 16);
+    for (int i = 1 - C::STAGES; i < n_units; ++i) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the buffer's last reads are done
+      const bool more = i + C::STAGES - 1 < n_units;
+      if (more) {
+        issue(i + C::STAGES - 1, next0, next1);
+        next0 = page_of(key_of(i + C::STAGES)), next1 = page_of(key_of(i + C::STAGES) + 16);
+      }
+      if (i < 0) continue;
+      if (more) wait_vmcnt<PER_STAGE * (C::STAGES - 1)>();
+      else wait_vmcnt<0>();
+      const int key0 = key_of(i);
+      if (key0 >= kend) continue;
+      const uint32_t buf = ring + (uint32_t)(i % C::STAGES) * C::STAGE;
+
+      const bool bad0 = page_of(key0) < 0, bad1 = page_of(key0 + 16) < 0;
+      const bool masked = key0 + 31 > first_limit || bad0 || bad1;
+      // The last of this lane's keys key0 + 16 u + 4 g + (0 .. 3) that its row attends to, as 0 .. 3 (below: none).
+      auto keys_at = [&](int t, int u) { return (u ? bad1 : bad0) ? -1 : limit[t] - (key0 + 16 * u + 4 * g); };
+      u32x4 p[MT];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        if (MT > 1 && 16 * t >= live_rows) continue;
+        float4_t s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          s[u] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int st = 0; st < ST; ++st)
+            s[u] = Elem<E>::mfma16(lds_read16(((buf + k_at) ^ (uint32_t)(64 * st)) + u * 16 * ROW), qf[t][st], s[u]);
+        }
+        if (masked) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int last = keys_at(t, u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e > last) s[u][e] = -__builtin_inff();
+          }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                         fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        mx = max_groups(mx);
+        if (__ballot(mx > limit_max[t])) {
+          const float mn = fmaxf(m[t], mx);
+          const float mcn = mn == -__builtin_inff() ? 0.0f : mn * scale_log2;
+          const float f = m[t] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mc[t] - mcn);
+          m[t] = mn;
+          mc[t] = mcn;
+          limit_max[t] = mn + slack;
+          sum[t] *= f;
+#pragma unroll
+          for (int c = 0; c < DT; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][c][e] *= f;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[u][e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], scale_log2, -mc[t]));
+            sum[t] += s[u][e];
+          }
+          p[t][2 * u] = Elem<E>::pack(s[u][0], s[u][1]);
+          p[t][2 * u + 1] = Elem<E>::pack(s[u][2], s[u][3]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < DT; ++c) {
+        const uint32_t va = (buf + v_at) ^ (uint32_t)(32 * c);
+        const u32x2 v0 = lds_read_tr(va), v1 = lds_read_tr(va + 16 * ROW);
+        u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
+        if (masked && __ballot(any_nonfinite<E>(v))) {
+          u32x4 nan, pos, neg;
+          split_nonfinite<E>(v, nan, pos, neg);
+          const float4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            u32x4 live;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const int last = keys_at(t, w >> 1) - 2 * (w & 1);
+              live[w] = last < 0 ? 0u : last == 0 ? Elem<E>::kOnes & 0xFFFFu : Elem<E>::kOnes;
+            }
+            const float4_t cn = Elem<E>::mfma16(nan, live, z), cp = Elem<E>::mfma16(pos, live, z);
+            const float4_t cm = Elem<E>::mfma16(neg, live, z);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][c][e] = with_nonfinite(o[t][c][e], cn[e], cp[e], cm[e]);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          if (MT > 1 && 16 * t >= live_rows) continue;
+          o[t][c] = Elem<E>::mfma16(v, p[t], o[t][c]);
+        }
+      }
+    }
+
+    // The wavefronts' maxima, sums and outputs meet in the buffers.
+    __syncthreads();  // every wavefront has read its last tile
+    const AttnArgs b = reload_args();
+    float* const acc = reinterpret_cast<float*>(smem);  // [WAVES][ROWS][HDP]
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const float total_sum = add_groups(sum[t]);
+      if (g == 0) {
+        stat[0][wave][16 * t + l16] = m[t] == -__builtin_inff() ? m[t] : mc[t];
+        stat[1][wave][16 * t + l16] = total_sum;
+      }
+#pragma unroll
+      for (int c = 0; c < DT; ++c)
+        *reinterpret_cast<float4_t*>(acc + (wave * C::ROWS + 16 * t + l16) * HDP + 16 * c + 4 * g) = o[t][c];
+    }
+    __syncthreads();
+    const bool whole = u0 == 0 && u1 == ku;
+    const int part = 2 * (int)blockIdx.x + (u0 == 0 ? 1 : 0);
+    float* const part_o = ws + (size_t)part * C::ROWS * (HDP + 2);
+    float* const part_s = part_o + C::ROWS * HDP;
+    for (int i = tid; i < min(live_rows, C::ROWS) * (HDP / 4); i += C::THREADS) {
+      const int r = i / (HDP / 4), d = 4 * (i % (HDP / 4));
+      float top = stat[0][0][r];
+#pragma unroll
+      for (int w = 1; w < C::WAVES; ++w) top = fmaxf(top, stat[0][w][r]);
+      float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+      float l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < C::WAVES; ++w) {
+        // A wavefront without keys for the row has m = -inf, sums of 0 and no part (0 here, not -inf - -inf).
+        const float f = stat[0][w][r] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(stat[0][w][r] - top);
+        const float4_t x = *reinterpret_cast<const float4_t*>(acc + (w * C::ROWS + r) * HDP + d);
+        // A NaN among a wavefront's scores is in its sum, whatever its maximum says.
+        l += stat[1][w][r] != stat[1][w][r] ? stat[1][w][r] : f * stat[1][w][r];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += f == 0.0f ? 0.0f : f * x[e];
+      }
+      if (whole) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no keys: zeros
+        const int row = row0 + r, tok = row / rep, head = kv * rep + (row - tok * rep);
+        if (d < b.head_dim)
+          store_global((E*)b.out + (size_t)(tok0 + tok) * b.out_token + (size_t)head * b.out_head + d,
+                       u32x2{Elem<E>::pack(v[0] * inv, v[1] * inv), Elem<E>::pack(v[2] * inv, v[3] * inv)});
+      } else {
+        *reinterpret_cast<float4_t*>(part_o + r * HDP + d) = v;
+        if (d == 0) {
+          part_s[r] = top;
+          part_s[C::ROWS + r] = l;
+        }
+      }
+    }
+    if (tid == 0 && u0 == 0 && !whole)
+      pieces[blockIdx.x] = Piece{seq, row0, kv, (item_at + ku - 1) / per};
+    __syncthreads();  // the sums have been read: the buffers are free
+    at = item_at + u1;
+  }
+}
+
+// Joins the pieces of the items that workgroup blockIdx.x of the first launch began and did not end.
+template <class E, int HDP, int MT>
+__global__ __launch_bounds__(256) void join_pieces_kernel(AttnArgs a, int rep, const float* ws, const Piece* pieces) {
+  using C = FewConfig<HDP, MT>;
+  const Piece pc = pieces[blockIdx.x];
+  if (pc.seq < 0) return;
+  const int tok0 = seq_offset(a.cu, pc.seq, a.seqs, a.tokens);
+  const int rows = (seq_offset(a.cu, pc.seq + 1, a.seqs, a.tokens) - tok0) * rep;
+  const int live_rows = min(rows - pc.row0, C::ROWS);
+  constexpr int STRIDE = C::ROWS * (HDP + 2);
+  const int first = blockIdx.x;
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < live_rows * (HDP / 4); i += 256 * gridDim.y) {
+    const int r = i / (HDP / 4), d = 4 * (i % (HDP / 4));
+    float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f, top = -__builtin_inff();
+    for (int w = first; w <= pc.last; ++w) {
+      const float* const p = ws + (size_t)(2 * w + (w == first ? 1 : 0)) * STRIDE;
+      const float mw = p[C::ROWS * HDP + r], lw = p[C::ROWS * HDP + C::ROWS + r];
+      const float4_t x = *reinterpret_cast<const float4_t*>(p + r * HDP + d);
+      const float mn = fmaxf(top, mw);
+      const float f0 = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top - mn);
+      const float f1 = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - mn);
+      l = (l != l ? l : f0 * l) + (lw != lw ? lw : f1 * lw);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (f0 == 0.0f ? 0.0f : f0 * v[e]) + (f1 == 0.0f ? 0.0f : f1 * x[e]);
+      top = mn;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int row = pc.row0 + r, tok = row / rep, head = pc.kv * rep + (row - tok * rep);
+    if (d < a.head_dim)
+      store_global((E*)a.out + (size_t)(tok0 + tok) * a.out_token + (size_t)head * a.out_head + d,
+                   u32x2{Elem<E>::pack(v[0] * inv, v[1] * inv), Elem<E>::pack(v[2] * inv, v[3] * inv)});
+  }
+}
+
+template <class E, int HDP, int MT>
+hipError_t launch(const AttnArgs& a, int max_rows, int grid, void* ws, hipStream_t stream) {
+  using C = FewConfig<HDP, MT>;
+  const int rep = a.heads / a.kv_heads;
+  float* const parts = static_cast<float*>(ws);
+  Piece* const pieces = reinterpret_cast<Piece*>(parts + (size_t)2 * grid * C::ROWS * (HDP + 2));
+  few_rows_kernel<E, HDP, MT><<<grid, C::THREADS, 0, stream>>>(a, rep, max_rows, a.scale * 1.44269504088896340736f,
+                                                              parts, pieces);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  join_pieces_kernel<E, HDP, MT><<<dim3(grid, MT), 256, 0, stream>>>(a, rep, parts, pieces);
+  return hipGetLastError();
+}
+
+template <class E, int HDP>
+hipError_t launch_rows(const AttnArgs& a, int row_tiles, int max_rows, int grid, void* ws, hipStream_t stream) {
+  if constexpr (HDP != 256) {  // one row tile of 256 dims fills the registers
+    if (row_tiles == 2) return launch<E, HDP, 2>(a, max_rows, grid, ws, stream);
+  }
+  return launch<E, HDP, 1>(a, max_rows, grid, ws, stream);
+}
+
+template <class E>
+hipError_t launch_dim(const AttnArgs& a, int row_tiles, int max_rows, int grid, void* ws, hipStream_t stream) {
+  if (a.head_dim <= 64) return launch_rows<E, 64>(a, row_tiles, max_rows, grid, ws, stream);
+  if (a.head_dim <= 128) return launch_rows<E, 128>(a, row_tiles, max_rows, grid, ws, stream);
+  return launch_rows<E, 256>(a, row_tiles, max_rows, grid, ws, stream);
+}
+
+}  // namespace
+
+int few_rows_tiles(int head_dim, int64_t rows) { return head_dim <= 128 && rows > 16 ? 2 : 1; }
+
+size_t few_rows_workspace_bytes(int head_dim, int row_tiles, int grid) {
+  const int padded = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+  return (size_t)grid * (2 * sizeof(float) * 16 * row_tiles * (padded + 2) + sizeof(Piece));
+}
+
+int64_t few_rows_units(const AttnArgs& a, int row_tiles) {
+  const int64_t keys = (int64_t)a.table_width << a.log2_block;
+  const int unit = a.head_dim <= 128 ? FewConfig<128, 1>::UNIT : FewConfig<256, 1>::UNIT;
+  return ((int64_t)a.tokens * (a.heads / a.kv_heads) / (16 * row_tiles) + a.seqs) * a.kv_heads * (keys / unit + 1);
+}
+
+hipError_t few_rows_launch(const AttnArgs& a, bool bf16, int row_tiles, int max_rows, int grid, void* ws,
+                           hipStream_t stream) {
+  return bf16 ? launch_dim<bhalf_t>(a, row_tiles, max_rows, grid, ws, stream)
+              : launch_dim<half_t>(a, row_tiles, max_rows, grid, ws, stream);
+}
+
+}  // namespace kf

@@ -48,6 +48,42 @@ class RopeCache(ctypes.Structure):
                 ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("max_seq", ctypes.c_int)]
 
 
+_I64 = ctypes.c_int64
+
+
+class PagedTablesArgs(ctypes.Structure):
+    """kf_paged_tables_args of include/kf_int4.h."""
+    _fields_ = [(n, _VP) for n in ("block_table", "context_lens", "new_lens", "free_pages", "free_count", "cu_new",
+                                   "seq_lens", "positions", "slots", "free_left")] + \
+        [("table_stride", _I64)] + \
+        [(n, _I) for n in ("seqs", "table_width", "block_size", "free_capacity", "max_tokens")]
+
+
+class RopePagedArgs(ctypes.Structure):
+    """kf_rope_paged_args of include/kf_int4.h."""
+    _fields_ = [(n, _VP) for n in ("qkv", "cos", "sin", "positions", "slots", "qk", "cache_k", "cache_v")] + \
+        [(n, _I64) for n in ("qkv_stride", "k_page", "k_head", "k_token", "v_page", "v_head", "v_token")] + \
+        [(n, _I) for n in ("tokens", "heads", "kv_heads", "head_dim", "max_pos", "num_pages", "block_size", "dtype")]
+
+
+class PromptAttentionArgs(ctypes.Structure):
+    """kf_prompt_attention_args of include/kf_int4.h."""
+    _fields_ = [(n, _VP) for n in ("q", "k", "v", "out", "cu_seqlens")] + \
+        [(n, _I64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "out_token", "out_head")] + \
+        [(n, _I) for n in ("tokens", "seqs", "heads", "kv_heads", "head_dim", "dtype")] + \
+        [("scale", ctypes.c_float), ("zero_rest", _I)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """kf_paged_attention_args of include/kf_int4.h."""
+    _fields_ = [(n, _VP) for n in ("q", "cache_k", "cache_v", "out", "block_table", "cu_new", "seq_lens")] + \
+        [(n, _I64) for n in ("q_token", "q_head", "out_token", "out_head", "k_page", "k_head", "k_token", "v_page",
+                             "v_head", "v_token", "table_stride")] + \
+        [(n, _I) for n in ("tokens", "seqs", "heads", "kv_heads", "head_dim", "dtype", "table_width", "num_pages",
+                           "block_size", "max_new")] + \
+        [("scale", ctypes.c_float), ("zero_rest", _I)]
+
+
 SIGNATURES = {
     "kf_abi_version": (_I, []),
     "kf_last_error": (ctypes.c_char_p, []),
@@ -73,6 +109,11 @@ SIGNATURES = {
     "kf_bw_write": (_I, [_VP, _SZ, _I, _VP]),
     "kf_bw_read_store": (_I, [_VP, _VP, _SZ, _I, _VP]),
     "kf_decode_attention": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP]),
+    "kf_paged_tables": (_I, [ctypes.POINTER(PagedTablesArgs), _VP]),
+    "kf_rope_paged_cache": (_I, [ctypes.POINTER(RopePagedArgs), _VP]),
+    "kf_prompt_attention": (_I, [ctypes.POINTER(PromptAttentionArgs), _VP]),
+    "kf_paged_attention_workspace_bytes": (_SZ, [ctypes.POINTER(PagedAttentionArgs)]),
+    "kf_paged_attention": (_I, [ctypes.POINTER(PagedAttentionArgs), _VP, _SZ, _VP]),
     "kf_decode_argmax_step": (_I, [_VP, _I, _VP, _VP, _VP, _I, _VP, _VP]),
 }
 

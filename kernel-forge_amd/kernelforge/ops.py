@@ -15,7 +15,8 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-from typing import Optional
+import math
+from typing import NamedTuple, Optional
 
 import torch
 from torch.autograd import forward_ad
@@ -805,3 +806,373 @@ def decode_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
                                          kv_heads, q.shape[1], mask.shape[1], mask.stride(0), _stream_ptr(q.device))
     _lib.check(status, "decode_attention")
     return out
+
+
+# ---- several requests at once: a paged KV cache ---------------------------------------------------------
+#
+# cache_k, cache_v: fp16 or bf16 [num_pages, kv_heads, block_size, head_dim], the last dimension contiguous, block_size a
+# power of two from 16 up.  block_table int32 [requests, width]: the pages of each request in order; token i of
+# request r lies in slot block_table[r, i // block_size] * block_size + i % block_size.  One step of a server is
+# paged_tables, the q|k|v projection, rope_paged_cache, paged_attention (or prompt_attention where the step
+# is whole prompts only).  Inference only.
+
+_HALF_TYPES = {torch.float16: 1, torch.bfloat16: 2}  # KF_DTYPE_F16, KF_DTYPE_BF16
+
+
+class PagedStep(NamedTuple):
+    """What paged_tables makes of a step's lengths."""
+
+    cu_new: torch.Tensor      # int32 [requests + 1]: where each request's new tokens begin
+    seq_lens: torch.Tensor    # int32 [requests]: tokens of each request, the new ones included
+    positions: torch.Tensor   # int64 [max_tokens]: position of every new token in its request, -1 behind the last
+    slots: torch.Tensor       # int64 [max_tokens]: its slot of the cache, -1 where it has none
+    free_count: torch.Tensor  # int32 [1]: pages left on the stack
+
+
+def _check_plain(what: str, tensors) -> None:
+    """Refuses what a kernel launch would get wrong silently: transforms and gradients."""
+    if _transformed():
+        raise RuntimeError(f"{what} launches a kernel; it cannot be transformed")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} is inference only; an input requires a gradient (use torch.no_grad())")
+
+
+def _check_memory(name: str, t: torch.Tensor, device: torch.device) -> None:
+    if isinstance(t, FakeTensor) or t.is_meta:
+        raise RuntimeError(f"{name} has no device memory (a fake or meta tensor)")
+    if not t.is_cuda or t.device != device:
+        raise RuntimeError(f"{name} must be on {device}, a CUDA device, got {t.device}")
+
+
+def _check_int(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} tensor of shape {list(shape)}, got "
+                         f"{str(t.dtype)[6:]} {list(t.shape)}")
+
+
+def _check_table(block_table: torch.Tensor, requests: int) -> None:
+    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != requests
+            or block_table.shape[1] < 1 or block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be int32 [{requests}, width] with contiguous rows, got "
+                         f"{str(block_table.dtype)[6:]} {list(block_table.shape)}")
+
+
+def _check_block_size(block_size: int) -> None:
+    if block_size < 16 or block_size > 1 << 20 or block_size & (block_size - 1):
+        raise ValueError(f"block_size must be a power of two from 16 to 2^20, got {block_size}")
+
+
+def _check_cache(cache_k: torch.Tensor, cache_v: torch.Tensor, dtype: torch.dtype) -> None:
+    """The two caches of one shape and type, laid out as the kernels read them."""
+    if cache_k.dim() != 4 or cache_k.shape != cache_v.shape:
+        raise ValueError(f"cache_k and cache_v must be [num_pages, kv_heads, block_size, head_dim], got "
+                         f"{list(cache_k.shape)} and {list(cache_v.shape)}")
+    if cache_k.numel() == 0:
+        raise ValueError("cache_k and cache_v must not be empty")
+    _check_block_size(cache_k.shape[2])
+    for name, t in (("cache_k", cache_k), ("cache_v", cache_v)):
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must have the type of the queries, {str(dtype)[6:]}, got {str(t.dtype)[6:]}")
+        if not _rows_ok(t):
+            raise ValueError(f"{name} must have a contiguous last dimension, other strides of multiples of 8 and a "
+                             "16-byte aligned start")
+
+
+def _rows_ok(t: torch.Tensor) -> bool:
+    """Whether the kernels can read t's last dimension in 16-byte pieces."""
+    *strides, last = t.stride()
+    return last == 1 and all(s % 8 == 0 for s in strides) and (isinstance(t, FakeTensor) or t.data_ptr() % 16 == 0)
+
+
+def _check_heads(heads: int, kv_heads: int, head_dim: int) -> None:
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"kv_heads={kv_heads} must divide heads={heads}")
+    if head_dim < 8 or head_dim % 8 or head_dim > _ATTN_MAX_HEAD_DIM:
+        raise ValueError(f"head_dim must be a multiple of 8 up to {_ATTN_MAX_HEAD_DIM}, got {head_dim}")
+
+
+def _check_scale(scale: float | None, head_dim: int) -> float:
+    if scale is None:
+        return 1.0 / math.sqrt(head_dim)
+    if not 0.0 < scale < 3.0e38:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    return float(scale)
+
+
+def _check_out(out: torch.Tensor | None, q: torch.Tensor) -> None:
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not _rows_ok(out)):
+        raise ValueError(f"out must be {str(q.dtype)[6:]} {list(q.shape)} on {q.device} with a contiguous last dimension, "
+                         "other strides of multiples of 8 and a 16-byte aligned start")
+
+
+def paged_tables(block_table: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor,
+                 free_pages: torch.Tensor, free_count: torch.Tensor, *, block_size: int, max_tokens: int) -> PagedStep:
+    """The tables of one step from the requests' lengths, in one launch (kf_paged_tables).
+
+    block_table int32 [B, width] (updated in place); context_lens, new_lens int32 [B]: tokens of each
+    request in the cache and tokens that this step adds (0 for a request that pauses).  Pages that they need
+    beyond those they hold come from the stack free_pages int32 [F] with free_count int32 [1] pages on
+    it, the last first, and are entered into the table; -1 is entered once the stack is empty or where
+    context + new passes the table's width (no slot then).  max_tokens: rows of positions and slots (the step's tokens at least).
+    free_pages and free_count are not changed: PagedStep.free_count is the count after the step.
+    Lengths stay on the device, so a captured call follows them.  No reference counterpart.
+    """
+    b = block_table.shape[0] if block_table.dim() == 2 else -1
+    _check_table(block_table, b)
+    _check_int("context_lens", context_lens, torch.int32, (b,))
+    _check_int("new_lens", new_lens, torch.int32, (b,))
+    _check_int("free_count", free_count, torch.int32, (1,))
+    if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
+        raise ValueError("free_pages must be a contiguous 1-D int32 tensor")
+    _check_block_size(block_size)
+    if b < 1 or max_tokens < 0:
+        raise ValueError(f"paged_tables needs at least one request and max_tokens >= 0, got {b} and {max_tokens}")
+    args = (block_table, context_lens, new_lens, free_pages, free_count, int(block_size), int(max_tokens))
+    _check_plain("paged_tables", args[:5])
+    return PagedStep(*(_paged_tables_op(*args) if _traced(args[:5]) else _launch_paged_tables(*args)))
+
+
+def _launch_paged_tables(block_table, context_lens, new_lens, free_pages, free_count, block_size, max_tokens):
+    dev = block_table.device
+    for name, t in (("block_table", block_table), ("context_lens", context_lens), ("new_lens", new_lens),
+                    ("free_pages", free_pages), ("free_count", free_count)):
+        _check_memory(name, t, dev)
+    lib = _lib.load()
+    b, width = block_table.shape
+    cu_new = block_table.new_empty(b + 1)
+    seq_lens = block_table.new_empty(b)
+    free_left = block_table.new_empty(1)
+    positions = block_table.new_empty(max_tokens, dtype=torch.int64)
+    slots = torch.empty_like(positions)
+    args = _lib.PagedTablesArgs(_ptr(block_table), _ptr(context_lens), _ptr(new_lens), _ptr(free_pages),
+                                _ptr(free_count), _ptr(cu_new), _ptr(seq_lens), _ptr(positions), _ptr(slots),
+                                _ptr(free_left), block_table.stride(0), b, width, block_size, free_pages.numel(),
+                                max_tokens)
+    with _on(dev):
+        status = lib.kf_paged_tables(ctypes.byref(args), _stream_ptr(dev))
+    _lib.check(status, "paged_tables")
+    return cu_new, seq_lens, positions, slots, free_left
+
+
+@torch.library.custom_op("kernelforge::paged_tables", mutates_args=("block_table",))
+def _paged_tables_op(block_table: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor,
+                     free_pages: torch.Tensor, free_count: torch.Tensor, block_size: int, max_tokens: int
+                     ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _launch_paged_tables(block_table, context_lens, new_lens, free_pages, free_count, block_size, max_tokens)
+
+
+@_paged_tables_op.register_fake
+def _(block_table, context_lens, new_lens, free_pages, free_count, block_size, max_tokens):
+    b = block_table.shape[0]
+    return (block_table.new_empty(b + 1), block_table.new_empty(b), block_table.new_empty(max_tokens, dtype=torch.int64),
+            block_table.new_empty(max_tokens, dtype=torch.int64), block_table.new_empty(1))
+
+
+def rope_paged_cache(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                     slots: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, *,
+                     heads: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """RoPE on q and k of a q|k|v projection, and k and v into the cache's slots, in one launch (kf_rope_paged_cache).
+
+    qkv [T, (heads + 2 kv_heads) head_dim] (rows may be strided); cos, sin fp32 [max_pos, head_dim] (sin with the
+    rotate-half sign folded in, as in int4_qkv_rope_cache); positions, slots int64 [T] (PagedStep's).  Returns
+    the rotated q [T, heads, head_dim] and k [T, kv_heads, head_dim], views of one tensor, rotated in 32 bits and
+    rounded once; the caches get that k, and v as it is.  A slot outside the cache writes no cache entry, nor does a
+    position outside [0, max_pos), which rotates with row 0.  Slots must be distinct.  The form of
+    int4_qkv_rope_cache for many tokens and a paged cache; no reference counterpart.
+    """
+    if qkv.dim() != 2 or qkv.dtype not in _HALF_TYPES:
+        raise TypeError("qkv must be a 2-D fp16 or bf16 tensor [T, (heads + 2 kv_heads) head_dim]")
+    _check_cache(cache_k, cache_v, qkv.dtype)
+    kv_heads, d = cache_k.shape[1], cache_k.shape[3]
+    _check_heads(heads, kv_heads, d)
+    t = qkv.shape[0]
+    if qkv.shape[1] != (heads + 2 * kv_heads) * d:
+        raise ValueError(f"qkv has {qkv.shape[1]} columns, not (heads + 2 kv_heads) head_dim = "
+                         f"{(heads + 2 * kv_heads) * d}")
+    if cos.dim() != 2 or cos.shape[0] < 1:
+        raise ValueError(f"cos must be float32 [max_pos, {d}], got {list(cos.shape)}")
+    _check_int("cos", cos, torch.float32, (cos.shape[0], d))
+    _check_int("sin", sin, torch.float32, (cos.shape[0], d))
+    _check_int("positions", positions, torch.int64, (t,))
+    _check_int("slots", slots, torch.int64, (t,))
+    tensors = (qkv, cos, sin, positions, slots, cache_k, cache_v)
+    _check_plain("rope_paged_cache", tensors)
+    qk = (_rope_paged_op if _traced(tensors) else _launch_rope_paged)(*tensors, int(heads))
+    return qk[:, :heads], qk[:, heads:]
+
+
+def _launch_rope_paged(qkv, cos, sin, positions, slots, cache_k, cache_v, heads):
+    dev = qkv.device
+    for name, t in (("qkv", qkv), ("cos", cos), ("sin", sin), ("positions", positions), ("slots", slots),
+                    ("cache_k", cache_k), ("cache_v", cache_v)):
+        _check_memory(name, t, dev)
+    if not _rows_ok(qkv):
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    pages, kv_heads, block_size, d = cache_k.shape
+    qk = qkv.new_empty(qkv.shape[0], heads + kv_heads, d)
+    if qkv.shape[0] == 0:
+        return qk
+    cos, sin, positions, slots = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (cos, sin, positions, slots))
+    args = _lib.RopePagedArgs(_ptr(qkv), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(slots), _ptr(qk), _ptr(cache_k),
+                              _ptr(cache_v), qkv.stride(0), *cache_k.stride()[:3], *cache_v.stride()[:3], qkv.shape[0],
+                              heads, kv_heads, d, cos.shape[0], pages, block_size, _HALF_TYPES[qkv.dtype])
+    lib = _lib.load()
+    with _on(dev):
+        status = lib.kf_rope_paged_cache(ctypes.byref(args), _stream_ptr(dev))
+    _lib.check(status, "rope_paged_cache")
+    return qk
+
+
+@torch.library.custom_op("kernelforge::rope_paged_cache", mutates_args=("cache_k", "cache_v"))
+def _rope_paged_op(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                   slots: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, heads: int) -> torch.Tensor:
+    return _launch_rope_paged(qkv, cos, sin, positions, slots, cache_k, cache_v, heads)
+
+
+@_rope_paged_op.register_fake
+def _(qkv, cos, sin, positions, slots, cache_k, cache_v, heads):
+    return qkv.new_empty(qkv.shape[0], heads + cache_k.shape[1], cache_k.shape[3])
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, *,
+                     scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention over whole prompts, packed one after the other, in one launch (kf_prompt_attention).
+
+    q [T, heads, head_dim], k and v [T, kv_heads, head_dim], fp16 or bf16, any strides of the first two dimensions (views of a
+    fused projection are read in place); cu_seqlens int32 [B + 1] on the device: sequence s is rows
+    cu_seqlens[s] .. cu_seqlens[s + 1] - 1, ascending from 0, empty ones allowed.  Query head h reads KV head
+    h // (heads / kv_heads); scale defaults to 1 / sqrt(head_dim).  Scores, softmax and sums in 32 bits,
+    probabilities rounded to the inputs' type for their product with v.  Rows behind the last sequence are zeros
+    in a new output and left as they are in ``out``.  The form of decode_attention for prompts; no reference
+    counterpart (its models run torch's attention).
+    """
+    if q.dim() != 3 or q.dtype not in _HALF_TYPES:
+        raise TypeError("q must be a 3-D fp16 or bf16 tensor [T, heads, head_dim]")
+    t, heads, d = q.shape
+    if k.dim() != 3 or k.shape[0] != t or k.shape[2] != d or v.shape != k.shape:
+        raise ValueError(f"k and v must be [{t}, kv_heads, {d}], got {list(k.shape)} and {list(v.shape)}")
+    _check_heads(heads, k.shape[1], d)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"k and v must have the type of q, {str(q.dtype)[6:]}")
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
+        raise ValueError("cu_seqlens must be int32 [B + 1] with B >= 1")
+    _check_int("cu_seqlens", cu_seqlens, torch.int32, tuple(cu_seqlens.shape))
+    scale = _check_scale(scale, d)
+    _check_out(out, q)
+    tensors = (q, k, v, cu_seqlens)
+    _check_plain("prompt_attention", tensors)
+    if _traced(tensors):
+        if out is not None:
+            raise RuntimeError("prompt_attention with out updates it in place and has no traceable form")
+        return _prompt_attention_op(*tensors, scale)
+    return _launch_prompt(*tensors, scale, out)
+
+
+def _launch_prompt(q, k, v, cu_seqlens, scale, out=None):
+    dev = q.device
+    for name, t in (("q", q), ("k", k), ("v", v), ("cu_seqlens", cu_seqlens)):
+        _check_memory(name, t, dev)
+    q, k, v = (t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    zero_rest = out is None
+    if out is None:
+        out = q.new_empty(q.shape)
+    t, heads, d = q.shape
+    if t == 0:
+        return out
+    args = _lib.PromptAttentionArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(cu_seqlens), *q.stride()[:2],
+                                    *k.stride()[:2], *v.stride()[:2], *out.stride()[:2], t, cu_seqlens.numel() - 1, heads,
+                                    k.shape[1], d, _HALF_TYPES[q.dtype], scale, zero_rest)
+    lib = _lib.load()
+    with _on(dev):
+        status = lib.kf_prompt_attention(ctypes.byref(args), _stream_ptr(dev))
+    _lib.check(status, "prompt_attention")
+    return out
+
+
+@torch.library.custom_op("kernelforge::prompt_attention", mutates_args=())
+def _prompt_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                         scale: float) -> torch.Tensor:
+    return _launch_prompt(q, k, v, cu_seqlens, scale)
+
+
+@_prompt_attention_op.register_fake
+def _(q, k, v, cu_seqlens, scale):
+    return q.new_empty(q.shape)
+
+
+def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, block_table: torch.Tensor,
+                    cu_new: torch.Tensor, seq_lens: torch.Tensor, *, max_new: int | None = None,
+                    scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of every request's new tokens over its pages of the cache (kf_paged_attention).
+
+    q [T, heads, head_dim], fp16 or bf16, any strides of the first two dimensions; block_table int32 [B, width];
+    cu_new int32 [B + 1]: request r's new tokens are rows cu_new[r] .. cu_new[r + 1] - 1 of q, the
+    last ones of its seq_lens[r] tokens (int32 [B]), whose keys and values the cache holds already
+    (rope_paged_cache).  One token per request (decode), chunks of prompts and batches of both.  max_new: an upper bound
+    of a request's new tokens, if the caller knows one; it chooses kernels and splits only.  Tokens whose page is not
+    in the cache (-1) are not attended to; a row with no key gets zeros.  Rows behind the last request are zeros in a
+    new output and left as they are in ``out``.  Arithmetic as in prompt_attention; results do not change from
+    run to run.  The form of decode_attention for many requests; no reference counterpart.
+    """
+    if q.dim() != 3 or q.dtype not in _HALF_TYPES:
+        raise TypeError("q must be a 3-D fp16 or bf16 tensor [T, heads, head_dim]")
+    _check_cache(cache_k, cache_v, q.dtype)
+    if q.shape[2] != cache_k.shape[3]:
+        raise ValueError(f"q has head_dim {q.shape[2]}, the caches {cache_k.shape[3]}")
+    _check_heads(q.shape[1], cache_k.shape[1], q.shape[2])
+    b = seq_lens.numel()
+    _check_int("seq_lens", seq_lens, torch.int32, (b,))
+    _check_int("cu_new", cu_new, torch.int32, (b + 1,))
+    _check_table(block_table, b)
+    if b < 1:
+        raise ValueError("paged_attention needs at least one request")
+    if max_new is not None and max_new < 1:
+        raise ValueError(f"max_new must be positive, got {max_new}")
+    scale = _check_scale(scale, q.shape[2])
+    _check_out(out, q)
+    tensors = (q, cache_k, cache_v, block_table, cu_new, seq_lens)
+    _check_plain("paged_attention", tensors)
+    if _traced(tensors):
+        if out is not None:
+            raise RuntimeError("paged_attention with out updates it in place and has no traceable form")
+        return _paged_attention_op(*tensors, int(max_new or 0), scale)
+    return _launch_paged(*tensors, int(max_new or 0), scale, out)
+
+
+def _launch_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scale, out=None):
+    dev = q.device
+    for name, t in (("q", q), ("cache_k", cache_k), ("cache_v", cache_v), ("block_table", block_table),
+                    ("cu_new", cu_new), ("seq_lens", seq_lens)):
+        _check_memory(name, t, dev)
+    if not _rows_ok(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    zero_rest = out is None
+    if out is None:
+        out = q.new_empty(q.shape)
+    t, heads, d = q.shape
+    if t == 0:
+        return out
+    pages, kv_heads, block_size, _ = cache_k.shape
+    args = _lib.PagedAttentionArgs(_ptr(q), _ptr(cache_k), _ptr(cache_v), _ptr(out), _ptr(block_table), _ptr(cu_new),
+                                   _ptr(seq_lens), *q.stride()[:2], *out.stride()[:2], *cache_k.stride()[:3],
+                                   *cache_v.stride()[:3], block_table.stride(0), t, seq_lens.numel(), heads, kv_heads, d,
+                                   _HALF_TYPES[q.dtype], block_table.shape[1], pages, block_size, max_new, scale, zero_rest)
+    lib = _lib.load()
+    with _on(dev):
+        ws_bytes = lib.kf_paged_attention_workspace_bytes(ctypes.byref(args))
+        ws = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+        status = lib.kf_paged_attention(ctypes.byref(args), _ptr(ws) if ws is not None else None, ws_bytes,
+                                        _stream_ptr(dev))
+    _lib.check(status, "paged_attention")
+    return out
+
+
+@torch.library.custom_op("kernelforge::paged_attention", mutates_args=())
+def _paged_attention_op(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, block_table: torch.Tensor,
+                        cu_new: torch.Tensor, seq_lens: torch.Tensor, max_new: int, scale: float) -> torch.Tensor:
+    return _launch_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scale)
+
+
+@_paged_attention_op.register_fake
+def _(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scale):
+    return q.new_empty(q.shape)

@@ -1,0 +1,202 @@
+"""Attention of new tokens over a paged cache against float64 (needs a GPU): single tokens, chunks and both in one
+batch; lengths at the edges of pages, tiles and splits; pages that are not there; caches of other layouts."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from kernelforge import ops
+
+from attention_cases import attend64, check, offsets
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+class Batch:
+    """Requests of ctx[r] + new[r] tokens over shuffled pages; unused slots hold NaN."""
+
+    def __init__(self, ctx, new, heads, kv_heads, d, dtype, block, pad=0, extra_width=2, seed=0):
+        g = torch.Generator(device=DEV).manual_seed(seed + heads + d + block + sum(ctx))
+        self.ctx, self.new, self.block = ctx, new, block
+        need = [-(-(c + n) // block) for c, n in zip(ctx, new)]
+        pages = sum(need) + 2
+        perm = torch.randperm(pages, generator=g, device=DEV).int()
+        self.table = torch.full((len(ctx), max(need) + extra_width), -1, dtype=torch.int32, device=DEV)
+        self.cache_k = torch.full((pages, kv_heads, block, d), float("nan"), dtype=dtype, device=DEV)
+        self.cache_v = self.cache_k.clone()
+        self.k, self.v = [], []
+        at = 0
+        for r, (c, n) in enumerate(zip(ctx, new)):
+            self.table[r, :need[r]] = perm[at:at + need[r]]
+            at += need[r]
+            k, v = (torch.randn(c + n, kv_heads, d, generator=g, device=DEV).to(dtype) for _ in range(2))
+            self.k.append(k)
+            self.v.append(v)
+            i = torch.arange(c + n, device=DEV)
+            page = self.table[r].long()[i // block]
+            self.cache_k[page, :, i % block] = k
+            self.cache_v[page, :, i % block] = v
+        self.q = torch.randn(sum(new) + pad, heads, d, generator=g, device=DEV).to(dtype)
+        self.cu = offsets(new, DEV)
+        self.seq_lens = torch.tensor([c + n for c, n in zip(ctx, new)], dtype=torch.int32, device=DEV)
+
+    def __call__(self, **kw):
+        return ops.paged_attention(self.q, self.cache_k, self.cache_v, self.table, self.cu, self.seq_lens, **kw)
+
+    def check(self, out, there=None):
+        at, worst = 0, 0.0
+        for r, n in enumerate(self.new):
+            if n:
+                ref, bound = attend64(self.q[at:at + n], self.k[r], self.v[r], None if there is None else there[r])
+                worst = max(worst, check(out[at:at + n], ref, bound, f"request {r}"))
+            at += n
+        assert bool((out[at:] == 0).all())
+        return worst
+
+
+LAYOUTS = [(32, 4, 64), (12, 2, 128), (8, 8, 96), (16, 1, 80), (4, 2, 256), (3, 3, 8), (40, 1, 64), (24, 1, 200)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d", LAYOUTS)
+@pytest.mark.parametrize("block", [16, 64])
+def test_decode(dtype, heads, kv_heads, d, block):
+    b = Batch([0, 1, 15, 16, 31, 127, 128, 500, 1025], [1] * 9, heads, kv_heads, d, dtype, block, pad=2)
+    b.check(b(max_new=1))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d", LAYOUTS)
+@pytest.mark.parametrize("block", [16, 128])
+def test_mixed(dtype, heads, kv_heads, d, block):
+    b = Batch([0, 70, 300, 5, 640, 33], [130, 1, 17, 0, 3, 64], heads, kv_heads, d, dtype, block, pad=3)
+    b.check(b(max_new=130))
+    assert torch.equal(b(), b(max_new=130))
+
+
+@pytest.mark.parametrize("ctx,new", [([20000], [1]), ([9000, 3], [1, 1]), ([4000], [300]), ([0], [777]), ([5000] * 3, [2] * 3),
+                                     ([40] * 300, [1] * 300), ([3000, 0, 17], [1, 900, 2])],
+                         ids=["long", "uneven", "chunk", "prompt", "few", "many", "both"])
+def test_lengths(ctx, new):
+    b = Batch(ctx, new, 8, 2, 64, torch.float16, 16)
+    b.check(b(max_new=max(new)))
+
+
+def test_hint_only_chooses_kernels():
+    """A hint that is too small costs time, never rows."""
+    b = Batch([100, 40], [90, 1], 8, 2, 64, torch.float16, 16)
+    b.check(b(max_new=1))
+
+
+def test_pages_that_are_not_there():
+    """Holes in a table: their keys are not attended to, whatever number stands there; rows without any key are zeros."""
+    for ctx, new in (([200, 64, 10], [1, 1, 1]), ([200, 0, 10], [100, 90, 6])):
+        b = Batch(ctx, new, 8, 2, 128, torch.bfloat16, 16)
+        there = [torch.ones(c + n, dtype=torch.bool, device=DEV) for c, n in zip(ctx, new)]
+        for r, page, value in ((0, 0, -1), (0, 5, 1 << 30), (0, 12, b.cache_k.shape[0]), (2, 0, -7)):
+            b.table[r, page] = value
+            there[r][16 * page:16 * page + 16] = False
+        out = b(max_new=max(new))
+        b.check(out, there)
+        assert bool((out[int(b.cu[2])] == 0).all()) or bool(there[2][:11].any())
+
+
+def test_lengths_that_do_not_fit_stay_inside():
+    """Wrong lengths and offsets give some result, from inside the arrays."""
+    b = Batch([50, 20], [1, 1], 4, 2, 64, torch.float16, 16)
+    b.seq_lens.copy_(torch.tensor([1 << 30, -5]))
+    out = b(max_new=1)
+    assert bool((out[1] == 0).all())
+    b = Batch([50, 20], [40, 40], 4, 2, 64, torch.float16, 16)
+    b.seq_lens.copy_(torch.tensor([3, 0]))  # fewer keys than new tokens: the first rows have none
+    out = b()
+    assert bool((out[:37] == 0).all()) and bool(out[37:40].isfinite().all()) and bool((out[40:] == 0).all())
+    b.cu.copy_(torch.tensor([0, 1 << 30, -4]))
+    b()
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_later_and_unused_slots_do_not_reach_a_row(new, bad):
+    """Slots behind a request's last token hold NaN in every test here; a later token's value does not reach
+    the rows before it."""
+    b = Batch([37, 90], [new, new], 8, 2, 64, torch.float16, 16)
+    want = b(max_new=new)
+    last = 37 + new - 1
+    page = int(b.table[0, last // 16])
+    b.cache_v[page, 1, last % 16, 5] = bad
+    out = b(max_new=new)
+    hit = out[new - 1, 4:, 5]
+    assert bool(hit.isnan().all()) if bad != bad else bool((hit == bad).all())
+    out[new - 1, 4:, 5] = want[new - 1, 4:, 5]
+    assert torch.equal(out, want)
+
+
+def test_cache_layouts_and_strides():
+    """Slots before heads, and both caches in one array: the same bits."""
+    b = Batch([300, 12, 70], [1, 60, 2], 8, 2, 64, torch.float16, 32)
+    want = b(max_new=60)
+    k, v = b.cache_k, b.cache_v
+    b.cache_k = k.transpose(1, 2).contiguous().transpose(1, 2)
+    b.cache_v = v.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(b(max_new=60), want)
+    both = torch.stack([k, v], 1)
+    b.cache_k, b.cache_v = both[:, 0], both[:, 1]
+    wide = torch.full((3, b.table.shape[1] + 5), -1, dtype=torch.int32, device=DEV)
+    wide[:, :b.table.shape[1]] = b.table
+    b.table = wide[:, :b.table.shape[1]]
+    q = b.q
+    b.q = torch.cat([q, q], 2)[..., :64]
+    assert torch.equal(b(max_new=60), want)
+    out = torch.full_like(q, 3.0)
+    assert torch.equal(b(max_new=60, out=out), want)
+
+
+def test_far_pages_pass_32_bits():
+    """A cache of more than 2^32 bytes per array: the last pages are read."""
+    pages = 70000
+    k = torch.zeros(pages, 4, 64, 128, dtype=torch.bfloat16, device=DEV)
+    v = torch.zeros_like(k)
+    b = Batch([500, 100], [1, 80], 8, 4, 128, torch.bfloat16, 64)
+    n = b.cache_k.shape[0]
+    k[pages - n:], v[pages - n:] = b.cache_k, b.cache_v
+    want = b(max_new=80)
+    b.cache_k, b.cache_v = k, v
+    b.table = torch.where(b.table >= 0, b.table + (pages - n), b.table)
+    assert torch.equal(b(max_new=80), want)
+
+
+def test_captured_and_replayed():
+    """Captured calls follow the lengths on the device; every replay equals the eager call, other work between."""
+    b = Batch([600, 40, 0], [1, 1, 1], 8, 2, 64, torch.float16, 16, extra_width=40)
+    b(max_new=1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = b(max_new=1)
+        out2 = b()
+    for lens in ([601, 41, 1], [3, 41, 1], [601, 2, 1], [17, 16, 0]):
+        b.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        want = b(max_new=1)
+        junk = torch.randn(1 << 20, device=DEV).sum()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(out2, want) and bool(junk.isfinite())
+
+
+def test_two_streams_at_once():
+    """Two calls that may overlap have workspaces of their own."""
+    a = Batch([9000, 100], [1, 1], 8, 2, 64, torch.float16, 16)
+    b = Batch([70, 7000], [1, 1], 8, 2, 64, torch.float16, 16, seed=5)
+    want = a(max_new=1), b(max_new=1)
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(3):
+        for x, s in zip((a, b), streams):
+            with torch.cuda.stream(s):
+                got.append(x(max_new=1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got))
