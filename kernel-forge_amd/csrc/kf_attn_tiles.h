@@ -93,25 +93,27 @@ __device__ __forceinline__ constexpr int swizzle_v16(int key) {
   return HDP == 64 ? 2 * ((key >> 1) & 3) : 2 * (key & 7);
 }
 
-// Copies 16 keys of K and of V into tiles, swizzled.  The source offsets of a lane do not change, so a copy of 16 keys
+// Copies ROWS keys of K and of V into tiles, swizzled.  The source offsets of a lane do not change, so a copy of keys
 // that are all there is one instruction per KiB.
-template <class E, int HDP, bool V16>
-struct Copy16 {
+template <class E, int HDP, bool V16, int ROWS = 16>
+struct TileCopy {
   static constexpr int CPR = HDP / 8;    // 16-byte pieces per row
   static constexpr int RPI = 64 / CPR;   // rows per copy instruction
-  static constexpr int N = 16 / RPI;     // instructions per tile
+  static constexpr int N = ROWS / RPI;   // instructions per tile
   uint32_t vo_k[N], vo_v[N];
   int pieces;  // of a row that are there
+  int row0;    // the first key's row in the tile, mod 16 (ROWS < 16 only)
 
-  __device__ __forceinline__ static int piece_k(int j, int lane) {
-    return (lane % CPR) ^ swizzle_k<HDP>(RPI * j + lane / CPR);
+  __device__ __forceinline__ int piece_k(int j, int lane) const {
+    return (lane % CPR) ^ swizzle_k<HDP>(row0 + RPI * j + lane / CPR);
   }
-  __device__ __forceinline__ static int piece_v(int j, int lane) {
-    const int r = RPI * j + lane / CPR;
+  __device__ __forceinline__ int piece_v(int j, int lane) const {
+    const int r = row0 + RPI * j + lane / CPR;
     return (lane % CPR) ^ (V16 ? swizzle_v16<HDP>(r) : swizzle_v<HDP>(r));
   }
   // Strides of at most 2^26 elements (checked by the caller), so offsets fit 32 bits.
-  __device__ __forceinline__ Copy16(int64_t k_token, int64_t v_token, int head_dim, int lane) : pieces(head_dim / 8) {
+  __device__ __forceinline__ TileCopy(int64_t k_token, int64_t v_token, int head_dim, int lane, int tile_row = 0)
+      : pieces(head_dim / 8), row0(ROWS < 16 ? tile_row & 15 : 0) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const uint32_t r = RPI * j + lane / CPR;
@@ -119,11 +121,11 @@ struct Copy16 {
       vo_v[j] = 2u * (r * (uint32_t)v_token + 8u * piece_v(j, lane));
     }
   }
-  // kb, vb: the first key's values; `rows` of the 16 keys are there (any value), the others and the pieces past
+  // kb, vb: the first key's values; `rows` of the keys are there (any value), the others and the pieces past
   // the head size become zeros.
   __device__ __forceinline__ void operator()(uint32_t dst_k, uint32_t dst_v, const E* kb, const E* vb, int rows,
                                              int lane) const {
-    if (rows >= 16 && pieces == CPR) {
+    if (rows >= ROWS && pieces == CPR) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         lds_dma16(dst_k + 1024 * j, kb, vo_k[j]);
@@ -173,30 +175,38 @@ __device__ __forceinline__ bool any_nonfinite(u32x4 v) {
 }
 
 // A piece of V next to masked keys.  A masked key may hold infinities or NaN, which a probability of zero does not
-// cancel.  They are taken out of v, and come back as ones where v had NaN, +inf and -inf: with ones for the
-// probabilities of the keys that a row attends to, a product counts how many of them the row meets.
+// cancel.  So where a tile has both, they are taken out of the product (finite_only), and three more products with ones for
+// the probabilities of the keys that a row attends to and ones where V has NaN, +inf or -inf (kind 0, 1, 2) count how
+// many of each a row meets.
 template <class E>
-__device__ __forceinline__ void split_nonfinite(u32x4& v, u32x4& nan, u32x4& pos, u32x4& neg) {
+__device__ __forceinline__ u32x4 finite_only(u32x4 v) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t wn = 0, wp = 0, wm = 0, keep = 0;
+    const uint32_t inf = Elem<E>::kExp;
+    if ((v[i] & inf & 0xFFFFu) == (inf & 0xFFFFu)) v[i] &= 0xFFFF0000u;
+    if ((v[i] & inf & 0xFFFF0000u) == (inf & 0xFFFF0000u)) v[i] &= 0x0000FFFFu;
+  }
+  return v;
+}
+template <class E>
+__device__ __forceinline__ u32x4 nonfinite_ones(u32x4 v, int kind) {
+  constexpr uint32_t inf = Elem<E>::kExp & 0xFFFFu, one = Elem<E>::kOnes & 0xFFFFu;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w = 0;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const uint32_t x = (v[i] >> (16 * e)) & 0xFFFFu, ex = Elem<E>::kExp & 0xFFFFu;
-      const uint32_t one = (Elem<E>::kOnes & 0xFFFFu) << (16 * e);
-      if ((x & ex) != ex) keep |= 0xFFFFu << (16 * e);
-      else if (x == ex) wp |= one;
-      else if (x == (ex | 0x8000u)) wm |= one;
-      else wn |= one;
+      const uint32_t x = (v[i] >> (16 * e)) & 0xFFFFu;
+      const bool hit = kind == 0 ? (x & 0x7FFFu) > inf : x == (kind == 1 ? inf : inf | 0x8000u);
+      w |= hit ? one << (16 * e) : 0u;
     }
-    nan[i] = wn, pos[i] = wp, neg[i] = wm;
-    v[i] &= keep;
+    v[i] = w;
   }
+  return v;
 }
-__device__ __forceinline__ float with_nonfinite(float o, float nan, float pos, float neg) {
-  if (pos > 0.0f) o += __builtin_inff();
-  if (neg > 0.0f) o -= __builtin_inff();
-  return nan > 0.0f ? __builtin_nanf("") : o;
+__device__ __forceinline__ float add_nonfinite(float o, float count, int kind) {
+  const float x = kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
+  return count > 0.0f ? o + x : o;
 }
 
 // Lengths, offsets and pages do not change while a kernel runs: scalar loads where the index is uniform.

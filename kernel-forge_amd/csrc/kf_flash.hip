@@ -4,7 +4,7 @@
 //   out[t, h] = sum_s softmax_s(scale q[t, h] . k[s, kv]) v[s, kv],   s <= position of t,   kv = h / rep
 //
 // A workgroup owns 128 rows of one KV head (kf_attn_tiles.h), 32 per wavefront, and walks their keys 64 at a
-// time through two LDS buffers.  Scores, maximum, sum and outputs are held in 32 bits; probabilities are rounded to
+// time (32 for heads of more than 128, whose outputs fill half the registers) through two LDS buffers.  Scores, maximum, sum and outputs are held in 32 bits; probabilities are rounded to
 // the inputs' type for the second matrix product (half a step of that type, as inputs are), the outputs once
 // more when they are stored.  The maximum that the exponentials are taken against follows the true one only when it is
 // exceeded by a factor 2^8: outputs and sums are then rescaled, which most tiles after the first spare.
@@ -16,16 +16,23 @@ namespace {
 
 constexpr int kFlashWaves = 4, kFlashThreads = 64 * kFlashWaves;
 constexpr int kFlashRows = 32 * kFlashWaves;
-constexpr int kFlashKeys = 64;
+
+// Wavefronts per SIMD that the registers have to allow: one computes scores while another works on its
+// softmax.  From two on the products also accumulate in ordinary registers, without moves.
+constexpr int flash_waves_per_simd(int hdp) { return hdp == 64 ? 3 : hdp == 128 ? 2 : 1; }
 
 template <class E, int HDP, bool PAGED>
-__global__ __launch_bounds__(kFlashThreads) void flash_attention_kernel(AttnArgs a, int rep, int min_rows,
+__global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flash_attention_kernel(AttnArgs a, int rep, int min_rows,
                                                                         float scale_log2) {
   constexpr int ROW = HDP * 2;                      // bytes
-  constexpr int TILE = kFlashKeys * ROW;
+  constexpr int KEYS = HDP == 256 ? 32 : 64, KU = KEYS / 32, KK = KEYS / 16;
+  constexpr int MINE = KEYS / kFlashWaves;           // keys of a tile that a wavefront fetches
+  constexpr int TILE = KEYS * ROW;
   constexpr int ST = HDP / 16;                      // k steps of the first product
   constexpr int DT = HDP / 32;                      // 32-row tiles of O^T
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
+  // Queries of more than 128 dims leave no registers for themselves beside the outputs: each lane's stay in LDS.
+  constexpr bool Q_LDS = HDP == 256;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE + (Q_LDS ? kFlashRows * ROW : 0)];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -61,14 +68,18 @@ __global__ __launch_bounds__(kFlashThreads) void flash_attention_kernel(AttnArgs
   const int wave_row = row0 + 32 * wave;
   const int wave_lo = shift + min(wave_row, rows - 1) / rep, wave_hi = shift + min(wave_row + 31, rows - 1) / rep;
   const int kend = shift + min(row0 + kFlashRows - 1, rows - 1) / rep + 1;
-  const int tiles = kend <= 0 ? 0 : (kend + kFlashKeys - 1) / kFlashKeys;
+  const int tiles = kend <= 0 ? 0 : (kend + KEYS - 1) / KEYS;
 
-  u32x4 qf[ST];
+  u32x4 qf[Q_LDS ? 1 : ST];
+  u32x4* const q_lds = reinterpret_cast<u32x4*>(smem + 4 * TILE) + wave * ST * 64 + lane;
   {
     const E* const qp = (const E*)a.q + (size_t)(tok0 + tok) * a.q_token + (size_t)head * a.q_head;
 #pragma unroll
-    for (int s = 0; s < ST; ++s)
-      qf[s] = 2 * s + half < a.head_dim / 8 ? load_global16(qp + 16 * s + 8 * half) : u32x4{0, 0, 0, 0};
+    for (int s = 0; s < ST; ++s) {
+      const u32x4 x = 2 * s + half < a.head_dim / 8 ? load_global16(qp + 16 * s + 8 * half) : u32x4{0, 0, 0, 0};
+      if constexpr (Q_LDS) q_lds[64 * s] = x;
+      else qf[s] = x;
+    }
   }
 
   // Copies.  A wavefront fetches rows 16 wave .. + 15 of both tiles: one page, as pages hold 16 keys at least.
@@ -77,12 +88,12 @@ __global__ __launch_bounds__(kFlashThreads) void flash_attention_kernel(AttnArgs
     const int p = load_const(a.table, table_at + (min(key, kend - 1) >> a.log2_block));
     return (unsigned)p < (unsigned)a.num_pages ? p : -1;
   };
-  const Copy16<E, HDP, false> copy(a.k_token, a.v_token, a.head_dim, lane);
+  const TileCopy<E, HDP, false, MINE> copy(a.k_token, a.v_token, a.head_dim, lane, MINE * wave);
   auto issue = [&](int kt, uint32_t buf, int page) {
-    const int key0 = kt * kFlashKeys + 16 * wave;
+    const int key0 = kt * KEYS + MINE * wave;
     const E* const k = (const E*)a.k + kv * a.k_head;
     const E* const v = (const E*)a.v + kv * a.v_head;
-    const uint32_t dst = lds + buf + (uint32_t)(16 * wave) * ROW;
+    const uint32_t dst = lds + buf + (uint32_t)(MINE * wave) * ROW;
     if constexpr (PAGED) {
       const int slot = key0 & ((1 << a.log2_block) - 1);
       copy(dst, dst + TILE, k + page * a.k_page + slot * a.k_token, v + page * a.v_page + slot * a.v_token,
@@ -112,53 +123,70 @@ __global__ __launch_bounds__(kFlashThreads) void flash_attention_kernel(AttnArgs
 
   int page = 0;
   if (tiles > 0) {
-    if constexpr (PAGED) page = page_of(16 * wave);
+    if constexpr (PAGED) page = page_of(MINE * wave);
     issue(0, 0, page);
-    if constexpr (PAGED) page = page_of(min(kFlashKeys, kend - 1) + 16 * wave);
+    if constexpr (PAGED) page = page_of(min(KEYS, kend - 1) + MINE * wave);
   }
   for (int kt = 0; kt < tiles; ++kt) {
     const uint32_t buf = (kt & 1) * 2 * TILE;
     dma_barrier();
     if (kt + 1 < tiles) {
       issue(kt + 1, 2 * TILE - buf, page);
-      if constexpr (PAGED) page = page_of((kt + 2) * kFlashKeys + 16 * wave);
+      if constexpr (PAGED) page = page_of((kt + 2) * KEYS + MINE * wave);
     }
-    const int key0 = kt * kFlashKeys;
+    const int key0 = kt * KEYS;
     if (key0 > wave_hi) continue;  // only other wavefronts have keys here
 
-    float16_t s[2];
+    float16_t s[KU];
     const uint32_t kb = lds + buf + k_at;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < KU; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
 #pragma unroll
-      for (int st = 0; st < ST; ++st)
-        s[u] = Elem<E>::mfma32(lds_read16((kb ^ (uint32_t)(32 * st)) + u * 32 * ROW), qf[st], s[u]);
-    }
+    for (int st = 0; st < ST; ++st)
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+        s[u] = Elem<E>::mfma32(lds_read16((kb ^ (uint32_t)(32 * st)) + u * 32 * ROW), Q_LDS ? q_lds[64 * st] : qf[Q_LDS ? 0 : st], s[u]);
 
     // Masks: keys past a row's own, pages that are not there.
     uint32_t bad = 0;  // bit i: keys key0 + 16 i .. + 15 are not there
     if constexpr (PAGED) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) bad |= page_of(key0 + 16 * i) < 0 ? 1u << i : 0u;
+      for (int i = 0; i < KK; ++i) bad |= page_of(key0 + 16 * i) < 0 ? 1u << i : 0u;
     }
-    const bool masked = key0 + kFlashKeys - 1 > wave_lo || bad != 0;
+    const bool masked = key0 + KEYS - 1 > wave_lo || bad != 0;
     // The last of this lane's keys key0 + 8 q + 4 half + (0 .. 3) that its row attends to, as 0 .. 3 (below: none).
     auto keys_at = [&](int q) { return (bad >> (q >> 1)) & 1 ? -1 : limit - (key0 + 8 * q + 4 * half); };
+    const uint32_t vb = lds + buf + v_at;
+    auto v_block = [&](int kk, int t) {
+      const uint32_t at = (vb ^ (uint32_t)(64 * t)) + kk * 16 * ROW;
+      const u32x2 v0 = lds_read_tr(at), v1 = lds_read_tr(at + 8 * ROW);
+      return u32x4{v0[0], v0[1], v1[0], v1[1]};
+    };
+    bool nonfinite = false;
     if (masked) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
+      for (int q = 0; q < 2 * KK; ++q) {
         const int last = keys_at(q);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (e > last) s[q >> 2][4 * (q & 3) + e] = -__builtin_inff();
       }
+      bool any = false;
+#pragma unroll 1
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          any |= any_nonfinite<E>(v_block(kk, t));
+          if constexpr (HDP == 256) __builtin_amdgcn_sched_barrier(0);
+        }
+      nonfinite = __ballot(any) != 0;
     }
 
     float mx = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i >> 4][i & 15]);
+    for (int i = 1; i < 16 * KU; ++i) mx = fmaxf(mx, s[i >> 4][i & 15]);
     mx = max_halves(mx);
     if (__ballot(mx > limit_max)) {
       const float mn = fmaxf(m, mx);
@@ -173,43 +201,49 @@ __global__ __launch_bounds__(kFlashThreads) void flash_attention_kernel(AttnArgs
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] *= f;
     }
+    u32x4 p[KK];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int kk = 0; kk < KK; ++kk) {
+      float e[8];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], scale_log2, -mc));
-        sum += s[u][i];
+      for (int i = 0; i < 8; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(fmaf(s[kk >> 1][8 * (kk & 1) + i], scale_log2, -mc));
+        sum += e[i];
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[kk][i] = Elem<E>::pack(e[2 * i], e[2 * i + 1]);
+      asm volatile("" : "+v"(sum));  // the sums are taken here: the 32-bit probabilities are not kept
+    }
 
-    const uint32_t vb = lds + buf + v_at;
+    if (!nonfinite) {
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      u32x4 p;
+      for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = Elem<E>::pack(s[kk >> 1][8 * (kk & 1) + 2 * i], s[kk >> 1][8 * (kk & 1) + 2 * i + 1]);
+        for (int t = 0; t < DT; ++t) o[t] = Elem<E>::mfma32(v_block(kk, t), p[kk], o[t]);
+    } else {
+#pragma unroll 1
+      for (int kk = 0; kk < KK; ++kk) {
+        const u32x4 pk = kk == 0 ? p[0] : kk == 1 ? p[1] : kk == 2 ? p[KK - 2] : p[KK - 1];
+        u32x4 live;
 #pragma unroll
-      for (int t = 0; t < DT; ++t) {
-        const uint32_t at = (vb ^ (uint32_t)(64 * t)) + kk * 16 * ROW;
-        const u32x2 v0 = lds_read_tr(at), v1 = lds_read_tr(at + 8 * ROW);
-        u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
-        if (masked && __ballot(any_nonfinite<E>(v))) {
-          u32x4 live;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int last = keys_at(2 * kk + (i >> 1)) - 2 * (i & 1);
-            live[i] = last < 0 ? 0u : last == 0 ? Elem<E>::kOnes & 0xFFFFu : Elem<E>::kOnes;
-          }
-          u32x4 nan, pos, neg;
-          split_nonfinite<E>(v, nan, pos, neg);
-          float16_t z;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) z[i] = 0.0f;
-          const float16_t cn = Elem<E>::mfma32(nan, live, z), cp = Elem<E>::mfma32(pos, live, z);
-          const float16_t cm = Elem<E>::mfma32(neg, live, z);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[t][i] = with_nonfinite(o[t][i], cn[i], cp[i], cm[i]);
+        for (int i = 0; i < 4; ++i) {
+          const int last = keys_at(2 * kk + (i >> 1)) - 2 * (i & 1);
+          live[i] = last < 0 ? 0u : last == 0 ? Elem<E>::kOnes & 0xFFFFu : Elem<E>::kOnes;
         }
-        o[t] = Elem<E>::mfma32(v, p, o[t]);
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          o[t] = Elem<E>::mfma32(finite_only<E>(v_block(kk, t)), pk, o[t]);
+#pragma unroll 1
+          for (int kind = 0; kind < 3; ++kind) {
+            float16_t c;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) c[i] = 0.0f;
+            c = Elem<E>::mfma32(nonfinite_ones<E>(v_block(kk, t), kind), live, c);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t][i] = add_nonfinite(o[t][i], c[i], kind);
+          }
+          __builtin_amdgcn_sched_barrier(0);  // one block at a time: no registers for this rare path
+        }
       }
     }
   }

@@ -60,7 +60,7 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
                                                                                  float scale_log2, float* ws,
                                                                                  Piece* pieces) {
   using C = FewConfig<HDP, MT>;
-  using Copy = Copy16<E, HDP, true>;
+  using Copy = TileCopy<E, HDP, true>;
   constexpr int PER_STAGE = 4 * Copy::N, ROW = C::ROW;  // copy instructions of a stage
   constexpr int ST = HDP / 32, DT = HDP / 16;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
@@ -266,33 +266,47 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
           p[t][2 * u + 1] = Elem<E>::pack(s[u][2], s[u][3]);
         }
       }
-#pragma unroll
-      for (int c = 0; c < DT; ++c) {
+      auto v_block = [&](int c) {
         const uint32_t va = (buf + v_at) ^ (uint32_t)(32 * c);
         const u32x2 v0 = lds_read_tr(va), v1 = lds_read_tr(va + 16 * ROW);
-        u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
-        if (masked && __ballot(any_nonfinite<E>(v))) {
-          u32x4 nan, pos, neg;
-          split_nonfinite<E>(v, nan, pos, neg);
-          const float4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
+        return u32x4{v0[0], v0[1], v1[0], v1[1]};
+      };
+      bool nonfinite = false;
+      if (masked) {
+        bool any = false;
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            u32x4 live;
+        for (int c = 0; c < DT; ++c) any |= any_nonfinite<E>(v_block(c));
+        nonfinite = __ballot(any) != 0;
+      }
+      if (!nonfinite) {
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const int last = keys_at(t, w >> 1) - 2 * (w & 1);
-              live[w] = last < 0 ? 0u : last == 0 ? Elem<E>::kOnes & 0xFFFFu : Elem<E>::kOnes;
-            }
-            const float4_t cn = Elem<E>::mfma16(nan, live, z), cp = Elem<E>::mfma16(pos, live, z);
-            const float4_t cm = Elem<E>::mfma16(neg, live, z);
+        for (int c = 0; c < DT; ++c) {
+          const u32x4 v = v_block(c);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[t][c][e] = with_nonfinite(o[t][c][e], cn[e], cp[e], cm[e]);
-          }
+          for (int t = 0; t < MT; ++t)
+            if (MT == 1 || 16 * t < live_rows) o[t][c] = Elem<E>::mfma16(v, p[t], o[t][c]);
         }
+      } else {
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           if (MT > 1 && 16 * t >= live_rows) continue;
-          o[t][c] = Elem<E>::mfma16(v, p[t], o[t][c]);
+          u32x4 live;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int last = keys_at(t, w >> 1) - 2 * (w & 1);
+            live[w] = last < 0 ? 0u : last == 0 ? Elem<E>::kOnes & 0xFFFFu : Elem<E>::kOnes;
+          }
+#pragma unroll
+          for (int c = 0; c < DT; ++c) {
+            o[t][c] = Elem<E>::mfma16(finite_only<E>(v_block(c)), p[t], o[t][c]);
+#pragma unroll 1
+            for (int kind = 0; kind < 3; ++kind) {
+              const float4_t n =
+                  Elem<E>::mfma16(nonfinite_ones<E>(v_block(c), kind), live, float4_t{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[t][c][e] = add_nonfinite(o[t][c][e], n[e], kind);
+            }
+          }
         }
       }
     }
