@@ -27,7 +27,7 @@ template <class E>
 struct Elem;
 template <>
 struct Elem<half_t> {
-  static constexpr uint32_t kExp = 0x7C007C00u, kExpLow = 0x04000400u, kOnes = 0x3C003C00u;
+  static constexpr uint32_t kExp = 0x7C007C00u, kExpLow = 0x04000400u;
   static __device__ __forceinline__ float16_t mfma32(u32x4 a, u32x4 b, float16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<half8_t>(a), bit_cast<half8_t>(b), c, 0, 0, 0);
   }
@@ -43,7 +43,7 @@ struct Elem<half_t> {
 };
 template <>
 struct Elem<bhalf_t> {
-  static constexpr uint32_t kExp = 0x7F807F80u, kExpLow = 0x00800080u, kOnes = 0x3F803F80u;
+  static constexpr uint32_t kExp = 0x7F807F80u, kExpLow = 0x00800080u;
   static __device__ __forceinline__ float16_t mfma32(u32x4 a, u32x4 b, float16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bit_cast<bhalf8_t>(a), bit_cast<bhalf8_t>(b), c, 0, 0, 0);
   }
@@ -74,6 +74,21 @@ __device__ __forceinline__ void dma_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+}
+
+// The same for LDS alone: copies go on.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The loads into v end here.  Without it the compiler waits for them where v is used, in the loop, by waiting for all
+// vector memory operations: the copies of the next tile, of which it does not know, among them.
+template <int N>
+__device__ __forceinline__ void arrived(u32x4 (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
 }
 
 // The 16-byte pieces of a row of a tile are stored at piece ^ swizzle(row), so that the 16 (K) or 4 (V) rows which
@@ -138,8 +153,10 @@ struct TileCopy {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const bool row_ok = RPI * j + lane_here / CPR < rows;
-      const char* const sk = reinterpret_cast<const char*>(kb) + vo_k[j];
-      const char* const sv = reinterpret_cast<const char*>(vb) + vo_v[j];
+      uint32_t ok = vo_k[j], ov = vo_v[j];
+      asm volatile("" : "+v"(ok), "+v"(ov));  // nor are offsets as 64 bits
+      const char* const sk = reinterpret_cast<const char*>(kb) + ok;
+      const char* const sv = reinterpret_cast<const char*>(vb) + ov;
       lds_dma16(dst_k + 1024 * j, row_ok && piece_k(j, lane_here) < there ? sk : (const char*)g_attn_zeros);
       lds_dma16(dst_v + 1024 * j, row_ok && piece_v(j, lane_here) < there ? sv : (const char*)g_attn_zeros);
     }
@@ -153,6 +170,11 @@ __device__ __forceinline__ u32x2 lds_read_tr(uint32_t lds) {
 }
 __device__ __forceinline__ u32x4 lds_read16(uint32_t lds) {
   typedef const __attribute__((address_space(3))) u32x4* ptr_t;
+  return *(ptr_t)(uintptr_t)lds;
+}
+
+__device__ __forceinline__ u32x2 lds_read8(uint32_t lds) {
+  typedef const __attribute__((address_space(3))) u32x2* ptr_t;
   return *(ptr_t)(uintptr_t)lds;
 }
 
@@ -174,10 +196,9 @@ __device__ __forceinline__ bool any_nonfinite(u32x4 v) {
   return (t & 0x80008000u) != 0;
 }
 
-// A piece of V next to masked keys.  A masked key may hold infinities or NaN, which a probability of zero does not
-// cancel.  So where a tile has both, they are taken out of the product (finite_only), and three more products with ones for
-// the probabilities of the keys that a row attends to and ones where V has NaN, +inf or -inf (kind 0, 1, 2) count how
-// many of each a row meets.
+// V next to masked keys.  A masked key may hold infinities or NaN, which a probability of zero does not cancel.  So
+// where a tile has both, the values that are not finite become zeros in LDS before its product, and are added to the
+// outputs of the rows that attend to their keys one key after the other.
 template <class E>
 __device__ __forceinline__ u32x4 finite_only(u32x4 v) {
 #pragma unroll
@@ -188,25 +209,30 @@ __device__ __forceinline__ u32x4 finite_only(u32x4 v) {
   }
   return v;
 }
+// ... of `kib` KiB of a tile from lds on, read and written by one wavefront.
 template <class E>
-__device__ __forceinline__ u32x4 nonfinite_ones(u32x4 v, int kind) {
-  constexpr uint32_t inf = Elem<E>::kExp & 0xFFFFu, one = Elem<E>::kOnes & 0xFFFFu;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const uint32_t x = (v[i] >> (16 * e)) & 0xFFFFu;
-      const bool hit = kind == 0 ? (x & 0x7FFFu) > inf : x == (kind == 1 ? inf : inf | 0x8000u);
-      w |= hit ? one << (16 * e) : 0u;
-    }
-    v[i] = w;
-  }
-  return v;
+__device__ __forceinline__ bool lds_any_nonfinite(uint32_t lds, int kib, int lane) {
+  bool any = false;
+  for (int i = 0; i < kib; ++i) any |= any_nonfinite<E>(lds_read16(lds + 1024 * i + 16 * lane));
+  return __ballot(any) != 0;
 }
-__device__ __forceinline__ float add_nonfinite(float o, float count, int kind) {
-  const float x = kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
-  return count > 0.0f ? o + x : o;
+template <class E>
+__device__ __forceinline__ void lds_finite_only(uint32_t lds, int kib, int lane) {
+  typedef __attribute__((address_space(3))) u32x4* ptr_t;
+#pragma unroll 1
+  for (int i = 0; i < kib; ++i) {
+    const uint32_t at = lds + 1024 * i + 16 * lane;
+    *(ptr_t)(uintptr_t)at = finite_only<E>(lds_read16(at));
+  }
+}
+// Four values of a row of V with zeros for the finite ones.
+template <class E>
+__device__ __forceinline__ float4_t nonfinite_of(u32x2 v) {
+  const float4_t x = {Elem<E>::lo(v[0]), Elem<E>::hi(v[0]), Elem<E>::lo(v[1]), Elem<E>::hi(v[1])};
+  float4_t y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = fabsf(x[e]) < __builtin_inff() ? 0.0f : x[e];
+  return y;
 }
 
 // Lengths, offsets and pages do not change while a kernel runs: scalar loads where the index is uniform.

@@ -19,7 +19,7 @@ constexpr int kFlashRows = 32 * kFlashWaves;
 
 // Wavefronts per SIMD that the registers have to allow: one computes scores while another works on its
 // softmax.  From two on the products also accumulate in ordinary registers, without moves.
-constexpr int flash_waves_per_simd(int hdp) { return hdp == 64 ? 3 : hdp == 128 ? 2 : 1; }
+constexpr int flash_waves_per_simd(int hdp) { return hdp == 64 ? 4 : hdp == 128 ? 2 : 1; }
 
 template <class E, int HDP, bool PAGED>
 __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flash_attention_kernel(AttnArgs a, int rep, int min_rows,
@@ -33,6 +33,7 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
   // Queries of more than 128 dims leave no registers for themselves beside the outputs: each lane's stay in LDS.
   constexpr bool Q_LDS = HDP == 256;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE + (Q_LDS ? kFlashRows * ROW : 0)];
+  __shared__ int found[2][kFlashWaves];  // infinities or NaN in a masked tile
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -67,6 +68,7 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
   const int limit = shift + tok;  // may be negative: no keys
   const int wave_row = row0 + 32 * wave;
   const int wave_lo = shift + min(wave_row, rows - 1) / rep, wave_hi = shift + min(wave_row + 31, rows - 1) / rep;
+  const int first_limit = shift + row0 / rep;  // the workgroup's first row's
   const int kend = shift + min(row0 + kFlashRows - 1, rows - 1) / rep + 1;
   const int tiles = kend <= 0 ? 0 : (kend + KEYS - 1) / KEYS;
 
@@ -80,6 +82,7 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
       if constexpr (Q_LDS) q_lds[64 * s] = x;
       else qf[s] = x;
     }
+    arrived(qf);
   }
 
   // Copies.  A wavefront fetches rows 16 wave .. + 15 of both tiles: one page, as pages hold 16 keys at least.
@@ -121,6 +124,7 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
                         16u * (uint32_t)((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swizzle_v<HDP>(vrow)) +
                         8u * (uint32_t)(lane & 1) + TILE;
 
+  int patch_from = 0x7fffffff;  // first key of a tile with masks whose infinities and NaN were taken out
   int page = 0;
   if (tiles > 0) {
     if constexpr (PAGED) page = page_of(MINE * wave);
@@ -135,6 +139,28 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
       if constexpr (PAGED) page = page_of((kt + 2) * KEYS + MINE * wave);
     }
     const int key0 = kt * KEYS;
+
+    // Masks: keys past a row's own, pages that are not there.
+    uint32_t bad = 0;  // bit i: keys key0 + 16 i .. + 15 are not there
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int i = 0; i < KK; ++i) bad |= page_of(key0 + 16 * i) < 0 ? 1u << i : 0u;
+    }
+    const uint32_t my_v = lds + buf + TILE + (uint32_t)(MINE * wave) * ROW;  // the rows of V that this wavefront looks after
+    bool nonfinite = false;
+    if (__builtin_expect(key0 + KEYS - 1 > first_limit || bad != 0, 0)) {  // the same in all wavefronts
+      const bool any = lds_any_nonfinite<E>(my_v, MINE * ROW / 1024, lane);
+      if (lane == 0) found[kt & 1][wave] = any;
+      lds_barrier();
+#pragma unroll
+      for (int w = 0; w < kFlashWaves; ++w) nonfinite |= found[kt & 1][w] != 0;
+      nonfinite = __builtin_amdgcn_readfirstlane(nonfinite);
+    }
+    if (__builtin_expect(nonfinite, 0)) {
+      lds_finite_only<E>(my_v, MINE * ROW / 1024, lane);
+      lds_barrier();
+      patch_from = min(patch_from, key0);
+    }
     if (key0 > wave_hi) continue;  // only other wavefronts have keys here
 
     float16_t s[KU];
@@ -149,12 +175,6 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
       for (int u = 0; u < KU; ++u)
         s[u] = Elem<E>::mfma32(lds_read16((kb ^ (uint32_t)(32 * st)) + u * 32 * ROW), Q_LDS ? q_lds[64 * st] : qf[Q_LDS ? 0 : st], s[u]);
 
-    // Masks: keys past a row's own, pages that are not there.
-    uint32_t bad = 0;  // bit i: keys key0 + 16 i .. + 15 are not there
-    if constexpr (PAGED) {
-#pragma unroll
-      for (int i = 0; i < KK; ++i) bad |= page_of(key0 + 16 * i) < 0 ? 1u << i : 0u;
-    }
     const bool masked = key0 + KEYS - 1 > wave_lo || bad != 0;
     // The last of this lane's keys key0 + 8 q + 4 half + (0 .. 3) that its row attends to, as 0 .. 3 (below: none).
     auto keys_at = [&](int q) { return (bad >> (q >> 1)) & 1 ? -1 : limit - (key0 + 8 * q + 4 * half); };
@@ -164,8 +184,7 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
       const u32x2 v0 = lds_read_tr(at), v1 = lds_read_tr(at + 8 * ROW);
       return u32x4{v0[0], v0[1], v1[0], v1[1]};
     };
-    bool nonfinite = false;
-    if (masked) {
+    if (__builtin_expect(masked, 0)) {
 #pragma unroll
       for (int q = 0; q < 2 * KK; ++q) {
         const int last = keys_at(q);
@@ -173,22 +192,13 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
         for (int e = 0; e < 4; ++e)
           if (e > last) s[q >> 2][4 * (q & 3) + e] = -__builtin_inff();
       }
-      bool any = false;
-#pragma unroll 1
-      for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-          any |= any_nonfinite<E>(v_block(kk, t));
-          if constexpr (HDP == 256) __builtin_amdgcn_sched_barrier(0);
-        }
-      nonfinite = __ballot(any) != 0;
     }
 
     float mx = s[0][0];
 #pragma unroll
     for (int i = 1; i < 16 * KU; ++i) mx = fmaxf(mx, s[i >> 4][i & 15]);
     mx = max_halves(mx);
-    if (__ballot(mx > limit_max)) {
+    if (__builtin_expect(__ballot(mx > limit_max) != 0, 0)) {
       const float mn = fmaxf(m, mx);
       const float mcn = mn == -__builtin_inff() ? 0.0f : mn * scale_log2;
       const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mc - mcn);
@@ -212,40 +222,13 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) p[kk][i] = Elem<E>::pack(e[2 * i], e[2 * i + 1]);
-      asm volatile("" : "+v"(sum));  // the sums are taken here: the 32-bit probabilities are not kept
+      asm volatile("" : "+v"(sum), "+v"(p[kk]));  // summed and rounded here: the 32-bit probabilities are not kept
     }
 
-    if (!nonfinite) {
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
+    for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-        for (int t = 0; t < DT; ++t) o[t] = Elem<E>::mfma32(v_block(kk, t), p[kk], o[t]);
-    } else {
-#pragma unroll 1
-      for (int kk = 0; kk < KK; ++kk) {
-        const u32x4 pk = kk == 0 ? p[0] : kk == 1 ? p[1] : kk == 2 ? p[KK - 2] : p[KK - 1];
-        u32x4 live;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int last = keys_at(2 * kk + (i >> 1)) - 2 * (i & 1);
-          live[i] = last < 0 ? 0u : last == 0 ? Elem<E>::kOnes & 0xFFFFu : Elem<E>::kOnes;
-        }
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-          o[t] = Elem<E>::mfma32(finite_only<E>(v_block(kk, t)), pk, o[t]);
-#pragma unroll 1
-          for (int kind = 0; kind < 3; ++kind) {
-            float16_t c;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) c[i] = 0.0f;
-            c = Elem<E>::mfma32(nonfinite_ones<E>(v_block(kk, t), kind), live, c);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[t][i] = add_nonfinite(o[t][i], c[i], kind);
-          }
-          __builtin_amdgcn_sched_barrier(0);  // one block at a time: no registers for this rare path
-        }
-      }
-    }
+      for (int t = 0; t < DT; ++t) o[t] = Elem<E>::mfma32(v_block(kk, t), p[kk], o[t]);
   }
 
   sum = add_halves(sum);
@@ -260,6 +243,28 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
           *(u32x2*)(out + d) = u32x2{Elem<E>::pack(o[t][4 * i] * inv, o[t][4 * i + 1] * inv),
                                      Elem<E>::pack(o[t][4 * i + 2] * inv, o[t][4 * i + 3] * inv)};
       }
+  }
+
+  // What was taken out of tiles with masks belongs to the rows that do attend to it.
+  if (__builtin_expect(patch_from < kend, 0) && my_row < rows) {
+    for (int c = half; c < a.head_dim / 4; c += 2) {
+      float4_t add = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int key = patch_from; key < kend; ++key) {
+        const E* v = (const E*)a.v + kv * a.v_head + 4 * c;
+        if constexpr (PAGED) {
+          const int p = page_of(key);
+          if (p < 0) continue;
+          v += p * a.v_page + (key & ((1 << a.log2_block) - 1)) * a.v_token;
+        } else {
+          v += (int64_t)(tok0 + key) * a.v_token;
+        }
+        if (key <= limit) add += nonfinite_of<E>(*reinterpret_cast<const u32x2*>(v));
+      }
+      u32x2* const at = reinterpret_cast<u32x2*>(out + 4 * c);
+      const u32x2 x = *at;
+      *at = u32x2{Elem<E>::pack(Elem<E>::lo(x[0]) + add[0], Elem<E>::hi(x[0]) + add[1]),
+                  Elem<E>::pack(Elem<E>::lo(x[1]) + add[2], Elem<E>::hi(x[1]) + add[3])};
+    }
   }
 }
 

@@ -165,6 +165,8 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
       for (int s = 0; s < ST; ++s)
         qf[t][s] = 4 * s + g < a.head_dim / 8 ? load_global16(qp + 32 * s + 8 * g) : u32x4{0, 0, 0, 0};
     }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) arrived(qf[t]);
     const int kend = shift + min(row0 + C::ROWS - 1, rows - 1) / rep + 1;  // keys of the tile's last row
     const int first_limit = shift + row0 / rep;
 
@@ -221,6 +223,7 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
       u32x4 p[MT];
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
+        p[t] = u32x4{0, 0, 0, 0};
         if (MT > 1 && 16 * t >= live_rows) continue;
         float4_t s[2];
 #pragma unroll
@@ -242,7 +245,7 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
         float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         mx = max_groups(mx);
-        if (__ballot(mx > limit_max[t])) {
+        if (__builtin_expect(__ballot(mx > limit_max[t]) != 0, 0)) {
           const float mn = fmaxf(m[t], mx);
           const float mcn = mn == -__builtin_inff() ? 0.0f : mn * scale_log2;
           const float f = m[t] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mc[t] - mcn);
@@ -271,43 +274,29 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
         const u32x2 v0 = lds_read_tr(va), v1 = lds_read_tr(va + 16 * ROW);
         return u32x4{v0[0], v0[1], v1[0], v1[1]};
       };
-      bool nonfinite = false;
-      if (masked) {
-        bool any = false;
+      const uint32_t v_tile = buf + 32 * ROW;
+      if (__builtin_expect(masked, 0) && lds_any_nonfinite<E>(v_tile, 32 * ROW / 1024, lane)) {
 #pragma unroll
-        for (int c = 0; c < DT; ++c) any |= any_nonfinite<E>(v_block(c));
-        nonfinite = __ballot(any) != 0;
-      }
-      if (!nonfinite) {
-#pragma unroll
-        for (int c = 0; c < DT; ++c) {
-          const u32x4 v = v_block(c);
-#pragma unroll
-          for (int t = 0; t < MT; ++t)
-            if (MT == 1 || 16 * t < live_rows) o[t][c] = Elem<E>::mfma16(v, p[t], o[t][c]);
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          if (MT > 1 && 16 * t >= live_rows) continue;
-          u32x4 live;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int last = keys_at(t, w >> 1) - 2 * (w & 1);
-            live[w] = last < 0 ? 0u : last == 0 ? Elem<E>::kOnes & 0xFFFFu : Elem<E>::kOnes;
-          }
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
           for (int c = 0; c < DT; ++c) {
-            o[t][c] = Elem<E>::mfma16(finite_only<E>(v_block(c)), p[t], o[t][c]);
+            float4_t add = {0.0f, 0.0f, 0.0f, 0.0f};  // of dims 16 c + 4 g + (0 .. 3)
 #pragma unroll 1
-            for (int kind = 0; kind < 3; ++kind) {
-              const float4_t n =
-                  Elem<E>::mfma16(nonfinite_ones<E>(v_block(c), kind), live, float4_t{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[t][c][e] = add_nonfinite(o[t][c][e], n[e], kind);
-            }
+            for (int k = 0; k < 32; ++k)
+              if (key0 + k <= limit[t] && !(k >> 4 ? bad1 : bad0))
+                add += nonfinite_of<E>(lds_read8(v_tile + k * ROW + 16 * ((2 * c + (g >> 1)) ^ swizzle_v16<HDP>(k)) + 8 * (g & 1)));
+            o[t][c] += add;
+            asm volatile("" : "+v"(o[t][c]));  // here, not for all tiles at the end: this rare path takes no registers from the others
           }
-        }
+        lds_finite_only<E>(v_tile, 32 * ROW / 1024, lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+#pragma unroll
+      for (int c = 0; c < DT; ++c) {
+        const u32x4 v = v_block(c);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          if (MT == 1 || 16 * t < live_rows) o[t][c] = Elem<E>::mfma16(v, p[t], o[t][c]);
       }
     }
 
