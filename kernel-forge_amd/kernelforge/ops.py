@@ -837,6 +837,20 @@ def _check_plain(what: str, tensors) -> None:
         raise RuntimeError(f"{what} is inference only; an input requires a gradient (use torch.no_grad())")
 
 
+def _direct(index: int, tensors) -> bool:
+    """Plain tensors on the current device `index`, seen by no tracer, transform or gradient: with right types and
+    shapes their call goes straight to its launch.  One pass over the attributes, as in _eager_shape; anything else takes
+    the checks one by one, which name what is wrong (they cost 6 of a call's 17 us of host time)."""
+    if (index < 0 or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0 or _transformed()
+            or index != torch._C._cuda_getDevice()):
+        return False
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if type(t) not in _PLAIN or t.get_device() != index or (grad and t.requires_grad):
+            return False
+    return True
+
+
 def _check_memory(name: str, t: torch.Tensor, device: torch.device) -> None:
     if isinstance(t, FakeTensor) or t.is_meta:
         raise RuntimeError(f"{name} has no device memory (a fake or meta tensor)")
@@ -878,6 +892,19 @@ def _check_cache(cache_k: torch.Tensor, cache_v: torch.Tensor, dtype: torch.dtyp
                              "16-byte aligned start")
 
 
+def _caches_ok(cache_k: torch.Tensor, cache_v: torch.Tensor, dtype: torch.dtype) -> bool:
+    """_check_cache as one test, for plain tensors; dtype one of _HALF_TYPES as well."""
+    if cache_k.dim() != 4 or cache_k.dtype != dtype or cache_v.dtype != dtype or dtype not in _HALF_TYPES:
+        return False
+    shape = cache_k.shape
+    a, b, c, one = cache_k.stride()
+    e, f, g, last = cache_v.stride() if cache_v.dim() == 4 else (0, 0, 0, 0)
+    block = shape[2]
+    return (cache_v.shape == shape and one == 1 and last == 1 and not (a | b | c | e | f | g) & 7
+            and not (cache_k.data_ptr() | cache_v.data_ptr()) & 15 and 16 <= block <= 1 << 20
+            and not block & (block - 1) and cache_k.numel() > 0)
+
+
 def _rows_ok(t: torch.Tensor) -> bool:
     """Whether the kernels can read t's last dimension in 16-byte pieces."""
     *strides, last = t.stride()
@@ -917,6 +944,16 @@ def paged_tables(block_table: torch.Tensor, context_lens: torch.Tensor, new_lens
     free_pages and free_count are not changed: PagedStep.free_count is the count after the step.
     Lengths stay on the device, so a captured call follows them.  No reference counterpart.
     """
+    args = (block_table, context_lens, new_lens, free_pages, free_count, int(block_size), int(max_tokens))
+    if _direct(block_table.get_device(), args[:5]) and block_table.dim() == 2:
+        b, width = block_table.shape
+        i32 = torch.int32
+        if (context_lens.shape == (b,) and new_lens.shape == (b,) and free_count.shape == (1,) and free_pages.dim() == 1
+                and block_table.dtype == i32 and context_lens.dtype == i32 and new_lens.dtype == i32
+                and free_pages.dtype == i32 and free_count.dtype == i32 and b > 0 and width > 0 and max_tokens >= 0
+                and block_table.stride(1) == 1 and context_lens.is_contiguous() and new_lens.is_contiguous()
+                and free_pages.is_contiguous() and 16 <= block_size <= 1 << 20 and not block_size & (block_size - 1)):
+            return PagedStep(*_run_paged_tables(*args))
     b = block_table.shape[0] if block_table.dim() == 2 else -1
     _check_table(block_table, b)
     _check_int("context_lens", context_lens, torch.int32, (b,))
@@ -927,7 +964,6 @@ def paged_tables(block_table: torch.Tensor, context_lens: torch.Tensor, new_lens
     _check_block_size(block_size)
     if b < 1 or max_tokens < 0:
         raise ValueError(f"paged_tables needs at least one request and max_tokens >= 0, got {b} and {max_tokens}")
-    args = (block_table, context_lens, new_lens, free_pages, free_count, int(block_size), int(max_tokens))
     _check_plain("paged_tables", args[:5])
     return PagedStep(*(_paged_tables_op(*args) if _traced(args[:5]) else _launch_paged_tables(*args)))
 
@@ -937,6 +973,12 @@ def _launch_paged_tables(block_table, context_lens, new_lens, free_pages, free_c
     for name, t in (("block_table", block_table), ("context_lens", context_lens), ("new_lens", new_lens),
                     ("free_pages", free_pages), ("free_count", free_count)):
         _check_memory(name, t, dev)
+    with _on(dev):
+        return _run_paged_tables(block_table, context_lens, new_lens, free_pages, free_count, block_size, max_tokens)
+
+
+def _run_paged_tables(block_table, context_lens, new_lens, free_pages, free_count, block_size, max_tokens):
+    """kf_paged_tables on checked arguments of the current device."""
     lib = _lib.load()
     b, width = block_table.shape
     cu_new = block_table.new_empty(b + 1)
@@ -948,9 +990,9 @@ def _launch_paged_tables(block_table, context_lens, new_lens, free_pages, free_c
                                 _ptr(free_count), _ptr(cu_new), _ptr(seq_lens), _ptr(positions), _ptr(slots),
                                 _ptr(free_left), block_table.stride(0), b, width, block_size, free_pages.numel(),
                                 max_tokens)
-    with _on(dev):
-        status = lib.kf_paged_tables(ctypes.byref(args), _stream_ptr(dev))
-    _lib.check(status, "paged_tables")
+    status = lib.kf_paged_tables(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(block_table.get_device()))
+    if status:
+        _lib.check(status, "paged_tables")
     return cu_new, seq_lens, positions, slots, free_left
 
 
@@ -980,6 +1022,20 @@ def rope_paged_cache(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, po
     position outside [0, max_pos), which rotates with row 0.  Slots must be distinct.  The form of
     int4_qkv_rope_cache for many tokens and a paged cache; no reference counterpart.
     """
+    tensors = (qkv, cos, sin, positions, slots, cache_k, cache_v)
+    if _direct(qkv.get_device(), tensors) and qkv.dim() == 2 and cos.dim() == 2 and _caches_ok(cache_k, cache_v, qkv.dtype):
+        t, columns = qkv.shape
+        kv_heads, d = cache_k.shape[1], cache_k.shape[3]
+        row, one = qkv.stride()
+        if (heads > 0 and heads % kv_heads == 0 and columns == (heads + 2 * kv_heads) * d and d % 8 == 0
+                and d <= _ATTN_MAX_HEAD_DIM and t > 0 and one == 1 and row % 8 == 0 and cos.shape[0] > 0
+                and cos.shape == sin.shape and cos.shape[1] == d and positions.shape == (t,) and slots.shape == (t,)
+                and cos.dtype == torch.float32 and sin.dtype == torch.float32 and positions.dtype == torch.int64
+                and slots.dtype == torch.int64 and cos.is_contiguous() and sin.is_contiguous()
+                and positions.is_contiguous() and slots.is_contiguous()
+                and not (qkv.data_ptr() | cos.data_ptr() | sin.data_ptr() | positions.data_ptr() | slots.data_ptr()) & 15):
+            qk = _run_rope_paged(*tensors, int(heads))
+            return qk.split_with_sizes((heads, kv_heads), 1)
     if qkv.dim() != 2 or qkv.dtype not in _HALF_TYPES:
         raise TypeError("qkv must be a 2-D fp16 or bf16 tensor [T, (heads + 2 kv_heads) head_dim]")
     _check_cache(cache_k, cache_v, qkv.dtype)
@@ -995,7 +1051,6 @@ def rope_paged_cache(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, po
     _check_int("sin", sin, torch.float32, (cos.shape[0], d))
     _check_int("positions", positions, torch.int64, (t,))
     _check_int("slots", slots, torch.int64, (t,))
-    tensors = (qkv, cos, sin, positions, slots, cache_k, cache_v)
     _check_plain("rope_paged_cache", tensors)
     qk = (_rope_paged_op if _traced(tensors) else _launch_rope_paged)(*tensors, int(heads))
     return qk[:, :heads], qk[:, heads:]
@@ -1008,18 +1063,24 @@ def _launch_rope_paged(qkv, cos, sin, positions, slots, cache_k, cache_v, heads)
         _check_memory(name, t, dev)
     if not _rows_ok(qkv):
         qkv = qkv.clone(memory_format=torch.contiguous_format)
-    pages, kv_heads, block_size, d = cache_k.shape
-    qk = qkv.new_empty(qkv.shape[0], heads + kv_heads, d)
     if qkv.shape[0] == 0:
-        return qk
+        return qkv.new_empty(0, heads + cache_k.shape[1], cache_k.shape[3])
     cos, sin, positions, slots = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (cos, sin, positions, slots))
+    with _on(dev):
+        return _run_rope_paged(qkv, cos, sin, positions, slots, cache_k, cache_v, heads)
+
+
+def _run_rope_paged(qkv, cos, sin, positions, slots, cache_k, cache_v, heads):
+    """kf_rope_paged_cache on checked arguments of the current device."""
+    pages, kv_heads, block_size, d = cache_k.shape
+    qk = qkv.new_empty((qkv.shape[0], heads + kv_heads, d))
     args = _lib.RopePagedArgs(_ptr(qkv), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(slots), _ptr(qk), _ptr(cache_k),
                               _ptr(cache_v), qkv.stride(0), *cache_k.stride()[:3], *cache_v.stride()[:3], qkv.shape[0],
                               heads, kv_heads, d, cos.shape[0], pages, block_size, _HALF_TYPES[qkv.dtype])
-    lib = _lib.load()
-    with _on(dev):
-        status = lib.kf_rope_paged_cache(ctypes.byref(args), _stream_ptr(dev))
-    _lib.check(status, "rope_paged_cache")
+    status = _lib.load().kf_rope_paged_cache(ctypes.byref(args),
+                                             torch._C._cuda_getCurrentRawStream(qkv.get_device()))
+    if status:
+        _lib.check(status, "rope_paged_cache")
     return qk
 
 
@@ -1046,6 +1107,20 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     in a new output and left as they are in ``out``.  The form of decode_attention for prompts; no reference
     counterpart (its models run torch's attention).
     """
+    tensors = (q, k, v, cu_seqlens)
+    if _direct(q.get_device(), tensors) and out is None and q.dim() == 3 and k.dim() == 3 and v.dim() == 3:
+        t, heads, d = q.shape
+        kt, kv_heads, kd = k.shape
+        dtype = q.dtype
+        a, b, one = q.stride()
+        c, e, two = k.stride()
+        f, g, three = v.stride()
+        if (dtype in _HALF_TYPES and k.dtype == dtype and v.dtype == dtype and v.shape == k.shape and kt == t and kd == d
+                and t > 0 and kv_heads > 0 and heads > 0 and heads % kv_heads == 0 and 0 < d <= _ATTN_MAX_HEAD_DIM
+                and not d & 7 and one == 1 and two == 1 and three == 1 and not (a | b | c | e | f | g) & 7
+                and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15 and cu_seqlens.dtype == torch.int32
+                and cu_seqlens.dim() == 1 and cu_seqlens.numel() > 1 and cu_seqlens.is_contiguous()):
+            return _run_prompt(*tensors, _check_scale(scale, d), q.new_empty((t, heads, d)), True)
     if q.dim() != 3 or q.dtype not in _HALF_TYPES:
         raise TypeError("q must be a 3-D fp16 or bf16 tensor [T, heads, head_dim]")
     t, heads, d = q.shape
@@ -1059,7 +1134,6 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     _check_int("cu_seqlens", cu_seqlens, torch.int32, tuple(cu_seqlens.shape))
     scale = _check_scale(scale, d)
     _check_out(out, q)
-    tensors = (q, k, v, cu_seqlens)
     _check_plain("prompt_attention", tensors)
     if _traced(tensors):
         if out is not None:
@@ -1076,16 +1150,21 @@ def _launch_prompt(q, k, v, cu_seqlens, scale, out=None):
     zero_rest = out is None
     if out is None:
         out = q.new_empty(q.shape)
-    t, heads, d = q.shape
-    if t == 0:
+    if q.shape[0] == 0:
         return out
+    with _on(dev):
+        return _run_prompt(q, k, v, cu_seqlens, scale, out, zero_rest)
+
+
+def _run_prompt(q, k, v, cu_seqlens, scale, out, zero_rest):
+    """kf_prompt_attention on checked arguments of the current device."""
+    t, heads, d = q.shape
     args = _lib.PromptAttentionArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(cu_seqlens), *q.stride()[:2],
                                     *k.stride()[:2], *v.stride()[:2], *out.stride()[:2], t, cu_seqlens.numel() - 1, heads,
                                     k.shape[1], d, _HALF_TYPES[q.dtype], scale, zero_rest)
-    lib = _lib.load()
-    with _on(dev):
-        status = lib.kf_prompt_attention(ctypes.byref(args), _stream_ptr(dev))
-    _lib.check(status, "prompt_attention")
+    status = _lib.load().kf_prompt_attention(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(q.get_device()))
+    if status:
+        _lib.check(status, "prompt_attention")
     return out
 
 
@@ -1114,6 +1193,20 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
     new output and left as they are in ``out``.  Arithmetic as in prompt_attention; results do not change from
     run to run.  The form of decode_attention for many requests; no reference counterpart.
     """
+    tensors = (q, cache_k, cache_v, block_table, cu_new, seq_lens)
+    if (_direct(q.get_device(), tensors) and out is None and q.dim() == 3 and block_table.dim() == 2
+            and _caches_ok(cache_k, cache_v, q.dtype)):
+        t, heads, d = q.shape
+        _, kv_heads, _, kd = cache_k.shape
+        b, width = block_table.shape
+        a, c, one = q.stride()
+        i32 = torch.int32
+        if (d == kd and t > 0 and heads > 0 and heads % kv_heads == 0 and d <= _ATTN_MAX_HEAD_DIM and not d & 7 and one == 1
+                and not (a | c) & 7 and not q.data_ptr() & 15 and b > 0 and width > 0 and block_table.stride(1) == 1
+                and block_table.dtype == i32 and cu_new.dtype == i32 and seq_lens.dtype == i32 and cu_new.shape == (b + 1,)
+                and seq_lens.shape == (b,) and cu_new.is_contiguous() and seq_lens.is_contiguous()
+                and (max_new is None or max_new > 0)):
+            return _run_paged(*tensors, int(max_new or 0), _check_scale(scale, d), q.new_empty((t, heads, d)), True)
     if q.dim() != 3 or q.dtype not in _HALF_TYPES:
         raise TypeError("q must be a 3-D fp16 or bf16 tensor [T, heads, head_dim]")
     _check_cache(cache_k, cache_v, q.dtype)
@@ -1130,7 +1223,6 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
         raise ValueError(f"max_new must be positive, got {max_new}")
     scale = _check_scale(scale, q.shape[2])
     _check_out(out, q)
-    tensors = (q, cache_k, cache_v, block_table, cu_new, seq_lens)
     _check_plain("paged_attention", tensors)
     if _traced(tensors):
         if out is not None:
@@ -1149,21 +1241,28 @@ def _launch_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, s
     zero_rest = out is None
     if out is None:
         out = q.new_empty(q.shape)
-    t, heads, d = q.shape
-    if t == 0:
+    if q.shape[0] == 0:
         return out
+    with _on(dev):
+        return _run_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scale, out, zero_rest)
+
+
+def _run_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scale, out, zero_rest):
+    """kf_paged_attention on checked arguments of the current device."""
+    t, heads, d = q.shape
     pages, kv_heads, block_size, _ = cache_k.shape
     args = _lib.PagedAttentionArgs(_ptr(q), _ptr(cache_k), _ptr(cache_v), _ptr(out), _ptr(block_table), _ptr(cu_new),
                                    _ptr(seq_lens), *q.stride()[:2], *out.stride()[:2], *cache_k.stride()[:3],
                                    *cache_v.stride()[:3], block_table.stride(0), t, seq_lens.numel(), heads, kv_heads, d,
                                    _HALF_TYPES[q.dtype], block_table.shape[1], pages, block_size, max_new, scale, zero_rest)
     lib = _lib.load()
-    with _on(dev):
-        ws_bytes = lib.kf_paged_attention_workspace_bytes(ctypes.byref(args))
-        ws = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
-        status = lib.kf_paged_attention(ctypes.byref(args), _ptr(ws) if ws is not None else None, ws_bytes,
-                                        _stream_ptr(dev))
-    _lib.check(status, "paged_attention")
+    ref = ctypes.byref(args)
+    ws_bytes = lib.kf_paged_attention_workspace_bytes(ref)
+    ws = q.new_empty((ws_bytes + 1) // 2) if ws_bytes else None  # two bytes a value
+    status = lib.kf_paged_attention(ref, ws.data_ptr() if ws is not None else None, ws_bytes,
+                                    torch._C._cuda_getCurrentRawStream(q.get_device()))
+    if status:
+        _lib.check(status, "paged_attention")
     return out
 
 

@@ -131,3 +131,16 @@ def test_another_stream():
         got = ops.prompt_attention(q, k, v, cu)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+def test_many_small_probabilities(dtype):
+    """One key far above the others: their probabilities are subnormal in fp16 against it, and add up to as much
+    as it has."""
+    n = 3001
+    q, k, v, cu = make([n], 2, 1, 64, dtype)
+    q = torch.zeros_like(q)
+    q[..., 0] = 8.0
+    k = k.contiguous() * 0.01
+    k[0, 0, 0] = 8.0 * 1.29  # score 10.3: the others' probabilities are about 3.3e-5 of its
+    against64([n], q, k, v, ops.prompt_attention(q, k, v, cu))
