@@ -218,21 +218,35 @@ int check_strides(const int64_t* s, int count) {
 // Which kernels a paged_attention call launches.  few: the one that splits the keys; many: the one that splits the rows.
 struct PagedPlan {
   bool few, many;
-  int row_tiles, grid, log2_block;
+  int64_t rows;  // (token, query head of a group) rows of a request that the first one has to expect
+  kf::AttnArgs args;
 };
 int paged_plan(const kf_paged_attention_args& a, PagedPlan* p) {
   if (int st = check_attention(a.tokens, a.seqs, a.heads, a.kv_heads, a.head_dim, a.dtype, a.scale)) return st;
-  if (int st = check_block(a.block_size, &p->log2_block)) return st;
+  kf::AttnArgs& t = p->args;
+  t = {};
+  if (int st = check_block(a.block_size, &t.log2_block)) return st;
   if (a.table_width < 1 || a.num_pages < 1 || a.max_new < 0)
     return fail(KF_ERR_INVALID_ARG, "need table_width, num_pages >= 1 and max_new >= 0, got %d, %d, %d", a.table_width,
                 a.num_pages, a.max_new);
-  if ((int64_t)a.table_width << p->log2_block >= (int64_t)1 << 30)
+  if ((int64_t)a.table_width << t.log2_block >= (int64_t)1 << 30)
     return fail(KF_ERR_UNSUPPORTED, "tables of %d pages of %d tokens are too long", a.table_width, a.block_size);
   const int64_t rows = (int64_t)(a.max_new ? std::min(a.max_new, a.tokens) : a.tokens) * (a.heads / a.kv_heads);
   p->many = rows > kFewRows;
   p->few = !p->many || a.seqs > 1;
-  p->row_tiles = kf::few_rows_tiles(a.head_dim, std::min<int64_t>(rows, kFewRows));
-  p->grid = 0;
+  p->rows = std::min<int64_t>(rows, kFewRows);
+  t.q = a.q, t.k = a.cache_k, t.v = a.cache_v, t.out = a.out;
+  t.cu = static_cast<const int*>(a.cu_new);
+  t.seq_lens = static_cast<const int*>(a.seq_lens);
+  t.table = static_cast<const int*>(a.block_table);
+  t.table_stride = a.table_stride;
+  t.q_token = a.q_token, t.q_head = a.q_head, t.out_token = a.out_token, t.out_head = a.out_head;
+  t.k_page = a.k_page, t.k_head = a.k_head, t.k_token = a.k_token;
+  t.v_page = a.v_page, t.v_head = a.v_head, t.v_token = a.v_token;
+  t.tokens = a.tokens, t.seqs = a.seqs, t.heads = a.heads, t.kv_heads = a.kv_heads, t.head_dim = a.head_dim;
+  t.table_width = a.table_width, t.num_pages = a.num_pages;
+  t.zero_rest = a.zero_rest;
+  t.scale = a.scale;
   return KF_OK;
 }
 
@@ -700,8 +714,9 @@ int kf_prompt_attention(const kf_prompt_attention_args* a, void* stream) {
 
 size_t kf_paged_attention_workspace_bytes(const kf_paged_attention_args* a) {
   PagedPlan p;
-  if (!a || paged_plan(*a, &p) || (p.few && cu_count(&p.grid))) return 0;
-  return p.few ? kf::few_rows_workspace_bytes(a->head_dim, p.row_tiles, p.grid) : 0;
+  int cus;
+  if (!a || paged_plan(*a, &p) || !p.few || cu_count(&cus)) return 0;
+  return kf::few_rows_workspace_bytes(a->head_dim, kf::few_rows_plan(p.args, p.rows, cus));
 }
 
 int kf_paged_attention(const kf_paged_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -717,36 +732,26 @@ int kf_paged_attention(const kf_paged_attention_args* a, void* ws, size_t ws_byt
   if (int st = check_strides(strides, 10)) return st;
   if (a->k_token > kMaxTokenStride || a->v_token > kMaxTokenStride)
     return fail(KF_ERR_UNSUPPORTED, "token strides of the caches go up to %d elements", kMaxTokenStride);
-  kf::AttnArgs t = {};
-  t.q = a->q, t.k = a->cache_k, t.v = a->cache_v, t.out = a->out;
-  t.cu = static_cast<const int*>(a->cu_new);
-  t.seq_lens = static_cast<const int*>(a->seq_lens);
-  t.table = static_cast<const int*>(a->block_table);
-  t.table_stride = a->table_stride;
-  t.q_token = a->q_token, t.q_head = a->q_head, t.out_token = a->out_token, t.out_head = a->out_head;
-  t.k_page = a->k_page, t.k_head = a->k_head, t.k_token = a->k_token;
-  t.v_page = a->v_page, t.v_head = a->v_head, t.v_token = a->v_token;
-  t.tokens = a->tokens, t.seqs = a->seqs, t.heads = a->heads, t.kv_heads = a->kv_heads, t.head_dim = a->head_dim;
-  t.table_width = a->table_width, t.log2_block = p.log2_block, t.num_pages = a->num_pages;
-  t.zero_rest = a->zero_rest;
-  t.scale = a->scale;
   const bool bf16 = a->dtype == KF_DTYPE_BF16;
   if (p.few) {
-    if (int st = cu_count(&p.grid)) return st;
-    const size_t need = kf::few_rows_workspace_bytes(a->head_dim, p.row_tiles, p.grid);
-    if (!ws || ws_bytes < need)
-      return fail(KF_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, ws ? ws_bytes : (size_t)0);
-    if (!aligned(ws, 16)) return fail(KF_ERR_WORKSPACE, "the workspace must be 16-byte aligned");
-    if (kf::few_rows_units(t, p.row_tiles) >= (int64_t)1 << 31)
+    int cus;
+    if (int st = cu_count(&cus)) return st;
+    const kf::FewPlan plan = kf::few_rows_plan(p.args, p.rows, cus);
+    if (plan.most_units >= (int64_t)1 << 31)
       return fail(KF_ERR_UNSUPPORTED, "%d tokens over tables of %d pages are more than one launch takes", a->tokens,
                   a->table_width);
+    const size_t need = kf::few_rows_workspace_bytes(a->head_dim, plan);
+    if (need && (!ws || ws_bytes < need))
+      return fail(KF_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, ws ? ws_bytes : (size_t)0);
+    if (need && !aligned(ws, 16)) return fail(KF_ERR_WORKSPACE, "the workspace must be 16-byte aligned");
     const int max_rows = p.many ? kFewRows : 0x7fffffff;
-    if (int st = hip_status(kf::few_rows_launch(t, bf16, p.row_tiles, max_rows, p.grid, ws, static_cast<hipStream_t>(stream)),
+    if (int st = hip_status(kf::few_rows_launch(p.args, bf16, plan, max_rows, ws, static_cast<hipStream_t>(stream)),
                             "paged_attention launch"))
       return st;
   }
   if (p.many)
-    return hip_status(kf::flash_attention_launch(t, true, bf16, p.few ? kFewRows + 1 : 0, static_cast<hipStream_t>(stream)),
+    return hip_status(kf::flash_attention_launch(p.args, true, bf16, p.few ? kFewRows + 1 : 0,
+                                                 static_cast<hipStream_t>(stream)),
                       "paged_attention launch");
   return KF_OK;
 }

@@ -240,13 +240,17 @@ struct AttnArgs {
 hipError_t flash_attention_launch(const AttnArgs& a, bool paged, bool bf16, int min_rows, hipStream_t stream);
 
 // ---- attention of few rows per request over a paged cache (kf_paged_attn.hip) -----
-// row_tiles: 16-row tiles that share a pass over the keys; requests of more than max_rows rows are left to the other
-// kernel.  ws: few_rows_workspace_bytes, 16-byte aligned.
-int few_rows_tiles(int head_dim, int64_t rows);
-size_t few_rows_workspace_bytes(int head_dim, int row_tiles, int grid);
-int64_t few_rows_units(const AttnArgs& a, int row_tiles);  // an upper bound of the kernel's work units
-hipError_t few_rows_launch(const AttnArgs& a, bool bf16, int row_tiles, int max_rows, int grid, void* ws,
-                           hipStream_t stream);
+struct FewPlan {
+  int row_tiles;       // 16-row tiles that share a pass over the keys
+  bool cut;            // items may be cut, and a second launch joins them
+  int grid;
+  int64_t most_units;  // an upper bound of the kernel's work units: below 2^31
+};
+// rows: (token, query head of a group) rows of a request, at most.
+FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int cu_count);
+size_t few_rows_workspace_bytes(int head_dim, const FewPlan& p);
+// Requests of more than max_rows rows are left to the other kernel.  ws: few_rows_workspace_bytes, 16-byte aligned.
+hipError_t few_rows_launch(const AttnArgs& a, bool bf16, const FewPlan& p, int max_rows, void* ws, hipStream_t stream);
 
 // ---- the paged cache's tables and writer (kf_paged.hip) -----------------------
 struct TablesArgs {

@@ -2,13 +2,15 @@
 //
 //   out[t, h] = sum_s softmax_s(scale q[t, h] . k[s, kv]) v[s, kv],   s <= position of t,   kv = h / rep
 //
-// What bounds it: the bytes of K and V, read once.  So the work of all requests is laid end to end, in units of 128
-// keys of one (request, row tile, KV head), and cut into one equal stretch per workgroup whatever the lengths
-// are; a workgroup finds its stretch from the lengths by itself (they are read on the device only, so a captured launch
+// What bounds it: the bytes of K and V, read once.  So the work of all requests is laid end to end, in units of 64
+// keys (32 for heads of more than 128) of one item (request, row tile, KV head), and cut into one equal stretch per workgroup
+// whatever the lengths are; a workgroup finds its stretch from the lengths by itself (they are read on the device only, so a captured launch
 // follows them).  The wavefronts of a workgroup take 32 keys each and do not wait for each other: each keeps its keys' tiles of K
 // and V coming through LDS buffers of its own by asynchronous copies, and they meet at the end of an item.
 // An item inside one stretch is finished there; the pieces of one that is cut go to the workspace (maximum, sum,
 // unscaled outputs, 32 bits) and a second launch joins them, in the order of the keys: results do not depend on timing.
+#include <algorithm>
+
 #include "kf_attn_tiles.h"
 #include "kf_launch.h"
 
@@ -17,7 +19,7 @@ namespace {
 
 template <int HDP, int MT>
 struct FewConfig {
-  static constexpr int WAVES = HDP == 256 ? 2 : 4;
+  static constexpr int WAVES = HDP == 256 ? 1 : 2;
   static constexpr int THREADS = 64 * WAVES;
   static constexpr int STAGES = HDP == 64 ? 4 : 2;
   static constexpr int ROW = HDP * 2;
@@ -25,7 +27,10 @@ struct FewConfig {
   static constexpr int RING = STAGES * STAGE;        // of one wavefront
   static constexpr int ROWS = 16 * MT;
   static constexpr int UNIT = 32 * WAVES;            // keys
-  static constexpr int LDS = WAVES * RING;           // 128 KiB
+  // Beginning and ending an item takes about as long as these many units: they count for it when the work is cut,
+  // or workgroups with many short items would be the last ones.
+  static constexpr int ITEM = 2;
+  static constexpr int LDS = WAVES * RING;           // 64 KiB: two workgroups per CU
   static_assert(WAVES * ROWS * HDP * 4 <= LDS, "the wavefronts' sums meet in the buffers");
 };
 
@@ -37,13 +42,28 @@ struct Piece {
 __device__ __forceinline__ int few_seq_len(const AttnArgs& a, int s) {
   return min(max(load_const(a.seq_lens, s), 0), a.table_width << a.log2_block);
 }
-// Units of a request: (row tiles) x (KV heads) x (units of keys), one at least where it has rows, so that they are written.
+// A request's items, (row tiles) x (KV heads), each of *key_units units of keys (one at least, so that every row is
+// written); what one item counts is item_cost: its units and ITEM, or 1 where items are not cut.
 template <class C>
-__device__ __forceinline__ int few_units(const AttnArgs& a, int s, int rep, int max_rows, int* key_units) {
+__device__ __forceinline__ int few_items(const AttnArgs& a, int s, int rep, int max_rows, int* key_units) {
   const int rows = max(seq_offset(a.cu, s + 1, a.seqs, a.tokens) - seq_offset(a.cu, s, a.seqs, a.tokens), 0) * rep;
-  const int ku = max((few_seq_len(a, s) + C::UNIT - 1) / C::UNIT, 1);
-  *key_units = ku;
-  return rows > max_rows ? 0 : (rows + C::ROWS - 1) / C::ROWS * a.kv_heads * ku;
+  *key_units = max((few_seq_len(a, s) + C::UNIT - 1) / C::UNIT, 1);
+  return rows > max_rows ? 0 : (rows + C::ROWS - 1) / C::ROWS * a.kv_heads;
+}
+template <class C, bool CUT>
+__device__ __forceinline__ int item_cost(int key_units) {
+  return CUT ? key_units + C::ITEM : 1;
+}
+
+// Inclusive prefix sums over a wavefront.
+__device__ __forceinline__ int wave_prefix(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
 }
 
 __device__ __forceinline__ float max_groups(float v) {  // of lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -55,7 +75,8 @@ __device__ __forceinline__ float add_groups(float v) {
   return add_halves(bit_cast<float>((uint32_t)s[0]) + bit_cast<float>((uint32_t)s[1]));
 }
 
-template <class E, int HDP, int MT>
+// CUT: items may be cut; otherwise every workgroup takes whole ones, and nothing is left to join.
+template <class E, int HDP, int MT, bool CUT>
 __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel(AttnArgs args, int rep, int max_rows,
                                                                                  float scale_log2, float* ws,
                                                                                  Piece* pieces) {
@@ -65,8 +86,7 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
   constexpr int ST = HDP / 32, DT = HDP / 16;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
   __shared__ float stat[2][C::WAVES][C::ROWS];
-  __shared__ int64_t scan[C::WAVES];
-  __shared__ int found[2];
+  __shared__ int scan[C::WAVES], found[2];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -76,35 +96,34 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
   const AttnArgs& a = args;
   // This workgroup's stretch.  Every thread sums a run of requests; the one whose run holds the stretch's
   // first unit says which request that is.
+  // Sums that pass 31 bits (offsets that do not ascend; the launch checks the others) end in no work or in work of
+  // some request, never outside.
   const int run = (a.seqs + C::THREADS - 1) / C::THREADS;
   const int s0 = min(tid * run, a.seqs), s1 = min(s0 + run, a.seqs);
-  int ku;
-  int64_t mine = 0;
-  for (int s = s0; s < s1; ++s) mine += few_units<C>(a, s, rep, max_rows, &ku);
-  int64_t upto = mine;  // inclusive prefix in the wavefront
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t v = __shfl_up(upto, off);
-    if (lane >= off) upto += v;
+  int ku, mine = 0;
+  for (int s = s0; s < s1; ++s) {
+    const int n = few_items<C>(a, s, rep, max_rows, &ku);
+    mine += n * item_cost<C, CUT>(ku);
   }
+  const int upto = wave_prefix(mine);
   if (lane == 63) scan[wave] = upto;
+  if (tid == 0) found[0] = -1;
   __syncthreads();
-  int64_t sum_all = 0, before = upto - mine;
+  int total = 0, before = upto - mine;
 #pragma unroll
   for (int w = 0; w < C::WAVES; ++w) {
     if (w < wave) before += scan[w];
-    sum_all += scan[w];
+    total += scan[w];
   }
-  // The launch checks that ascending offsets stay below 2^31 units; with others there is no work.
-  const int total = __builtin_amdgcn_readfirstlane(sum_all < 0x7fffffff ? (int)sum_all : 0);
+  total = max(__builtin_amdgcn_readfirstlane(total), 0);
   per = total / (int)gridDim.x + (total % (int)gridDim.x ? 1 : 0);
   // 64 bits: workgroups past the end begin past it.
   begin = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
   end = begin + min(per, total - begin);
   if (begin >= before && begin < before + mine) {
-    int at = (int)before;
+    int at = before;
     for (int s = s0; s < s1; ++s) {
-      const int n = few_units<C>(a, s, rep, max_rows, &ku);
+      const int n = few_items<C>(a, s, rep, max_rows, &ku) * item_cost<C, CUT>(ku);
       if (begin < at + n) {
         found[0] = s;
         found[1] = at;
@@ -113,7 +132,7 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
       at += n;
     }
   }
-  if (tid == 0) pieces[blockIdx.x].seq = -1;
+  if (CUT && tid == 0) pieces[blockIdx.x].seq = -1;
   __syncthreads();
 
   // Rows in no sequence.
@@ -127,7 +146,7 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
       *(u32x4*)((E*)a.out + (t0 + t) * a.out_token + h * a.out_head + 8 * (r - h * cpr)) = u32x4{0, 0, 0, 0};
     }
   }
-  if (begin >= end) return;
+  if (begin >= end || found[0] < 0) return;
   }
 
   int seq = __builtin_amdgcn_readfirstlane(found[0]);
@@ -142,12 +161,16 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
     const AttnArgs a = reload_args();
     const Copy copy(a.k_token, a.v_token, a.head_dim, lane);
     int n, ku;
-    while ((n = few_units<C>(a, seq, rep, max_rows, &ku)) <= at - seq_at) {  // next request with units
+    while ((n = few_items<C>(a, seq, rep, max_rows, &ku) * item_cost<C, CUT>(ku)) <= at - seq_at) {  // next request with items
       seq_at += n;
-      ++seq;
+      if (++seq >= a.seqs) return;
     }
-    const int item = (at - seq_at) / ku, item_at = seq_at + item * ku;
-    const int u0 = at - item_at, u1 = min(ku, end - item_at);
+    const int cost = item_cost<C, CUT>(ku), item = (at - seq_at) / cost, item_at = seq_at + item * cost;
+    // The stretch's part of the item; of what it counts, the beginning comes first.
+    const int first_unit = item_at + (CUT ? C::ITEM : 0);
+    const int u0 = CUT ? max(at - first_unit, 0) : 0, u1 = CUT ? min(ku, end - first_unit) : ku;
+    at = item_at + cost;
+    if (u1 <= u0) break;  // not even its first unit
     const int kv = item % a.kv_heads, row0 = item / a.kv_heads * C::ROWS;
     const int tok0 = seq_offset(a.cu, seq, a.seqs, a.tokens);
     const int len = seq_offset(a.cu, seq + 1, a.seqs, a.tokens) - tok0, rows = len * rep;
@@ -311,12 +334,14 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
         stat[0][wave][16 * t + l16] = m[t] == -__builtin_inff() ? m[t] : mc[t];
         stat[1][wave][16 * t + l16] = total_sum;
       }
+      if (16 * t + l16 < live_rows) {
 #pragma unroll
-      for (int c = 0; c < DT; ++c)
-        *reinterpret_cast<float4_t*>(acc + (wave * C::ROWS + 16 * t + l16) * HDP + 16 * c + 4 * g) = o[t][c];
+        for (int c = 0; c < DT; ++c)
+          *reinterpret_cast<float4_t*>(acc + (wave * C::ROWS + 16 * t + l16) * HDP + 16 * c + 4 * g) = o[t][c];
+      }
     }
     __syncthreads();
-    const bool whole = u0 == 0 && u1 == ku;
+    const bool whole = !CUT || (u0 == 0 && u1 == ku);
     const int part = 2 * (int)blockIdx.x + (u0 == 0 ? 1 : 0);
     float* const part_o = ws + (size_t)part * C::ROWS * (HDP + 2);
     float* const part_s = part_o + C::ROWS * HDP;
@@ -352,9 +377,8 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
       }
     }
     if (tid == 0 && u0 == 0 && !whole)
-      pieces[blockIdx.x] = Piece{seq, row0, kv, (item_at + ku - 1) / per};
+      pieces[blockIdx.x] = Piece{seq, row0, kv, (item_at + cost - 1) / per};
     __syncthreads();  // the sums have been read: the buffers are free
-    at = item_at + u1;
   }
 }
 
@@ -371,19 +395,20 @@ __global__ __launch_bounds__(256) void join_pieces_kernel(AttnArgs a, int rep, c
   const int first = blockIdx.x;
   for (int i = blockIdx.y * 256 + threadIdx.x; i < live_rows * (HDP / 4); i += 256 * gridDim.y) {
     const int r = i / (HDP / 4), d = 4 * (i % (HDP / 4));
+    auto part = [&](int w) { return ws + (size_t)(2 * w + (w == first ? 1 : 0)) * STRIDE; };
+    float top = -__builtin_inff(), l = 0.0f;
+#pragma unroll 4
+    for (int w = first; w <= pc.last; ++w) top = fmaxf(top, part(w)[C::ROWS * HDP + r]);
     float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f, top = -__builtin_inff();
+#pragma unroll 4
     for (int w = first; w <= pc.last; ++w) {
-      const float* const p = ws + (size_t)(2 * w + (w == first ? 1 : 0)) * STRIDE;
+      const float* const p = part(w);
       const float mw = p[C::ROWS * HDP + r], lw = p[C::ROWS * HDP + C::ROWS + r];
       const float4_t x = *reinterpret_cast<const float4_t*>(p + r * HDP + d);
-      const float mn = fmaxf(top, mw);
-      const float f0 = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top - mn);
-      const float f1 = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - mn);
-      l = (l != l ? l : f0 * l) + (lw != lw ? lw : f1 * lw);
+      const float f = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
+      l += lw != lw ? lw : f * lw;  // a NaN among a piece's scores is in its sum, whatever its maximum says
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (f0 == 0.0f ? 0.0f : f0 * v[e]) + (f1 == 0.0f ? 0.0f : f1 * x[e]);
-      top = mn;
+      for (int e = 0; e < 4; ++e) v[e] += f == 0.0f ? 0.0f : f * x[e];
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int row = pc.row0 + r, tok = row / rep, head = pc.kv * rep + (row - tok * rep);
@@ -394,13 +419,17 @@ __global__ __launch_bounds__(256) void join_pieces_kernel(AttnArgs a, int rep, c
 }
 
 template <class E, int HDP, int MT>
-hipError_t launch(const AttnArgs& a, int max_rows, int grid, void* ws, hipStream_t stream) {
+hipError_t launch(const AttnArgs& a, int max_rows, bool cut, int grid, void* ws, hipStream_t stream) {
   using C = FewConfig<HDP, MT>;
   const int rep = a.heads / a.kv_heads;
+  const float scale_log2 = a.scale * 1.44269504088896340736f;
+  if (!cut) {
+    few_rows_kernel<E, HDP, MT, false><<<grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, nullptr, nullptr);
+    return hipGetLastError();
+  }
   float* const parts = static_cast<float*>(ws);
   Piece* const pieces = reinterpret_cast<Piece*>(parts + (size_t)2 * grid * C::ROWS * (HDP + 2));
-  few_rows_kernel<E, HDP, MT><<<grid, C::THREADS, 0, stream>>>(a, rep, max_rows, a.scale * 1.44269504088896340736f,
-                                                              parts, pieces);
+  few_rows_kernel<E, HDP, MT, true><<<grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, parts, pieces);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   join_pieces_kernel<E, HDP, MT><<<dim3(grid, MT), 256, 0, stream>>>(a, rep, parts, pieces);
@@ -408,39 +437,44 @@ hipError_t launch(const AttnArgs& a, int max_rows, int grid, void* ws, hipStream
 }
 
 template <class E, int HDP>
-hipError_t launch_rows(const AttnArgs& a, int row_tiles, int max_rows, int grid, void* ws, hipStream_t stream) {
+hipError_t launch_rows(const AttnArgs& a, int row_tiles, int max_rows, bool cut, int grid, void* ws, hipStream_t stream) {
   if constexpr (HDP != 256) {  // one row tile of 256 dims fills the registers
-    if (row_tiles == 2) return launch<E, HDP, 2>(a, max_rows, grid, ws, stream);
+    if (row_tiles == 2) return launch<E, HDP, 2>(a, max_rows, cut, grid, ws, stream);
   }
-  return launch<E, HDP, 1>(a, max_rows, grid, ws, stream);
+  return launch<E, HDP, 1>(a, max_rows, cut, grid, ws, stream);
 }
 
 template <class E>
-hipError_t launch_dim(const AttnArgs& a, int row_tiles, int max_rows, int grid, void* ws, hipStream_t stream) {
-  if (a.head_dim <= 64) return launch_rows<E, 64>(a, row_tiles, max_rows, grid, ws, stream);
-  if (a.head_dim <= 128) return launch_rows<E, 128>(a, row_tiles, max_rows, grid, ws, stream);
-  return launch_rows<E, 256>(a, row_tiles, max_rows, grid, ws, stream);
+hipError_t launch_dim(const AttnArgs& a, int row_tiles, int max_rows, bool cut, int grid, void* ws, hipStream_t stream) {
+  if (a.head_dim <= 64) return launch_rows<E, 64>(a, row_tiles, max_rows, cut, grid, ws, stream);
+  if (a.head_dim <= 128) return launch_rows<E, 128>(a, row_tiles, max_rows, cut, grid, ws, stream);
+  return launch_rows<E, 256>(a, row_tiles, max_rows, cut, grid, ws, stream);
 }
 
 }  // namespace
 
-int few_rows_tiles(int head_dim, int64_t rows) { return head_dim <= 128 && rows > 16 ? 2 : 1; }
-
-size_t few_rows_workspace_bytes(int head_dim, int row_tiles, int grid) {
-  const int padded = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
-  return (size_t)grid * (2 * sizeof(float) * 16 * row_tiles * (padded + 2) + sizeof(Piece));
-}
-
-int64_t few_rows_units(const AttnArgs& a, int row_tiles) {
-  const int64_t keys = (int64_t)a.table_width << a.log2_block;
+FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int cu_count) {
+  FewPlan p;
+  p.row_tiles = a.head_dim <= 128 && rows > 16 ? 2 : 1;
   const int unit = a.head_dim <= 128 ? FewConfig<128, 1>::UNIT : FewConfig<256, 1>::UNIT;
-  return ((int64_t)a.tokens * (a.heads / a.kv_heads) / (16 * row_tiles) + a.seqs) * a.kv_heads * (keys / unit + 1);
+  const int64_t key_units = (((int64_t)a.table_width << a.log2_block) + unit - 1) / unit;
+  const int64_t items = ((int64_t)a.tokens * (a.heads / a.kv_heads) / (16 * p.row_tiles) + a.seqs) * a.kv_heads;
+  // Tables of up to 512 keys are worked off faster than a second launch begins.
+  p.cut = key_units * unit > 512;
+  p.most_units = items * (key_units + FewConfig<128, 1>::ITEM);
+  p.grid = (int)std::min<int64_t>(2 * cu_count, p.cut ? p.most_units : items);
+  return p;
 }
 
-hipError_t few_rows_launch(const AttnArgs& a, bool bf16, int row_tiles, int max_rows, int grid, void* ws,
-                           hipStream_t stream) {
-  return bf16 ? launch_dim<bhalf_t>(a, row_tiles, max_rows, grid, ws, stream)
-              : launch_dim<half_t>(a, row_tiles, max_rows, grid, ws, stream);
+size_t few_rows_workspace_bytes(int head_dim, const FewPlan& p) {
+  if (!p.cut) return 0;
+  const int padded = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+  return (size_t)p.grid * (2 * sizeof(float) * 16 * p.row_tiles * (padded + 2) + sizeof(Piece));
+}
+
+hipError_t few_rows_launch(const AttnArgs& a, bool bf16, const FewPlan& p, int max_rows, void* ws, hipStream_t stream) {
+  return bf16 ? launch_dim<bhalf_t>(a, p.row_tiles, max_rows, p.cut, p.grid, ws, stream)
+              : launch_dim<half_t>(a, p.row_tiles, max_rows, p.cut, p.grid, ws, stream);
 }
 
 }  // namespace kf
