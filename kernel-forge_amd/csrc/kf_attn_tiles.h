@@ -65,8 +65,11 @@ static __device__ __attribute__((aligned(16))) uint32_t g_attn_zeros[4] = {0, 0,
 __device__ __forceinline__ void lds_dma16(uint32_t lds, const void* src) {
   asm volatile("global_load_lds_dwordx4 %1, off" ::"{m0}"(lds), "v"(src) : "memory");
 }
+// ONCE: no other workgroup reads these bytes.
+template <bool ONCE>
 __device__ __forceinline__ void lds_dma16(uint32_t lds, const void* base, uint32_t offset) {
-  asm volatile("global_load_lds_dwordx4 %1, %2" ::"{m0}"(lds), "v"(offset), "s"(base) : "memory");
+  if constexpr (ONCE) asm volatile("global_load_lds_dwordx4 %1, %2 nt" ::"{m0}"(lds), "v"(offset), "s"(base) : "memory");
+  else asm volatile("global_load_lds_dwordx4 %1, %2" ::"{m0}"(lds), "v"(offset), "s"(base) : "memory");
 }
 // All of this wavefront's copies have landed and its reads are done, and every wavefront of the workgroup has come
 // here.
@@ -110,7 +113,8 @@ __device__ __forceinline__ constexpr int swizzle_v16(int key) {
 
 // Copies ROWS keys of K and of V into tiles, swizzled.  The source offsets of a lane do not change, so a copy of keys
 // that are all there is one instruction per KiB.
-template <class E, int HDP, bool V16, int ROWS = 16>
+// FEW: for the kernel of few rows, whose products are 16 x 16 and whose keys no other workgroup reads.
+template <class E, int HDP, bool FEW, int ROWS = 16>
 struct TileCopy {
   static constexpr int CPR = HDP / 8;    // 16-byte pieces per row
   static constexpr int RPI = 64 / CPR;   // rows per copy instruction
@@ -124,7 +128,7 @@ struct TileCopy {
   }
   __device__ __forceinline__ int piece_v(int j, int lane) const {
     const int r = row0 + RPI * j + lane / CPR;
-    return (lane % CPR) ^ (V16 ? swizzle_v16<HDP>(r) : swizzle_v<HDP>(r));
+    return (lane % CPR) ^ (FEW ? swizzle_v16<HDP>(r) : swizzle_v<HDP>(r));
   }
   // Strides of at most 2^26 elements (checked by the caller), so offsets fit 32 bits.
   __device__ __forceinline__ TileCopy(int64_t k_token, int64_t v_token, int head_dim, int lane, int tile_row = 0)
@@ -143,8 +147,8 @@ struct TileCopy {
     if (rows >= ROWS && pieces == CPR) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        lds_dma16(dst_k + 1024 * j, kb, vo_k[j]);
-        lds_dma16(dst_v + 1024 * j, vb, vo_v[j]);
+        lds_dma16<FEW>(dst_k + 1024 * j, kb, vo_k[j]);
+        lds_dma16<FEW>(dst_v + 1024 * j, vb, vo_v[j]);
       }
       return;
     }

@@ -2,8 +2,8 @@
 //
 //   out[t, h] = sum_s softmax_s(scale q[t, h] . k[s, kv]) v[s, kv],   s <= position of t,   kv = h / rep
 //
-// What bounds it: the bytes of K and V, read once.  So the work of all requests is laid end to end, in units of 64
-// keys (32 for heads of more than 128) of one item (request, row tile, KV head), and cut into one equal stretch per workgroup
+// What bounds it: the bytes of K and V, read once.  So the work of all requests is laid end to end, in units of 128
+// keys (64 for heads of more than 128) of one item (request, row tile, KV head), and cut into one equal stretch per workgroup
 // whatever the lengths are; a workgroup finds its stretch from the lengths by itself (they are read on the device only, so a captured launch
 // follows them).  The wavefronts of a workgroup take 32 keys each and do not wait for each other: each keeps its keys' tiles of K
 // and V coming through LDS buffers of its own by asynchronous copies, and they meet at the end of an item.
@@ -19,7 +19,7 @@ namespace {
 
 template <int HDP, int MT>
 struct FewConfig {
-  static constexpr int WAVES = HDP == 256 ? 1 : 2;
+  static constexpr int WAVES = HDP == 256 ? 2 : 4;
   static constexpr int THREADS = 64 * WAVES;
   static constexpr int STAGES = HDP == 64 ? 4 : 2;
   static constexpr int ROW = HDP * 2;
@@ -30,7 +30,7 @@ struct FewConfig {
   // Beginning and ending an item takes about as long as these many units: they count for it when the work is cut,
   // or workgroups with many short items would be the last ones.
   static constexpr int ITEM = 2;
-  static constexpr int LDS = WAVES * RING;           // 64 KiB: two workgroups per CU
+  static constexpr int LDS = WAVES * RING;           // 128 KiB, of which half or more is on its way
   static_assert(WAVES * ROWS * HDP * 4 <= LDS, "the wavefronts' sums meet in the buffers");
 };
 
@@ -462,7 +462,7 @@ FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int cu_count) {
   // Tables of up to 512 keys are worked off faster than a second launch begins.
   p.cut = key_units * unit > 512;
   p.most_units = items * (key_units + FewConfig<128, 1>::ITEM);
-  p.grid = (int)std::min<int64_t>(2 * cu_count, p.cut ? p.most_units : items);
+  p.grid = (int)std::min<int64_t>(cu_count, p.cut ? p.most_units : items);
   return p;
 }
 
