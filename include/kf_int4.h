@@ -335,7 +335,8 @@ int kf_rope_paged_cache(const kf_rope_paged_args* args, void* stream);
  *   out[t, h] = sum_{u <= t} softmax_u(scale q[t, h] . k[u, kv]) v[u, kv],  kv = h / (heads / kv_heads),
  * with 32-bit scores, maxima and sums; probabilities are rounded to the inputs' type for the second product, out
  * once more.  Keys after a token do not reach it whatever they hold.  Rows in no sequence are zeroed where
- * zero_rest is set and left as they are otherwise.  Strides in elements, multiples of 8; head_dim a multiple of 8
+ * zero_rest is set and left as they are otherwise.  ws: at least kf_prompt_attention_workspace_bytes(args)
+ * bytes, 16-byte aligned, not shared with a call that may run at the same time.  Strides in elements, multiples of 8; head_dim a multiple of 8
  * up to KF_ATTN_MAX_HEAD_DIM; scale positive. */
 typedef struct {
   const void* q;          /* [tokens, heads, head_dim] */
@@ -348,7 +349,8 @@ typedef struct {
   float scale;
   int zero_rest;
 } kf_prompt_attention_args;
-int kf_prompt_attention(const kf_prompt_attention_args* args, void* stream);
+size_t kf_prompt_attention_workspace_bytes(const kf_prompt_attention_args* args);
+int kf_prompt_attention(const kf_prompt_attention_args* args, void* ws, size_t ws_bytes, void* stream);
 
 /* Causal attention of every request's new tokens over its pages of the cache (which hold the new tokens' keys and
  * values already): request r's new tokens are rows cu_new[r] .. cu_new[r + 1] - 1 of q, the last of its

@@ -250,6 +250,35 @@ int paged_plan(const kf_paged_attention_args& a, PagedPlan* p) {
   return KF_OK;
 }
 
+size_t paged_workspace(const PagedPlan& p, int cus) {
+  size_t need = 0;
+  if (p.few) need = kf::few_rows_workspace_bytes(p.args.head_dim, kf::few_rows_plan(p.args, p.rows, cus));
+  if (p.many) need = std::max(need, kf::flash_workspace_bytes(p.args.head_dim, kf::flash_plan(p.args, true, cus)));
+  return need;
+}
+
+int check_workspace(const void* ws, size_t have, size_t need) {
+  if (!need) return KF_OK;
+  if (!ws || have < need)
+    return fail(KF_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, ws ? have : (size_t)0);
+  if (!aligned(ws, 16)) return fail(KF_ERR_WORKSPACE, "the workspace must be 16-byte aligned");
+  return KF_OK;
+}
+
+int prompt_args(const kf_prompt_attention_args& a, kf::AttnArgs* p) {
+  if (int st = check_attention(a.tokens, a.seqs, a.heads, a.kv_heads, a.head_dim, a.dtype, a.scale)) return st;
+  kf::AttnArgs& t = *p;
+  t = {};
+  t.q = a.q, t.k = a.k, t.v = a.v, t.out = a.out;
+  t.cu = static_cast<const int*>(a.cu_seqlens);
+  t.q_token = a.q_token, t.q_head = a.q_head, t.out_token = a.out_token, t.out_head = a.out_head;
+  t.k_token = a.k_token, t.k_head = a.k_head, t.v_token = a.v_token, t.v_head = a.v_head;
+  t.tokens = a.tokens, t.seqs = a.seqs, t.heads = a.heads, t.kv_heads = a.kv_heads, t.head_dim = a.head_dim;
+  t.zero_rest = a.zero_rest;
+  t.scale = a.scale;
+  return KF_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -689,34 +718,39 @@ int kf_rope_paged_cache(const kf_rope_paged_args* a, void* stream) {
                     "rope_paged_cache launch");
 }
 
-int kf_prompt_attention(const kf_prompt_attention_args* a, void* stream) {
+size_t kf_prompt_attention_workspace_bytes(const kf_prompt_attention_args* a) {
+  kf::AttnArgs t;
+  int cus;
+  if (!a || prompt_args(*a, &t) || cu_count(&cus)) return 0;
+  return kf::flash_workspace_bytes(a->head_dim, kf::flash_plan(t, false, cus));
+}
+
+int kf_prompt_attention(const kf_prompt_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
   if (!a) return fail(KF_ERR_INVALID_ARG, "args must be non-null");
-  if (int st = check_attention(a->tokens, a->seqs, a->heads, a->kv_heads, a->head_dim, a->dtype, a->scale)) return st;
+  kf::AttnArgs t;
+  if (int st = prompt_args(*a, &t)) return st;
   if (a->tokens == 0) return KF_OK;
-  const void* const p[] = {a->q, a->k, a->v, a->out, a->cu_seqlens};
+  const void* const p[] = {a->q, a->k, a->v, a->out};
   if (int st = check_arrays(p, 4)) return st;
   if (!a->cu_seqlens) return fail(KF_ERR_INVALID_ARG, "every array must be non-null");
   const int64_t strides[] = {a->q_token, a->q_head, a->k_token, a->k_head, a->v_token, a->v_head, a->out_token, a->out_head};
   if (int st = check_strides(strides, 8)) return st;
   if (a->k_token > kMaxTokenStride || a->v_token > kMaxTokenStride)
     return fail(KF_ERR_UNSUPPORTED, "token strides of k and v go up to %d elements", kMaxTokenStride);
-  kf::AttnArgs t = {};
-  t.q = a->q, t.k = a->k, t.v = a->v, t.out = a->out;
-  t.cu = static_cast<const int*>(a->cu_seqlens);
-  t.q_token = a->q_token, t.q_head = a->q_head, t.out_token = a->out_token, t.out_head = a->out_head;
-  t.k_token = a->k_token, t.k_head = a->k_head, t.v_token = a->v_token, t.v_head = a->v_head;
-  t.tokens = a->tokens, t.seqs = a->seqs, t.heads = a->heads, t.kv_heads = a->kv_heads, t.head_dim = a->head_dim;
-  t.zero_rest = a->zero_rest;
-  t.scale = a->scale;
-  return hip_status(kf::flash_attention_launch(t, false, a->dtype == KF_DTYPE_BF16, 0, static_cast<hipStream_t>(stream)),
+  int cus;
+  if (int st = cu_count(&cus)) return st;
+  const kf::FlashPlan plan = kf::flash_plan(t, false, cus);
+  if (int st = check_workspace(ws, ws_bytes, kf::flash_workspace_bytes(a->head_dim, plan))) return st;
+  return hip_status(kf::flash_attention_launch(t, false, a->dtype == KF_DTYPE_BF16, plan, 0, ws,
+                                               static_cast<hipStream_t>(stream)),
                     "prompt_attention launch");
 }
 
 size_t kf_paged_attention_workspace_bytes(const kf_paged_attention_args* a) {
   PagedPlan p;
   int cus;
-  if (!a || paged_plan(*a, &p) || !p.few || cu_count(&cus)) return 0;
-  return kf::few_rows_workspace_bytes(a->head_dim, kf::few_rows_plan(p.args, p.rows, cus));
+  if (!a || paged_plan(*a, &p) || cu_count(&cus)) return 0;
+  return paged_workspace(p, cus);
 }
 
 int kf_paged_attention(const kf_paged_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -733,26 +767,27 @@ int kf_paged_attention(const kf_paged_attention_args* a, void* ws, size_t ws_byt
   if (a->k_token > kMaxTokenStride || a->v_token > kMaxTokenStride)
     return fail(KF_ERR_UNSUPPORTED, "token strides of the caches go up to %d elements", kMaxTokenStride);
   const bool bf16 = a->dtype == KF_DTYPE_BF16;
+  int cus;
+  if (int st = cu_count(&cus)) return st;
+  // The two launches follow each other on the stream: they share the workspace.
+  if (int st = check_workspace(ws, ws_bytes, paged_workspace(p, cus))) return st;
   if (p.few) {
-    int cus;
-    if (int st = cu_count(&cus)) return st;
     const kf::FewPlan plan = kf::few_rows_plan(p.args, p.rows, cus);
     if (plan.most_units >= (int64_t)1 << 31)
       return fail(KF_ERR_UNSUPPORTED, "%d tokens over tables of %d pages are more than one launch takes", a->tokens,
                   a->table_width);
-    const size_t need = kf::few_rows_workspace_bytes(a->head_dim, plan);
-    if (need && (!ws || ws_bytes < need))
-      return fail(KF_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, ws ? ws_bytes : (size_t)0);
-    if (need && !aligned(ws, 16)) return fail(KF_ERR_WORKSPACE, "the workspace must be 16-byte aligned");
     const int max_rows = p.many ? kFewRows : 0x7fffffff;
     if (int st = hip_status(kf::few_rows_launch(p.args, bf16, plan, max_rows, ws, static_cast<hipStream_t>(stream)),
                             "paged_attention launch"))
       return st;
   }
-  if (p.many)
-    return hip_status(kf::flash_attention_launch(p.args, true, bf16, p.few ? kFewRows + 1 : 0,
+  if (p.many) {
+    kf::AttnArgs t = p.args;
+    if (p.few) t.zero_rest = 0;  // done
+    return hip_status(kf::flash_attention_launch(t, true, bf16, kf::flash_plan(t, true, cus), p.few ? kFewRows + 1 : 0, ws,
                                                  static_cast<hipStream_t>(stream)),
                       "paged_attention launch");
+  }
   return KF_OK;
 }
 

@@ -267,6 +267,17 @@ __device__ __forceinline__ AttnArgs reload_args() {
   return bit_cast<AttnArgs>(v);
 }
 
+// Inclusive prefix sums over a wavefront.
+__device__ __forceinline__ int wave_prefix(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // Sequences of packed tokens: [offset(s), offset(s + 1)) for s < seqs, then the rows in no sequence as sequence
 // `seqs`.  Offsets outside [0, tokens] are clamped, so no row index made from them leaves the tensors.
 __device__ __forceinline__ int seq_offset(const int* cu, int s, int seqs, int tokens) {
@@ -295,5 +306,50 @@ __device__ __forceinline__ int find_seq(const int* cu, int seqs, int tokens, int
   *first = lo == 0 ? 0 : seq_offset(cu, lo, seqs, tokens) * rep / BM + lo;
   return lo;
 }
+
+// What the second launch needs to know of a cut item, left by the workgroup in whose stretch it begins.
+struct Piece {
+  int seq, row0, kv, last;  // last: the workgroup in whose stretch it ends; seq < 0: nothing begins and goes on here
+};
+
+// A piece's output against the maximum of them all.  A factor of zero leaves nothing of it but infinities and NaN.
+__device__ __forceinline__ float scaled(float x, float f) { return fabsf(x) < __builtin_inff() ? f * x : x; }
+
+namespace {
+// Joins the pieces of the items that workgroup blockIdx.x of the first launch began and did not end.
+template <class E, int HDP, int ROWS>
+__global__ __launch_bounds__(256) void join_pieces_kernel(AttnArgs a, int rep, const float* ws, const Piece* pieces) {
+  const Piece pc = pieces[blockIdx.x];
+  if (pc.seq < 0) return;
+  const int tok0 = seq_offset(a.cu, pc.seq, a.seqs, a.tokens);
+  const int rows = (seq_offset(a.cu, pc.seq + 1, a.seqs, a.tokens) - tok0) * rep;
+  const int live_rows = min(rows - pc.row0, ROWS);
+  constexpr int STRIDE = ROWS * (HDP + 2);
+  const int first = blockIdx.x;
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < live_rows * (HDP / 4); i += 256 * gridDim.y) {
+    const int r = i / (HDP / 4), d = 4 * (i % (HDP / 4));
+    auto part = [&](int w) { return ws + (size_t)(2 * w + (w == first ? 1 : 0)) * STRIDE; };
+    float top = -__builtin_inff(), l = 0.0f;
+#pragma unroll 4
+    for (int w = first; w <= pc.last; ++w) top = fmaxf(top, part(w)[ROWS * HDP + r]);
+    float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int w = first; w <= pc.last; ++w) {
+      const float* const p = part(w);
+      const float mw = p[ROWS * HDP + r], lw = p[ROWS * HDP + ROWS + r];
+      const float4_t x = *reinterpret_cast<const float4_t*>(p + r * HDP + d);
+      const float f = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
+      l += lw != lw ? lw : f * lw;  // a NaN among a piece's scores is in its sum, whatever its maximum says
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += scaled(x[e], f);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int row = pc.row0 + r, tok = row / rep, head = pc.kv * rep + (row - tok * rep);
+    if (d < a.head_dim)
+      store_global((E*)a.out + (size_t)(tok0 + tok) * a.out_token + (size_t)head * a.out_head + d,
+                   u32x2{Elem<E>::pack(v[0] * inv, v[1] * inv), Elem<E>::pack(v[2] * inv, v[3] * inv)});
+  }
+}
+}  // namespace
 
 }  // namespace kf

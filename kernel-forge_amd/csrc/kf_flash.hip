@@ -8,6 +8,9 @@
 // the inputs' type for the second matrix product (half a step of that type, as inputs are), the outputs once
 // more when they are stored.  The maximum that the exponentials are taken against follows the true one only when it is
 // exceeded by a factor 2^8: outputs and sums are then rescaled, which most tiles after the first spare.
+#include <math.h>
+#include <stdlib.h>
+
 #include "kf_attn_tiles.h"
 #include "kf_launch.h"
 
@@ -19,49 +22,57 @@ constexpr int kFlashRows = 32 * kFlashWaves;
 
 // Wavefronts per SIMD that the registers have to allow: one computes scores while another works on its
 // softmax.  From two on the products also accumulate in ordinary registers, without moves.
-constexpr int flash_waves_per_simd(int hdp) { return hdp == 64 ? 4 : hdp == 128 ? 2 : 1; }
+// The kernel that cuts the work needs some registers more.
+constexpr int flash_waves_per_simd(int hdp, bool cut) { return hdp == 64 ? (cut ? 3 : 4) : hdp == 128 ? 2 : 1; }
 
-template <class E, int HDP, bool PAGED>
-__global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flash_attention_kernel(AttnArgs a, int rep, int min_rows,
-                                                                        float scale_log2) {
-  constexpr int ROW = HDP * 2;                      // bytes
-  constexpr int KEYS = HDP == 256 ? 32 : 64, KU = KEYS / 32, KK = KEYS / 16;
-  constexpr int MINE = KEYS / kFlashWaves;           // keys of a tile that a wavefront fetches
-  constexpr int TILE = KEYS * ROW;
+// Two groups where their buffers fit.
+constexpr int flash_groups(int hdp) { return hdp == 256 ? 1 : 2; }
+
+template <int HDP>
+struct FlashConfig {
+  static constexpr int ROW = HDP * 2;  // bytes
+  static constexpr int KEYS = HDP == 256 ? 32 : 64;
+  static constexpr int TILE = KEYS * ROW;
+  // Queries of more than 128 dims leave no registers for themselves beside the outputs: each lane's stay in LDS.
+  static constexpr bool Q_LDS = HDP == 256;
+  static constexpr int LDS = 4 * TILE + (Q_LDS ? kFlashRows * ROW : 0);
+};
+// GROUPS of four wavefronts work on the same rows, each on every GROUPS-th tile of keys, and join at the end: where
+// there are fewer row tiles than the GPU holds workgroups, an item then ends sooner.
+template <int HDP, int GROUPS>
+struct FlashShared {
+  __attribute__((aligned(1024))) unsigned char smem[GROUPS * FlashConfig<HDP>::LDS];
+  int found[2][GROUPS * kFlashWaves];  // infinities or NaN in a masked tile
+  int patch_from;
+  float stat[GROUPS > 1 ? 2 * 64 * kFlashWaves : 1];
+};
+
+// Rows row0 .. + 127 of a sequence over its key tiles tile0 .. tiles - 1 (those that it has of them).
+// part: nullptr, or where the maximum, sum and unscaled outputs of an item that is cut go.
+template <class E, int HDP, bool PAGED, int GROUPS>
+__device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, GROUPS>& sh, int rep, float scale_log2, int seq,
+                                           int row0, int kv, int tile0, int tiles, float* part) {
+  using C = FlashConfig<HDP>;
+  constexpr int ROW = C::ROW, KEYS = C::KEYS, KU = KEYS / 32, KK = KEYS / 16, TILE = C::TILE;
+  constexpr int MINE = KEYS / kFlashWaves;          // keys of a tile that a wavefront fetches
   constexpr int ST = HDP / 16;                      // k steps of the first product
   constexpr int DT = HDP / 32;                      // 32-row tiles of O^T
-  // Queries of more than 128 dims leave no registers for themselves beside the outputs: each lane's stay in LDS.
-  constexpr bool Q_LDS = HDP == 256;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE + (Q_LDS ? kFlashRows * ROW : 0)];
-  __shared__ int found[2][kFlashWaves];  // infinities or NaN in a masked tile
-  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
-
+  constexpr bool Q_LDS = C::Q_LDS;
+  auto& found = sh.found;
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kv = blockIdx.x % a.kv_heads;
-  // The last tiles of a sequence have the most keys: they start first.
-  const int tile = (int)(gridDim.x / a.kv_heads) - 1 - (int)(blockIdx.x / a.kv_heads);
-
-  int first;
-  const int seq = find_seq<kFlashRows>(a.cu, a.seqs, a.tokens, rep, tile, lane, &first);
+  const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % kFlashWaves);
+  const int group = GROUPS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+  unsigned char* const smem = sh.smem + group * C::LDS;
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
   const int tok0 = seq_offset(a.cu, seq, a.seqs, a.tokens);
   const int len = max(seq_offset(a.cu, seq + 1, a.seqs, a.tokens) - tok0, 0);
   const int rows = len * rep;
-  const int row0 = (tile - first) * kFlashRows;
-  if (row0 >= rows || (seq < a.seqs && rows < min_rows)) return;
 
   // This lane's row.  Rows past the end repeat the last one and are not stored.
   const int my_row = row0 + 32 * wave + (lane & 31);
   const int row = min(my_row, rows - 1);
   const int tok = row / rep;
   const int head = kv * rep + (row - tok * rep);
-  E* const out = (E*)a.out + (size_t)(tok0 + tok) * a.out_token + (size_t)head * a.out_head;
-  if (seq == a.seqs) {
-    if (a.zero_rest && my_row < rows)
-      for (int c = half; c < a.head_dim / 8; c += 2) *(u32x4*)(out + 8 * c) = u32x4{0, 0, 0, 0};
-    return;
-  }
-
   // Keys: positions before this lane's row's own, itself included.
   const int seq_len = PAGED ? min(max(load_const(a.seq_lens, seq), 0), a.table_width << a.log2_block) : len;
   const int shift = seq_len - len;
@@ -70,7 +81,8 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
   const int wave_lo = shift + min(wave_row, rows - 1) / rep, wave_hi = shift + min(wave_row + 31, rows - 1) / rep;
   const int first_limit = shift + row0 / rep;  // the workgroup's first row's
   const int kend = shift + min(row0 + kFlashRows - 1, rows - 1) / rep + 1;
-  const int tiles = kend <= 0 ? 0 : (kend + KEYS - 1) / KEYS;
+  tiles = min(tiles, kend <= 0 ? 0 : (kend + KEYS - 1) / KEYS);
+  const int mine0 = tile0 + group;  // this group's first tile
 
   u32x4 qf[Q_LDS ? 1 : ST];
   u32x4* const q_lds = reinterpret_cast<u32x4*>(smem + 4 * TILE) + wave * ST * 64 + lane;
@@ -126,42 +138,55 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
 
   int patch_from = 0x7fffffff;  // first key of a tile with masks whose infinities and NaN were taken out
   int page = 0;
-  if (tiles > 0) {
-    if constexpr (PAGED) page = page_of(MINE * wave);
-    issue(0, 0, page);
-    if constexpr (PAGED) page = page_of(min(KEYS, kend - 1) + MINE * wave);
+  if (mine0 < tiles) {
+    if constexpr (PAGED) page = page_of(mine0 * KEYS + MINE * wave);
+    issue(mine0, 0, page);
+    if constexpr (PAGED) page = page_of((mine0 + GROUPS) * KEYS + MINE * wave);
   }
-  for (int kt = 0; kt < tiles; ++kt) {
-    const uint32_t buf = (kt & 1) * 2 * TILE;
+  uint32_t buf = 2 * TILE;
+  for (int kt0 = tile0; kt0 < tiles; kt0 += GROUPS) {  // the groups' iterations and barriers are the same
+    const int kt = kt0 + group;
+    buf ^= 2 * TILE;
     dma_barrier();
-    if (kt + 1 < tiles) {
-      issue(kt + 1, 2 * TILE - buf, page);
-      if constexpr (PAGED) page = page_of((kt + 2) * KEYS + MINE * wave);
+    if (kt + GROUPS < tiles) {
+      issue(kt + GROUPS, 2 * TILE - buf, page);
+      if constexpr (PAGED) page = page_of((kt + 2 * GROUPS) * KEYS + MINE * wave);
     }
     const int key0 = kt * KEYS;
 
     // Masks: keys past a row's own, pages that are not there.
     uint32_t bad = 0;  // bit i: keys key0 + 16 i .. + 15 are not there
+    bool other_bad = false;
     if constexpr (PAGED) {
 #pragma unroll
-      for (int i = 0; i < KK; ++i) bad |= page_of(key0 + 16 * i) < 0 ? 1u << i : 0u;
+      for (int i = 0; i < GROUPS * KK; ++i) {
+        const bool missing = page_of(kt0 * KEYS + 16 * i) < 0;
+        if (GROUPS == 1 || i / KK == group) bad |= missing ? 1u << (i % KK) : 0u;
+        other_bad |= missing;
+      }
     }
     const uint32_t my_v = lds + buf + TILE + (uint32_t)(MINE * wave) * ROW;  // the rows of V that this wavefront looks after
-    bool nonfinite = false;
-    if (__builtin_expect(key0 + KEYS - 1 > first_limit || bad != 0, 0)) {  // the same in all wavefronts
-      const bool any = lds_any_nonfinite<E>(my_v, MINE * ROW / 1024, lane);
-      if (lane == 0) found[kt & 1][wave] = any;
+    // The same in all wavefronts: some group's tile has masks.
+    if (__builtin_expect((kt0 + GROUPS) * KEYS - 1 > first_limit || other_bad, 0)) {
+      const int flag = (buf != 0) ? 1 : 0;
+      const bool any = kt < tiles && lds_any_nonfinite<E>(my_v, MINE * ROW / 1024, lane);
+      if (lane == 0) found[flag][group * kFlashWaves + wave] = any;
       lds_barrier();
+      bool some = false, mine = false;
 #pragma unroll
-      for (int w = 0; w < kFlashWaves; ++w) nonfinite |= found[kt & 1][w] != 0;
-      nonfinite = __builtin_amdgcn_readfirstlane(nonfinite);
+      for (int w = 0; w < GROUPS * kFlashWaves; ++w) {
+        some |= found[flag][w] != 0;
+        mine |= w / kFlashWaves == group && found[flag][w] != 0;
+      }
+      if (__builtin_expect(__builtin_amdgcn_readfirstlane(some), 0)) {
+        if (__builtin_amdgcn_readfirstlane(mine)) {
+          lds_finite_only<E>(my_v, MINE * ROW / 1024, lane);
+          patch_from = min(patch_from, key0);
+        }
+        lds_barrier();
+      }
     }
-    if (__builtin_expect(nonfinite, 0)) {
-      lds_finite_only<E>(my_v, MINE * ROW / 1024, lane);
-      lds_barrier();
-      patch_from = min(patch_from, key0);
-    }
-    if (key0 > wave_hi) continue;  // only other wavefronts have keys here
+    if (key0 > wave_hi || kt >= tiles) continue;  // only other wavefronts have keys here
 
     float16_t s[KU];
     const uint32_t kb = lds + buf + k_at;
@@ -232,6 +257,84 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
   }
 
   sum = add_halves(sum);
+  if constexpr (GROUPS > 1) {
+    // The second group's outputs, maxima and sums go through the buffers to the first one.
+    static_assert(GROUPS == 2, "one joins the other");
+    const int t256 = 64 * wave + lane;
+    if (threadIdx.x == 0) sh.patch_from = 0x7fffffff;
+    lds_barrier();  // the tiles have been read
+    float4_t* const acc = reinterpret_cast<float4_t*>(sh.smem);  // [4 DT][256]
+    if (group == 1) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc[(4 * t + i) * 256 + t256] = float4_t{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+      sh.stat[t256] = m;
+      sh.stat[256 + t256] = sum;
+      if (lane == 0 && patch_from != 0x7fffffff) atomicMin(&sh.patch_from, patch_from);
+    }
+    lds_barrier();
+    if (group == 1) return;
+    const float m1 = sh.stat[t256], mn = fmaxf(m, m1);
+    const float mcn = mn == -__builtin_inff() ? 0.0f : mn * scale_log2;
+    const float f0 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mc - mcn);
+    const float f1 = m1 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m1 * scale_log2 - mcn);
+    // A NaN among a group's scores is in its sum, whatever its maximum says; without a maximum the others are zeros.
+    const float s1 = sh.stat[256 + t256];
+    sum = (sum != sum ? sum : f0 * sum) + (s1 != s1 ? s1 : f1 * s1);
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4_t x = acc[(4 * t + i) * 256 + t256];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[t][4 * i + e] = scaled(o[t][4 * i + e], f0) + scaled(x[e], f1);
+      }
+    m = mn;
+    mc = mcn;
+    patch_from = min(patch_from, sh.patch_from);
+  }
+  const AttnArgs b = reload_args();
+  // What was taken out of tiles with masks belongs to the rows that do attend to it.
+  auto patch_of = [&](int d) {  // dims d .. d + 3 of this lane's row
+    float4_t add = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int key = patch_from; key < min(kend, tiles * KEYS); ++key) {
+      const E* v = (const E*)b.v + kv * b.v_head + d;
+      if constexpr (PAGED) {
+        const int p = load_const(b.table, (int64_t)seq * b.table_stride + (key >> b.log2_block));
+        if ((unsigned)p >= (unsigned)b.num_pages) continue;
+        v += p * b.v_page + (key & ((1 << b.log2_block) - 1)) * b.v_token;
+      } else {
+        v += (int64_t)(tok0 + key) * b.v_token;
+      }
+      if (key <= limit) add += nonfinite_of<E>(*reinterpret_cast<const u32x2*>(v));
+    }
+    return add;
+  };
+  if (part) {
+    if (my_row < rows) {
+      const int r = my_row - row0;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          store_global(part + r * HDP + 32 * t + 8 * i + 4 * half,
+                       float4_t{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]});
+      int first_half = half;
+      asm volatile("" : "+v"(first_half));  // compared here, not kept in scalar registers for the whole loop
+      if (first_half == 0) {
+        store_global(part + kFlashRows * HDP + r, m == -__builtin_inff() ? m : mc);
+        store_global(part + kFlashRows * HDP + kFlashRows + r, sum);
+      }
+    }
+    if (__builtin_expect(patch_from < kend, 0) && my_row < rows)
+      for (int d = 4 * half; d < b.head_dim; d += 8) *reinterpret_cast<float4_t*>(part + (my_row - row0) * HDP + d) += patch_of(d);
+    return;
+  }
+  const int group_heads = b.heads / b.kv_heads, out_row = min(my_row, rows - 1), out_tok = out_row / group_heads;
+  const int out_head = kv * group_heads + (out_row - out_tok * group_heads);
+  E* const out = (E*)b.out + (size_t)(tok0 + out_tok) * b.out_token + (size_t)out_head * b.out_head;
   const float inv = m == -__builtin_inff() && sum == 0.0f ? 0.0f : 1.0f / sum;  // no keys: zeros
   if (my_row < rows) {
 #pragma unroll
@@ -239,28 +342,15 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = 32 * t + 8 * i + 4 * half;
-        if (d < a.head_dim)
-          *(u32x2*)(out + d) = u32x2{Elem<E>::pack(o[t][4 * i] * inv, o[t][4 * i + 1] * inv),
-                                     Elem<E>::pack(o[t][4 * i + 2] * inv, o[t][4 * i + 3] * inv)};
+        if (d < b.head_dim)
+          store_global(out + d, u32x2{Elem<E>::pack(o[t][4 * i] * inv, o[t][4 * i + 1] * inv),
+                                      Elem<E>::pack(o[t][4 * i + 2] * inv, o[t][4 * i + 3] * inv)});
       }
   }
-
-  // What was taken out of tiles with masks belongs to the rows that do attend to it.
   if (__builtin_expect(patch_from < kend, 0) && my_row < rows) {
-    for (int c = half; c < a.head_dim / 4; c += 2) {
-      float4_t add = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int key = patch_from; key < kend; ++key) {
-        const E* v = (const E*)a.v + kv * a.v_head + 4 * c;
-        if constexpr (PAGED) {
-          const int p = page_of(key);
-          if (p < 0) continue;
-          v += p * a.v_page + (key & ((1 << a.log2_block) - 1)) * a.v_token;
-        } else {
-          v += (int64_t)(tok0 + key) * a.v_token;
-        }
-        if (key <= limit) add += nonfinite_of<E>(*reinterpret_cast<const u32x2*>(v));
-      }
-      u32x2* const at = reinterpret_cast<u32x2*>(out + 4 * c);
+    for (int d = 4 * half; d < b.head_dim; d += 8) {
+      const float4_t add = patch_of(d);
+      u32x2* const at = reinterpret_cast<u32x2*>(out + d);
       const u32x2 x = *at;
       *at = u32x2{Elem<E>::pack(Elem<E>::lo(x[0]) + add[0], Elem<E>::hi(x[0]) + add[1]),
                   Elem<E>::pack(Elem<E>::lo(x[1]) + add[2], Elem<E>::hi(x[1]) + add[3])};
@@ -268,28 +358,270 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP)) void flas
   }
 }
 
-template <class E, int HDP>
-hipError_t launch(const AttnArgs& a, bool paged, int min_rows, hipStream_t stream) {
+// Zeros in the rows of out that are in no sequence.
+template <class E>
+__device__ __forceinline__ void zero_rows(const AttnArgs& a, int64_t at, int64_t step) {
+  const int t0 = seq_offset(a.cu, a.seqs, a.seqs, a.tokens);
+  const int cpr = a.head_dim / 8, per_row = a.heads * cpr;
+  for (int64_t i = at; i < (int64_t)(a.tokens - t0) * per_row; i += step) {
+    const int64_t t = i / per_row;
+    const int r = (int)(i - t * per_row), h = r / cpr;
+    store_global((E*)a.out + (t0 + t) * a.out_token + h * a.out_head + 8 * (r - h * cpr), u32x4{0, 0, 0, 0});
+  }
+}
+
+// Row tile number `rank` of all sequences' (64 at most) in the order of their last keys, the longest first: the workgroups
+// that take longest then start first, whatever order the sequences come in.  The length of tile i of a sequence is (its
+// cached keys x rep + 128 (i + 1)) >> q, so how many of its tiles are at least so long needs no loop: lane s counts those
+// of sequence s, and a search over lengths ends at the one of tile `rank`.  False: there are only *total tiles.
+template <bool PAGED>
+__device__ __forceinline__ bool longest_tile(const AttnArgs& a, int rep, int min_rows, int rank, int lane, int* seq,
+                                             int* tile, int* total) {
+  int rows = 0;
+  int64_t base = 0;
+  if (lane < a.seqs) {
+    const int len = max(seq_offset(a.cu, lane + 1, a.seqs, a.tokens) - seq_offset(a.cu, lane, a.seqs, a.tokens), 0);
+    const int keys = PAGED ? min(max(load_const(a.seq_lens, lane), 0), a.table_width << a.log2_block) : len;
+    rows = len * rep;
+    base = (int64_t)max(keys - len, 0) * rep;
+  }
+  const int tiles = rows < min_rows ? 0 : (rows + kFlashRows - 1) / kFlashRows;
+  const int q = 32 - __clz(64 * rep - 1);  // lengths in steps of 64 keys or a little more
+  auto at_least = [&](int length) {        // tiles of this lane's sequence
+    const int64_t above = ((int64_t)length << q) - base;
+    const int64_t first = above <= 0 ? 0 : (above + kFlashRows - 1) / kFlashRows - 1;
+    return tiles - (int)min(first, (int64_t)tiles);
+  };
+  int top = tiles ? (int)((base + (int64_t)tiles * kFlashRows) >> q) : 0;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) top = max(top, __shfl_xor(top, off));
+  auto all = [](int v) { return __builtin_amdgcn_readlane(wave_prefix(v), 63); };
+  *total = all(tiles);
+  if (rank >= *total) return false;
+  int lo = 0, hi = __builtin_amdgcn_readfirstlane(top) + 1;  // at least lo: more than `rank` tiles; at least hi: not
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (all(at_least(mid)) > rank) lo = mid;
+    else hi = mid;
+  }
+  const int longer = at_least(hi), here = at_least(lo) - longer;
+  const int index = rank - all(longer);  // among the tiles of this length, sequence by sequence
+  const int before = wave_prefix(here) - here;
+  const uint64_t mine = __ballot(index >= before && index < before + here);
+  if (mine == 0) return false;
+  const int owner = __builtin_amdgcn_readfirstlane(__builtin_ctzll(mine));
+  *seq = owner;
+  *tile = __builtin_amdgcn_readlane(tiles - at_least(lo) + index - before, owner);
+  return true;
+}
+
+// One workgroup per row tile and KV head.
+template <class E, int HDP, bool PAGED, int GROUPS>
+__global__ __launch_bounds__(GROUPS * kFlashThreads, flash_waves_per_simd(HDP, GROUPS > 1)) void flash_attention_kernel(
+    AttnArgs a, int rep, int min_rows, int longest_first, float scale_log2) {
+  __shared__ FlashShared<HDP, GROUPS> sh;
+  const int kv = blockIdx.x % a.kv_heads;
+  const int numbers = (int)(gridDim.x / a.kv_heads), number = (int)(blockIdx.x / a.kv_heads);
+  int seq, tile, total;
+  if (longest_first) {
+    if (!longest_tile<PAGED>(a, rep, min_rows, number, threadIdx.x & 63, &seq, &tile, &total)) {
+      if (a.zero_rest && kv == 0)
+        zero_rows<E>(a, (int64_t)(number - total) * GROUPS * kFlashThreads + threadIdx.x,
+                     (int64_t)(numbers - total) * GROUPS * kFlashThreads);
+      return;
+    }
+  } else {
+    // In the sequences' order, the last tiles, which have the most keys, first.
+    const int t = numbers - 1 - number;
+    int first;
+    seq = find_seq<kFlashRows>(a.cu, a.seqs, a.tokens, rep, t, threadIdx.x & 63, &first);
+    if (seq == a.seqs) {
+      if (a.zero_rest && kv == 0)
+        zero_rows<E>(a, (int64_t)(t - first) * GROUPS * kFlashThreads + threadIdx.x,
+                     (int64_t)(numbers - first) * GROUPS * kFlashThreads);
+      return;
+    }
+    tile = t - first;
+    const int rows =
+        max(seq_offset(a.cu, seq + 1, a.seqs, a.tokens) - seq_offset(a.cu, seq, a.seqs, a.tokens), 0) * rep;
+    if (tile * kFlashRows >= rows || rows < min_rows) return;
+  }
+  const int row0 = tile * kFlashRows;
+  flash_item<E, HDP, PAGED, GROUPS>(a, sh, rep, scale_log2, seq, row0, kv, 0, 0x7fffffff / FlashConfig<HDP>::KEYS, nullptr);
+}
+
+// Fewer row tiles than workgroups that the GPU holds, or tiles of very different length: the work of all is laid end to
+// end and cut into equal stretches, as in kf_paged_attn.hip.  A row tile i of a sequence counts base + 2 (i + 1) steps
+// of 64 / rep keys: its first row's keys and some for beginning and ending it, then the rows'.  Items are in the order
+// request, KV head, row tile, and neighbouring stretches run on one XCD, whose L2 then holds their head's keys.
+constexpr int kFlashItem = 128;  // keys that beginning and ending an item takes as long as
+struct FlashWork {
+  int rows, tiles, base, head_cost;  // head_cost: of a KV head's row tiles together
+  __device__ __forceinline__ int64_t upto(int n) const { return (int64_t)n * base + (int64_t)n * (n + 1); }
+};
+template <bool PAGED>
+__device__ __forceinline__ FlashWork flash_work(const AttnArgs& a, int s, int rep, int min_rows) {
+  const int len = max(seq_offset(a.cu, s + 1, a.seqs, a.tokens) - seq_offset(a.cu, s, a.seqs, a.tokens), 0);
+  FlashWork w;
+  w.rows = len * rep;
+  w.tiles = w.rows < min_rows ? 0 : (w.rows + kFlashRows - 1) / kFlashRows;
+  const int keys = PAGED ? min(max(load_const(a.seq_lens, s), 0), a.table_width << a.log2_block) : len;
+  w.base = (int)(((int64_t)(max(keys - len, 0) + kFlashItem) * rep) >> 6);
+  // Never reached by offsets that ascend (flash_plan); with others no cost is negative.
+  w.head_cost = (int)min(w.upto(w.tiles), (int64_t)(0x7fffffff / a.kv_heads));
+  return w;
+}
+
+template <class E, int HDP, bool PAGED>
+__global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) void flash_cut_kernel(
+    AttnArgs args) {
+  __shared__ FlashShared<HDP, 1> sh;
+  __shared__ int scan[kFlashWaves], found[2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Workgroups go to the 8 XCDs in turn: XCD x takes stretches x * grid / 8 and on.
+  const int me = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+  int begin, end, per;
+  {
+    const AttnArgs& a = args;
+    const int rep = a.rep, min_rows = a.min_rows;
+    if (a.zero_rest) zero_rows<E>(a, (int64_t)blockIdx.x * kFlashThreads + tid, (int64_t)gridDim.x * kFlashThreads);
+    const int run = (a.seqs + kFlashThreads - 1) / kFlashThreads;
+    const int s0 = min(tid * run, a.seqs), s1 = min(s0 + run, a.seqs);
+    int mine = 0;
+    for (int s = s0; s < s1; ++s) mine += flash_work<PAGED>(a, s, rep, min_rows).head_cost * a.kv_heads;
+    const int upto = wave_prefix(mine);
+    if (lane == 63) scan[wave] = upto;
+    if (tid == 0) {
+      found[0] = -1;
+      static_cast<Piece*>(a.pieces)[me].seq = -1;
+    }
+    __syncthreads();
+    int total = 0, before = upto - mine;
+#pragma unroll
+    for (int w = 0; w < kFlashWaves; ++w) {
+      if (w < wave) before += scan[w];
+      total += scan[w];
+    }
+    total = max(__builtin_amdgcn_readfirstlane(total), 0);
+    // No stretch is shorter than what a tile of keys counts: every piece between an item's first and last has some.
+    per = max(total / (int)gridDim.x + 1, 4 * rep + 8);
+    begin = (int)min((int64_t)me * per, (int64_t)total);
+    end = begin + min(per, total - begin);
+    if (begin < end && begin >= before && begin < before + mine) {
+      int at = before;
+      for (int s = s0; s < s1; ++s) {
+        const int n = flash_work<PAGED>(a, s, rep, min_rows).head_cost * a.kv_heads;
+        if (begin < at + n) {
+          found[0] = s;
+          found[1] = at;
+          break;
+        }
+        at += n;
+      }
+    }
+    __syncthreads();
+  }
+  int seq = __builtin_amdgcn_readfirstlane(found[0]), seq_at = __builtin_amdgcn_readfirstlane(found[1]);
+  if (seq < 0) return;
+  begin = __builtin_amdgcn_readfirstlane(begin), end = __builtin_amdgcn_readfirstlane(end);
+  per = __builtin_amdgcn_readfirstlane(per);
+  for (int at = begin; at < end;) {
+    const AttnArgs a = reload_args();
+    const int rep = a.rep, min_rows = a.min_rows;
+    FlashWork w;
+    while ((w = flash_work<PAGED>(a, seq, rep, min_rows)).head_cost * a.kv_heads <= at - seq_at) {
+      seq_at += w.head_cost * a.kv_heads;
+      if (++seq >= a.seqs) return;
+    }
+    const int kv = (at - seq_at) / w.head_cost, head_at = seq_at + kv * w.head_cost, rest = at - head_at;
+    // The last row tile whose predecessors count at most `rest`: n^2 + (1 + base) n <= rest.
+    const double h = 0.5 * (1.0 + w.base);
+    int tile = __builtin_amdgcn_readfirstlane(min(max((int)(sqrt(h * h + rest) - h), 0), w.tiles - 1));
+    while (tile > 0 && w.upto(tile) > rest) --tile;
+    while (tile + 1 < w.tiles && w.upto(tile + 1) <= rest) ++tile;
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    const int item_at = head_at + (int)w.upto(tile), cost = w.base + 2 * (tile + 1);
+    const int from = at - item_at, to = min(cost, end - item_at);
+    const int row0 = tile * kFlashRows, len = w.rows / rep;
+    const int keys = PAGED ? min(max(load_const(a.seq_lens, seq), 0), a.table_width << a.log2_block) : len;
+    const int kend = keys - len + min(row0 + kFlashRows - 1, w.rows - 1) / rep + 1;
+    // The part's tiles: floor(position * tiles / cost), the same for a piece's end and the next one's beginning.
+    const double tiles = max((kend + FlashConfig<HDP>::KEYS - 1) / FlashConfig<HDP>::KEYS, 1), each = cost;
+    const int t0 = __builtin_amdgcn_readfirstlane((int)(from * tiles / each));
+    const int t1 = __builtin_amdgcn_readfirstlane((int)(to * tiles / each));
+    at = item_at + cost;
+    if (t0 == t1) continue;
+    const bool whole = t0 == 0 && to == cost;
+    float* const part = static_cast<float*>(a.ws) + (size_t)(2 * me + (t0 == 0 ? 1 : 0)) * kFlashRows * (HDP + 2);
+    if (tid == 0 && t0 == 0 && !whole) static_cast<Piece*>(a.pieces)[me] = Piece{seq, row0, kv, (item_at + cost - 1) / per};
+    flash_item<E, HDP, PAGED, 1>(a, sh, rep, a.scale_log2, seq, row0, kv, t0, t1, whole ? nullptr : part);
+    lds_barrier();  // the tiles have been read: the buffers are free
+  }
+}
+
+template <class E, int HDP, bool PAGED>
+hipError_t launch(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws, hipStream_t stream) {
   const int rep = a.heads / a.kv_heads;
-  const unsigned tiles = (unsigned)((int64_t)a.tokens * rep / kFlashRows + a.seqs + 1);
-  const dim3 grid(tiles * (unsigned)a.kv_heads);
   const float scale_log2 = a.scale * 1.44269504088896340736f;
-  if (paged) flash_attention_kernel<E, HDP, true><<<grid, kFlashThreads, 0, stream>>>(a, rep, min_rows, scale_log2);
-  else flash_attention_kernel<E, HDP, false><<<grid, kFlashThreads, 0, stream>>>(a, rep, min_rows, scale_log2);
+  constexpr int GROUPS = flash_groups(HDP);
+  if (!p.cut) {
+    if (p.groups > 1)
+      flash_attention_kernel<E, HDP, PAGED, GROUPS><<<p.grid, GROUPS * kFlashThreads, 0, stream>>>(a, rep, min_rows, p.longest_first,
+                                                                                                           scale_log2);
+    else
+      flash_attention_kernel<E, HDP, PAGED, 1><<<p.grid, kFlashThreads, 0, stream>>>(a, rep, min_rows, p.longest_first, scale_log2);
+    return hipGetLastError();
+  }
+  float* const parts = static_cast<float*>(ws);
+  Piece* const pieces = reinterpret_cast<Piece*>(parts + (size_t)2 * p.grid * kFlashRows * (HDP + 2));
+  AttnArgs c = a;
+  c.scale_log2 = scale_log2, c.rep = rep, c.min_rows = min_rows, c.ws = parts, c.pieces = pieces;
+  flash_cut_kernel<E, HDP, PAGED><<<p.grid, kFlashThreads, 0, stream>>>(c);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  join_pieces_kernel<E, HDP, kFlashRows><<<dim3(p.grid, 4), 256, 0, stream>>>(a, rep, parts, pieces);
   return hipGetLastError();
 }
 
-template <class E>
-hipError_t launch_dim(const AttnArgs& a, bool paged, int min_rows, hipStream_t stream) {
-  if (a.head_dim <= 64) return launch<E, 64>(a, paged, min_rows, stream);
-  if (a.head_dim <= 128) return launch<E, 128>(a, paged, min_rows, stream);
-  return launch<E, 256>(a, paged, min_rows, stream);
+template <class E, bool PAGED>
+hipError_t launch_dim(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws, hipStream_t stream) {
+  if (a.head_dim <= 64) return launch<E, 64, PAGED>(a, p, min_rows, ws, stream);
+  if (a.head_dim <= 128) return launch<E, 128, PAGED>(a, p, min_rows, ws, stream);
+  return launch<E, 256, PAGED>(a, p, min_rows, ws, stream);
 }
 
 }  // namespace
 
-hipError_t flash_attention_launch(const AttnArgs& a, bool paged, bool bf16, int min_rows, hipStream_t stream) {
-  return bf16 ? launch_dim<bhalf_t>(a, paged, min_rows, stream) : launch_dim<half_t>(a, paged, min_rows, stream);
+FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count) {
+  FlashPlan p;
+  const int64_t rep = a.heads / a.kv_heads;
+  const int64_t tiles = a.tokens * rep / kFlashRows + a.seqs + 1;
+  const int hdp = a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256;
+  const int64_t keys = paged ? (int64_t)a.table_width << a.log2_block : a.tokens;
+  const int64_t most_cost = (tiles + a.seqs) * a.kv_heads * (((keys + kFlashItem) * rep >> 6) + 2 * tiles + 2);
+  const int64_t items = tiles * a.kv_heads;
+  const char* e1 = getenv("KF_CUT"); const char* e2 = getenv("KF_GRP");
+  p.cut = items < cu_count && keys * (cu_count - items) > (int64_t)1600 * cu_count && most_cost < (int64_t)1 << 31;
+  p.groups = 4 * items <= 5 * cu_count && keys > 256 ? flash_groups(hdp) : 1;
+  if (e1) p.cut = atoi(e1);
+  if (e2) p.groups = atoi(e2) > 1 ? flash_groups(hdp) : 1;
+  // One sequence has its longest tiles last in any case, and workgroups that all run at once need no order.
+  p.longest_first = a.seqs > 1 && a.seqs <= 64 && items * p.groups > cu_count * flash_waves_per_simd(hdp, false);
+  p.grid = p.cut ? cu_count * flash_waves_per_simd(hdp, true) : (int)items;
+  return p;
+}
+
+size_t flash_workspace_bytes(int head_dim, const FlashPlan& p) {
+  if (!p.cut) return 0;
+  const int padded = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+  return (size_t)p.grid * (2 * sizeof(float) * kFlashRows * (padded + 2) + sizeof(Piece));
+}
+
+hipError_t flash_attention_launch(const AttnArgs& a, bool paged, bool bf16, const FlashPlan& p, int min_rows, void* ws,
+                                  hipStream_t stream) {
+  if (paged) return bf16 ? launch_dim<bhalf_t, true>(a, p, min_rows, ws, stream) : launch_dim<half_t, true>(a, p, min_rows, ws, stream);
+  return bf16 ? launch_dim<bhalf_t, false>(a, p, min_rows, ws, stream) : launch_dim<half_t, false>(a, p, min_rows, ws, stream);
 }
 
 }  // namespace kf

@@ -235,9 +235,23 @@ struct AttnArgs {
   int table_width, log2_block, num_pages;
   int zero_rest;            // write zeros to the rows of out that are in no sequence
   float scale;
+  // Filled in by the launchers of kernels that read their arguments anew for every item.
+  float scale_log2;         // of the exponent to base 2
+  int rep, min_rows;        // heads / kv_heads; sequences of fewer rows are not theirs
+  void* ws;
+  void* pieces;
 };
-// Requests of fewer than min_rows rows are left to the other kernel.
-hipError_t flash_attention_launch(const AttnArgs& a, bool paged, bool bf16, int min_rows, hipStream_t stream);
+struct FlashPlan {
+  bool cut;    // the work of all row tiles is cut into equal stretches, and a second launch joins what was cut
+  int groups;  // of four wavefronts that share a row tile's keys
+  bool longest_first;  // row tiles start in the order of their lengths
+  int grid;
+};
+FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count);
+size_t flash_workspace_bytes(int head_dim, const FlashPlan& p);
+// Requests of fewer than min_rows rows are left to the other kernel.  ws: flash_workspace_bytes, 16-byte aligned.
+hipError_t flash_attention_launch(const AttnArgs& a, bool paged, bool bf16, const FlashPlan& p, int min_rows, void* ws,
+                                  hipStream_t stream);
 
 // ---- attention of few rows per request over a paged cache (kf_paged_attn.hip) -----
 struct FewPlan {

@@ -34,11 +34,6 @@ struct FewConfig {
   static_assert(WAVES * ROWS * HDP * 4 <= LDS, "the wavefronts' sums meet in the buffers");
 };
 
-// What the second launch needs to know of a cut item, left by the workgroup in whose stretch it begins.
-struct Piece {
-  int seq, row0, kv, last;  // last: the workgroup in whose stretch it ends; seq < 0: nothing begins and goes on here
-};
-
 __device__ __forceinline__ int few_seq_len(const AttnArgs& a, int s) {
   return min(max(load_const(a.seq_lens, s), 0), a.table_width << a.log2_block);
 }
@@ -53,17 +48,6 @@ __device__ __forceinline__ int few_items(const AttnArgs& a, int s, int rep, int 
 template <class C, bool CUT>
 __device__ __forceinline__ int item_cost(int key_units) {
   return CUT ? key_units + C::ITEM : 1;
-}
-
-// Inclusive prefix sums over a wavefront.
-__device__ __forceinline__ int wave_prefix(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
-  return v;
 }
 
 __device__ __forceinline__ float max_groups(float v) {  // of lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -360,7 +344,7 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
         // A NaN among a wavefront's scores is in its sum, whatever its maximum says.
         l += stat[1][w][r] != stat[1][w][r] ? stat[1][w][r] : f * stat[1][w][r];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += f == 0.0f ? 0.0f : f * x[e];
+        for (int e = 0; e < 4; ++e) v[e] += scaled(x[e], f);
       }
       if (whole) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no keys: zeros
@@ -382,42 +366,6 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
   }
 }
 
-// Joins the pieces of the items that workgroup blockIdx.x of the first launch began and did not end.
-template <class E, int HDP, int MT>
-__global__ __launch_bounds__(256) void join_pieces_kernel(AttnArgs a, int rep, const float* ws, const Piece* pieces) {
-  using C = FewConfig<HDP, MT>;
-  const Piece pc = pieces[blockIdx.x];
-  if (pc.seq < 0) return;
-  const int tok0 = seq_offset(a.cu, pc.seq, a.seqs, a.tokens);
-  const int rows = (seq_offset(a.cu, pc.seq + 1, a.seqs, a.tokens) - tok0) * rep;
-  const int live_rows = min(rows - pc.row0, C::ROWS);
-  constexpr int STRIDE = C::ROWS * (HDP + 2);
-  const int first = blockIdx.x;
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < live_rows * (HDP / 4); i += 256 * gridDim.y) {
-    const int r = i / (HDP / 4), d = 4 * (i % (HDP / 4));
-    auto part = [&](int w) { return ws + (size_t)(2 * w + (w == first ? 1 : 0)) * STRIDE; };
-    float top = -__builtin_inff(), l = 0.0f;
-#pragma unroll 4
-    for (int w = first; w <= pc.last; ++w) top = fmaxf(top, part(w)[C::ROWS * HDP + r]);
-    float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int w = first; w <= pc.last; ++w) {
-      const float* const p = part(w);
-      const float mw = p[C::ROWS * HDP + r], lw = p[C::ROWS * HDP + C::ROWS + r];
-      const float4_t x = *reinterpret_cast<const float4_t*>(p + r * HDP + d);
-      const float f = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
-      l += lw != lw ? lw : f * lw;  // a NaN among a piece's scores is in its sum, whatever its maximum says
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += f == 0.0f ? 0.0f : f * x[e];
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int row = pc.row0 + r, tok = row / rep, head = pc.kv * rep + (row - tok * rep);
-    if (d < a.head_dim)
-      store_global((E*)a.out + (size_t)(tok0 + tok) * a.out_token + (size_t)head * a.out_head + d,
-                   u32x2{Elem<E>::pack(v[0] * inv, v[1] * inv), Elem<E>::pack(v[2] * inv, v[3] * inv)});
-  }
-}
-
 template <class E, int HDP, int MT>
 hipError_t launch(const AttnArgs& a, int max_rows, bool cut, int grid, void* ws, hipStream_t stream) {
   using C = FewConfig<HDP, MT>;
@@ -432,7 +380,7 @@ hipError_t launch(const AttnArgs& a, int max_rows, bool cut, int grid, void* ws,
   few_rows_kernel<E, HDP, MT, true><<<grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, parts, pieces);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  join_pieces_kernel<E, HDP, MT><<<dim3(grid, MT), 256, 0, stream>>>(a, rep, parts, pieces);
+  join_pieces_kernel<E, HDP, C::ROWS><<<dim3(grid, MT), 256, 0, stream>>>(a, rep, parts, pieces);
   return hipGetLastError();
 }
 

@@ -111,7 +111,8 @@ SIGNATURES = {
     "kf_decode_attention": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP]),
     "kf_paged_tables": (_I, [ctypes.POINTER(PagedTablesArgs), _VP]),
     "kf_rope_paged_cache": (_I, [ctypes.POINTER(RopePagedArgs), _VP]),
-    "kf_prompt_attention": (_I, [ctypes.POINTER(PromptAttentionArgs), _VP]),
+    "kf_prompt_attention_workspace_bytes": (_SZ, [ctypes.POINTER(PromptAttentionArgs)]),
+    "kf_prompt_attention": (_I, [ctypes.POINTER(PromptAttentionArgs), _VP, _SZ, _VP]),
     "kf_paged_attention_workspace_bytes": (_SZ, [ctypes.POINTER(PagedAttentionArgs)]),
     "kf_paged_attention": (_I, [ctypes.POINTER(PagedAttentionArgs), _VP, _SZ, _VP]),
     "kf_decode_argmax_step": (_I, [_VP, _I, _VP, _VP, _VP, _I, _VP, _VP]),

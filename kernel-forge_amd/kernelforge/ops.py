@@ -1162,7 +1162,12 @@ def _run_prompt(q, k, v, cu_seqlens, scale, out, zero_rest):
     args = _lib.PromptAttentionArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(cu_seqlens), *q.stride()[:2],
                                     *k.stride()[:2], *v.stride()[:2], *out.stride()[:2], t, cu_seqlens.numel() - 1, heads,
                                     k.shape[1], d, _HALF_TYPES[q.dtype], scale, zero_rest)
-    status = _lib.load().kf_prompt_attention(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(q.get_device()))
+    lib = _lib.load()
+    ref = ctypes.byref(args)
+    ws_bytes = lib.kf_prompt_attention_workspace_bytes(ref)
+    ws = q.new_empty((ws_bytes + 1) // 2) if ws_bytes else None  # two bytes a value
+    status = lib.kf_prompt_attention(ref, ws.data_ptr() if ws is not None else None, ws_bytes,
+                                     torch._C._cuda_getCurrentRawStream(q.get_device()))
     if status:
         _lib.check(status, "prompt_attention")
     return out

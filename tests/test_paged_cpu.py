@@ -191,7 +191,7 @@ def _struct(cls, **change):
     (dict(tokens=1 << 30, heads=64, kv_heads=1), "more than one launch"),
 ])
 def test_prompt_attention_abi(change, match):
-    _err(_lib.load().kf_prompt_attention(ctypes.byref(_struct(_lib.PromptAttentionArgs, **change)), None), match)
+    _err(_lib.load().kf_prompt_attention(ctypes.byref(_struct(_lib.PromptAttentionArgs, **change)), None, 0, None), match)
 
 
 @pytest.mark.parametrize("change,match", [
@@ -224,9 +224,11 @@ def test_paged_tables_abi(change, match):
 
 def test_null_arguments_and_empty_batches():
     lib = _lib.load()
-    for fn in (lib.kf_prompt_attention, lib.kf_rope_paged_cache, lib.kf_paged_tables):
+    for fn in (lib.kf_rope_paged_cache, lib.kf_paged_tables):
         _err(fn(None, None), "args must be non-null")
+    _err(lib.kf_prompt_attention(None, None, 0, None), "args must be non-null")
+    assert lib.kf_prompt_attention_workspace_bytes(None) == 0
     _err(lib.kf_paged_attention(None, None, 0, None), "args must be non-null")
     assert lib.kf_paged_attention_workspace_bytes(None) == 0
-    assert lib.kf_prompt_attention(ctypes.byref(_struct(_lib.PromptAttentionArgs, tokens=0, q=None)), None) == 0
+    assert lib.kf_prompt_attention(ctypes.byref(_struct(_lib.PromptAttentionArgs, tokens=0, q=None)), None, 0, None) == 0
     assert lib.kf_rope_paged_cache(ctypes.byref(_struct(_lib.RopePagedArgs, tokens=0, qkv=None)), None) == 0
