@@ -9,7 +9,6 @@
 // more when they are stored.  The maximum that the exponentials are taken against follows the true one only when it is
 // exceeded by a factor 2^8: outputs and sums are then rescaled, which most tiles after the first spare.
 #include <math.h>
-#include <stdlib.h>
 
 #include "kf_attn_tiles.h"
 #include "kf_launch.h"
@@ -98,10 +97,12 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
   }
 
   // Copies.  A wavefront fetches rows 16 wave .. + 15 of both tiles: one page, as pages hold 16 keys at least.
-  const int64_t table_at = (int64_t)seq * a.table_stride;
-  auto page_of = [&](int key) {  // uniform; -1: not in the cache
-    const int p = load_const(a.table, table_at + (min(key, kend - 1) >> a.log2_block));
-    return (unsigned)p < (unsigned)a.num_pages ? p : -1;
+  // The pages of the groups' next tiles come by one vector load, lane i's those of 16 keys, a tile ahead of the copies.
+  const int* const table = a.table + (PAGED ? (int64_t)seq * a.table_stride : 0);
+  auto load_pages = [&](int kt0) {
+    const int key = kt0 * KEYS + 16 * (lane % (GROUPS * KK));
+    const int p = load_const(table, min(key, kend - 1) >> a.log2_block);
+    return (unsigned)p < (unsigned)a.num_pages ? p : -1;  // -1: not in the cache
   };
   const TileCopy<E, HDP, false, MINE> copy(a.k_token, a.v_token, a.head_dim, lane, MINE * wave);
   auto issue = [&](int kt, uint32_t buf, int page) {
@@ -137,37 +138,36 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
                         8u * (uint32_t)(lane & 1) + TILE;
 
   int patch_from = 0x7fffffff;  // first key of a tile with masks whose infinities and NaN were taken out
-  int page = 0;
-  if (mine0 < tiles) {
-    if constexpr (PAGED) page = page_of(mine0 * KEYS + MINE * wave);
-    issue(mine0, 0, page);
-    if constexpr (PAGED) page = page_of((mine0 + GROUPS) * KEYS + MINE * wave);
+  // Which of this wavefront's pages and of all groups' are not there, now and in the next tiles.
+  int pages = 0;
+  uint64_t missing = 0, next_missing = 0;
+  auto my_page = [&] { return __builtin_amdgcn_readlane(pages, group * KK + MINE * wave / 16); };
+  auto none = [&] { return __ballot(pages < 0) & ((1u << (GROUPS * KK)) - 1); };
+  if (tile0 < tiles) {
+    if constexpr (PAGED) {
+      pages = load_pages(tile0);
+      next_missing = none();
+    }
+    if (mine0 < tiles) issue(mine0, 0, PAGED ? my_page() : 0);
+    if constexpr (PAGED) pages = load_pages(tile0 + GROUPS);
   }
   uint32_t buf = 2 * TILE;
   for (int kt0 = tile0; kt0 < tiles; kt0 += GROUPS) {  // the groups' iterations and barriers are the same
     const int kt = kt0 + group;
     buf ^= 2 * TILE;
     dma_barrier();
-    if (kt + GROUPS < tiles) {
-      issue(kt + GROUPS, 2 * TILE - buf, page);
-      if constexpr (PAGED) page = page_of((kt + 2 * GROUPS) * KEYS + MINE * wave);
-    }
+    missing = next_missing;
+    if constexpr (PAGED) next_missing = none();
+    const int page = PAGED ? my_page() : 0;
+    if constexpr (PAGED) pages = load_pages(kt0 + 2 * GROUPS);  // before the copies: the wait for them is a wait for it
+    if (kt + GROUPS < tiles) issue(kt + GROUPS, 2 * TILE - buf, page);
     const int key0 = kt * KEYS;
 
-    // Masks: keys past a row's own, pages that are not there.
-    uint32_t bad = 0;  // bit i: keys key0 + 16 i .. + 15 are not there
-    bool other_bad = false;
-    if constexpr (PAGED) {
-#pragma unroll
-      for (int i = 0; i < GROUPS * KK; ++i) {
-        const bool missing = page_of(kt0 * KEYS + 16 * i) < 0;
-        if (GROUPS == 1 || i / KK == group) bad |= missing ? 1u << (i % KK) : 0u;
-        other_bad |= missing;
-      }
-    }
+    // Masks: keys past a row's own, pages that are not there (bit i of `bad`: keys key0 + 16 i .. + 15).
+    const uint32_t bad = (uint32_t)(missing >> (group * KK)) & ((1u << KK) - 1);
     const uint32_t my_v = lds + buf + TILE + (uint32_t)(MINE * wave) * ROW;  // the rows of V that this wavefront looks after
     // The same in all wavefronts: some group's tile has masks.
-    if (__builtin_expect((kt0 + GROUPS) * KEYS - 1 > first_limit || other_bad, 0)) {
+    if (__builtin_expect((kt0 + GROUPS) * KEYS - 1 > first_limit || missing != 0, 0)) {
       const int flag = (buf != 0) ? 1 : 0;
       const bool any = kt < tiles && lds_any_nonfinite<E>(my_v, MINE * ROW / 1024, lane);
       if (lane == 0) found[flag][group * kFlashWaves + wave] = any;
@@ -194,12 +194,15 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
     for (int u = 0; u < KU; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
+    // This wavefront's matrix products go before the other wavefronts' softmax: their results are waited for longest.
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int st = 0; st < ST; ++st)
 #pragma unroll
       for (int u = 0; u < KU; ++u)
         s[u] = Elem<E>::mfma32(lds_read16((kb ^ (uint32_t)(32 * st)) + u * 32 * ROW), Q_LDS ? q_lds[64 * st] : qf[Q_LDS ? 0 : st], s[u]);
 
+    __builtin_amdgcn_s_setprio(0);
     const bool masked = key0 + KEYS - 1 > wave_lo || bad != 0;
     // The last of this lane's keys key0 + 8 q + 4 half + (0 .. 3) that its row attends to, as 0 .. 3 (below: none).
     auto keys_at = [&](int q) { return (bad >> (q >> 1)) & 1 ? -1 : limit - (key0 + 8 * q + 4 * half); };
@@ -601,11 +604,8 @@ FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count) {
   const int64_t keys = paged ? (int64_t)a.table_width << a.log2_block : a.tokens;
   const int64_t most_cost = (tiles + a.seqs) * a.kv_heads * (((keys + kFlashItem) * rep >> 6) + 2 * tiles + 2);
   const int64_t items = tiles * a.kv_heads;
-  const char* e1 = getenv("KF_CUT"); const char* e2 = getenv("KF_GRP");
   p.cut = items < cu_count && keys * (cu_count - items) > (int64_t)1600 * cu_count && most_cost < (int64_t)1 << 31;
   p.groups = 4 * items <= 5 * cu_count && keys > 256 ? flash_groups(hdp) : 1;
-  if (e1) p.cut = atoi(e1);
-  if (e2) p.groups = atoi(e2) > 1 ? flash_groups(hdp) : 1;
   // One sequence has its longest tiles last in any case, and workgroups that all run at once need no order.
   p.longest_first = a.seqs > 1 && a.seqs <= 64 && items * p.groups > cu_count * flash_waves_per_simd(hdp, false);
   p.grid = p.cut ? cu_count * flash_waves_per_simd(hdp, true) : (int)items;
