@@ -19,6 +19,9 @@ positions in device tensors, one decode step captured in a HIP graph and replaye
 token is written back into the graph's input on the device, so replays run back to back.
 Attention of a decode step on the GPU is one launch (ops.decode_attention, fp32 inside); prompts and
 the CPU run plain PyTorch (fp16 matmuls on contiguous operands, fp32 softmax).
+
+``PagedDecoder`` serves several requests at once: their new tokens packed, keys and values in pages
+(ops.paged_tables, rope_paged_cache, prompt_attention for prompts, paged_attention for chunks and decode steps).
 """
 
 from __future__ import annotations
@@ -142,6 +145,26 @@ class Attention(nn.Module):
             y = self.qkv.forward_concat(x)                               # [1, T, (hq + 2 hkv) d]
             return y[..., :nqk], y[..., nqk:]
         return torch.cat([self.q_proj(x), self.k_proj(x)], dim=-1), self.v_proj(x)
+
+    def paged(self, x, step, rope, cache_k, cache_v, block_table, max_new, whole_prompts, norm=None):
+        """Attention of several requests' new tokens, x [1, T, H] packed (normalized unless `norm` is given), over
+        a paged cache: [1, T, heads d], before o_proj.  whole_prompts: no request has tokens in the cache yet."""
+        cfg = self.cfg
+        if self.qkv is None:
+            qkv = torch.cat(self.project(x, norm), dim=-1)
+        elif norm is not None:
+            qkv = _int4_fused(self.qkv, x, norm_weight=norm.weight, eps=norm.eps)
+        else:
+            qkv = self.qkv.forward_concat(x)
+        qkv = qkv.view(-1, qkv.shape[-1])
+        v = qkv[:, (cfg.heads + cfg.kv_heads) * cfg.head_dim:]
+        q, k = ops.rope_paged_cache(qkv, rope[0], rope[1], step.positions, step.slots, cache_k, cache_v,
+                                    heads=cfg.heads)
+        if whole_prompts:
+            out = ops.prompt_attention(q, k, v.unflatten(1, (cfg.kv_heads, cfg.head_dim)), step.cu_new)
+        else:
+            out = ops.paged_attention(q, cache_k, cache_v, block_table, step.cu_new, step.seq_lens, max_new=max_new)
+        return out.view(1, -1, cfg.heads * cfg.head_dim)
 
     def core(self, qk, v, pos, cos, sin, cache_k, cache_v, scores):
         """Attention of the new positions over the cache: [1, T, heads d], before o_proj.
@@ -268,6 +291,17 @@ class DecoderLayer(nn.Module):
         return x + m(self.post_attention_layernorm(x))
 
 
+    def paged(self, x, *args):
+        """The layer on several requests' packed new tokens (Attention.paged's arguments after x)."""
+        a, m = self.self_attn, self.mlp
+        if self.int4_fusable():
+            x = _int4_fused(a.o_proj, a.paged(x, *args, norm=self.input_layernorm), residual=x)
+            g, u = m.project(x, self.post_attention_layernorm)
+            return _int4_fused(m.down_proj, g, up=u, residual=x)
+        x = x + a.o_proj(a.paged(self.input_layernorm(x), *args))
+        return x + m(self.post_attention_layernorm(x))
+
+
 class TinyLlama(nn.Module):
     def __init__(self, cfg: TinyLlamaConfig):
         super().__init__()
@@ -295,6 +329,23 @@ class TinyLlama(nn.Module):
         transposed (read as [kv_heads, head_dim, max_seq]), the value slab V as laid out."""
         c = self.cfg
         return torch.zeros(c.layers, 2, c.kv_heads, c.max_seq, c.head_dim, device=device, dtype=dtype)
+
+    def new_paged_cache(self, num_pages: int, block_size: int, device, dtype=torch.float16) -> torch.Tensor:
+        """Paged KV cache [layers, 2, num_pages, kv_heads, block_size, head_dim] for ops.paged_attention."""
+        c = self.cfg
+        return torch.zeros(c.layers, 2, num_pages, c.kv_heads, block_size, c.head_dim, device=device, dtype=dtype)
+
+    @torch.no_grad()
+    def forward_paged(self, tokens, step: ops.PagedStep, cache, rope, block_table, *, max_new: int,
+                      whole_prompts: bool = False):
+        """Several requests at once: tokens int64 [T], packed request by request as `step` (ops.paged_tables) says; cache
+        from new_paged_cache; rope: the fp32 tables of _rope_tables.  Returns the logits after each request's last new
+        token, [requests, vocab] (of some other token for requests without new ones)."""
+        x = self.embed_tokens(tokens).unsqueeze(0)
+        for i, layer in enumerate(self.layers):
+            x = layer.paged(x, step, rope, cache[i, 0], cache[i, 1], block_table, max_new, whole_prompts)
+        last = (step.cu_new[1:].long() - 1).clamp(0, tokens.numel() - 1)
+        return self.lm_head(self.norm(x[0, last]))
 
     @torch.no_grad()
     def forward(self, tokens, pos, cache, rope, mask, logits_fp32: bool = True):
@@ -443,6 +494,149 @@ class GraphDecoder:
 
     def generated(self, prompt_len: int, steps: int) -> torch.Tensor:
         return self.history[prompt_len:prompt_len + steps + 1].clone()
+
+
+class PagedDecoder:
+    """Greedy decode of several requests at once over a paged KV cache, one HIP-graph-captured step for all.
+
+    Every request has a row.  ``admit`` gives prompts to free rows (whole, or in chunks between which nothing else runs),
+    ``decode`` appends one token per step to every row that holds a request, ``finish`` frees a row and returns its
+    pages.  Lengths, tables and the stack of free pages are on the device, where the step advances them; the host
+    keeps its own count of lengths and pages and refuses (ValueError) what would pass max_seq or the pages there are.
+    """
+
+    def __init__(self, model: TinyLlama, device, requests: int, num_pages: int, block_size: int = 16):
+        cfg = model.cfg
+        self.model, self.device, self.block_size, self.num_pages = model, device, block_size, num_pages
+        self.rope = tuple(t.contiguous() for t in _rope_tables(cfg, device))
+        self.cache = model.new_paged_cache(num_pages, block_size, device, model.embed_tokens.weight.dtype)
+        i32 = dict(dtype=torch.int32, device=device)
+        self.block_table = torch.full((requests, -(-cfg.max_seq // block_size)), -1, **i32)
+        self.context_lens = torch.zeros(requests, **i32)
+        self.active = torch.zeros(requests, **i32)  # 1: the row holds a request
+        self.free_pages = torch.arange(num_pages, **i32)
+        self.free_count = torch.full((1,), num_pages, **i32)
+        self.tokens = torch.zeros(requests, dtype=torch.long, device=device)
+        self.history = torch.zeros(requests, cfg.max_seq, dtype=torch.long, device=device)
+        self.graph = None
+        self.host_lens = [0] * requests  # tokens in the cache; 0: a free row
+
+    def _pages(self, tokens: int) -> int:
+        return -(-tokens // self.block_size)
+
+    def _reserve(self, new: list[int], what: str) -> None:
+        """Raises unless `new` more tokens per row stay inside max_seq and the pages that are left."""
+        last = self.model.cfg.max_seq - 1
+        after = [n + m for n, m in zip(self.host_lens, new)]
+        for row, n in enumerate(after):
+            if n > last:
+                raise ValueError(f"{what}: row {row} would hold {n} tokens, more than max_seq - 1 = {last}")
+        need = sum(self._pages(n) for n in after)
+        if need > self.num_pages:
+            raise ValueError(f"{what}: {need} pages are needed, and there are {self.num_pages}")
+
+    def _advance(self, tokens, new_lens, max_tokens: int, max_new: int, whole_prompts: bool) -> ops.PagedStep:
+        """One step of the model for rows with new tokens; the next token of each goes into self.tokens and the history."""
+        step = ops.paged_tables(self.block_table, self.context_lens, new_lens, self.free_pages, self.free_count,
+                                block_size=self.block_size, max_tokens=max_tokens)
+        logits = self.model.forward_paged(tokens, step, self.cache, self.rope, self.block_table, max_new=max_new,
+                                          whole_prompts=whole_prompts)
+        chosen = new_lens > 0
+        nxt = torch.where(chosen, torch.argmax(logits, dim=-1), self.tokens)
+        self.tokens.copy_(nxt)
+        # A row's next token stands behind the tokens that its cache holds; rows that paused write theirs again.
+        self.history.scatter_(1, step.seq_lens.long().unsqueeze(1), nxt.unsqueeze(1))
+        self.context_lens.copy_(step.seq_lens)
+        self.free_count.copy_(step.free_count)
+        return step
+
+    @torch.no_grad()
+    def admit(self, prompts: dict[int, torch.Tensor], chunk: int | None = None) -> None:
+        """Runs the prompts (row -> int64 tokens) of free rows together, `chunk` tokens of each at a time if given, and
+        leaves each row's first generated token."""
+        rows = sorted(prompts)
+        for row in rows:
+            if self.host_lens[row]:
+                raise ValueError(f"admit: row {row} holds a request")
+            if prompts[row].numel() < 1:
+                raise ValueError(f"admit: the prompt of row {row} is empty")
+        if chunk is not None and chunk < 1:
+            raise ValueError(f"admit: chunk must be positive, got {chunk}")
+        lens = [prompts[r].numel() if r in prompts else 0 for r in range(len(self.host_lens))]
+        self._reserve(lens, "admit")
+        done = [0] * len(lens)
+        for row in rows:
+            self.history[row] = 0
+            self.history[row, :lens[row]] = prompts[row]
+        while done != lens:
+            new = [min(n - d, chunk or n) for n, d in zip(lens, done)]
+            tokens = torch.cat([prompts[r][done[r]:done[r] + new[r]] for r in rows])
+            self._advance(tokens, torch.tensor(new, dtype=torch.int32, device=self.device), sum(new), max(new),
+                          whole_prompts=chunk is None and not any(self.host_lens))
+            done = [d + n for d, n in zip(done, new)]
+        for row in rows:
+            self.host_lens[row] = lens[row]
+            # The chunks' own next tokens are overwritten by the prompt's.
+            self.history[row, :lens[row]] = prompts[row]
+            self.active[row] = 1
+
+    def finish(self, row: int) -> None:
+        """Frees a row: its pages go back onto the stack."""
+        n = self._pages(self.host_lens[row])
+        if n == 0:
+            raise ValueError(f"finish: row {row} holds no request")
+        used = sum(self._pages(m) for m in self.host_lens)
+        free = self.num_pages - used
+        self.free_pages[free:free + n] = self.block_table[row, :n].clone()
+        self.free_count.fill_(free + n)
+        self.block_table[row] = -1
+        self.context_lens[row] = 0
+        self.active[row] = 0
+        self.host_lens[row] = 0
+
+    def _step(self) -> None:
+        # The tokens of the rows that hold requests, packed.
+        rows = self.tokens.numel()
+        ends = torch.cumsum(self.active, 0)
+        order = torch.searchsorted(ends, torch.arange(1, rows + 1, device=self.device)).clamp(max=rows - 1)
+        self._advance(self.tokens[order], self.active, rows, 1, whole_prompts=False)
+
+    @torch.no_grad()
+    def capture(self) -> None:
+        """Captures the step; the requests are left as they were."""
+        state = (self.cache, self.block_table, self.context_lens, self.free_count, self.tokens, self.history)
+        self._reserve([2 if n else 0 for n in self.host_lens], "capture (two warm-up steps)")
+        saved = [t.clone() for t in state]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                self._step()
+        torch.cuda.current_stream().wait_stream(side)
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self._step()
+        for t, old in zip(state, saved):
+            t.copy_(old)
+
+    @torch.no_grad()
+    def decode(self, steps: int, use_graph: bool = True) -> torch.Tensor:
+        """`steps` more tokens for every row that holds a request; returns the history [requests, max_seq]."""
+        if use_graph and self.graph is None:
+            raise ValueError("decode: capture first, or pass use_graph=False")
+        new = [steps if n else 0 for n in self.host_lens]
+        self._reserve(new, "decode")
+        for _ in range(steps):
+            if use_graph:
+                self.graph.replay()
+            else:
+                self._step()
+        self.host_lens = [n + m for n, m in zip(self.host_lens, new)]
+        return self.history
+
+    def generated(self, row: int, prompt_len: int) -> torch.Tensor:
+        """The tokens generated so far for a row, the one not yet in the cache included."""
+        return self.history[row, prompt_len:self.host_lens[row] + 1].clone()
 
 
 def build_int4_model(cfg: TinyLlamaConfig, device, seed: int = 0, group_size: int = 128,
