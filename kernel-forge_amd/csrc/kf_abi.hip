@@ -658,7 +658,11 @@ int kf_paged_tables(const kf_paged_tables_args* a, void* stream) {
       !a->cu_new || !a->seq_lens || (a->max_tokens && (!a->positions || !a->slots)) || !a->free_left)
     return fail(KF_ERR_INVALID_ARG, "every array must be non-null");
   if (a->free_left == a->free_count) return fail(KF_ERR_INVALID_ARG, "free_left must not be free_count");
-  if (a->seqs > (1 << 20)) return fail(KF_ERR_UNSUPPORTED, "paged_tables takes up to %d requests, got %d", 1 << 20, a->seqs);
+  // Every request's workgroup sums over the requests before it.
+  if (a->seqs > (1 << 16)) return fail(KF_ERR_UNSUPPORTED, "paged_tables takes up to %d requests, got %d", 1 << 16, a->seqs);
+  if (a->seqs > 1 && a->table_stride < a->table_width)
+    return fail(KF_ERR_INVALID_ARG, "rows of block_table overlap: stride %lld, width %d", (long long)a->table_stride,
+                a->table_width);
   kf::TablesArgs t;
   t.table = static_cast<int*>(a->block_table);
   t.context_lens = static_cast<const int*>(a->context_lens);

@@ -901,6 +901,7 @@ def _caches_ok(cache_k: torch.Tensor, cache_v: torch.Tensor, dtype: torch.dtype)
     e, f, g, last = cache_v.stride() if cache_v.dim() == 4 else (0, 0, 0, 0)
     block = shape[2]
     return (cache_v.shape == shape and one == 1 and last == 1 and not (a | b | c | e | f | g) & 7
+            and a and b and c and e and f and g
             and not (cache_k.data_ptr() | cache_v.data_ptr()) & 15 and 16 <= block <= 1 << 20
             and not block & (block - 1) and cache_k.numel() > 0)
 
@@ -926,10 +927,16 @@ def _check_scale(scale: float | None, head_dim: int) -> float:
     return float(scale)
 
 
+def _own_places(t: torch.Tensor) -> bool:
+    """Whether no dimension of a tensor that is written is expanded (stride 0)."""
+    return all(s != 0 or n <= 1 for s, n in zip(t.stride(), t.shape))
+
+
 def _check_out(out: torch.Tensor | None, q: torch.Tensor) -> None:
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not _rows_ok(out)):
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
+                            or not _rows_ok(out) or not _own_places(out)):
         raise ValueError(f"out must be {str(q.dtype)[6:]} {list(q.shape)} on {q.device} with a contiguous last dimension, "
-                         "other strides of multiples of 8 and a 16-byte aligned start")
+                         "other strides of multiples of 8, none of them 0, and a 16-byte aligned start")
 
 
 def paged_tables(block_table: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor,
@@ -951,11 +958,14 @@ def paged_tables(block_table: torch.Tensor, context_lens: torch.Tensor, new_lens
         if (context_lens.shape == (b,) and new_lens.shape == (b,) and free_count.shape == (1,) and free_pages.dim() == 1
                 and block_table.dtype == i32 and context_lens.dtype == i32 and new_lens.dtype == i32
                 and free_pages.dtype == i32 and free_count.dtype == i32 and b > 0 and width > 0 and max_tokens >= 0
-                and block_table.stride(1) == 1 and context_lens.is_contiguous() and new_lens.is_contiguous()
+                and block_table.stride(1) == 1 and (b == 1 or block_table.stride(0) >= width)
+                and context_lens.is_contiguous() and new_lens.is_contiguous()
                 and free_pages.is_contiguous() and 16 <= block_size <= 1 << 20 and not block_size & (block_size - 1)):
             return PagedStep(*_run_paged_tables(*args))
     b = block_table.shape[0] if block_table.dim() == 2 else -1
     _check_table(block_table, b)
+    if b > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("block_table is written: its rows must not overlap")
     _check_int("context_lens", context_lens, torch.int32, (b,))
     _check_int("new_lens", new_lens, torch.int32, (b,))
     _check_int("free_count", free_count, torch.int32, (1,))
@@ -1039,6 +1049,8 @@ def rope_paged_cache(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, po
     if qkv.dim() != 2 or qkv.dtype not in _HALF_TYPES:
         raise TypeError("qkv must be a 2-D fp16 or bf16 tensor [T, (heads + 2 kv_heads) head_dim]")
     _check_cache(cache_k, cache_v, qkv.dtype)
+    if not _own_places(cache_k) or not _own_places(cache_v):
+        raise ValueError("cache_k and cache_v are written: they must not be expanded")
     kv_heads, d = cache_k.shape[1], cache_k.shape[3]
     _check_heads(heads, kv_heads, d)
     t = qkv.shape[0]
@@ -1104,7 +1116,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     cu_seqlens[s] .. cu_seqlens[s + 1] - 1, ascending from 0, empty ones allowed.  Query head h reads KV head
     h // (heads / kv_heads); scale defaults to 1 / sqrt(head_dim).  Scores, softmax and sums in 32 bits,
     probabilities rounded to the inputs' type for their product with v.  Rows behind the last sequence are zeros
-    in a new output and left as they are in ``out``.  The form of decode_attention for prompts; no reference
+    in a new output and left as they are in ``out``, which must not overlap k or v.  The form of decode_attention for prompts; no reference
     counterpart (its models run torch's attention).
     """
     tensors = (q, k, v, cu_seqlens)
@@ -1195,7 +1207,7 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
     (rope_paged_cache).  One token per request (decode), chunks of prompts and batches of both.  max_new: an upper bound
     of a request's new tokens, if the caller knows one; it chooses kernels and splits only.  Tokens whose page is not
     in the cache (-1) are not attended to; a row with no key gets zeros.  Rows behind the last request are zeros in a
-    new output and left as they are in ``out``.  Arithmetic as in prompt_attention; results do not change from
+    new output and left as they are in ``out``, which must not overlap the caches.  Arithmetic as in prompt_attention; results do not change from
     run to run.  The form of decode_attention for many requests; no reference counterpart.
     """
     tensors = (q, cache_k, cache_v, block_table, cu_new, seq_lens)

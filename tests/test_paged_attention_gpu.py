@@ -200,3 +200,48 @@ def test_two_streams_at_once():
                 got.append(x(max_new=1))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got))
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (4, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize("ctx,new", [([20000], [100]), ([9000, 0], [200, 90]), ([300, 5000, 40], [150, 70, 1]),
+                                     ([700] * 30, [80] * 30)], ids=["cut", "cut2", "mixed", "ordered"])
+def test_every_plan(heads, kv_heads, d, ctx, new):
+    """Chunks over long contexts, cut over workgroups, beside short ones and single tokens."""
+    b = Batch(ctx, new, heads, kv_heads, d, torch.bfloat16, 32, pad=2)
+    b.check(b(max_new=max(new)))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_holes_and_infinities_in_cut_items(bad):
+    """A long item in pieces: a page that is missing in the middle, and values beyond a row's last key."""
+    b = Batch([20000], [100], 8, 2, 64, torch.float16, 16)
+    there = torch.ones(20100, dtype=torch.bool, device=DEV)
+    b.table[0, 400] = -1
+    there[6400:6416] = False
+    out = b(max_new=100)
+    b.check(out, [there])
+    last = 20099
+    b.cache_v[b.table[0, last // 16].long(), 1, last % 16, 5] = bad
+    hit = b(max_new=100)
+    got = hit[99, 4:, 5]
+    assert bool(got.isnan().all()) if bad != bad else bool((got == bad).all())
+    hit[99, 4:, 5] = out[99, 4:, 5]
+    assert torch.equal(hit, out)
+
+
+def test_registered_ops():
+    b = Batch([40, 3], [1, 5], 4, 2, 64, torch.float16, 16)
+    args = (b.q, b.cache_k.nan_to_num(), b.cache_v.nan_to_num(), b.table, b.cu, b.seq_lens, 5, 0.125)
+    torch.library.opcheck(ops._paged_attention_op, args, test_utils=("test_schema", "test_faketensor"))
+    assert torch.equal(torch.ops.kernelforge.paged_attention(*args), b(max_new=5))
+    t = torch.zeros(2, 9, dtype=torch.int32, device=DEV)
+    lens = torch.tensor([4, 0], dtype=torch.int32, device=DEV)
+    free, count = torch.arange(9, dtype=torch.int32, device=DEV), torch.tensor([9], dtype=torch.int32, device=DEV)
+    torch.library.opcheck(ops._paged_tables_op, (t, lens, lens, free, count, 16, 8),
+                          test_utils=("test_schema", "test_faketensor"))
+    pos, slots = torch.arange(4, device=DEV), torch.arange(4, device=DEV)
+    cos = torch.ones(8, 64, device=DEV)
+    caches = [torch.zeros(3, 2, 16, 64, dtype=torch.float16, device=DEV) for _ in range(2)]
+    qkv = torch.randn(4, 512, device=DEV).half()
+    torch.library.opcheck(ops._rope_paged_op, (qkv, cos, cos, pos, slots, *caches, 4),
+                          test_utils=("test_schema", "test_faketensor"))

@@ -46,6 +46,7 @@ def attention_args(dtype=H, t=6, heads=4, kv=2, d=64, block=16, b=2, width=3, pa
     (dict(scale=-1.0), ValueError, "scale"),
     (dict(out=torch.zeros(6, 4, 64)), ValueError, "out must be"),
     (dict(out=torch.zeros(6, 4, 65, dtype=H)[..., 1:]), ValueError, "out must be"),
+    (dict(out=torch.zeros(6, 1, 64, dtype=H).expand(6, 4, 64)), ValueError, "none of them 0"),
 ])
 def test_paged_attention_refusals(change, error, match):
     with pytest.raises(error, match=match):
@@ -102,6 +103,7 @@ def rope_args():
     (dict(positions=torch.zeros(6, dtype=torch.int32)), ValueError, "positions"),
     (dict(slots=torch.zeros(7, dtype=torch.int64)), ValueError, "slots"),
     (dict(cache_k=torch.zeros(5, 2, 16, 64)), TypeError, "cache_k"),
+    (dict(cache_v=torch.zeros(1, 2, 16, 64, dtype=H).expand(5, 2, 16, 64)), ValueError, "must not be expanded"),
     (dict(), RuntimeError, "CUDA device"),
 ])
 def test_rope_paged_cache_refusals(change, error, match):
@@ -123,6 +125,7 @@ def tables_args():
     (dict(free_pages=torch.zeros(4, dtype=torch.int64)), ValueError, "free_pages"),
     (dict(free_count=torch.zeros(2, dtype=torch.int32)), ValueError, "free_count"),
     (dict(block_size=17), ValueError, "power of two"),
+    (dict(block_table=torch.zeros(1, 3, dtype=torch.int32).expand(2, 3)), ValueError, "must not overlap"),
     (dict(max_tokens=-1), ValueError, "max_tokens"),
     (dict(), RuntimeError, "CUDA device"),
 ])
@@ -216,7 +219,8 @@ def test_rope_paged_cache_abi(change, match):
 
 @pytest.mark.parametrize("change,match", [
     (dict(slots=None), "non-null"), (dict(seqs=0), "seqs"), (dict(max_tokens=-1), "max_tokens"), (dict(block_size=0), "power of two"),
-    (dict(free_left=0x5000, free_count=0x5000), "must not be free_count"), (dict(seqs=(1 << 20) + 1), "up to"),
+    (dict(free_left=0x5000, free_count=0x5000), "must not be free_count"), (dict(seqs=(1 << 16) + 1), "up to"),
+    (dict(table_stride=2), "overlap"),
 ])
 def test_paged_tables_abi(change, match):
     _err(_lib.load().kf_paged_tables(ctypes.byref(_struct(_lib.PagedTablesArgs, **change)), None), match)

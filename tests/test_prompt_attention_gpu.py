@@ -144,3 +144,38 @@ def test_many_small_probabilities(dtype):
     k = k.contiguous() * 0.01
     k[0, 0, 0] = 8.0 * 1.29  # score 10.3: the others' probabilities are about 3.3e-5 of its
     against64([n], q, k, v, ops.prompt_attention(q, k, v, cu))
+
+
+def test_far_apart_tokens():
+    """Keys 128 MiB apart: offsets within a copy pass 31 bits, those of tokens 32."""
+    n, step = 33, 1 << 26
+    q, k, v, cu = make([n], 2, 1, 64, torch.float16)
+    want = ops.prompt_attention(q, k, v, cu)
+    big = torch.empty((n - 1) * step + 64, dtype=torch.float16, device=DEV)
+    far = big.as_strided((n, 1, 64), (step, 64, 1))
+    far.copy_(k)
+    assert torch.equal(ops.prompt_attention(q, far, v, cu), want)
+    far.copy_(v)
+    assert torch.equal(ops.prompt_attention(q, k, far, cu), want)
+    with pytest.raises(ValueError, match="token strides"):
+        big.resize_(0)
+        big = torch.empty((n - 1) * (step + 8) + 64, dtype=torch.float16, device=DEV)
+        ops.prompt_attention(q, big.as_strided((n, 1, 64), (step + 8, 64, 1)), v, cu)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (4, 2, 128), (4, 1, 256)])
+@pytest.mark.parametrize("lens", [[2000], [6000], [900, 1, 1700], [40] * 30 + [333] * 20, [1, 2500, 7, 0, 600]],
+                         ids=["groups", "cut", "few", "ordered", "uneven"])
+def test_every_plan(heads, kv_heads, d, lens):
+    """Row tiles whole, shared by two groups of wavefronts, cut over workgroups, and in the order of their lengths: prompts
+    of few and many row tiles, against 64 bits."""
+    q, k, v, cu = make(lens, heads, kv_heads, d, torch.bfloat16, pad=3)
+    out = ops.prompt_attention(q, k, v, cu)
+    against64(lens, q, k, v, out)
+    assert bool((out[sum(lens):] == 0).all())
+
+
+def test_registered_op():
+    q, k, v, cu = make([20, 9], 4, 2, 64, torch.float16)
+    torch.library.opcheck(ops._prompt_attention_op, (q, k, v, cu, 0.125), test_utils=("test_schema", "test_faketensor"))
+    assert torch.equal(torch.ops.kernelforge.prompt_attention(q, k, v, cu, 0.125), ops.prompt_attention(q, k, v, cu))
