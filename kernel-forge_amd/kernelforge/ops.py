@@ -961,7 +961,11 @@ def paged_tables(block_table: torch.Tensor, context_lens: torch.Tensor, new_lens
                 and block_table.stride(1) == 1 and (b == 1 or block_table.stride(0) >= width)
                 and context_lens.is_contiguous() and new_lens.is_contiguous()
                 and free_pages.is_contiguous() and 16 <= block_size <= 1 << 20 and not block_size & (block_size - 1)):
-            return PagedStep(*_run_paged_tables(*args))
+            cu_new, seq_lens, free_left = block_table.new_empty(2 * b + 2).split_with_sizes((b + 1, b, 1))
+            odd = max_tokens & 1  # slots start at 16 bytes as well
+            positions, _, slots = block_table.new_empty(2 * max_tokens + odd, dtype=torch.int64).split_with_sizes(
+                (max_tokens, odd, max_tokens))
+            return _run_paged_tables(*args, PagedStep(cu_new, seq_lens, positions, slots, free_left))
     b = block_table.shape[0] if block_table.dim() == 2 else -1
     _check_table(block_table, b)
     if b > 1 and block_table.stride(0) < block_table.shape[1]:
@@ -975,7 +979,7 @@ def paged_tables(block_table: torch.Tensor, context_lens: torch.Tensor, new_lens
     if b < 1 or max_tokens < 0:
         raise ValueError(f"paged_tables needs at least one request and max_tokens >= 0, got {b} and {max_tokens}")
     _check_plain("paged_tables", args[:5])
-    return PagedStep(*(_paged_tables_op(*args) if _traced(args[:5]) else _launch_paged_tables(*args)))
+    return PagedStep(*_paged_tables_op(*args)) if _traced(args[:5]) else _launch_paged_tables(*args)
 
 
 def _launch_paged_tables(block_table, context_lens, new_lens, free_pages, free_count, block_size, max_tokens):
@@ -983,34 +987,32 @@ def _launch_paged_tables(block_table, context_lens, new_lens, free_pages, free_c
     for name, t in (("block_table", block_table), ("context_lens", context_lens), ("new_lens", new_lens),
                     ("free_pages", free_pages), ("free_count", free_count)):
         _check_memory(name, t, dev)
+    b = block_table.shape[0]
+    step = PagedStep(block_table.new_empty(b + 1), block_table.new_empty(b),
+                     *(block_table.new_empty(max_tokens, dtype=torch.int64) for _ in range(2)), block_table.new_empty(1))
     with _on(dev):
-        return _run_paged_tables(block_table, context_lens, new_lens, free_pages, free_count, block_size, max_tokens)
+        return _run_paged_tables(block_table, context_lens, new_lens, free_pages, free_count, block_size, max_tokens, step)
 
 
-def _run_paged_tables(block_table, context_lens, new_lens, free_pages, free_count, block_size, max_tokens):
+def _run_paged_tables(block_table, context_lens, new_lens, free_pages, free_count, block_size, max_tokens, step):
     """kf_paged_tables on checked arguments of the current device."""
-    lib = _lib.load()
+    cu_new, seq_lens, positions, slots, free_left = step
     b, width = block_table.shape
-    cu_new = block_table.new_empty(b + 1)
-    seq_lens = block_table.new_empty(b)
-    free_left = block_table.new_empty(1)
-    positions = block_table.new_empty(max_tokens, dtype=torch.int64)
-    slots = torch.empty_like(positions)
-    args = _lib.PagedTablesArgs(_ptr(block_table), _ptr(context_lens), _ptr(new_lens), _ptr(free_pages),
-                                _ptr(free_count), _ptr(cu_new), _ptr(seq_lens), _ptr(positions), _ptr(slots),
-                                _ptr(free_left), block_table.stride(0), b, width, block_size, free_pages.numel(),
-                                max_tokens)
-    status = lib.kf_paged_tables(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(block_table.get_device()))
+    args = _lib.pack_paged_tables(block_table.data_ptr(), context_lens.data_ptr(), new_lens.data_ptr(),
+                                  free_pages.data_ptr(), free_count.data_ptr(), cu_new.data_ptr(), seq_lens.data_ptr(),
+                                  positions.data_ptr(), slots.data_ptr(), free_left.data_ptr(), block_table.stride(0), b,
+                                  width, block_size, free_pages.numel(), max_tokens)
+    status = _lib.load().kf_paged_tables(args, torch._C._cuda_getCurrentRawStream(block_table.get_device()))
     if status:
         _lib.check(status, "paged_tables")
-    return cu_new, seq_lens, positions, slots, free_left
+    return step
 
 
 @torch.library.custom_op("kernelforge::paged_tables", mutates_args=("block_table",))
 def _paged_tables_op(block_table: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor,
                      free_pages: torch.Tensor, free_count: torch.Tensor, block_size: int, max_tokens: int
                      ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _launch_paged_tables(block_table, context_lens, new_lens, free_pages, free_count, block_size, max_tokens)
+    return tuple(_launch_paged_tables(block_table, context_lens, new_lens, free_pages, free_count, block_size, max_tokens))
 
 
 @_paged_tables_op.register_fake
@@ -1086,11 +1088,13 @@ def _run_rope_paged(qkv, cos, sin, positions, slots, cache_k, cache_v, heads):
     """kf_rope_paged_cache on checked arguments of the current device."""
     pages, kv_heads, block_size, d = cache_k.shape
     qk = qkv.new_empty((qkv.shape[0], heads + kv_heads, d))
-    args = _lib.RopePagedArgs(_ptr(qkv), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(slots), _ptr(qk), _ptr(cache_k),
-                              _ptr(cache_v), qkv.stride(0), *cache_k.stride()[:3], *cache_v.stride()[:3], qkv.shape[0],
-                              heads, kv_heads, d, cos.shape[0], pages, block_size, _HALF_TYPES[qkv.dtype])
-    status = _lib.load().kf_rope_paged_cache(ctypes.byref(args),
-                                             torch._C._cuda_getCurrentRawStream(qkv.get_device()))
+    k_page, k_head, k_token, _ = cache_k.stride()
+    v_page, v_head, v_token, _ = cache_v.stride()
+    args = _lib.pack_rope_paged(qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+                                qk.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), qkv.stride(0), k_page, k_head,
+                                k_token, v_page, v_head, v_token, qkv.shape[0], heads, kv_heads, d, cos.shape[0], pages,
+                                block_size, _HALF_TYPES[qkv.dtype])
+    status = _lib.load().kf_rope_paged_cache(args, torch._C._cuda_getCurrentRawStream(qkv.get_device()))
     if status:
         _lib.check(status, "rope_paged_cache")
     return qk
@@ -1171,14 +1175,17 @@ def _launch_prompt(q, k, v, cu_seqlens, scale, out=None):
 def _run_prompt(q, k, v, cu_seqlens, scale, out, zero_rest):
     """kf_prompt_attention on checked arguments of the current device."""
     t, heads, d = q.shape
-    args = _lib.PromptAttentionArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(cu_seqlens), *q.stride()[:2],
-                                    *k.stride()[:2], *v.stride()[:2], *out.stride()[:2], t, cu_seqlens.numel() - 1, heads,
-                                    k.shape[1], d, _HALF_TYPES[q.dtype], scale, zero_rest)
+    q_token, q_head, _ = q.stride()
+    k_token, k_head, _ = k.stride()
+    v_token, v_head, _ = v.stride()
+    out_token, out_head, _ = out.stride()
+    args = _lib.pack_prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(),
+                                      q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head, t,
+                                      cu_seqlens.numel() - 1, heads, k.shape[1], d, _HALF_TYPES[q.dtype], scale, zero_rest)
     lib = _lib.load()
-    ref = ctypes.byref(args)
-    ws_bytes = lib.kf_prompt_attention_workspace_bytes(ref)
+    ws_bytes = lib.kf_prompt_attention_workspace_bytes(args)
     ws = q.new_empty((ws_bytes + 1) // 2) if ws_bytes else None  # two bytes a value
-    status = lib.kf_prompt_attention(ref, ws.data_ptr() if ws is not None else None, ws_bytes,
+    status = lib.kf_prompt_attention(args, ws.data_ptr() if ws is not None else None, ws_bytes,
                                      torch._C._cuda_getCurrentRawStream(q.get_device()))
     if status:
         _lib.check(status, "prompt_attention")
@@ -1268,15 +1275,19 @@ def _run_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scal
     """kf_paged_attention on checked arguments of the current device."""
     t, heads, d = q.shape
     pages, kv_heads, block_size, _ = cache_k.shape
-    args = _lib.PagedAttentionArgs(_ptr(q), _ptr(cache_k), _ptr(cache_v), _ptr(out), _ptr(block_table), _ptr(cu_new),
-                                   _ptr(seq_lens), *q.stride()[:2], *out.stride()[:2], *cache_k.stride()[:3],
-                                   *cache_v.stride()[:3], block_table.stride(0), t, seq_lens.numel(), heads, kv_heads, d,
-                                   _HALF_TYPES[q.dtype], block_table.shape[1], pages, block_size, max_new, scale, zero_rest)
+    q_token, q_head, _ = q.stride()
+    out_token, out_head, _ = out.stride()
+    k_page, k_head, k_token, _ = cache_k.stride()
+    v_page, v_head, v_token, _ = cache_v.stride()
+    args = _lib.pack_paged_attention(q.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), out.data_ptr(),
+                                     block_table.data_ptr(), cu_new.data_ptr(), seq_lens.data_ptr(), q_token, q_head,
+                                     out_token, out_head, k_page, k_head, k_token, v_page, v_head, v_token,
+                                     block_table.stride(0), t, seq_lens.numel(), heads, kv_heads, d, _HALF_TYPES[q.dtype],
+                                     block_table.shape[1], pages, block_size, max_new, scale, zero_rest)
     lib = _lib.load()
-    ref = ctypes.byref(args)
-    ws_bytes = lib.kf_paged_attention_workspace_bytes(ref)
+    ws_bytes = lib.kf_paged_attention_workspace_bytes(args)
     ws = q.new_empty((ws_bytes + 1) // 2) if ws_bytes else None  # two bytes a value
-    status = lib.kf_paged_attention(ref, ws.data_ptr() if ws is not None else None, ws_bytes,
+    status = lib.kf_paged_attention(args, ws.data_ptr() if ws is not None else None, ws_bytes,
                                     torch._C._cuda_getCurrentRawStream(q.get_device()))
     if status:
         _lib.check(status, "paged_attention")

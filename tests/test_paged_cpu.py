@@ -236,3 +236,16 @@ def test_null_arguments_and_empty_batches():
     assert lib.kf_paged_attention_workspace_bytes(None) == 0
     assert lib.kf_prompt_attention(ctypes.byref(_struct(_lib.PromptAttentionArgs, tokens=0, q=None)), None, 0, None) == 0
     assert lib.kf_rope_paged_cache(ctypes.byref(_struct(_lib.RopePagedArgs, tokens=0, qkv=None)), None) == 0
+
+
+@pytest.mark.parametrize("cls,pack", [
+    (_lib.PagedTablesArgs, _lib.pack_paged_tables), (_lib.RopePagedArgs, _lib.pack_rope_paged),
+    (_lib.PromptAttentionArgs, _lib.pack_prompt_attention), (_lib.PagedAttentionArgs, _lib.pack_paged_attention),
+])
+def test_packed_arguments_are_the_structure(cls, pack):
+    values = [0.375 if kind is ctypes.c_float else (1 << 40) + i if kind is not ctypes.c_int else i - 3
+              for i, (_, kind) in enumerate(cls._fields_)]
+    assert pack(*values) == bytes(cls(*values))
+    values[-1] = 1 << 32  # cut off in a structure
+    with pytest.raises(ValueError, match="more than one call takes"):
+        pack(*values)
