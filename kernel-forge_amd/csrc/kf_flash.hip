@@ -8,6 +8,15 @@
 // the inputs' type for the second matrix product (half a step of that type, as inputs are), the outputs once
 // more when they are stored.  The maximum that the exponentials are taken against follows the true one only when it is
 // exceeded by a factor 2^8: outputs and sums are then rescaled, which most tiles after the first spare.
+//
+// What bounds it: a tile of 64 keys costs a wavefront 16 (64 dims) or 32 (128 dims) matrix instructions of 32 cycles and
+// some 200 vector instructions for the softmax of its 32 x 64 scores, 32 of them exponentials at a quarter of the rate.
+// With 64 dims the two are alike: 16001 tokens of 32 heads take 1.09 ms, 960 TFLOP/s, vector pipe busy 81% of the time, matrix
+// cores 53%, no LDS bank conflicts, the clock down at 1.7 GHz.  With 128 dims the matrix cores lead: 8000 tokens of 32 heads take 0.49 ms,
+// 1070 TFLOP/s, of 1190 .. 1630 that matrix products of 4096 .. 16384 reach on the card.  Tried without gain: the next tile's
+// scores computed while a tile's exponentials are (0.50 .. 0.52 ms), tiles of 32 keys (0.49 ms; 16 ragged prompts 55 us, not 49).
+// A batch of a few hundred row tiles waits for its longest: 16 prompts of 19 .. 1455 tokens (12 heads on 2 of 128) take 49 us, of
+// which 25 are its work spread evenly.
 #include <math.h>
 
 #include "kf_attn_tiles.h"
@@ -195,6 +204,7 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
     // This wavefront's matrix products go before the other wavefronts' softmax: their results are waited for longest.
+    // (8000 tokens of 32 heads of 128: 507 -> 497 us; 64 dims and short prompts the same without.)
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int st = 0; st < ST; ++st)
@@ -596,6 +606,15 @@ hipError_t launch_dim(const AttnArgs& a, const FlashPlan& p, int min_rows, void*
 
 }  // namespace
 
+// How the row tiles are spread, by their number (`items`, from above) and the longest a sequence can be (`keys`).  The
+// kernel's time is at least its longest item's, so where there are few and they are long they are
+//   cut         into equal stretches that a second launch joins, where the CUs that would stay idle make up for writing and
+//               reading the pieces: 200 tokens over 60000 (8 KV heads of 128, 56 items) 1392 -> 285 us; but 2000 tokens of
+//               12 heads 35 -> 64, 16 ragged prompts 49 -> 79, a mixed batch 91 -> 102 us;
+//   shared      by two groups of four wavefronts, where they are hardly more than the CUs: 2000 tokens of 12 heads (192 items)
+//               45 -> 35 us, 4000 of 8 heads of 96 (250) 91 -> 70; but 16 ragged prompts (700) 49 -> 65, as eight wavefronts
+//               at one barrier overlap less than two workgroups do;
+//   longest first, where they do not all run at once: 16 ragged prompts 57 -> 49 us, a mixed batch 105 -> 91.
 FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count) {
   FlashPlan p;
   const int64_t rep = a.heads / a.kv_heads;

@@ -256,6 +256,7 @@ hipError_t flash_attention_launch(const AttnArgs& a, bool paged, bool bf16, cons
 // ---- attention of few rows per request over a paged cache (kf_paged_attn.hip) -----
 struct FewPlan {
   int row_tiles;       // 16-row tiles that share a pass over the keys
+  int waves;           // of a workgroup: 4, or 2 of which a CU holds two (one where head_dim > 128)
   bool cut;            // items may be cut, and a second launch joins them
   int grid;
   int64_t most_units;  // an upper bound of the kernel's work units: below 2^31

@@ -2,8 +2,10 @@
 //
 //   out[t, h] = sum_s softmax_s(scale q[t, h] . k[s, kv]) v[s, kv],   s <= position of t,   kv = h / rep
 //
-// What bounds it: the bytes of K and V, read once.  So the work of all requests is laid end to end, in units of 128
-// keys (64 for heads of more than 128) of one item (request, row tile, KV head), and cut into one equal stretch per workgroup
+// What bounds it: the bytes of K and V, read once.  Three requests of up to 131071 tokens (8 KV heads of 128) take 205 us, 6.3 TB/s
+// of the 7.1 that a plain read of the card reaches; 64 of 100 .. 8191 tokens (2 of 128), 112 MB, take 25.5 us, 15.8 of
+// them at that rate, the rest the second launch (6) and finding the stretches until the first keys are there.  So the work of all requests is laid end to end, in units of 32
+// keys a wavefront of one item (request, row tile, KV head), and cut into one equal stretch per workgroup
 // whatever the lengths are; a workgroup finds its stretch from the lengths by itself (they are read on the device only, so a captured launch
 // follows them).  The wavefronts of a workgroup take 32 keys each and do not wait for each other: each keeps its keys' tiles of K
 // and V coming through LDS buffers of its own by asynchronous copies, and they meet at the end of an item.
@@ -17,9 +19,14 @@
 namespace kf {
 namespace {
 
-template <int HDP, int MT>
+// Beginning and ending an item takes about as long as these many units: they count for it when the work is cut, or
+// workgroups with many short items would be the last ones.  With 0, 1, 2, 3: 39.6, 28.4, 25.6, 25.1 us for 64 requests of
+// 100 .. 8191 tokens (2 KV heads of 128), 58.6, 45.6, 41.7, 41.7 for 128 of 50 .. 900 (8 of 128, four wavefronts).
+constexpr int kFewItem = 2;
+
+template <int HDP, int MT, int WAVES_>
 struct FewConfig {
-  static constexpr int WAVES = HDP == 256 ? 2 : 4;
+  static constexpr int WAVES = WAVES_;
   static constexpr int THREADS = 64 * WAVES;
   static constexpr int STAGES = HDP == 64 ? 4 : 2;
   static constexpr int ROW = HDP * 2;
@@ -27,10 +34,7 @@ struct FewConfig {
   static constexpr int RING = STAGES * STAGE;        // of one wavefront
   static constexpr int ROWS = 16 * MT;
   static constexpr int UNIT = 32 * WAVES;            // keys
-  // Beginning and ending an item takes about as long as these many units: they count for it when the work is cut,
-  // or workgroups with many short items would be the last ones.
-  static constexpr int ITEM = 2;
-  static constexpr int LDS = WAVES * RING;           // 128 KiB, of which half or more is on its way
+  static constexpr int LDS = WAVES * RING;           // 32 KiB a wavefront, of which half or more is on its way
   static_assert(WAVES * ROWS * HDP * 4 <= LDS, "the wavefronts' sums meet in the buffers");
 };
 
@@ -47,7 +51,7 @@ __device__ __forceinline__ int few_items(const AttnArgs& a, int s, int rep, int 
 }
 template <class C, bool CUT>
 __device__ __forceinline__ int item_cost(int key_units) {
-  return CUT ? key_units + C::ITEM : 1;
+  return CUT ? key_units + kFewItem : 1;
 }
 
 __device__ __forceinline__ float max_groups(float v) {  // of lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -60,11 +64,11 @@ __device__ __forceinline__ float add_groups(float v) {
 }
 
 // CUT: items may be cut; otherwise every workgroup takes whole ones, and nothing is left to join.
-template <class E, int HDP, int MT, bool CUT>
-__global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel(AttnArgs args, int rep, int max_rows,
+template <class E, int HDP, int MT, int WAVES, bool CUT>
+__global__ __launch_bounds__((FewConfig<HDP, MT, WAVES>::THREADS)) void few_rows_kernel(AttnArgs args, int rep, int max_rows,
                                                                                  float scale_log2, float* ws,
                                                                                  Piece* pieces) {
-  using C = FewConfig<HDP, MT>;
+  using C = FewConfig<HDP, MT, WAVES>;
   using Copy = TileCopy<E, HDP, true>;
   constexpr int PER_STAGE = 4 * Copy::N, ROW = C::ROW;  // copy instructions of a stage
   constexpr int ST = HDP / 32, DT = HDP / 16;
@@ -151,7 +155,7 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
     }
     const int cost = item_cost<C, CUT>(ku), item = (at - seq_at) / cost, item_at = seq_at + item * cost;
     // The stretch's part of the item; of what it counts, the beginning comes first.
-    const int first_unit = item_at + (CUT ? C::ITEM : 0);
+    const int first_unit = item_at + (CUT ? kFewItem : 0);
     const int u0 = CUT ? max(at - first_unit, 0) : 0, u1 = CUT ? min(ku, end - first_unit) : ku;
     at = item_at + cost;
     if (u1 <= u0) break;  // not even its first unit
@@ -366,37 +370,42 @@ __global__ __launch_bounds__((FewConfig<HDP, MT>::THREADS)) void few_rows_kernel
   }
 }
 
-template <class E, int HDP, int MT>
-hipError_t launch(const AttnArgs& a, int max_rows, bool cut, int grid, void* ws, hipStream_t stream) {
-  using C = FewConfig<HDP, MT>;
+template <class E, int HDP, int MT, int WAVES>
+hipError_t launch(const AttnArgs& a, const FewPlan& p, int max_rows, void* ws, hipStream_t stream) {
+  using C = FewConfig<HDP, MT, WAVES>;
   const int rep = a.heads / a.kv_heads;
   const float scale_log2 = a.scale * 1.44269504088896340736f;
-  if (!cut) {
-    few_rows_kernel<E, HDP, MT, false><<<grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, nullptr, nullptr);
+  if (!p.cut) {
+    few_rows_kernel<E, HDP, MT, WAVES, false><<<p.grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, nullptr, nullptr);
     return hipGetLastError();
   }
   float* const parts = static_cast<float*>(ws);
-  Piece* const pieces = reinterpret_cast<Piece*>(parts + (size_t)2 * grid * C::ROWS * (HDP + 2));
-  few_rows_kernel<E, HDP, MT, true><<<grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, parts, pieces);
+  Piece* const pieces = reinterpret_cast<Piece*>(parts + (size_t)2 * p.grid * C::ROWS * (HDP + 2));
+  few_rows_kernel<E, HDP, MT, WAVES, true><<<p.grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, parts, pieces);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  join_pieces_kernel<E, HDP, C::ROWS><<<dim3(grid, MT), 256, 0, stream>>>(a, rep, parts, pieces);
+  join_pieces_kernel<E, HDP, C::ROWS><<<dim3(p.grid, MT), 256, 0, stream>>>(a, rep, parts, pieces);
   return hipGetLastError();
 }
 
 template <class E, int HDP>
-hipError_t launch_rows(const AttnArgs& a, int row_tiles, int max_rows, bool cut, int grid, void* ws, hipStream_t stream) {
-  if constexpr (HDP != 256) {  // one row tile of 256 dims fills the registers
-    if (row_tiles == 2) return launch<E, HDP, 2>(a, max_rows, cut, grid, ws, stream);
+hipError_t launch_rows(const AttnArgs& a, const FewPlan& p, int max_rows, void* ws, hipStream_t stream) {
+  if constexpr (HDP == 256) {  // one row tile of 256 dims fills the registers, two wavefronts the buffers
+    return launch<E, HDP, 1, 2>(a, p, max_rows, ws, stream);
+  } else {
+    if (p.waves == 2)
+      return p.row_tiles == 2 ? launch<E, HDP, 2, 2>(a, p, max_rows, ws, stream)
+                              : launch<E, HDP, 1, 2>(a, p, max_rows, ws, stream);
+    return p.row_tiles == 2 ? launch<E, HDP, 2, 4>(a, p, max_rows, ws, stream)
+                            : launch<E, HDP, 1, 4>(a, p, max_rows, ws, stream);
   }
-  return launch<E, HDP, 1>(a, max_rows, cut, grid, ws, stream);
 }
 
 template <class E>
-hipError_t launch_dim(const AttnArgs& a, int row_tiles, int max_rows, bool cut, int grid, void* ws, hipStream_t stream) {
-  if (a.head_dim <= 64) return launch_rows<E, 64>(a, row_tiles, max_rows, cut, grid, ws, stream);
-  if (a.head_dim <= 128) return launch_rows<E, 128>(a, row_tiles, max_rows, cut, grid, ws, stream);
-  return launch_rows<E, 256>(a, row_tiles, max_rows, cut, grid, ws, stream);
+hipError_t launch_dim(const AttnArgs& a, const FewPlan& p, int max_rows, void* ws, hipStream_t stream) {
+  if (a.head_dim <= 64) return launch_rows<E, 64>(a, p, max_rows, ws, stream);
+  if (a.head_dim <= 128) return launch_rows<E, 128>(a, p, max_rows, ws, stream);
+  return launch_rows<E, 256>(a, p, max_rows, ws, stream);
 }
 
 }  // namespace
@@ -404,13 +413,20 @@ hipError_t launch_dim(const AttnArgs& a, int row_tiles, int max_rows, bool cut, 
 FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int cu_count) {
   FewPlan p;
   p.row_tiles = a.head_dim <= 128 && rows > 16 ? 2 : 1;
-  const int unit = a.head_dim <= 128 ? FewConfig<128, 1>::UNIT : FewConfig<256, 1>::UNIT;
-  const int64_t key_units = (((int64_t)a.table_width << a.log2_block) + unit - 1) / unit;
   const int64_t items = ((int64_t)a.tokens * (a.heads / a.kv_heads) / (16 * p.row_tiles) + a.seqs) * a.kv_heads;
-  // Tables of up to 512 keys are worked off faster than a second launch begins.
+  const int64_t keys = (int64_t)a.table_width << a.log2_block;
+  // A CU holds one workgroup of four wavefronts or two of two, one of which then copies while the other begins or ends an
+  // item.  That pays where there are an item or more for each CU and they are short; otherwise the second
+  // workgroup's pieces only cost.  Four / two, us: 128 requests of up to 700 tokens, 8 KV heads of 128, 44 / 35, of
+  // up to 2000 82 / 85, 4 heads of 64 34 / 30, of up to 6000 66 / 66; 16 of up to 700, 4 of 64, 11.5 / 12.5.
+  p.waves = a.head_dim > 128 || (items >= cu_count && keys * (a.head_dim <= 64 ? 64 : 128) <= 1 << 17) ? 2 : 4;
+  const int unit = 32 * p.waves, fits = (a.head_dim <= 128 && p.waves == 2 ? 2 : 1) * cu_count;
+  const int64_t key_units = (keys + unit - 1) / unit;
+  // Up to 512 keys are worked off whole, without the second launch.  Whole / cut, us: 16 requests of up to 450 tokens 8.7 / 11.2,
+  // of up to 900 11.3 / 11.8, of up to 1900 17.2 / 12.8; one of 900 15.6 / 11.5.
   p.cut = key_units * unit > 512;
-  p.most_units = items * (key_units + FewConfig<128, 1>::ITEM);
-  p.grid = (int)std::min<int64_t>(cu_count, p.cut ? p.most_units : items);
+  p.most_units = items * (key_units + kFewItem);
+  p.grid = (int)std::min<int64_t>(fits, p.cut ? p.most_units : items);
   return p;
 }
 
@@ -421,8 +437,7 @@ size_t few_rows_workspace_bytes(int head_dim, const FewPlan& p) {
 }
 
 hipError_t few_rows_launch(const AttnArgs& a, bool bf16, const FewPlan& p, int max_rows, void* ws, hipStream_t stream) {
-  return bf16 ? launch_dim<bhalf_t>(a, p.row_tiles, max_rows, p.cut, p.grid, ws, stream)
-              : launch_dim<half_t>(a, p.row_tiles, max_rows, p.cut, p.grid, ws, stream);
+  return bf16 ? launch_dim<bhalf_t>(a, p, max_rows, ws, stream) : launch_dim<half_t>(a, p, max_rows, ws, stream);
 }
 
 }  // namespace kf

@@ -211,6 +211,21 @@ def test_every_plan(heads, kv_heads, d, ctx, new):
     b.check(b(max_new=max(new)))
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(32, 8, 64), (16, 8, 128), (8, 8, 96)])
+@pytest.mark.parametrize("longest,new", [(15, 1), (500, 1), (980, 1), (980, 9)])
+def test_many_short_requests(heads, kv_heads, d, longest, new):
+    """An item or more for each of a few hundred CUs: whole ones and cut ones, one and two row tiles, pages missing."""
+    count = 41
+    b = Batch([(i * 37 * longest // 600) % longest if i % 9 else 0 for i in range(count)],
+              [0 if i == 7 else 1 + i * 5 % new for i in range(count)], heads, kv_heads, d, torch.float16, 16, pad=1)
+    lens = b.seq_lens.tolist()
+    there = [torch.ones(n, dtype=torch.bool, device=DEV) for n in lens]
+    long = max(range(count), key=lens.__getitem__)
+    b.table[long, 0] = -1
+    there[long][:16] = False
+    b.check(b(max_new=new), there)
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_holes_and_infinities_in_cut_items(bad):
     """A long item in pieces: a page that is missing in the middle, and values beyond a row's last key."""
