@@ -252,11 +252,28 @@ int paged_plan(const kf_paged_attention_args& a, PagedPlan* p) {
   return KF_OK;
 }
 
-size_t paged_workspace(const PagedPlan& p, int cus) {
-  size_t need = 0;
-  if (p.few) need = kf::few_rows_workspace_bytes(p.args.head_dim, kf::few_rows_plan(p.args, p.rows, cus));
-  if (p.many) need = std::max(need, kf::flash_workspace_bytes(p.args.head_dim, kf::flash_plan(p.args, true, cus)));
-  return need;
+struct PagedLaunches {
+  kf::FewPlan few;
+  kf::FlashPlan many;
+  bool together;  // one launch for both kinds of requests
+  size_t workspace;
+};
+PagedLaunches paged_launches(const PagedPlan& p, int cus) {
+  PagedLaunches l = {};
+  if (p.many) l.many = kf::flash_plan(p.args, true, cus);
+  if (p.few) {
+    // Where the row tiles are more than the CUs, and the others are cut.
+    l.together = p.many && !l.many.cut && l.many.groups == 1 && l.many.grid < 1 << 30 && p.args.head_dim <= 128;
+    if (l.together) {
+      l.few = kf::few_rows_plan(p.args, p.rows, cus, true);
+      l.together = l.few.cut;
+    }
+    if (!l.together) l.few = kf::few_rows_plan(p.args, p.rows, cus, false);
+    l.workspace = kf::few_rows_workspace_bytes(p.args.head_dim, l.few);
+  }
+  // Launches that follow each other on the stream share the workspace.
+  if (p.many) l.workspace = std::max(l.workspace, kf::flash_workspace_bytes(p.args.head_dim, l.many));
+  return l;
 }
 
 int check_workspace(const void* ws, size_t have, size_t need) {
@@ -756,7 +773,7 @@ size_t kf_paged_attention_workspace_bytes(const kf_paged_attention_args* a) {
   PagedPlan p;
   int cus;
   if (!a || paged_plan(*a, &p) || cu_count(&cus)) return 0;
-  return paged_workspace(p, cus);
+  return paged_launches(p, cus).workspace;
 }
 
 int kf_paged_attention(const kf_paged_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -775,22 +792,24 @@ int kf_paged_attention(const kf_paged_attention_args* a, void* ws, size_t ws_byt
   const bool bf16 = a->dtype == KF_DTYPE_BF16;
   int cus;
   if (int st = cu_count(&cus)) return st;
-  // The two launches follow each other on the stream: they share the workspace.
-  if (int st = check_workspace(ws, ws_bytes, paged_workspace(p, cus))) return st;
+  const PagedLaunches l = paged_launches(p, cus);
+  if (int st = check_workspace(ws, ws_bytes, l.workspace)) return st;
+  if (p.few && l.few.most_units >= (int64_t)1 << 31)
+    return fail(KF_ERR_UNSUPPORTED, "%d tokens over tables of %d pages are more than one launch takes", a->tokens,
+                a->table_width);
+  if (l.together)
+    return hip_status(kf::mixed_attention_launch(p.args, bf16, l.few, l.many, kFewRows, ws, static_cast<hipStream_t>(stream)),
+                      "paged_attention launch");
   if (p.few) {
-    const kf::FewPlan plan = kf::few_rows_plan(p.args, p.rows, cus);
-    if (plan.most_units >= (int64_t)1 << 31)
-      return fail(KF_ERR_UNSUPPORTED, "%d tokens over tables of %d pages are more than one launch takes", a->tokens,
-                  a->table_width);
     const int max_rows = p.many ? kFewRows : 0x7fffffff;
-    if (int st = hip_status(kf::few_rows_launch(p.args, bf16, plan, max_rows, ws, static_cast<hipStream_t>(stream)),
+    if (int st = hip_status(kf::few_rows_launch(p.args, bf16, l.few, max_rows, ws, static_cast<hipStream_t>(stream)),
                             "paged_attention launch"))
       return st;
   }
   if (p.many) {
     kf::AttnArgs t = p.args;
     if (p.few) t.zero_rest = 0;  // done
-    return hip_status(kf::flash_attention_launch(t, true, bf16, kf::flash_plan(t, true, cus), p.few ? kFewRows + 1 : 0, ws,
+    return hip_status(kf::flash_attention_launch(t, true, bf16, l.many, p.few ? kFewRows + 1 : 0, ws,
                                                  static_cast<hipStream_t>(stream)),
                       "paged_attention launch");
   }

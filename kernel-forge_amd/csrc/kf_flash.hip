@@ -19,7 +19,7 @@
 // which 25 are its work spread evenly.
 #include <math.h>
 
-#include "kf_attn_tiles.h"
+#include "kf_few_rows.h"
 #include "kf_launch.h"
 
 namespace kf {
@@ -428,13 +428,12 @@ __device__ __forceinline__ bool longest_tile(const AttnArgs& a, int rep, int min
   return true;
 }
 
-// One workgroup per row tile and KV head.
+// One workgroup per row tile and KV head: `block` of `blocks`.
 template <class E, int HDP, bool PAGED, int GROUPS>
-__global__ __launch_bounds__(GROUPS * kFlashThreads, flash_waves_per_simd(HDP, GROUPS > 1)) void flash_attention_kernel(
-    AttnArgs a, int rep, int min_rows, int longest_first, float scale_log2) {
-  __shared__ FlashShared<HDP, GROUPS> sh;
-  const int kv = blockIdx.x % a.kv_heads;
-  const int numbers = (int)(gridDim.x / a.kv_heads), number = (int)(blockIdx.x / a.kv_heads);
+__device__ __forceinline__ void flash_block(const AttnArgs& a, FlashShared<HDP, GROUPS>& sh, unsigned block, unsigned blocks,
+                                            int rep, int min_rows, int longest_first, float scale_log2) {
+  const int kv = (int)(block % a.kv_heads);
+  const int numbers = (int)(blocks / a.kv_heads), number = (int)(block / a.kv_heads);
   int seq, tile, total;
   if (longest_first) {
     if (!longest_tile<PAGED>(a, rep, min_rows, number, threadIdx.x & 63, &seq, &tile, &total)) {
@@ -461,6 +460,41 @@ __global__ __launch_bounds__(GROUPS * kFlashThreads, flash_waves_per_simd(HDP, G
   }
   const int row0 = tile * kFlashRows;
   flash_item<E, HDP, PAGED, GROUPS>(a, sh, rep, scale_log2, seq, row0, kv, 0, 0x7fffffff / FlashConfig<HDP>::KEYS, nullptr);
+}
+
+template <class E, int HDP, bool PAGED, int GROUPS>
+__global__ __launch_bounds__(GROUPS * kFlashThreads, flash_waves_per_simd(HDP, GROUPS > 1)) void flash_attention_kernel(
+    AttnArgs a, int rep, int min_rows, int longest_first, float scale_log2) {
+  __shared__ FlashShared<HDP, GROUPS> sh;
+  flash_block<E, HDP, PAGED, GROUPS>(a, sh, blockIdx.x, gridDim.x, rep, min_rows, longest_first, scale_log2);
+}
+
+// A batch of both kinds of requests in one launch: the first few_grid workgroups, of which two wavefronts work, take the
+// requests of at most few_rows rows (kf_few_rows.h), the others the row tiles of the rest.  The ones wait for memory
+// and the others for the matrix cores, and a CU holds some of each.  24 requests of 1 .. 700 tokens over 30 .. 4000 (8 KV heads of
+// 128) take 73 us, in two launches 91; 4 heads of 64 61 (73); 64 of 1 .. 200 over 500 .. 8000 216 (252).
+template <int HDP>
+using MixedFew = FewConfig<HDP, 2, 2, 2>;  // 64 dims: half the buffers, so that a CU holds four workgroups as without it
+template <int HDP>
+union MixedShared {
+  FewShared<MixedFew<HDP>> few;
+  FlashShared<HDP, 1> many;
+};
+template <class E, int HDP>
+__global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, false)) void mixed_attention_kernel(AttnArgs a, int rep, int few_rows, int few_grid,
+                                                                           int longest_first, float scale_log2, float* ws,
+                                                                           Piece* pieces) {
+  __shared__ MixedShared<HDP> sh;
+  if ((int)blockIdx.x < few_grid) {  // zeros the rows behind the last request too
+    if (threadIdx.x >= MixedFew<HDP>::THREADS) return;
+    few_rows_stretch<E, MixedFew<HDP>, true>(a, sh.few, (int)blockIdx.x, few_grid, rep, few_rows, scale_log2,
+                                         ws, pieces);
+  } else {
+    AttnArgs b = a;
+    b.zero_rest = 0;
+    flash_block<E, HDP, true, 1>(b, sh.many, blockIdx.x - few_grid, gridDim.x - few_grid, rep,
+                                 few_rows + 1, longest_first, scale_log2);
+  }
 }
 
 // Fewer row tiles than workgroups that the GPU holds, or tiles of very different length: the work of all is laid end to
@@ -597,6 +631,22 @@ hipError_t launch(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws,
   return hipGetLastError();
 }
 
+template <class E, int HDP>
+hipError_t launch_mixed(const AttnArgs& a, const FewPlan& f, const FlashPlan& p, int few_rows, void* ws, hipStream_t stream) {
+  const int rep = a.heads / a.kv_heads;
+  const float scale_log2 = a.scale * 1.44269504088896340736f;
+  float* const parts = static_cast<float*>(ws);
+  Piece* const pieces = reinterpret_cast<Piece*>(parts + (size_t)2 * f.grid * 32 * (HDP + 2));
+  constexpr int OWN = sizeof(MixedShared<HDP>);
+  const size_t more_lds = p.lds > OWN ? p.lds - OWN : 0;
+  mixed_attention_kernel<E, HDP><<<f.grid + p.grid, kFlashThreads, more_lds, stream>>>(
+      a, rep, few_rows, f.grid, p.longest_first, scale_log2, parts, pieces);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  join_pieces_kernel<E, HDP, 32><<<dim3(f.grid, 2), 256, 0, stream>>>(a, rep, parts, pieces);
+  return hipGetLastError();
+}
+
 template <class E, bool PAGED>
 hipError_t launch_dim(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws, hipStream_t stream) {
   if (a.head_dim <= 64) return launch<E, 64, PAGED>(a, p, min_rows, ws, stream);
@@ -614,7 +664,11 @@ hipError_t launch_dim(const AttnArgs& a, const FlashPlan& p, int min_rows, void*
 //   shared      by two groups of four wavefronts, where they are hardly more than the CUs: 2000 tokens of 12 heads (192 items)
 //               45 -> 35 us, 4000 of 8 heads of 96 (250) 91 -> 70; but 16 ragged prompts (700) 49 -> 65, as eight wavefronts
 //               at one barrier overlap less than two workgroups do;
-//   longest first, where they do not all run at once: 16 ragged prompts 57 -> 49 us, a mixed batch 105 -> 91.
+//   longest first, where they do not all run at once: 16 ragged prompts 57 -> 49 us, a mixed batch 105 -> 91;
+//   kept apart, in a launch for both kinds of requests, where a CU could hold more of them (four, of up to 64 dims) than there are
+//               for each: they are not dealt out evenly by themselves.  Two up to 5/2 of the CUs, three up to 3: 4 requests'
+//               512 tokens over 4000 (4 KV heads of 64, 512 items) 126 -> 111 us, a mixed batch 65 -> 61; single prompts
+//               (500 .. 1000 items) within 1% either way, so they go without.
 FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count) {
   FlashPlan p;
   const int64_t rep = a.heads / a.kv_heads;
@@ -627,6 +681,7 @@ FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count) {
   p.groups = 4 * items <= 5 * cu_count && keys > 256 ? flash_groups(hdp) : 1;
   // One sequence has its longest tiles last in any case, and workgroups that all run at once need no order.
   p.longest_first = a.seqs > 1 && a.seqs <= 64 && items * p.groups > cu_count * flash_waves_per_simd(hdp, false);
+  p.lds = hdp > 64 ? 0 : 2 * items <= 5 * cu_count ? 54 << 10 : items <= 3 * cu_count ? 41 << 10 : 0;
   p.grid = p.cut ? cu_count * flash_waves_per_simd(hdp, true) : (int)items;
   return p;
 }
@@ -641,6 +696,13 @@ hipError_t flash_attention_launch(const AttnArgs& a, bool paged, bool bf16, cons
                                   hipStream_t stream) {
   if (paged) return bf16 ? launch_dim<bhalf_t, true>(a, p, min_rows, ws, stream) : launch_dim<half_t, true>(a, p, min_rows, ws, stream);
   return bf16 ? launch_dim<bhalf_t, false>(a, p, min_rows, ws, stream) : launch_dim<half_t, false>(a, p, min_rows, ws, stream);
+}
+
+hipError_t mixed_attention_launch(const AttnArgs& a, bool bf16, const FewPlan& f, const FlashPlan& p, int few_rows, void* ws,
+                                  hipStream_t stream) {
+  if (a.head_dim <= 64)
+    return bf16 ? launch_mixed<bhalf_t, 64>(a, f, p, few_rows, ws, stream) : launch_mixed<half_t, 64>(a, f, p, few_rows, ws, stream);
+  return bf16 ? launch_mixed<bhalf_t, 128>(a, f, p, few_rows, ws, stream) : launch_mixed<half_t, 128>(a, f, p, few_rows, ws, stream);
 }
 
 }  // namespace kf

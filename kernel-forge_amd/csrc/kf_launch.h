@@ -245,6 +245,7 @@ struct FlashPlan {
   bool cut;    // the work of all row tiles is cut into equal stretches, and a second launch joins what was cut
   int groups;  // of four wavefronts that share a row tile's keys
   bool longest_first;  // row tiles start in the order of their lengths
+  int lds;             // mixed_attention_launch: bytes that a workgroup takes at least, so that a CU holds no more than it should
   int grid;
 };
 FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count);
@@ -261,11 +262,15 @@ struct FewPlan {
   int grid;
   int64_t most_units;  // an upper bound of the kernel's work units: below 2^31
 };
-// rows: (token, query head of a group) rows of a request, at most.
-FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int cu_count);
+// rows: (token, query head of a group) rows of a request, at most.  beside: for mixed_attention_launch.
+FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int cu_count, bool beside);
 size_t few_rows_workspace_bytes(int head_dim, const FewPlan& p);
 // Requests of more than max_rows rows are left to the other kernel.  ws: few_rows_workspace_bytes, 16-byte aligned.
 hipError_t few_rows_launch(const AttnArgs& a, bool bf16, const FewPlan& p, int max_rows, void* ws, hipStream_t stream);
+// Requests of at most few_rows rows by the plan f and the others by p, in one launch; then what f cut is joined.  f: with
+// `beside` and cut, head_dim <= 128; p: neither cut nor in groups.  ws: f's.
+hipError_t mixed_attention_launch(const AttnArgs& a, bool bf16, const FewPlan& f, const FlashPlan& p, int few_rows, void* ws,
+                                  hipStream_t stream);
 
 // ---- the paged cache's tables and writer (kf_paged.hip) -----------------------
 struct TablesArgs {

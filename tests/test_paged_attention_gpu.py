@@ -226,6 +226,50 @@ def test_many_short_requests(heads, kv_heads, d, longest, new):
     b.check(b(max_new=new), there)
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(32, 4, 64), (32, 8, 128), (16, 16, 96)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+def test_chunks_beside_single_tokens(heads, kv_heads, d, dtype):
+    """Many row tiles of chunks, and single tokens over long contexts, in one launch: the rows at which a request goes to the
+    other kind of workgroups, empty requests, pages that are missing in either kind, infinities behind a row's last key."""
+    rep = heads // kv_heads
+    edge = 64 // rep
+    ctx = [0, 2900, 40, 700, 1300, 0, 16, 511, 1024, 5, 1900, 64]
+    new = [300, 1, edge, edge + 1, 400, 0, 250, 1, 129, 2, 1, 333]
+    b = Batch(ctx, new, heads, kv_heads, d, dtype, 16, pad=3)
+    there = [torch.ones(c + n, dtype=torch.bool, device=DEV) for c, n in zip(ctx, new)]
+    for r, page in ((1, 100), (4, 7), (8, 65)):
+        b.table[r, page] = -1
+        there[r][16 * page:16 * page + 16] = False
+    out = b(max_new=400)
+    b.check(out, there)
+    assert torch.equal(out, b())
+    last = ctx[4] + new[4] - 1
+    b.cache_v[b.table[4, last // 16].long(), 0, last % 16, 3] = float("inf")
+    got = b()
+    row = sum(new[:5]) - 1
+    assert bool((got[row, :rep, 3] == float("inf")).all())
+    got[row, :rep, 3] = out[row, :rep, 3]
+    assert torch.equal(got, out)
+
+
+def test_chunks_beside_single_tokens_in_a_graph():
+    """One captured call, whose requests change from chunks to single tokens and back between replays."""
+    b = Batch([700] * 16, [90] * 16, 32, 8, 128, torch.float16, 16)
+    b()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = b()
+    for new in ([90] * 16, [1] * 16, [1, 179] * 8, [0] * 15 + [1440]):
+        b.cu.copy_(offsets(new, DEV))
+        b.seq_lens.copy_(torch.tensor([max(n, 790 - n) for n in new], dtype=torch.int32))
+        want = b()
+        junk = torch.randn(1 << 20, device=DEV).sum()
+        graph.replay()
+        torch.cuda.synchronize()
+        # Bits: the last request's keys go on into a page's unused slots, which hold NaN.
+        assert torch.equal(out.view(torch.int16), want.view(torch.int16)) and bool(junk.isfinite())
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_holes_and_infinities_in_cut_items(bad):
     """A long item in pieces: a page that is missing in the middle, and values beyond a row's last key."""
