@@ -316,36 +316,84 @@ struct Piece {
 __device__ __forceinline__ float scaled(float x, float f) { return fabsf(x) < __builtin_inff() ? f * x : x; }
 
 namespace {
-// Joins the pieces of the items that workgroup blockIdx.x of the first launch began and did not end.
+// Joins the pieces of the items that workgroup blockIdx.x of the first launch began and did not end.  A long item can have
+// hundreds, which is what takes the time: the wavefronts of a workgroup take every kJoinWaves-th piece of the same 64 x 4 values,
+// kJoinAhead of them loaded at once, and the workgroups in y share an item's values, 32 at most: 8 requests of 1 .. 12 tokens over
+// up to 32000 (2 KV heads of 128) take 79 us in all, with 16 workgroups 87, with 8 107; 64 single tokens 25.4 either way.
+constexpr int kJoinWaves = 4, kJoinAhead = 8;
+template <int HDP, int ROWS>
+constexpr int join_blocks() { return ROWS * HDP / 256 < 32 ? ROWS * HDP / 256 : 32; }
+
 template <class E, int HDP, int ROWS>
-__global__ __launch_bounds__(256) void join_pieces_kernel(AttnArgs a, int rep, const float* ws, const Piece* pieces) {
+__global__ __launch_bounds__(64 * kJoinWaves) void join_pieces_kernel(AttnArgs a, int rep, const float* ws, const Piece* pieces) {
+  __shared__ float stat[2][kJoinWaves][64];
+  __shared__ float4_t parts[kJoinWaves][64];
   const Piece pc = pieces[blockIdx.x];
   if (pc.seq < 0) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tok0 = seq_offset(a.cu, pc.seq, a.seqs, a.tokens);
   const int rows = (seq_offset(a.cu, pc.seq + 1, a.seqs, a.tokens) - tok0) * rep;
   const int live_rows = min(rows - pc.row0, ROWS);
   constexpr int STRIDE = ROWS * (HDP + 2);
   const int first = blockIdx.x;
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < live_rows * (HDP / 4); i += 256 * gridDim.y) {
+  for (int i0 = blockIdx.y * 64; i0 < live_rows * (HDP / 4); i0 += 64 * gridDim.y) {
+    const int i = min(i0 + lane, live_rows * (HDP / 4) - 1);
     const int r = i / (HDP / 4), d = 4 * (i % (HDP / 4));
-    auto part = [&](int w) { return ws + (size_t)(2 * w + (w == first ? 1 : 0)) * STRIDE; };
     float top = -__builtin_inff(), l = 0.0f;
-#pragma unroll 4
-    for (int w = first; w <= pc.last; ++w) top = fmaxf(top, part(w)[ROWS * HDP + r]);
     float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int w = first; w <= pc.last; ++w) {
-      const float* const p = part(w);
-      const float mw = p[ROWS * HDP + r], lw = p[ROWS * HDP + ROWS + r];
-      const float4_t x = *reinterpret_cast<const float4_t*>(p + r * HDP + d);
-      const float f = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
-      l += lw != lw ? lw : f * lw;  // a NaN among a piece's scores is in its sum, whatever its maximum says
+    // A factor for a maximum against a higher one; a piece without keys has none (0, not exp2(-inf - -inf)).
+    auto factor = [](float m, float high) { return m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - high); };
+    // A NaN among a piece's scores is in its sum, whatever its maximum says.
+    auto sum = [](float l, float f) { return l != l ? l : f * l; };
+    for (int w0 = first + wave; w0 <= pc.last; w0 += kJoinWaves * kJoinAhead) {
+      float m[kJoinAhead], lw[kJoinAhead];
+      float4_t x[kJoinAhead];
+      float high = top;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += scaled(x[e], f);
+      for (int j = 0; j < kJoinAhead; ++j) {
+        const int w = min(w0 + kJoinWaves * j, pc.last);
+        const float* const p = ws + (size_t)(2 * w + (w == first ? 1 : 0)) * STRIDE;
+        m[j] = p[ROWS * HDP + r];
+        lw[j] = p[ROWS * HDP + ROWS + r];
+        x[j] = *reinterpret_cast<const float4_t*>(p + r * HDP + d);
+      }
+#pragma unroll
+      for (int j = 0; j < kJoinAhead; ++j)
+        if (w0 + kJoinWaves * j <= pc.last) high = fmaxf(high, m[j]);
+      const float old = factor(top, high);
+      l = sum(l, old);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = scaled(v[e], old);
+#pragma unroll
+      for (int j = 0; j < kJoinAhead; ++j) {
+        if (w0 + kJoinWaves * j > pc.last) break;
+        const float f = factor(m[j], high);
+        l += sum(lw[j], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += scaled(x[j][e], f);
+      }
+      top = high;
+    }
+    __syncthreads();  // the last values have been read
+    stat[0][wave][lane] = top;
+    stat[1][wave][lane] = l;
+    parts[wave][lane] = v;
+    __syncthreads();
+    if (wave != 0) continue;
+#pragma unroll
+    for (int w = 1; w < kJoinWaves; ++w) top = fmaxf(top, stat[0][w][lane]);
+    l = 0.0f;
+    v = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) {
+      const float f = factor(stat[0][w][lane], top);
+      l += sum(stat[1][w][lane], f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += scaled(parts[w][lane][e], f);
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int row = pc.row0 + r, tok = row / rep, head = pc.kv * rep + (row - tok * rep);
-    if (d < a.head_dim)
+    if (d < a.head_dim && i0 + lane < live_rows * (HDP / 4))
       store_global((E*)a.out + (size_t)(tok0 + tok) * a.out_token + (size_t)head * a.out_head + d,
                    u32x2{Elem<E>::pack(v[0] * inv, v[1] * inv), Elem<E>::pack(v[2] * inv, v[3] * inv)});
   }

@@ -627,7 +627,7 @@ hipError_t launch(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws,
   flash_cut_kernel<E, HDP, PAGED><<<p.grid, kFlashThreads, 0, stream>>>(c);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  join_pieces_kernel<E, HDP, kFlashRows><<<dim3(p.grid, 4), 256, 0, stream>>>(a, rep, parts, pieces);
+  join_pieces_kernel<E, HDP, kFlashRows><<<dim3(p.grid, join_blocks<HDP, kFlashRows>()), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
   return hipGetLastError();
 }
 
@@ -643,7 +643,7 @@ hipError_t launch_mixed(const AttnArgs& a, const FewPlan& f, const FlashPlan& p,
       a, rep, few_rows, f.grid, p.longest_first, scale_log2, parts, pieces);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  join_pieces_kernel<E, HDP, 32><<<dim3(f.grid, 2), 256, 0, stream>>>(a, rep, parts, pieces);
+  join_pieces_kernel<E, HDP, 32><<<dim3(f.grid, join_blocks<HDP, 32>()), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
   return hipGetLastError();
 }
 

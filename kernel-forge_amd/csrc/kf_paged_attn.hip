@@ -28,7 +28,7 @@ hipError_t launch(const AttnArgs& a, const FewPlan& p, int max_rows, void* ws, h
   few_rows_kernel<E, C, true><<<p.grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, parts, pieces);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  join_pieces_kernel<E, HDP, C::ROWS><<<dim3(p.grid, MT), 256, 0, stream>>>(a, rep, parts, pieces);
+  join_pieces_kernel<E, HDP, C::ROWS><<<dim3(p.grid, join_blocks<HDP, C::ROWS>()), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
   return hipGetLastError();
 }
 
