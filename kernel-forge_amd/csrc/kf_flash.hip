@@ -665,10 +665,11 @@ hipError_t launch_dim(const AttnArgs& a, const FlashPlan& p, int min_rows, void*
 //               45 -> 35 us, 4000 of 8 heads of 96 (250) 91 -> 70; but 16 ragged prompts (700) 49 -> 65, as eight wavefronts
 //               at one barrier overlap less than two workgroups do;
 //   longest first, where they do not all run at once: 16 ragged prompts 57 -> 49 us, a mixed batch 105 -> 91;
-//   kept apart, in a launch for both kinds of requests, where a CU could hold more of them (four, of up to 64 dims) than there are
-//               for each: they are not dealt out evenly by themselves.  Two up to 5/2 of the CUs, three up to 3: 4 requests'
-//               512 tokens over 4000 (4 KV heads of 64, 512 items) 126 -> 111 us, a mixed batch 65 -> 61; single prompts
-//               (500 .. 1000 items) within 1% either way, so they go without.
+//   kept apart, in a launch for both kinds of requests, where a CU could hold more of them (four, of up to 64 dims) than there
+//               are for each: they are not dealt out evenly by themselves.  Two where they are at most twice the CUs, three
+//               at most thrice: 4 requests' 512 tokens over 4000 (4 KV heads of 64, 512 items) 124 -> 107 us, a mixed
+//               batch 66 -> 61; 540 tokens (540 items) are 125 with three and 146 with two.  Single prompts and chunks
+//               stayed within 1% with it, so they go without.
 FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count) {
   FlashPlan p;
   const int64_t rep = a.heads / a.kv_heads;
@@ -681,7 +682,8 @@ FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count) {
   p.groups = 4 * items <= 5 * cu_count && keys > 256 ? flash_groups(hdp) : 1;
   // One sequence has its longest tiles last in any case, and workgroups that all run at once need no order.
   p.longest_first = a.seqs > 1 && a.seqs <= 64 && items * p.groups > cu_count * flash_waves_per_simd(hdp, false);
-  p.lds = hdp > 64 ? 0 : 2 * items <= 5 * cu_count ? 54 << 10 : items <= 3 * cu_count ? 41 << 10 : 0;
+  const int64_t full = (int64_t)a.tokens * rep / kFlashRows * a.kv_heads;  // without what `items` has to spare
+  p.lds = hdp > 64 ? 0 : full <= 2 * cu_count ? 54 << 10 : full <= 3 * cu_count ? 41 << 10 : 0;
   p.grid = p.cut ? cu_count * flash_waves_per_simd(hdp, true) : (int)items;
   return p;
 }
