@@ -471,8 +471,8 @@ __global__ __launch_bounds__(GROUPS * kFlashThreads, flash_waves_per_simd(HDP, G
 
 // A batch of both kinds of requests in one launch: the first few_grid workgroups, of which two wavefronts work, take the
 // requests of at most few_rows rows (kf_few_rows.h), the others the row tiles of the rest.  The ones wait for memory
-// and the others for the matrix cores, and a CU holds some of each.  24 requests of 1 .. 700 tokens over 30 .. 4000 (8 KV heads of
-// 128) take 73 us, in two launches 91; 4 heads of 64 61 (73); 64 of 1 .. 200 over 500 .. 8000 216 (252).
+// and the others for the matrix cores, and a CU holds some of each.  24 requests of 1 .. 700 tokens over 30 .. 4000 (8 KV
+// heads of 128) take 71 us, in two launches 91; 64 of 1 .. 200 over 500 .. 8000 213 (252).
 template <int HDP>
 using MixedFew = FewConfig<HDP, 2, 2, 2>;  // 64 dims: half the buffers, so that a CU holds four workgroups as without it
 template <int HDP>
@@ -637,10 +637,8 @@ hipError_t launch_mixed(const AttnArgs& a, const FewPlan& f, const FlashPlan& p,
   const float scale_log2 = a.scale * 1.44269504088896340736f;
   float* const parts = static_cast<float*>(ws);
   Piece* const pieces = reinterpret_cast<Piece*>(parts + (size_t)2 * f.grid * 32 * (HDP + 2));
-  constexpr int OWN = sizeof(MixedShared<HDP>);
-  const size_t more_lds = p.lds > OWN ? p.lds - OWN : 0;
-  mixed_attention_kernel<E, HDP><<<f.grid + p.grid, kFlashThreads, more_lds, stream>>>(
-      a, rep, few_rows, f.grid, p.longest_first, scale_log2, parts, pieces);
+  mixed_attention_kernel<E, HDP><<<f.grid + p.grid, kFlashThreads, 0, stream>>>(a, rep, few_rows, f.grid, p.longest_first,
+                                                                                scale_log2, parts, pieces);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   join_pieces_kernel<E, HDP, 32><<<dim3(f.grid, join_blocks<HDP, 32>()), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
@@ -661,15 +659,11 @@ hipError_t launch_dim(const AttnArgs& a, const FlashPlan& p, int min_rows, void*
 //   cut         into equal stretches that a second launch joins, where the CUs that would stay idle make up for writing and
 //               reading the pieces: 200 tokens over 60000 (8 KV heads of 128, 56 items) 1392 -> 285 us; but 2000 tokens of
 //               12 heads 35 -> 64, 16 ragged prompts 49 -> 79, a mixed batch 91 -> 102 us;
-//   shared      by two groups of four wavefronts, where they are hardly more than the CUs: 2000 tokens of 12 heads (192 items)
-//               45 -> 35 us, 4000 of 8 heads of 96 (250) 91 -> 70; but 16 ragged prompts (700) 49 -> 65, as eight wavefronts
-//               at one barrier overlap less than two workgroups do;
-//   longest first, where they do not all run at once: 16 ragged prompts 57 -> 49 us, a mixed batch 105 -> 91;
-//   kept apart, in a launch for both kinds of requests, where a CU could hold more of them (four, of up to 64 dims) than there
-//               are for each: they are not dealt out evenly by themselves.  Two where they are at most twice the CUs, three
-//               at most thrice: 4 requests' 512 tokens over 4000 (4 KV heads of 64, 512 items) 124 -> 107 us, a mixed
-//               batch 66 -> 61; 540 tokens (540 items) are 125 with three and 146 with two.  Single prompts and chunks
-//               stayed within 1% with it, so they go without.
+//   shared      by two groups of four wavefronts, where a CU gets hardly more than half the workgroups it could hold (four of
+//               up to 64 dims, two of 128): 2000 tokens of 12 heads of 128 (192 items) 45 -> 35 us, 4000 of 8 of 96 (250)
+//               91 -> 70, 2047 tokens of 32 of 64 over 29999 (512) 666 -> 613, 1600 (400) 27.9 -> 24.4; but 16 ragged prompts
+//               of 128 dims (700) 49 -> 65, as eight wavefronts at one barrier overlap less than two workgroups do;
+//   longest first, where they do not all run at once: 16 ragged prompts 57 -> 49 us, a mixed batch 105 -> 91.
 FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count) {
   FlashPlan p;
   const int64_t rep = a.heads / a.kv_heads;
@@ -679,11 +673,9 @@ FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count) {
   const int64_t most_cost = (tiles + a.seqs) * a.kv_heads * (((keys + kFlashItem) * rep >> 6) + 2 * tiles + 2);
   const int64_t items = tiles * a.kv_heads;
   p.cut = items < cu_count && keys * (cu_count - items) > (int64_t)1600 * cu_count && most_cost < (int64_t)1 << 31;
-  p.groups = 4 * items <= 5 * cu_count && keys > 256 ? flash_groups(hdp) : 1;
+  p.groups = (hdp == 64 ? 2 : 4) * items <= 5 * cu_count && keys > 256 ? flash_groups(hdp) : 1;
   // One sequence has its longest tiles last in any case, and workgroups that all run at once need no order.
   p.longest_first = a.seqs > 1 && a.seqs <= 64 && items * p.groups > cu_count * flash_waves_per_simd(hdp, false);
-  const int64_t full = (int64_t)a.tokens * rep / kFlashRows * a.kv_heads;  // without what `items` has to spare
-  p.lds = hdp > 64 ? 0 : full <= 2 * cu_count ? 54 << 10 : full <= 3 * cu_count ? 41 << 10 : 0;
   p.grid = p.cut ? cu_count * flash_waves_per_simd(hdp, true) : (int)items;
   return p;
 }

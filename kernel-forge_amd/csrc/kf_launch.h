@@ -245,7 +245,6 @@ struct FlashPlan {
   bool cut;    // the work of all row tiles is cut into equal stretches, and a second launch joins what was cut
   int groups;  // of four wavefronts that share a row tile's keys
   bool longest_first;  // row tiles start in the order of their lengths
-  int lds;             // mixed_attention_launch: bytes that a workgroup takes at least, so that a CU holds no more than it should
   int grid;
 };
 FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count);
