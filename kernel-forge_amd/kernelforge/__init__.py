@@ -2,7 +2,7 @@
 
 Submodules:
   quantize  the packed INT4 format (producer, reference kernelforge/quantize.py)
-  ops       int4_gemv / int4_gemm / int4_matmul / int4_linear + torch.library op
+  ops       int4_gemv / int4_gemm / int4_matmul / int4_linear + torch.library op; attention and tables of a paged KV cache
   modules   KFLinearInt4 and quantize_linears_
   _lib      ctypes binding of libkf_int4.so
   build     hipcc build of libkf_int4.so

@@ -226,7 +226,7 @@ def test_many_short_requests(heads, kv_heads, d, longest, new):
     b.check(b(max_new=new), there)
 
 
-@pytest.mark.parametrize("heads,kv_heads,d", [(32, 4, 64), (32, 8, 128), (16, 16, 96)])
+@pytest.mark.parametrize("heads,kv_heads,d", [(32, 4, 64), (64, 8, 64), (32, 8, 128), (16, 16, 96)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
 def test_chunks_beside_single_tokens(heads, kv_heads, d, dtype):
     """Many row tiles of chunks, and single tokens over long contexts, in one launch: the rows at which a request goes to the
