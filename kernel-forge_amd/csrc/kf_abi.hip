@@ -262,11 +262,11 @@ PagedLaunches paged_launches(const PagedPlan& p, int cus) {
   PagedLaunches l = {};
   if (p.many) l.many = kf::flash_plan(p.args, true, cus);
   if (p.few) {
-    // Where the row tiles are more than the CUs, and the others are cut.
-    l.together = p.many && !l.many.cut && l.many.groups == 1 && l.many.grid < 1 << 30 && p.args.head_dim <= 128;
+    // Where there are many row tiles, and the others are cut; the grid stays below 2^31 work-items.
+    l.together = p.many && !l.many.cut && l.many.groups == 1 && p.args.head_dim <= 128;
     if (l.together) {
       l.few = kf::few_rows_plan(p.args, p.rows, cus, true);
-      l.together = l.few.cut;
+      l.together = l.few.cut && ((int64_t)l.many.grid + l.few.grid) * 256 < (int64_t)1 << 31;
     }
     if (!l.together) l.few = kf::few_rows_plan(p.args, p.rows, cus, false);
     l.workspace = kf::few_rows_workspace_bytes(p.args.head_dim, l.few);

@@ -252,6 +252,15 @@ def test_chunks_beside_single_tokens(heads, kv_heads, d, dtype):
     assert torch.equal(got, out)
 
 
+def test_chunks_beside_single_tokens_of_many_requests():
+    """More requests than are put in the order of their lengths."""
+    count = 90
+    ctx = [(i * 211) % 700 for i in range(count)]
+    new = [1 if i % 3 else 30 + i for i in range(count)]
+    b = Batch(ctx, new, 32, 8, 128, torch.float16, 32, pad=5)
+    b.check(b(max_new=max(new)))
+
+
 def test_chunks_beside_single_tokens_in_a_graph():
     """One captured call, whose requests change from chunks to single tokens and back between replays."""
     b = Batch([700] * 16, [90] * 16, 32, 8, 128, torch.float16, 16)
