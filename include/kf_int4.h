@@ -284,7 +284,8 @@ int kf_decode_attention(const void* q, const void* cache_k, const void* cache_v,
  * request's page table row names its pages in order; token i of it lies in slot
  * row[i / block_size] * block_size + i % block_size.  No counterpart in the reference, which serves one stream.
  * Every length, offset, position, slot and page that the kernels read is bounded before it is used: wrong
- * ones give wrong results, never an access outside the arrays.  Pointers 16-byte aligned. */
+ * ones give wrong results, never an access outside the arrays.  Pointers 16-byte aligned, those of
+ * int32 arrays 4-byte aligned. */
 
 /* The tables of one step, from the requests' lengths, in one launch.  Request r has context_lens[r] tokens in the
  * cache and gets new_lens[r] more (negative: 0).  Where they need new pages (up to table_width in all), these are taken
@@ -336,7 +337,8 @@ int kf_rope_paged_cache(const kf_rope_paged_args* args, void* stream);
  * with 32-bit scores, maxima and sums; probabilities are rounded to the inputs' type for the second product, out
  * once more.  Keys after a token do not reach it whatever they hold.  Rows in no sequence are zeroed where
  * zero_rest is set and left as they are otherwise.  ws: at least kf_prompt_attention_workspace_bytes(args)
- * bytes, 16-byte aligned, not shared with a call that may run at the same time.  Strides in elements, multiples of 8; head_dim a multiple of 8
+ * bytes, 16-byte aligned, not shared with a call that may run at the same time.  Strides in elements, multiples
+ * of 8; head_dim a multiple of 8
  * up to KF_ATTN_MAX_HEAD_DIM; scale positive. */
 typedef struct {
   const void* q;          /* [tokens, heads, head_dim] */

@@ -316,13 +316,14 @@ struct Piece {
 __device__ __forceinline__ float scaled(float x, float f) { return fabsf(x) < __builtin_inff() ? f * x : x; }
 
 namespace {
-// Joins the pieces of the items that workgroup blockIdx.x of the first launch began and did not end.  A long item can have
-// hundreds, which is what takes the time: the wavefronts of a workgroup take every kJoinWaves-th piece of the same 64 x 4 values,
-// kJoinAhead of them loaded at once, and the workgroups in y share an item's values, 32 at most: 8 requests of 1 .. 12 tokens over
-// up to 32000 (2 KV heads of 128) take 79 us in all, with 16 workgroups 87, with 8 107; 64 single tokens 25.4 either way.
+// Joins the pieces of the items that workgroup blockIdx.x of the first launch began and did not end.  A long item can
+// have hundreds, which is what takes the time: the wavefronts of a workgroup take every kJoinWaves-th piece of the
+// same 64 x 4 values, kJoinAhead of them loaded at once, and the workgroups in y share an item's values, 32 at most:
+// 8 requests of 1 .. 12 tokens over up to 32000 (2 KV heads of 128) take 79 us in all, with 16 workgroups 87, with 8
+// 107; 64 single tokens 25.4 either way.
 constexpr int kJoinWaves = 4, kJoinAhead = 8;
 template <int HDP, int ROWS>
-constexpr int join_blocks() { return ROWS * HDP / 256 < 32 ? ROWS * HDP / 256 : 32; }
+dim3 join_grid(int stretches) { return dim3(stretches, ROWS * HDP / 256 < 32 ? ROWS * HDP / 256 : 32); }
 
 template <class E, int HDP, int ROWS>
 __global__ __launch_bounds__(64 * kJoinWaves) void join_pieces_kernel(AttnArgs a, int rep, const float* ws, const Piece* pieces) {

@@ -3,20 +3,21 @@
 //
 //   out[t, h] = sum_s softmax_s(scale q[t, h] . k[s, kv]) v[s, kv],   s <= position of t,   kv = h / rep
 //
-// A workgroup owns 128 rows of one KV head (kf_attn_tiles.h), 32 per wavefront, and walks their keys 64 at a
-// time (32 for heads of more than 128, whose outputs fill half the registers) through two LDS buffers.  Scores, maximum, sum and outputs are held in 32 bits; probabilities are rounded to
-// the inputs' type for the second matrix product (half a step of that type, as inputs are), the outputs once
-// more when they are stored.  The maximum that the exponentials are taken against follows the true one only when it is
-// exceeded by a factor 2^8: outputs and sums are then rescaled, which most tiles after the first spare.
+// A workgroup owns 128 rows of one KV head (kf_attn_tiles.h), 32 per wavefront, and walks their keys 64 at a time (32
+// for heads of more than 128, whose outputs fill half the registers) through two LDS buffers.  Scores, maximum, sum
+// and outputs are held in 32 bits; probabilities are rounded to the inputs' type for the second matrix product (half
+// a step of that type, as inputs are), the outputs once more when they are stored.  The maximum that the exponentials
+// are taken against follows the true one only when it is exceeded by a factor 2^8: outputs and sums are then
+// rescaled, which most tiles after the first spare.
 //
-// What bounds it: a tile of 64 keys costs a wavefront 16 (64 dims) or 32 (128 dims) matrix instructions of 32 cycles and
-// some 200 vector instructions for the softmax of its 32 x 64 scores, 32 of them exponentials at a quarter of the rate.
-// With 64 dims the two are alike: 16001 tokens of 32 heads take 1.09 ms, 960 TFLOP/s, vector pipe busy 81% of the time, matrix
-// cores 53%, no LDS bank conflicts, the clock down at 1.7 GHz.  With 128 dims the matrix cores lead: 8000 tokens of 32 heads take 0.49 ms,
-// 1070 TFLOP/s, of 1190 .. 1630 that matrix products of 4096 .. 16384 reach on the card.  Tried without gain: the next tile's
-// scores computed while a tile's exponentials are (0.50 .. 0.52 ms), tiles of 32 keys (0.49 ms; 16 ragged prompts 55 us, not 49).
-// A batch of a few hundred row tiles waits for its longest: 16 prompts of 19 .. 1455 tokens (12 heads on 2 of 128) take 49 us, of
-// which 25 are its work spread evenly.
+// What bounds it: a tile of 64 keys costs a wavefront 16 (64 dims) or 32 (128 dims) matrix instructions of 32 cycles
+// and some 200 vector instructions for the softmax of its 32 x 64 scores, 32 of them exponentials at a quarter of the
+// rate. With 64 dims the two are alike: 16001 tokens of 32 heads take 1.09 ms, 960 TFLOP/s, vector pipe busy 81% of
+// the time, matrix cores 53%, no LDS bank conflicts, the clock down at 1.7 GHz.  With 128 dims the matrix cores lead:
+// 8000 tokens of 32 heads take 0.49 ms, 1070 TFLOP/s, of 1190 .. 1630 that matrix products of 4096 .. 16384 reach on
+// the card.  Tried without gain: the next tile's scores computed while a tile's exponentials are (0.50 .. 0.52 ms),
+// tiles of 32 keys (0.49 ms; 16 ragged prompts 55 us, not 49). A batch of a few hundred row tiles waits for its
+// longest: 16 prompts of 19 .. 1455 tokens (12 heads on 2 of 128) take 49 us, of which 25 are its work spread evenly.
 #include <math.h>
 
 #include "kf_few_rows.h"
@@ -627,7 +628,7 @@ hipError_t launch(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws,
   flash_cut_kernel<E, HDP, PAGED><<<p.grid, kFlashThreads, 0, stream>>>(c);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  join_pieces_kernel<E, HDP, kFlashRows><<<dim3(p.grid, join_blocks<HDP, kFlashRows>()), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
+  join_pieces_kernel<E, HDP, kFlashRows><<<join_grid<HDP, kFlashRows>(p.grid), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
   return hipGetLastError();
 }
 
@@ -641,7 +642,7 @@ hipError_t launch_mixed(const AttnArgs& a, const FewPlan& f, const FlashPlan& p,
                                                                                 scale_log2, parts, pieces);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  join_pieces_kernel<E, HDP, 32><<<dim3(f.grid, join_blocks<HDP, 32>()), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
+  join_pieces_kernel<E, HDP, 32><<<join_grid<HDP, 32>(f.grid), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
   return hipGetLastError();
 }
 

@@ -28,7 +28,7 @@ hipError_t launch(const AttnArgs& a, const FewPlan& p, int max_rows, void* ws, h
   few_rows_kernel<E, C, true><<<p.grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, parts, pieces);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  join_pieces_kernel<E, HDP, C::ROWS><<<dim3(p.grid, join_blocks<HDP, C::ROWS>()), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
+  join_pieces_kernel<E, HDP, C::ROWS><<<join_grid<HDP, C::ROWS>(p.grid), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
   return hipGetLastError();
 }
 
@@ -66,8 +66,8 @@ FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int cu_count, bool beside
   p.waves = beside || a.head_dim > 128 || (items >= cu_count && keys * (a.head_dim <= 64 ? 64 : 128) <= 1 << 17) ? 2 : 4;
   const int unit = 32 * p.waves, fits = (a.head_dim <= 128 && p.waves == 2 && !beside ? 2 : 1) * cu_count;
   const int64_t key_units = (keys + unit - 1) / unit;
-  // Up to 512 keys are worked off whole, without the second launch.  Whole / cut, us: 16 requests of up to 450 tokens 8.7 / 11.2,
-  // of up to 900 11.3 / 11.8, of up to 1900 17.2 / 12.8; one of 900 15.6 / 11.5.
+  // Up to 512 keys are worked off whole, without the second launch.  Whole / cut, us: 16 requests of up to 450 tokens
+  // 8.7 / 11.2, of up to 900 11.3 / 11.8, of up to 1900 17.2 / 12.8; one of 900 15.6 / 11.5.
   p.cut = key_units * unit > 512;
   p.most_units = items * (key_units + kFewItem);
   p.grid = (int)std::min<int64_t>(fits, p.cut ? p.most_units : items);
