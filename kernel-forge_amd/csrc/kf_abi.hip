@@ -233,8 +233,17 @@ int paged_plan(const kf_paged_attention_args& a, PagedPlan* p) {
                 a.num_pages, a.max_new);
   if ((int64_t)a.table_width << t.log2_block >= (int64_t)1 << 30)
     return fail(KF_ERR_UNSUPPORTED, "tables of %d pages of %d tokens are too long", a.table_width, a.block_size);
-  const int64_t rows = (int64_t)(a.max_new ? std::min(a.max_new, a.tokens) : a.tokens) * (a.heads / a.kv_heads);
-  p->many = rows > kFewRows;
+  const int64_t rep = a.heads / a.kv_heads;
+  const int64_t rows = (int64_t)(a.max_new ? std::min(a.max_new, a.tokens) : a.tokens) * rep;
+  // Up to twice as many rows stay there where the requests have few on the average and caches that are soon read, as the other
+  // kernel's launches would take longer than reading keys again for the further rows.  Both kernels / this one alone, us:
+  // 16 requests of 1 .. 32 tokens over 300 .. 3000 (8 KV heads of 128) 67 / 40, 64 of 1 .. 16 over 500 .. 4000 (4 of 64)
+  // 78 / 59, 8 of 1 .. 12 over up to 32000 (2 of 128) 79 / 47; but 4 of 1 .. 32 over 60000 (8 of 128) 254 / 279, 64 of 1 .. 32
+  // over 4000 .. 16000 467 / 573, 64 of 16 over 500 .. 4000 (4 of 64) 54 / 115.
+  const bool few_on_average = rows <= 2 * kFewRows && a.tokens * rep <= (int64_t)kFewRows * a.seqs && a.head_dim <= 128 &&
+                              ((int64_t)a.table_width << t.log2_block) * a.seqs * a.kv_heads * (a.head_dim <= 64 ? 64 : 128) <=
+                                  (1 << 27);
+  p->many = rows > kFewRows && !few_on_average;
   p->few = !p->many || a.seqs > 1;
   p->rows = std::min<int64_t>(rows, kFewRows);
   t.q = a.q, t.k = a.cache_k, t.v = a.cache_v, t.out = a.out;

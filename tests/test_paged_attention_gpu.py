@@ -252,6 +252,18 @@ def test_chunks_beside_single_tokens(heads, kv_heads, d, dtype):
     assert torch.equal(got, out)
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(16, 4, 64), (32, 8, 128), (8, 8, 96), (8, 2, 256)])
+@pytest.mark.parametrize("pad", [0, 9])
+def test_short_chunks(heads, kv_heads, d, pad):
+    """A few requests of some tokens, single tokens for the most part: both sides of every bound on their rows."""
+    rep = heads // kv_heads
+    for most in (64 // rep, 64 // rep + 1, 128 // rep, 128 // rep + 1):
+        new = [1, most, 0, 2, most // 2, 1, 1, 3, 1, 1, 1, 1]
+        b = Batch([(i * 401 + 7) % 1500 for i in range(12)], new, heads, kv_heads, d, torch.bfloat16, 16, pad=pad)
+        b.check(b(max_new=most))
+        b.check(b())
+
+
 def test_chunks_beside_single_tokens_of_many_requests():
     """More requests than are put in the order of their lengths."""
     count = 90
