@@ -18,6 +18,7 @@
 
 #include "kf_int4.h"
 #include "kf_launch.h"
+#include "kf_stretch.h"
 
 static_assert(KF_DTYPE_F32 == kf::kQuantF32 && KF_DTYPE_F16 == kf::kQuantF16 && KF_DTYPE_BF16 == kf::kQuantBF16,
               "dtype codes of the C ABI and the kernels differ");
@@ -803,7 +804,7 @@ int kf_paged_attention(const kf_paged_attention_args* a, void* ws, size_t ws_byt
   if (int st = cu_count(&cus)) return st;
   const PagedLaunches l = paged_launches(p, cus);
   if (int st = check_workspace(ws, ws_bytes, l.workspace)) return st;
-  if (p.few && l.few.most_units >= (int64_t)1 << 31)
+  if (p.few && l.few.most_units >= kf::kNoWork)
     return fail(KF_ERR_UNSUPPORTED, "%d tokens over tables of %d pages are more than one launch takes", a->tokens,
                 a->table_width);
   if (l.together)

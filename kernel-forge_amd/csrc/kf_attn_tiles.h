@@ -15,6 +15,7 @@
 #pragma once
 
 #include "kf_device.h"
+#include "kf_stretch.h"
 
 namespace kf {
 
@@ -275,6 +276,17 @@ __device__ __forceinline__ int wave_prefix(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
   v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
+// The same of work (kf_stretch.h).
+__device__ __forceinline__ int work_prefix(int v) {
+  v = add_work(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
+  v = add_work(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+  v = add_work(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+  v = add_work(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+  v = add_work(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+  v = add_work(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
   return v;
 }
 

@@ -90,60 +90,58 @@ __device__ __forceinline__ void few_rows_stretch(const AttnArgs& args, FewShared
 
   int begin, end, per;
   {
-  const AttnArgs& a = args;
-  // This workgroup's stretch.  Every thread sums a run of requests; the one whose run holds the stretch's
-  // first unit says which request that is.
-  // Sums that pass 31 bits (offsets that do not ascend; the launch checks the others) end in no work or in work of
-  // some request, never outside.
-  const int run = (a.seqs + C::THREADS - 1) / C::THREADS;
-  const int s0 = min(tid * run, a.seqs), s1 = min(s0 + run, a.seqs);
-  int ku, mine = 0;
-  for (int s = s0; s < s1; ++s) {
-    const int n = few_items<C>(a, s, rep, max_rows, &ku);
-    mine += n * item_cost<C, CUT>(ku);
-  }
-  const int upto = wave_prefix(mine);
-  if (lane == 63) scan[wave] = upto;
-  if (tid == 0) found[0] = -1;
-  __syncthreads();
-  int total = 0, before = upto - mine;
-#pragma unroll
-  for (int w = 0; w < C::WAVES; ++w) {
-    if (w < wave) before += scan[w];
-    total += scan[w];
-  }
-  total = max(__builtin_amdgcn_readfirstlane(total), 0);
-  per = total / stretches + (total % stretches ? 1 : 0);
-  // 64 bits: workgroups past the end begin past it.
-  begin = (int)min((int64_t)me * per, (int64_t)total);
-  end = begin + min(per, total - begin);
-  if (begin >= before && begin < before + mine) {
-    int at = before;
+    const AttnArgs& a = args;
+    // This workgroup's stretch.  Every thread sums a run of requests; the one whose run holds the stretch's
+    // first unit says which request that is.
+    const int run = (a.seqs + C::THREADS - 1) / C::THREADS;
+    const int s0 = min(tid * run, a.seqs), s1 = min(s0 + run, a.seqs);
+    int ku, mine = 0;
     for (int s = s0; s < s1; ++s) {
-      const int n = few_items<C>(a, s, rep, max_rows, &ku) * item_cost<C, CUT>(ku);
-      if (begin < at + n) {
-        found[0] = s;
-        found[1] = at;
-        break;
+      const int n = few_items<C>(a, s, rep, max_rows, &ku);
+      mine = add_work(mine, n * item_cost<C, CUT>(ku));
+    }
+    const int upto = work_prefix(mine);
+    if (lane == 63) scan[wave] = upto;
+    if (tid == 0) found[0] = -1;
+    __syncthreads();
+    int total = 0, before = upto - mine;
+#pragma unroll
+    for (int w = 0; w < C::WAVES; ++w) {
+      if (w < wave) before = add_work(before, scan[w]);
+      total = add_work(total, scan[w]);
+    }
+    total = __builtin_amdgcn_readfirstlane(total);
+    if (total == kNoWork) total = 0;
+    per = total / stretches + (total % stretches ? 1 : 0);
+    const Stretch stretch = stretch_of(total, per, me);
+    begin = stretch.begin, end = stretch.end;
+    if (stretch.begins_in(before, mine)) {
+      int at = before;
+      for (int s = s0; s < s1; ++s) {
+        const int n = few_items<C>(a, s, rep, max_rows, &ku) * item_cost<C, CUT>(ku);
+        if (begin < at + n) {
+          found[0] = s;
+          found[1] = at;
+          break;
+        }
+        at += n;
       }
-      at += n;
     }
-  }
-  if (CUT && tid == 0) pieces[me].seq = -1;
-  __syncthreads();
+    if (CUT && tid == 0) pieces[me].seq = -1;
+    __syncthreads();
 
-  // Rows in no sequence.
-  if (a.zero_rest) {
-    const int t0 = seq_offset(a.cu, a.seqs, a.seqs, a.tokens);
-    const int cpr = a.head_dim / 8, per_row = a.heads * cpr;
-    for (int64_t i = (int64_t)me * C::THREADS + tid; i < (int64_t)(a.tokens - t0) * per_row;
-         i += (int64_t)stretches * C::THREADS) {
-      const int64_t t = i / per_row;
-      const int r = (int)(i - t * per_row), h = r / cpr;
-      *(u32x4*)((E*)a.out + (t0 + t) * a.out_token + h * a.out_head + 8 * (r - h * cpr)) = u32x4{0, 0, 0, 0};
+    // Rows in no sequence.
+    if (a.zero_rest) {
+      const int t0 = seq_offset(a.cu, a.seqs, a.seqs, a.tokens);
+      const int cpr = a.head_dim / 8, per_row = a.heads * cpr;
+      for (int64_t i = (int64_t)me * C::THREADS + tid; i < (int64_t)(a.tokens - t0) * per_row;
+           i += (int64_t)stretches * C::THREADS) {
+        const int64_t t = i / per_row;
+        const int r = (int)(i - t * per_row), h = r / cpr;
+        *(u32x4*)((E*)a.out + (t0 + t) * a.out_token + h * a.out_head + 8 * (r - h * cpr)) = u32x4{0, 0, 0, 0};
+      }
     }
-  }
-  if (begin >= end || found[0] < 0) return;
+    if (begin >= end || found[0] < 0) return;
   }
 
   int seq = __builtin_amdgcn_readfirstlane(found[0]);
@@ -374,7 +372,7 @@ __device__ __forceinline__ void few_rows_stretch(const AttnArgs& args, FewShared
       }
     }
     if (tid == 0 && u0 == 0 && !whole)
-      pieces[me] = Piece{seq, row0, kv, (item_at + cost - 1) / per};
+      pieces[me] = Piece{seq, row0, kv, last_stretch(item_at, cost, per)};
     __syncthreads();  // the sums have been read: the buffers are free
   }
 }

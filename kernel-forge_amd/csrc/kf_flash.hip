@@ -515,7 +515,7 @@ __device__ __forceinline__ FlashWork flash_work(const AttnArgs& a, int s, int re
   w.tiles = w.rows < min_rows ? 0 : (w.rows + kFlashRows - 1) / kFlashRows;
   const int keys = PAGED ? min(max(load_const(a.seq_lens, s), 0), a.table_width << a.log2_block) : len;
   w.base = (int)(((int64_t)(max(keys - len, 0) + kFlashItem) * rep) >> 6);
-  // Never reached by offsets that ascend (flash_plan); with others no cost is negative.
+  // Never reached by offsets that ascend (flash_plan); with others no cost is above kNoWork.
   w.head_cost = (int)min(w.upto(w.tiles), (int64_t)(0x7fffffff / a.kv_heads));
   return w;
 }
@@ -537,8 +537,8 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
     const int run = (a.seqs + kFlashThreads - 1) / kFlashThreads;
     const int s0 = min(tid * run, a.seqs), s1 = min(s0 + run, a.seqs);
     int mine = 0;
-    for (int s = s0; s < s1; ++s) mine += flash_work<PAGED>(a, s, rep, min_rows).head_cost * a.kv_heads;
-    const int upto = wave_prefix(mine);
+    for (int s = s0; s < s1; ++s) mine = add_work(mine, flash_work<PAGED>(a, s, rep, min_rows).head_cost * a.kv_heads);
+    const int upto = work_prefix(mine);
     if (lane == 63) scan[wave] = upto;
     if (tid == 0) {
       found[0] = -1;
@@ -548,15 +548,16 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
     int total = 0, before = upto - mine;
 #pragma unroll
     for (int w = 0; w < kFlashWaves; ++w) {
-      if (w < wave) before += scan[w];
-      total += scan[w];
+      if (w < wave) before = add_work(before, scan[w]);
+      total = add_work(total, scan[w]);
     }
-    total = max(__builtin_amdgcn_readfirstlane(total), 0);
+    total = __builtin_amdgcn_readfirstlane(total);
+    if (total == kNoWork) total = 0;
     // No stretch is shorter than what a tile of keys counts: every piece between an item's first and last has some.
     per = max(total / (int)gridDim.x + 1, 4 * rep + 8);
-    begin = (int)min((int64_t)me * per, (int64_t)total);
-    end = begin + min(per, total - begin);
-    if (begin < end && begin >= before && begin < before + mine) {
+    const Stretch stretch = stretch_of(total, per, me);
+    begin = stretch.begin, end = stretch.end;
+    if (stretch.begins_in(before, mine)) {
       int at = before;
       for (int s = s0; s < s1; ++s) {
         const int n = flash_work<PAGED>(a, s, rep, min_rows).head_cost * a.kv_heads;
@@ -602,7 +603,7 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
     if (t0 == t1) continue;
     const bool whole = t0 == 0 && to == cost;
     float* const part = static_cast<float*>(a.ws) + (size_t)(2 * me + (t0 == 0 ? 1 : 0)) * kFlashRows * (HDP + 2);
-    if (tid == 0 && t0 == 0 && !whole) static_cast<Piece*>(a.pieces)[me] = Piece{seq, row0, kv, (item_at + cost - 1) / per};
+    if (tid == 0 && t0 == 0 && !whole) static_cast<Piece*>(a.pieces)[me] = Piece{seq, row0, kv, last_stretch(item_at, cost, per)};
     flash_item<E, HDP, PAGED, 1>(a, sh, rep, a.scale_log2, seq, row0, kv, t0, t1, whole ? nullptr : part);
     lds_barrier();  // the tiles have been read: the buffers are free
   }
@@ -673,7 +674,7 @@ FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count) {
   const int64_t keys = paged ? (int64_t)a.table_width << a.log2_block : a.tokens;
   const int64_t most_cost = (tiles + a.seqs) * a.kv_heads * (((keys + kFlashItem) * rep >> 6) + 2 * tiles + 2);
   const int64_t items = tiles * a.kv_heads;
-  p.cut = items < cu_count && keys * (cu_count - items) > (int64_t)1600 * cu_count && most_cost < (int64_t)1 << 31;
+  p.cut = items < cu_count && keys * (cu_count - items) > (int64_t)1600 * cu_count && most_cost < kNoWork;
   p.groups = (hdp == 64 ? 2 : 4) * items <= 5 * cu_count && keys > 256 ? flash_groups(hdp) : 1;
   // One sequence has its longest tiles last in any case, and workgroups that all run at once need no order.
   p.longest_first = a.seqs > 1 && a.seqs <= 64 && items * p.groups > cu_count * flash_waves_per_simd(hdp, false);

@@ -259,7 +259,7 @@ struct FewPlan {
   int waves;           // of a workgroup: 4, or 2 of which a CU holds two (one where head_dim > 128)
   bool cut;            // items may be cut, and a second launch joins them
   int grid;
-  int64_t most_units;  // an upper bound of the kernel's work units: below 2^31
+  int64_t most_units;  // an upper bound of the kernel's work units: below kNoWork
 };
 // rows: (token, query head of a group) rows of a request, at most.  beside: for mixed_attention_launch.
 FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int cu_count, bool beside);
