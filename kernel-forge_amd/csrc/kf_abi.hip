@@ -222,6 +222,7 @@ int check_strides(const int64_t* s, int count) {
 struct PagedPlan {
   bool few, many;
   int64_t rows;  // (token, query head of a group) rows of a request that the first one has to expect
+  int max_rows;  // ... and up to which it takes requests
   kf::AttnArgs args;
 };
 int paged_plan(const kf_paged_attention_args& a, PagedPlan* p) {
@@ -247,6 +248,7 @@ int paged_plan(const kf_paged_attention_args& a, PagedPlan* p) {
   p->many = rows > kFewRows && !few_on_average;
   p->few = !p->many || a.seqs > 1;
   p->rows = std::min<int64_t>(rows, kFewRows);
+  p->max_rows = p->many ? kFewRows : 0x7fffffff;
   t.q = a.q, t.k = a.cache_k, t.v = a.cache_v, t.out = a.out;
   t.cu = static_cast<const int*>(a.cu_new);
   t.seq_lens = static_cast<const int*>(a.seq_lens);
@@ -275,10 +277,10 @@ PagedLaunches paged_launches(const PagedPlan& p, int cus) {
     // Where there are many row tiles, and the others are cut; the grid stays below 2^31 work-items.
     l.together = p.many && !l.many.cut && l.many.groups == 1 && p.args.head_dim <= 128;
     if (l.together) {
-      l.few = kf::few_rows_plan(p.args, p.rows, cus, true);
+      l.few = kf::few_rows_plan(p.args, p.rows, p.max_rows, cus, true);
       l.together = l.few.cut && ((int64_t)l.many.grid + l.few.grid) * 256 < (int64_t)1 << 31;
     }
-    if (!l.together) l.few = kf::few_rows_plan(p.args, p.rows, cus, false);
+    if (!l.together) l.few = kf::few_rows_plan(p.args, p.rows, p.max_rows, cus, false);
     l.workspace = kf::few_rows_workspace_bytes(p.args.head_dim, l.few);
   }
   // Launches that follow each other on the stream share the workspace.
@@ -811,8 +813,7 @@ int kf_paged_attention(const kf_paged_attention_args* a, void* ws, size_t ws_byt
     return hip_status(kf::mixed_attention_launch(p.args, bf16, l.few, l.many, kFewRows, ws, static_cast<hipStream_t>(stream)),
                       "paged_attention launch");
   if (p.few) {
-    const int max_rows = p.many ? kFewRows : 0x7fffffff;
-    if (int st = hip_status(kf::few_rows_launch(p.args, bf16, l.few, max_rows, ws, static_cast<hipStream_t>(stream)),
+    if (int st = hip_status(kf::few_rows_launch(p.args, bf16, l.few, p.max_rows, ws, static_cast<hipStream_t>(stream)),
                             "paged_attention launch"))
       return st;
   }

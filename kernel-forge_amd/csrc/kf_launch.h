@@ -261,8 +261,9 @@ struct FewPlan {
   int grid;
   int64_t most_units;  // an upper bound of the kernel's work units: below kNoWork
 };
-// rows: (token, query head of a group) rows of a request, at most.  beside: for mixed_attention_launch.
-FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int cu_count, bool beside);
+// rows: (token, query head of a group) rows to expect of a request, at most.  max_rows: as for few_rows_launch.  beside: for
+// mixed_attention_launch.
+FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int max_rows, int cu_count, bool beside);
 size_t few_rows_workspace_bytes(int head_dim, const FewPlan& p);
 // Requests of more than max_rows rows are left to the other kernel.  ws: few_rows_workspace_bytes, 16-byte aligned.
 hipError_t few_rows_launch(const AttnArgs& a, bool bf16, const FewPlan& p, int max_rows, void* ws, hipStream_t stream);

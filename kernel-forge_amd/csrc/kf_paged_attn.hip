@@ -54,10 +54,13 @@ hipError_t launch_dim(const AttnArgs& a, const FewPlan& p, int max_rows, void* w
 
 }  // namespace
 
-FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int cu_count, bool beside) {
+FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int max_rows, int cu_count, bool beside) {
   FewPlan p;
   p.row_tiles = beside || (a.head_dim <= 128 && rows > 16) ? 2 : 1;
-  const int64_t items = ((int64_t)a.tokens * (a.heads / a.kv_heads) / (16 * p.row_tiles) + a.seqs) * a.kv_heads;
+  // By the rows of all requests, and by the most that a request of this kernel's has.
+  const int64_t tile = 16 * p.row_tiles;
+  const int64_t items = std::min((int64_t)a.tokens * (a.heads / a.kv_heads) / tile + a.seqs,
+                                 a.seqs * ((max_rows + tile - 1) / tile)) * a.kv_heads;
   const int64_t keys = (int64_t)a.table_width << a.log2_block;
   // A CU holds one workgroup of four wavefronts or two of two, one of which then copies while the other begins or ends an
   // item.  That pays where there are an item or more for each CU and they are short; otherwise the second

@@ -7,6 +7,7 @@ csrc/kf_stretch.h is plain arithmetic; it is compiled for the host, and walked a
 
 from __future__ import annotations
 
+import ctypes
 import subprocess
 
 import pytest
@@ -115,3 +116,51 @@ def test_offsets_that_do_not_ascend(walk, requests, tokens):
 def test_offsets_that_ascend(walk, requests, items, cost, grid):
     last, units = walk(requests, items, cost, grid, 1)
     assert 0 <= last < grid and units == sum(items * (cost + i % 7) for i in range(requests))
+
+
+class AttnArgs(ctypes.Structure):
+    """kf::AttnArgs of csrc/kf_launch.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "cu", "seq_lens", "table")] + \
+        [(n, ctypes.c_int64) for n in ("table_stride", "q_token", "q_head", "out_token", "out_head", "k_page", "k_head",
+                                       "k_token", "v_page", "v_head", "v_token")] + \
+        [(n, ctypes.c_int) for n in ("tokens", "seqs", "heads", "kv_heads", "head_dim", "table_width", "log2_block",
+                                     "num_pages", "zero_rest")] + \
+        [("scale", ctypes.c_float), ("scale_log2", ctypes.c_float), ("rep", ctypes.c_int), ("min_rows", ctypes.c_int),
+         ("ws", ctypes.c_void_p), ("pieces", ctypes.c_void_p)]
+
+
+class FewPlan(ctypes.Structure):
+    """kf::FewPlan of csrc/kf_launch.h."""
+    _fields_ = [("row_tiles", ctypes.c_int), ("waves", ctypes.c_int), ("cut", ctypes.c_bool), ("grid", ctypes.c_int),
+                ("most_units", ctypes.c_int64)]
+
+
+def few_rows_plan(tokens, seqs, heads, kv_heads, d, keys, rows, max_rows, beside):
+    plan = ctypes.CDLL(str(build.LIB_PATH))._ZN2kf13few_rows_planERKNS_8AttnArgsEliib
+    plan.restype = FewPlan
+    plan.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_bool]
+    args = AttnArgs(tokens=tokens, seqs=seqs, heads=heads, kv_heads=kv_heads, head_dim=d, table_width=keys // 16, log2_block=4)
+    return plan(ctypes.byref(args), rows, max_rows, 256, beside)
+
+
+ALL = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("beside", [False, True])
+@pytest.mark.parametrize("tokens,seqs,heads,kv_heads,d,keys", [
+    (32768, 2, 128, 8, 128, 1 << 20), (4096, 2, 1024, 8, 8, 1 << 20), (40000, 3, 64, 8, 64, 1 << 20)])
+def test_work_beside_long_requests(tokens, seqs, heads, kv_heads, d, keys, beside):
+    """Requests of more rows than the kernel of few rows takes are none of its work: a long chunk beside a single token
+    over long tables is not more than a launch takes."""
+    p = few_rows_plan(tokens, seqs, heads, kv_heads, d, keys, 64, 64, beside)
+    unit = 32 * p.waves
+    items = seqs * -(-64 // (16 * p.row_tiles)) * kv_heads
+    assert p.most_units == items * (keys // unit + 2) < 2 ** 31 - 1
+
+
+def test_work_of_one_kernel_for_all():
+    """Without the other kernel every row counts: both sides of what a launch takes."""
+    for tokens, fits in ((32000, True), (33000, False)):
+        p = few_rows_plan(tokens, 2, 128, 8, 128, 1 << 20, 64, ALL, True)
+        items = (tokens * 16 // 32 + 2) * 8
+        assert p.most_units == items * ((1 << 20) // 64 + 2) and (p.most_units < 2 ** 31 - 1) == fits
