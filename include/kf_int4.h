@@ -356,9 +356,10 @@ int kf_prompt_attention(const kf_prompt_attention_args* args, void* ws, size_t w
 
 /* Causal attention of every request's new tokens over its pages of the cache (which hold the new tokens' keys and
  * values already): request r's new tokens are rows cu_new[r] .. cu_new[r + 1] - 1 of q, the last of its
- * seq_lens[r] tokens.  Otherwise as kf_prompt_attention.  Tokens whose page is not in [0, num_pages) are not
- * attended to; a row that is left with no key gets zeros.  max_new: an upper bound of the new tokens of a
- * request if the caller knows one, else 0; it chooses kernels and splits, results hold for any value.
+ * seq_lens[r] tokens.  Otherwise as kf_prompt_attention.  Tokens whose page is not in [0, num_pages), or
+ * behind the table's last one, are not attended to; a row that is left with no key gets zeros.  max_new: an upper bound
+ * of the new tokens of a request if the caller knows one, else 0; it chooses kernels and splits, results hold for any
+ * value.
  * ws: at least kf_paged_attention_workspace_bytes(args) bytes, 16-byte aligned, not shared with a call that may run
  * at the same time. */
 typedef struct {

@@ -296,6 +296,20 @@ __device__ __forceinline__ int seq_offset(const int* cu, int s, int seqs, int to
   return s <= 0 ? 0 : s > seqs ? tokens : min(max(load_const(cu, s), 0), tokens);
 }
 
+// The keys of sequence s whose last `len` tokens are new: `keys` of them have a place in its table, and the new token t is at
+// position shift + t, which may be behind them (a table that is too narrow: it attends to what has a place) or negative
+// (fewer keys than new tokens: none).
+struct SeqKeys {
+  int keys, shift;
+  __device__ __forceinline__ int last_key(int t) const { return min(shift + t, keys - 1); }  // that token t attends to
+  __device__ __forceinline__ int before() const { return min(max(shift, 0), keys); }         // of the keys, not new ones
+};
+template <bool PAGED>
+__device__ __forceinline__ SeqKeys seq_keys(const AttnArgs& a, int s, int len) {
+  const int n = PAGED ? max(load_const(a.seq_lens, s), 0) : len;
+  return SeqKeys{PAGED ? min(n, a.table_width << a.log2_block) : n, n - len};
+}
+
 // Tiles of BM rows over the packed sequences, numbered so that a tile finds its sequence without a scan: sequence
 // s owns the numbers from offset(s) * rep / BM + s on, enough for its rows, as
 // floor(a + b) + 1 >= floor(a) + ceil(b).  Returns the largest s <= seqs whose first number is at most t.

@@ -39,15 +39,12 @@ struct FewConfig {
   static_assert(WAVES * ROWS * HDP * 4 <= LDS, "the wavefronts' sums meet in the buffers");
 };
 
-__device__ __forceinline__ int few_seq_len(const AttnArgs& a, int s) {
-  return min(max(load_const(a.seq_lens, s), 0), a.table_width << a.log2_block);
-}
 // A request's items, (row tiles) x (KV heads), each of *key_units units of keys (one at least, so that every row is
 // written); what one item counts is item_cost: its units and ITEM, or 1 where items are not cut.
 template <class C>
 __device__ __forceinline__ int few_items(const AttnArgs& a, int s, int rep, int max_rows, int* key_units) {
   const int rows = max(seq_offset(a.cu, s + 1, a.seqs, a.tokens) - seq_offset(a.cu, s, a.seqs, a.tokens), 0) * rep;
-  *key_units = max((few_seq_len(a, s) + C::UNIT - 1) / C::UNIT, 1);
+  *key_units = max((seq_keys<true>(a, s, 0).keys + C::UNIT - 1) / C::UNIT, 1);
   return rows > max_rows ? 0 : (rows + C::ROWS - 1) / C::ROWS * a.kv_heads;
 }
 template <class C, bool CUT>
@@ -169,7 +166,7 @@ __device__ __forceinline__ void few_rows_stretch(const AttnArgs& args, FewShared
     const int kv = item % a.kv_heads, row0 = item / a.kv_heads * C::ROWS;
     const int tok0 = seq_offset(a.cu, seq, a.seqs, a.tokens);
     const int len = seq_offset(a.cu, seq + 1, a.seqs, a.tokens) - tok0, rows = len * rep;
-    const int seq_len = few_seq_len(a, seq), shift = seq_len - len;
+    const SeqKeys sk = seq_keys<true>(a, seq, len);
     const int64_t table_at = (int64_t)seq * a.table_stride;
 
     u32x4 qf[MT][ST];
@@ -177,7 +174,7 @@ __device__ __forceinline__ void few_rows_stretch(const AttnArgs& args, FewShared
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       const int row = min(row0 + 16 * t + l16, rows - 1), tok = row / rep, head = kv * rep + (row - tok * rep);
-      limit[t] = shift + tok;
+      limit[t] = sk.last_key(tok);
       const E* const qp = (const E*)a.q + (size_t)(tok0 + tok) * a.q_token + (size_t)head * a.q_head;
 #pragma unroll
       for (int s = 0; s < ST; ++s)
@@ -185,8 +182,8 @@ __device__ __forceinline__ void few_rows_stretch(const AttnArgs& args, FewShared
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) arrived(qf[t]);
-    const int kend = shift + min(row0 + C::ROWS - 1, rows - 1) / rep + 1;  // keys of the tile's last row
-    const int first_limit = shift + row0 / rep;
+    const int kend = sk.last_key(min(row0 + C::ROWS - 1, rows - 1) / rep) + 1;  // keys of the tile's last row
+    const int first_limit = sk.last_key(row0 / rep);
 
     auto page_of = [&](int key) {  // uniform; -1: not in the cache
       if (kend <= 0) return -1;

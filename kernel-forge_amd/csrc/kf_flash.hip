@@ -83,13 +83,12 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
   const int tok = row / rep;
   const int head = kv * rep + (row - tok * rep);
   // Keys: positions before this lane's row's own, itself included.
-  const int seq_len = PAGED ? min(max(load_const(a.seq_lens, seq), 0), a.table_width << a.log2_block) : len;
-  const int shift = seq_len - len;
-  const int limit = shift + tok;  // may be negative: no keys
+  const SeqKeys sk = seq_keys<PAGED>(a, seq, len);
+  const int limit = sk.last_key(tok);  // may be negative: no keys
   const int wave_row = row0 + 32 * wave;
-  const int wave_lo = shift + min(wave_row, rows - 1) / rep, wave_hi = shift + min(wave_row + 31, rows - 1) / rep;
-  const int first_limit = shift + row0 / rep;  // the workgroup's first row's
-  const int kend = shift + min(row0 + kFlashRows - 1, rows - 1) / rep + 1;
+  const int wave_lo = sk.last_key(min(wave_row, rows - 1) / rep), wave_hi = sk.last_key(min(wave_row + 31, rows - 1) / rep);
+  const int first_limit = sk.last_key(row0 / rep);  // the workgroup's first row's
+  const int kend = sk.last_key(min(row0 + kFlashRows - 1, rows - 1) / rep) + 1;
   tiles = min(tiles, kend <= 0 ? 0 : (kend + KEYS - 1) / KEYS);
   const int mine0 = tile0 + group;  // this group's first tile
 
@@ -395,9 +394,8 @@ __device__ __forceinline__ bool longest_tile(const AttnArgs& a, int rep, int min
   int64_t base = 0;
   if (lane < a.seqs) {
     const int len = max(seq_offset(a.cu, lane + 1, a.seqs, a.tokens) - seq_offset(a.cu, lane, a.seqs, a.tokens), 0);
-    const int keys = PAGED ? min(max(load_const(a.seq_lens, lane), 0), a.table_width << a.log2_block) : len;
     rows = len * rep;
-    base = (int64_t)max(keys - len, 0) * rep;
+    base = (int64_t)seq_keys<PAGED>(a, lane, len).before() * rep;
   }
   const int tiles = rows < min_rows ? 0 : (rows + kFlashRows - 1) / kFlashRows;
   const int q = 32 - __clz(64 * rep - 1);  // lengths in steps of 64 keys or a little more
@@ -513,8 +511,7 @@ __device__ __forceinline__ FlashWork flash_work(const AttnArgs& a, int s, int re
   FlashWork w;
   w.rows = len * rep;
   w.tiles = w.rows < min_rows ? 0 : (w.rows + kFlashRows - 1) / kFlashRows;
-  const int keys = PAGED ? min(max(load_const(a.seq_lens, s), 0), a.table_width << a.log2_block) : len;
-  w.base = (int)(((int64_t)(max(keys - len, 0) + kFlashItem) * rep) >> 6);
+  w.base = (int)(((int64_t)(seq_keys<PAGED>(a, s, len).before() + kFlashItem) * rep) >> 6);
   // Never reached by offsets that ascend (flash_plan); with others no cost is above kNoWork.
   w.head_cost = (int)min(w.upto(w.tiles), (int64_t)(0x7fffffff / a.kv_heads));
   return w;
@@ -553,7 +550,7 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
     }
     total = __builtin_amdgcn_readfirstlane(total);
     if (total == kNoWork) total = 0;
-    // No stretch is shorter than what a tile of keys counts: every piece between an item's first and last has some.
+    // No stretch is shorter than what a tile of keys counts.
     per = max(total / (int)gridDim.x + 1, 4 * rep + 8);
     const Stretch stretch = stretch_of(total, per, me);
     begin = stretch.begin, end = stretch.end;
@@ -593,14 +590,15 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
     const int item_at = head_at + (int)w.upto(tile), cost = w.base + 2 * (tile + 1);
     const int from = at - item_at, to = min(cost, end - item_at);
     const int row0 = tile * kFlashRows, len = w.rows / rep;
-    const int keys = PAGED ? min(max(load_const(a.seq_lens, seq), 0), a.table_width << a.log2_block) : len;
-    const int kend = keys - len + min(row0 + kFlashRows - 1, w.rows - 1) / rep + 1;
+    const int kend = seq_keys<PAGED>(a, seq, len).last_key(min(row0 + kFlashRows - 1, w.rows - 1) / rep) + 1;
     // The part's tiles: floor(position * tiles / cost), the same for a piece's end and the next one's beginning.
     const double tiles = max((kend + FlashConfig<HDP>::KEYS - 1) / FlashConfig<HDP>::KEYS, 1), each = cost;
     const int t0 = __builtin_amdgcn_readfirstlane((int)(from * tiles / each));
     const int t1 = __builtin_amdgcn_readfirstlane((int)(to * tiles / each));
     at = item_at + cost;
-    if (t0 == t1) continue;
+    // Not begun yet.  Further on a piece has a tile, or, where a table is too narrow for its request, may have none: that
+    // is written as such.
+    if (t1 == 0) continue;
     const bool whole = t0 == 0 && to == cost;
     float* const part = static_cast<float*>(a.ws) + (size_t)(2 * me + (t0 == 0 ? 1 : 0)) * kFlashRows * (HDP + 2);
     if (tid == 0 && t0 == 0 && !whole) static_cast<Piece*>(a.pieces)[me] = Piece{seq, row0, kv, last_stretch(item_at, cost, per)};

@@ -1213,9 +1213,10 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
     its seq_lens[r] tokens (int32 [B]), whose keys and values the cache holds already (rope_paged_cache). One
     token per request (decode), chunks of prompts and batches of both. max_new: an upper bound of a request's new
     tokens, if the caller knows one; it chooses kernels and splits only. Tokens whose page is not in the cache
-    (-1) are not attended to; a row with no key gets zeros. Rows behind the last request are zeros in a new output
-    and left as they are in ``out``, which must not overlap the caches. Arithmetic as in prompt_attention; results
-    do not change from run to run. The form of decode_attention for many requests; no reference counterpart.
+    (-1) and those behind the table's last page are not attended to; a row with no key gets zeros. Rows behind the
+    last request are zeros in a new output and left as they are in ``out``, which must not overlap the caches.
+    Arithmetic as in prompt_attention; results do not change from run to run. The form of decode_attention for many
+    requests; no reference counterpart.
     """
     tensors = (q, cache_k, cache_v, block_table, cu_new, seq_lens)
     if (_direct(q.get_device(), tensors) and out is None and q.dim() == 3 and block_table.dim() == 2

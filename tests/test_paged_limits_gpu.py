@@ -8,6 +8,7 @@ import torch
 from kernelforge import ops
 
 from attention_cases import attend64, check, offsets
+from test_paged_attention_gpu import Batch
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -48,3 +49,46 @@ def test_long_chunks_over_wide_tables():
         keys, values = (c[table[r, :n // block].long()].transpose(1, 2).reshape(n, kv_heads, d) for c in (k, v))
         ref, bound = attend64(q[rows][:, some], keys, values)
         check(out[rows][:, some], ref, bound, f"request {r}")
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (4, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize("ctx,new,width", [([60, 64, 70, 3], [1, 1, 1, 1], 4), ([60, 0, 40, 10], [8, 90, 30, 1], 4),
+                                           ([3, 300, 0, 100], [200, 5, 700, 300], 16), ([5000, 30], [300, 1], 320),
+                                           ([300, 0, 20] * 8, [80, 300, 1] * 8, 20), ([2500], [100], 160)],
+                         ids=["single", "short", "chunks", "long", "both", "cut"])
+def test_tables_that_are_too_narrow(heads, kv_heads, d, ctx, new, width):
+    """Requests that pass their table's width: new tokens keep their positions and attend to the keys that have a
+    place, as single tokens, in chunks and in both kinds of cut items."""
+    b = Batch(ctx, new, heads, kv_heads, d, torch.float16, 16, pad=2)
+    b.table = b.table[:, :width]
+    there = [torch.arange(c + n, device=DEV) < 16 * width for c, n in zip(ctx, new)]
+    assert not all(bool(t.all()) for t in there)
+    b.check(b(max_new=max(new)), there)
+    b.check(b(), there)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_cut_prompt_far_past_its_table(d):
+    """Row tiles whose keys end with the table while their number goes on: pieces without a key."""
+    b = Batch([0], [9000], 1, 1, d, torch.bfloat16, 16)
+    b.table = b.table[:, :250]
+    b.check(b(max_new=9000), [torch.arange(9000, device=DEV) < 4000])
+
+
+def test_a_step_that_passes_its_table():
+    """paged_tables gives such tokens no slot, rope_paged_cache leaves the cache, and paged_attention attends to the rest."""
+    heads, kv_heads, d, block = 4, 2, 64, 16
+    g = torch.Generator(device=DEV).manual_seed(9)
+    caches = [torch.randn(9, kv_heads, block, d, generator=g, device=DEV).half() for _ in range(2)]
+    table = i32([[5, 2, 7, -1], [1, -1, -1, -1]])
+    step = ops.paged_tables(table, i32([45, 10]), i32([30, 2]), i32([0, 8, 3]), i32([3]), block_size=block, max_tokens=32)
+    qkv = torch.randn(32, (heads + 2 * kv_heads) * d, generator=g, device=DEV).half()
+    cos, sin = (torch.rand(128, d, generator=g, device=DEV) for _ in range(2))
+    q, _ = ops.rope_paged_cache(qkv, cos, sin, step.positions, step.slots, *caches, heads=heads)
+    out = ops.paged_attention(q, *caches, table, step.cu_new, step.seq_lens, max_new=30)
+    assert table.tolist() == [[5, 2, 7, 3], [1, -1, -1, -1]]
+    for r, (rows, n) in enumerate(((slice(0, 30), 75), (slice(30, 32), 12))):
+        pages = table[r][table[r] >= 0].long()
+        k, v = (torch.cat([c[pages].transpose(1, 2).reshape(-1, kv_heads, d), c.new_zeros(32, kv_heads, d)])[:n] for c in caches)
+        ref, bound = attend64(q[rows], k, v, torch.arange(n, device=DEV) < 16 * pages.numel())
+        check(out[rows], ref, bound, f"request {r}")
