@@ -834,7 +834,7 @@ def _check_plain(what: str, tensors) -> None:
     if _transformed():
         raise RuntimeError(f"{what} launches a kernel; it cannot be transformed")
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} is inference only; an input requires a gradient (use torch.no_grad())")
+        raise RuntimeError(f"{what} is inference only; a tensor requires a gradient (use torch.no_grad())")
 
 
 def _direct(index: int, tensors) -> bool:
@@ -1150,7 +1150,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     _check_int("cu_seqlens", cu_seqlens, torch.int32, tuple(cu_seqlens.shape))
     scale = _check_scale(scale, d)
     _check_out(out, q)
-    _check_plain("prompt_attention", tensors)
+    _check_plain("prompt_attention", tensors if out is None else (*tensors, out))
     if _traced(tensors):
         if out is not None:
             raise RuntimeError("prompt_attention with out updates it in place and has no traceable form")
@@ -1248,7 +1248,7 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
         raise ValueError(f"max_new must be positive, got {max_new}")
     scale = _check_scale(scale, q.shape[2])
     _check_out(out, q)
-    _check_plain("paged_attention", tensors)
+    _check_plain("paged_attention", tensors if out is None else (*tensors, out))
     if _traced(tensors):
         if out is not None:
             raise RuntimeError("paged_attention with out updates it in place and has no traceable form")
