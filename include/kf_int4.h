@@ -338,8 +338,8 @@ int kf_rope_paged_cache(const kf_rope_paged_args* args, void* stream);
  * once more.  Keys after a token do not reach it whatever they hold.  Rows in no sequence are zeroed where
  * zero_rest is set and left as they are otherwise.  ws: at least kf_prompt_attention_workspace_bytes(args)
  * bytes, 16-byte aligned, not shared with a call that may run at the same time.  Strides in elements, multiples
- * of 8; head_dim a multiple of 8
- * up to KF_ATTN_MAX_HEAD_DIM; scale positive. */
+ * of 8, those of k's and v's tokens at most 2^26; head_dim a multiple of 8 up to KF_ATTN_MAX_HEAD_DIM; scale positive, at
+ * most 2.35e38. */
 typedef struct {
   const void* q;          /* [tokens, heads, head_dim] */
   const void* k;          /* [tokens, kv_heads, head_dim] */

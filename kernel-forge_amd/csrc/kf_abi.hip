@@ -195,7 +195,9 @@ int check_heads(int heads, int kv_heads, int head_dim, int dtype) {
 int check_attention(int tokens, int seqs, int heads, int kv_heads, int head_dim, int dtype, float scale) {
   if (tokens < 0 || seqs < 1) return fail(KF_ERR_INVALID_ARG, "need tokens >= 0 and seqs >= 1, got %d, %d", tokens, seqs);
   if (int st = check_heads(heads, kv_heads, head_dim, dtype)) return st;
-  if (!(scale > 0.0f) || scale > 3.0e38f) return fail(KF_ERR_INVALID_ARG, "scale must be positive and finite, got %g", scale);
+  // Finite in units of the exponent to base 2 as well.
+  if (!(scale > 0.0f) || scale > 2.35e38f)
+    return fail(KF_ERR_INVALID_ARG, "scale must be positive and at most 2.35e38, got %g", scale);
   // Row numbers (tokens x query heads of a group), and the grid in work-items, fit 31 bits.
   const int64_t rep = heads / kv_heads;
   if (tokens * rep >= (int64_t)1 << 31 || (tokens * rep / 128 + seqs + 1) * kv_heads * 256 >= (int64_t)1 << 31)

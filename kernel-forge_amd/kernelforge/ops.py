@@ -922,8 +922,8 @@ def _check_heads(heads: int, kv_heads: int, head_dim: int) -> None:
 def _check_scale(scale: float | None, head_dim: int) -> float:
     if scale is None:
         return 1.0 / math.sqrt(head_dim)
-    if not 0.0 < scale < 3.0e38:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 0.0 < scale <= 2.35e38:  # finite in units of the exponent to base 2 as well
+        raise ValueError(f"scale must be positive and at most 2.35e38, got {scale}")
     return float(scale)
 
 
