@@ -592,6 +592,8 @@ class PagedDecoder:
         self.block_table[row] = -1
         self.context_lens[row] = 0
         self.active[row] = 0
+        # Steps write a row's token again where it has no new one: at a free row's first place of the history.
+        self.tokens[row] = self.history[row, 0]
         self.host_lens[row] = 0
 
     def _step(self) -> None:
