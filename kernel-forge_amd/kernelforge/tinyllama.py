@@ -605,21 +605,23 @@ class PagedDecoder:
 
     @torch.no_grad()
     def capture(self) -> None:
-        """Captures the step; the requests are left as they were."""
-        state = (self.cache, self.block_table, self.context_lens, self.free_count, self.tokens, self.history)
-        self._reserve([2 if n else 0 for n in self.host_lens], "capture (two warm-up steps)")
-        saved = [t.clone() for t in state]
-        side = torch.cuda.Stream()
-        side.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(side):
-            for _ in range(2):
+        """Captures the step.  Warm-up and capture run without active rows, so they write no token and take no page: the
+        requests are left as they were."""
+        active = self.active.clone()
+        self.active.zero_()
+        try:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                for _ in range(2):
+                    self._step()
+            torch.cuda.current_stream().wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
                 self._step()
-        torch.cuda.current_stream().wait_stream(side)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
-            self._step()
-        for t, old in zip(state, saved):
-            t.copy_(old)
+            self.graph = graph
+        finally:
+            self.active.copy_(active)
 
     @torch.no_grad()
     def decode(self, steps: int, use_graph: bool = True) -> torch.Tensor:

@@ -32,3 +32,46 @@ def test_a_finished_row_keeps_its_history(model):
     dec.finish(0)
     dec.decode(2, use_graph=False)
     assert torch.equal(dec.history[0], want) and torch.equal(dec.history[0, :20], a)
+
+
+def test_capture_needs_no_room(model):
+    """Rows one token below max_seq and without a free page are captured, a large cache without a second one, and nothing
+    of the requests changes."""
+    last = model.cfg.max_seq - 1
+    a, b = prompts(last, 16)
+    dec = tl.PagedDecoder(model, DEV, requests=3, num_pages=14)
+    dec.admit({0: a, 2: b})
+    assert int(dec.free_count) == 0
+    before, lens = state(dec), list(dec.host_lens)
+    dec.capture()
+    same(dec, before)
+    assert dec.host_lens == lens
+    dec = tl.PagedDecoder(model, DEV, requests=2, num_pages=8000)
+    dec.admit({0: b})
+    dec.decode(1, use_graph=False)
+    size = dec.cache.numel() * dec.cache.element_size()
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    dec.capture()
+    assert torch.cuda.max_memory_allocated() - held < size // 2
+
+
+def test_a_capture_that_fails_leaves_the_requests(model, monkeypatch):
+    a, b = prompts(20, 9)
+    dec = tl.PagedDecoder(model, DEV, requests=2, num_pages=20)
+    dec.admit({0: a, 1: b})
+    before = state(dec)
+    forward = model.forward_paged
+    calls = []
+
+    def failing(*args, **kw):
+        calls.append(1)
+        if len(calls) == 2:
+            raise RuntimeError("planted")
+        return forward(*args, **kw)
+    monkeypatch.setattr(model, "forward_paged", failing)
+    with pytest.raises(RuntimeError, match="planted"):
+        dec.capture()
+    same(dec, before)
+    assert dec.graph is None
