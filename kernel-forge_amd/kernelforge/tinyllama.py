@@ -628,6 +628,8 @@ class PagedDecoder:
         """`steps` more tokens for every row that holds a request; returns the history [requests, max_seq]."""
         if use_graph and self.graph is None:
             raise ValueError("decode: capture first, or pass use_graph=False")
+        if steps < 0:
+            raise ValueError(f"decode: the number of steps must not be negative, got {steps}")
         new = [steps if n else 0 for n in self.host_lens]
         self._reserve(new, "decode")
         for _ in range(steps):

@@ -75,3 +75,14 @@ def test_a_capture_that_fails_leaves_the_requests(model, monkeypatch):
         dec.capture()
     same(dec, before)
     assert dec.graph is None
+
+
+def test_a_negative_number_of_steps(model):
+    (a,) = prompts(30)
+    dec = tl.PagedDecoder(model, DEV, requests=2, num_pages=8)
+    dec.admit({0: a})
+    with pytest.raises(ValueError, match="steps"):
+        dec.decode(-20, use_graph=False)
+    assert dec.host_lens == [30, 0] and torch.equal(dec.decode(0, use_graph=False), dec.history)
+    dec.finish(0)
+    assert int(dec.free_count) == 8 and sorted(dec.free_pages.tolist()) == list(range(8))
