@@ -556,9 +556,15 @@ class PagedDecoder:
         leaves each row's first generated token."""
         rows = sorted(prompts)
         for row in rows:
+            if not 0 <= row < len(self.host_lens):
+                raise ValueError(f"admit: there is no row {row}, only 0 to {len(self.host_lens) - 1}")
             if self.host_lens[row]:
                 raise ValueError(f"admit: row {row} holds a request")
-            if prompts[row].numel() < 1:
+            prompt = prompts[row]
+            if prompt.dim() != 1 or prompt.dtype not in (torch.int64, torch.int32) or prompt.device != self.tokens.device:
+                raise ValueError(f"admit: the prompt of row {row} must be 1-D int64 on {self.tokens.device}, got "
+                                 f"{str(prompt.dtype)[6:]} {list(prompt.shape)} on {prompt.device}")
+            if prompt.numel() < 1:
                 raise ValueError(f"admit: the prompt of row {row} is empty")
         if chunk is not None and chunk < 1:
             raise ValueError(f"admit: chunk must be positive, got {chunk}")

@@ -86,3 +86,25 @@ def test_a_negative_number_of_steps(model):
     assert dec.host_lens == [30, 0] and torch.equal(dec.decode(0, use_graph=False), dec.history)
     dec.finish(0)
     assert int(dec.free_count) == 8 and sorted(dec.free_pages.tolist()) == list(range(8))
+
+
+@pytest.mark.parametrize("row", [-1, 2, 7])
+def test_rows_that_there_are_not(model, row):
+    a, b = prompts(20, 9)
+    dec = tl.PagedDecoder(model, DEV, requests=2, num_pages=20)
+    before = state(dec)
+    for prompts_of in ({row: a}, {0: b, row: a}):
+        with pytest.raises(ValueError, match=f"no row {row}"):
+            dec.admit(prompts_of)
+    same(dec, before)
+    assert dec.host_lens == [0, 0]
+
+
+def test_prompts_of_other_shapes(model):
+    (a,) = prompts(20)
+    dec = tl.PagedDecoder(model, DEV, requests=2, num_pages=20)
+    before = state(dec)
+    for prompt in (a[None], a.float(), a.cpu()):
+        with pytest.raises(ValueError, match="prompt of row 1"):
+            dec.admit({1: prompt}, chunk=7)
+    same(dec, before)
