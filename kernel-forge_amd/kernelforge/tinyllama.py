@@ -148,7 +148,8 @@ class Attention(nn.Module):
 
     def paged(self, x, step, rope, cache_k, cache_v, block_table, max_new, whole_prompts, norm=None):
         """Attention of several requests' new tokens, x [1, T, H] packed (normalized unless `norm` is given), over
-        a paged cache: [1, T, heads d], before o_proj.  whole_prompts: no request has tokens in the cache yet."""
+        a paged cache: [1, T, heads d], before o_proj.  whole_prompts: no request with new tokens has any in the
+        cache yet."""
         cfg = self.cfg
         if self.qkv is None:
             qkv = torch.cat(self.project(x, norm), dim=-1)
@@ -578,7 +579,7 @@ class PagedDecoder:
             new = [min(n - d, chunk or n) for n, d in zip(lens, done)]
             tokens = torch.cat([prompts[r][done[r]:done[r] + new[r]] for r in rows])
             self._advance(tokens, torch.tensor(new, dtype=torch.int32, device=self.device), sum(new), max(new),
-                          whole_prompts=chunk is None and not any(self.host_lens))
+                          whole_prompts=chunk is None)
             done = [d + n for d, n in zip(done, new)]
         for row in rows:
             self.host_lens[row] = lens[row]

@@ -108,3 +108,28 @@ def test_prompts_of_other_shapes(model):
         with pytest.raises(ValueError, match="prompt of row 1"):
             dec.admit({1: prompt}, chunk=7)
     same(dec, before)
+
+
+@torch.no_grad()
+def test_whole_prompts_beside_running_rows(model, monkeypatch):
+    """They are whole prompts whatever the other rows hold, which have no new tokens then."""
+    a, b, c = prompts(40, 70, 33)
+    dec = tl.PagedDecoder(model, DEV, requests=4, num_pages=40)
+    dec.admit({1: a})
+    dec.decode(2, use_graph=False)
+    running = dec.history[1].clone()
+    calls = []
+    for name in ("prompt_attention", "paged_attention"):
+        def counted(*args, op=getattr(tl.ops, name), name=name, **kw):
+            calls.append(name)
+            return op(*args, **kw)
+        monkeypatch.setattr(tl.ops, name, counted)
+    dec.admit({0: b, 3: c})
+    assert calls == ["prompt_attention"] * model.cfg.layers
+    assert torch.equal(dec.history[1], running) and dec.host_lens == [70, 42, 0, 33]
+    dec.decode(3, use_graph=False)
+    for row, p in ((0, b), (1, a), (3, c)):
+        for at in range(p.numel(), dec.host_lens[row] + 1):
+            logits = single(model, dec.history[row, :at])
+            best, chosen = logits.max(), logits[dec.history[row, at]]
+            assert float(best - chosen) <= 2 * BOUND * float(logits.abs().max())
