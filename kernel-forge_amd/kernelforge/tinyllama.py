@@ -575,12 +575,19 @@ class PagedDecoder:
         for row in rows:
             self.history[row] = 0
             self.history[row, :lens[row]] = prompts[row]
-        while done != lens:
-            new = [min(n - d, chunk or n) for n, d in zip(lens, done)]
-            tokens = torch.cat([prompts[r][done[r]:done[r] + new[r]] for r in rows])
-            self._advance(tokens, torch.tensor(new, dtype=torch.int32, device=self.device), sum(new), max(new),
-                          whole_prompts=chunk is None)
-            done = [d + n for d, n in zip(done, new)]
+        try:
+            while done != lens:
+                new = [min(n - d, chunk or n) for n, d in zip(lens, done)]
+                tokens = torch.cat([prompts[r][done[r]:done[r] + new[r]] for r in rows])
+                self._advance(tokens, torch.tensor(new, dtype=torch.int32, device=self.device), sum(new), max(new),
+                              whole_prompts=chunk is None)
+                done = [d + n for d, n in zip(done, new)]
+        except BaseException:
+            # The rows are free again.  Pages are taken by counting down the stack, so the old count has them back.
+            for row in rows:
+                self._clear(row)
+            self.free_count.fill_(self.num_pages - sum(self._pages(m) for m in self.host_lens))
+            raise
         for row in rows:
             self.host_lens[row] = lens[row]
             # The chunks' own next tokens are overwritten by the prompt's.
@@ -596,12 +603,16 @@ class PagedDecoder:
         free = self.num_pages - used
         self.free_pages[free:free + n] = self.block_table[row, :n].clone()
         self.free_count.fill_(free + n)
+        self._clear(row)
+        self.host_lens[row] = 0
+
+    def _clear(self, row: int) -> None:
+        """Leaves a row without a request on the device."""
         self.block_table[row] = -1
         self.context_lens[row] = 0
         self.active[row] = 0
         # Steps write a row's token again where it has no new one: at a free row's first place of the history.
         self.tokens[row] = self.history[row, 0]
-        self.host_lens[row] = 0
 
     def _step(self) -> None:
         # The tokens of the rows that hold requests, packed.
@@ -637,14 +648,17 @@ class PagedDecoder:
             raise ValueError("decode: capture first, or pass use_graph=False")
         if steps < 0:
             raise ValueError(f"decode: the number of steps must not be negative, got {steps}")
-        new = [steps if n else 0 for n in self.host_lens]
-        self._reserve(new, "decode")
-        for _ in range(steps):
-            if use_graph:
-                self.graph.replay()
-            else:
-                self._step()
-        self.host_lens = [n + m for n, m in zip(self.host_lens, new)]
+        self._reserve([steps if n else 0 for n in self.host_lens], "decode")
+        done = 0
+        try:
+            for _ in range(steps):
+                if use_graph:
+                    self.graph.replay()
+                else:
+                    self._step()
+                done += 1
+        finally:
+            self.host_lens = [n + done if n else 0 for n in self.host_lens]
         return self.history
 
     def generated(self, row: int, prompt_len: int) -> torch.Tensor:

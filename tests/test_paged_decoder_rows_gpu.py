@@ -133,3 +133,60 @@ def test_whole_prompts_beside_running_rows(model, monkeypatch):
             logits = single(model, dec.history[row, :at])
             best, chosen = logits.max(), logits[dec.history[row, at]]
             assert float(best - chosen) <= 2 * BOUND * float(logits.abs().max())
+
+
+def fail_at(monkeypatch, model, call):
+    """The model's call number `call` from here on raises, before it computes anything."""
+    forward, calls = model.forward_paged, []
+
+    def failing(*args, **kw):
+        calls.append(1)
+        if len(calls) == call:
+            raise RuntimeError("planted")
+        return forward(*args, **kw)
+    monkeypatch.setattr(model, "forward_paged", failing)
+
+
+def test_an_admission_that_fails(model, monkeypatch):
+    """Its rows are free again, with their pages; the others go on."""
+    a, b, c = prompts(40, 70, 33)
+    outs = []
+    for fails in (False, True):
+        dec = tl.PagedDecoder(model, DEV, requests=3, num_pages=30)
+        dec.admit({1: a})
+        dec.decode(2, use_graph=False)
+        if fails:
+            with monkeypatch.context() as m:
+                fail_at(m, model, 3)
+                with pytest.raises(RuntimeError, match="planted"):
+                    dec.admit({0: b, 2: c}, chunk=20)
+            assert dec.host_lens == [0, 42, 0] and dec.context_lens.tolist() == [0, 42, 0]
+            assert int(dec.free_count) == 27 and bool((dec.block_table[[0, 2]] == -1).all())
+        dec.admit({0: b, 2: c}, chunk=20)
+        dec.decode(4, use_graph=False)
+        outs.append([dec.generated(r, p.numel()) for r, p in ((0, b), (1, a), (2, c))])
+        assert int(dec.free_count) == 30 - sum(-(-n // 16) for n in dec.host_lens)
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)
+
+
+def test_a_step_that_fails(model, monkeypatch):
+    """The steps before it count, on the host as on the device, and the next call goes on from there."""
+    a, b = prompts(30, 14)
+    outs = []
+    for fails in (False, True):
+        dec = tl.PagedDecoder(model, DEV, requests=2, num_pages=12)
+        dec.admit({0: a, 1: b})
+        done = 0
+        if fails:
+            with monkeypatch.context() as m:
+                fail_at(m, model, 4)  # the step in which both rows take a new page
+                with pytest.raises(RuntimeError, match="planted"):
+                    dec.decode(6, use_graph=False)
+            done = 3
+            assert dec.host_lens == dec.context_lens.tolist() == [33, 17]
+        dec.decode(6 - done, use_graph=False)
+        assert dec.host_lens == dec.context_lens.tolist() == [36, 20]
+        assert int(dec.free_count) == 12 - 3 - 2
+        outs.append(dec.history.clone())
+    assert torch.equal(*outs)
