@@ -190,3 +190,27 @@ def test_a_step_that_fails(model, monkeypatch):
         assert int(dec.free_count) == 12 - 3 - 2
         outs.append(dec.history.clone())
     assert torch.equal(*outs)
+
+
+def test_rows_come_and_go_around_a_captured_step(model):
+    """One capture, then requests that end and begin between its replays: what eager steps of the same rows give, with
+    the model's other work between the replays."""
+    ps = prompts(50, 21, 77, 5)
+    outs = []
+    for use_graph in (False, True):
+        dec = tl.PagedDecoder(model, DEV, requests=3, num_pages=30)
+        if use_graph:
+            dec.capture()  # before any request
+        dec.admit({0: ps[0], 1: ps[1]})
+        dec.decode(3, use_graph=use_graph)
+        dec.finish(0)
+        dec.decode(2, use_graph=use_graph)
+        dec.admit({0: ps[2]}, chunk=30)
+        dec.decode(2, use_graph=use_graph)
+        dec.admit({2: ps[3]})
+        dec.decode(5, use_graph=use_graph)
+        outs.append({**state(dec), "lens": torch.tensor(dec.host_lens)})
+        assert dec.host_lens == [84, 33, 10] == dec.context_lens.tolist()
+    for name in outs[0]:
+        if name != "cache":
+            assert torch.equal(outs[0][name], outs[1][name]), name
