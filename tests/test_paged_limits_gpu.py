@@ -92,3 +92,14 @@ def test_a_step_that_passes_its_table():
         k, v = (torch.cat([c[pages].transpose(1, 2).reshape(-1, kv_heads, d), c.new_zeros(32, kv_heads, d)])[:n] for c in caches)
         ref, bound = attend64(q[rows], k, v, torch.arange(n, device=DEV) < 16 * pages.numel())
         check(out[rows], ref, bound, f"request {r}")
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(32, 4, 64), (12, 2, 128), (8, 8, 96), (4, 1, 256), (16, 1, 80)])
+@pytest.mark.parametrize("ctx,new", [([0, 17, 130, 400], [1, 1, 1, 1]), ([40] * 70, [1] * 70), ([0], [300]), ([900, 3], [33, 1]),
+                                     ([0, 70, 500], [0, 260, 2]), ([100] * 12, [1, 200, 1, 9] * 3), ([5], [1])],
+                         ids=["decode", "many", "prompt", "short", "chunk", "mixed", "one"])
+def test_tables_much_wider_than_the_requests(heads, kv_heads, d, ctx, new):
+    """A server's table is as wide as its longest request may get, and the plans go by its width."""
+    b = Batch(ctx, new, heads, kv_heads, d, torch.bfloat16, 16, pad=1, extra_width=6000)
+    b.check(b(max_new=max(new)))
+    b.check(b())
