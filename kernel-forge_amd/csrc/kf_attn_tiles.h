@@ -96,7 +96,7 @@ __device__ __forceinline__ void arrived(u32x4 (&v)[N]) {
 }
 
 // The 16-byte pieces of a row of a tile are stored at piece ^ swizzle(row), so that the 16 (K) or 4 (V) rows which
-// one read touches lie in different banks.
+// one read touches lie in different banks.  (Measured: none of the kernel of many rows' LDS cycles are conflicts.)
 template <int HDP>
 __device__ __forceinline__ constexpr int swizzle_k(int key) {
   return HDP == 64 ? (key >> 1) & 7 : key & 15;
@@ -154,7 +154,8 @@ struct TileCopy {
       return;
     }
     int there = pieces, lane_here = lane;
-    asm volatile("" : "+s"(there), "+v"(lane_here));  // the comparisons below are made here, not kept in registers for the whole loop
+    // The comparisons below are made here, not kept in registers for the whole loop.
+    asm volatile("" : "+s"(there), "+v"(lane_here));
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const bool row_ok = RPI * j + lane_here / CPR < rows;

@@ -2,9 +2,10 @@
 //
 //   out[t, h] = sum_s softmax_s(scale q[t, h] . k[s, kv]) v[s, kv],   s <= position of t,   kv = h / rep
 //
-// What bounds it: the bytes of K and V, read once.  Three requests of up to 131071 tokens (8 KV heads of 128) take 205 us,
-// 6.3 TB/s of the 7.1 that a plain read of the card reaches; 64 of 100 .. 8191 tokens (2 of 128), 112 MB, take 25.5 us, 15.8
-// of them at that rate, the rest the second launch (6) and finding the stretches until the first keys are there.  So the
+// What bounds it: the bytes of K and V, read once.  Three requests of up to 131071 tokens (8 KV heads of 128) take 204 us,
+// 6.3 TB/s of the 7.1 that a plain read of the card reaches; 64 of 100 .. 8191 tokens (2 of 128), 112 MB, take 25 us: 21 the
+// first launch, of which 15.8 at that rate, the rest finding the stretches until the first keys are there, and 4 the second.
+// LDS bank conflicts are 27% of its LDS cycles there, which bound nothing: the vector pipe is busy 13% of the time.  So the
 // work of all requests is laid end to end, in units of 32 keys a wavefront of one item (request, row tile, KV head), and cut
 // into one equal stretch per workgroup whatever the lengths are; a workgroup finds its stretch from the lengths by itself
 // (they are read on the device only, so a captured launch follows them).  The wavefronts of a workgroup take 32 keys each
@@ -299,9 +300,11 @@ __device__ __forceinline__ void few_rows_stretch(const AttnArgs& args, FewShared
 #pragma unroll 1
             for (int k = 0; k < 32; ++k)
               if (key0 + k <= limit[t] && !(k >> 4 ? bad1 : bad0))
-                add += nonfinite_of<E>(lds_read8(v_tile + k * ROW + 16 * ((2 * c + (g >> 1)) ^ swizzle_v16<HDP>(k)) + 8 * (g & 1)));
+                add += nonfinite_of<E>(
+                    lds_read8(v_tile + k * ROW + 16 * ((2 * c + (g >> 1)) ^ swizzle_v16<HDP>(k)) + 8 * (g & 1)));
             o[t][c] += add;
-            asm volatile("" : "+v"(o[t][c]));  // here, not for all tiles at the end: this rare path takes no registers from the others
+            // Here, not for all tiles at the end: this rare path takes no registers from the others.
+            asm volatile("" : "+v"(o[t][c]));
           }
         lds_finite_only<E>(v_tile, 32 * ROW / 1024, lane);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

@@ -11,13 +11,14 @@
 // rescaled, which most tiles after the first spare.
 //
 // What bounds it: a tile of 64 keys costs a wavefront 16 (64 dims) or 32 (128 dims) matrix instructions of 32 cycles
-// and some 200 vector instructions for the softmax of its 32 x 64 scores, 32 of them exponentials at a quarter of the
-// rate. With 64 dims the two are alike: 16001 tokens of 32 heads take 1.09 ms, 960 TFLOP/s, vector pipe busy 81% of
-// the time, matrix cores 53%, no LDS bank conflicts, the clock down at 1.7 GHz.  With 128 dims the matrix cores lead:
-// 8000 tokens of 32 heads take 0.49 ms, 1070 TFLOP/s, of 1190 .. 1630 that matrix products of 4096 .. 16384 reach on
-// the card.  Tried without gain: the next tile's scores computed while a tile's exponentials are (0.50 .. 0.52 ms),
-// tiles of 32 keys (0.49 ms; 16 ragged prompts 55 us, not 49). A batch of a few hundred row tiles waits for its
-// longest: 16 prompts of 19 .. 1455 tokens (12 heads on 2 of 128) take 49 us, of which 25 are its work spread evenly.
+// and some 150 vector instructions for the softmax of its 32 x 64 scores, 32 of them exponentials, which take two slots.
+// With 64 dims the vector pipe leads: 16001 tokens of 32 heads take 1.11 ms, 950 TFLOP/s, vector pipe busy 89% of the
+// CUs' cycles, matrix cores 58%, no LDS bank conflicts, the clock at 1.64 GHz.  With 128 dims neither is full, at two
+// wavefronts per SIMD: 8000 tokens of 32 heads take 0.49 ms, 1070 TFLOP/s, matrix cores 55%, vector pipe 48%, of 1190 ..
+// 1630 TFLOP/s that matrix products of 4096 .. 16384 reach on the card.  Tried without gain: the next tile's scores
+// computed while a tile's exponentials are (0.50 .. 0.52 ms), tiles of 32 keys (0.49 ms; 16 ragged prompts 55 us, not
+// 49).  A batch of a few hundred row tiles waits for its longest: 16 prompts of 19 .. 1455 tokens (12 heads on 2 of 128)
+// take 45 .. 49 us, the longest row tile 23 tiles of keys where the work spread evenly is 14.
 #include <math.h>
 
 #include "kf_few_rows.h"
@@ -210,7 +211,8 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
     for (int st = 0; st < ST; ++st)
 #pragma unroll
       for (int u = 0; u < KU; ++u)
-        s[u] = Elem<E>::mfma32(lds_read16((kb ^ (uint32_t)(32 * st)) + u * 32 * ROW), Q_LDS ? q_lds[64 * st] : qf[Q_LDS ? 0 : st], s[u]);
+        s[u] = Elem<E>::mfma32(lds_read16((kb ^ (uint32_t)(32 * st)) + u * 32 * ROW),
+                               Q_LDS ? q_lds[64 * st] : qf[Q_LDS ? 0 : st], s[u]);
 
     __builtin_amdgcn_s_setprio(0);
     const bool masked = key0 + KEYS - 1 > wave_lo || bad != 0;
@@ -342,7 +344,8 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
       }
     }
     if (__builtin_expect(patch_from < kend, 0) && my_row < rows)
-      for (int d = 4 * half; d < b.head_dim; d += 8) *reinterpret_cast<float4_t*>(part + (my_row - row0) * HDP + d) += patch_of(d);
+      for (int d = 4 * half; d < b.head_dim; d += 8)
+        *reinterpret_cast<float4_t*>(part + (my_row - row0) * HDP + d) += patch_of(d);
     return;
   }
   const int group_heads = b.heads / b.kv_heads, out_row = min(my_row, rows - 1), out_tok = out_row / group_heads;
@@ -480,9 +483,8 @@ union MixedShared {
   FlashShared<HDP, 1> many;
 };
 template <class E, int HDP>
-__global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, false)) void mixed_attention_kernel(AttnArgs a, int rep, int few_rows, int few_grid,
-                                                                           int longest_first, float scale_log2, float* ws,
-                                                                           Piece* pieces) {
+__global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, false)) void mixed_attention_kernel(
+    AttnArgs a, int rep, int few_rows, int few_grid, int longest_first, float scale_log2, float* ws, Piece* pieces) {
   __shared__ MixedShared<HDP> sh;
   if ((int)blockIdx.x < few_grid) {  // zeros the rows behind the last request too
     if (threadIdx.x >= MixedFew<HDP>::THREADS) return;
@@ -614,10 +616,11 @@ hipError_t launch(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws,
   constexpr int GROUPS = flash_groups(HDP);
   if (!p.cut) {
     if (p.groups > 1)
-      flash_attention_kernel<E, HDP, PAGED, GROUPS><<<p.grid, GROUPS * kFlashThreads, 0, stream>>>(a, rep, min_rows, p.longest_first,
-                                                                                                           scale_log2);
+      flash_attention_kernel<E, HDP, PAGED, GROUPS>
+          <<<p.grid, GROUPS * kFlashThreads, 0, stream>>>(a, rep, min_rows, p.longest_first, scale_log2);
     else
-      flash_attention_kernel<E, HDP, PAGED, 1><<<p.grid, kFlashThreads, 0, stream>>>(a, rep, min_rows, p.longest_first, scale_log2);
+      flash_attention_kernel<E, HDP, PAGED, 1>
+          <<<p.grid, kFlashThreads, 0, stream>>>(a, rep, min_rows, p.longest_first, scale_log2);
     return hipGetLastError();
   }
   float* const parts = static_cast<float*>(ws);
@@ -627,7 +630,8 @@ hipError_t launch(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws,
   flash_cut_kernel<E, HDP, PAGED><<<p.grid, kFlashThreads, 0, stream>>>(c);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  join_pieces_kernel<E, HDP, kFlashRows><<<join_grid<HDP, kFlashRows>(p.grid), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
+  join_pieces_kernel<E, HDP, kFlashRows>
+      <<<join_grid<HDP, kFlashRows>(p.grid), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
   return hipGetLastError();
 }
 
@@ -654,7 +658,9 @@ hipError_t launch_dim(const AttnArgs& a, const FlashPlan& p, int min_rows, void*
 
 }  // namespace
 
-// How the row tiles are spread, by their number (`items`, from above) and the longest a sequence can be (`keys`).  The
+// How the row tiles are spread, by their number (`items`, from above) and the longest a sequence can be (`keys`: over a
+// cache the table's width, as lengths are on the device; a first chunk of 2000 tokens, 12 heads on 2 of 128, takes 39 us
+// with a table of its length and, cut, 56 with one of 131072 tokens).  The
 // kernel's time is at least its longest item's, so where there are few and they are long they are
 //   cut         into equal stretches that a second launch joins, where the CUs that would stay idle make up for writing and
 //               reading the pieces: 200 tokens over 60000 (8 KV heads of 128, 56 items) 1392 -> 285 us; but 2000 tokens of
@@ -688,15 +694,20 @@ size_t flash_workspace_bytes(int head_dim, const FlashPlan& p) {
 
 hipError_t flash_attention_launch(const AttnArgs& a, bool paged, bool bf16, const FlashPlan& p, int min_rows, void* ws,
                                   hipStream_t stream) {
-  if (paged) return bf16 ? launch_dim<bhalf_t, true>(a, p, min_rows, ws, stream) : launch_dim<half_t, true>(a, p, min_rows, ws, stream);
-  return bf16 ? launch_dim<bhalf_t, false>(a, p, min_rows, ws, stream) : launch_dim<half_t, false>(a, p, min_rows, ws, stream);
+  if (paged)
+    return bf16 ? launch_dim<bhalf_t, true>(a, p, min_rows, ws, stream)
+                : launch_dim<half_t, true>(a, p, min_rows, ws, stream);
+  return bf16 ? launch_dim<bhalf_t, false>(a, p, min_rows, ws, stream)
+              : launch_dim<half_t, false>(a, p, min_rows, ws, stream);
 }
 
 hipError_t mixed_attention_launch(const AttnArgs& a, bool bf16, const FewPlan& f, const FlashPlan& p, int few_rows, void* ws,
                                   hipStream_t stream) {
   if (a.head_dim <= 64)
-    return bf16 ? launch_mixed<bhalf_t, 64>(a, f, p, few_rows, ws, stream) : launch_mixed<half_t, 64>(a, f, p, few_rows, ws, stream);
-  return bf16 ? launch_mixed<bhalf_t, 128>(a, f, p, few_rows, ws, stream) : launch_mixed<half_t, 128>(a, f, p, few_rows, ws, stream);
+    return bf16 ? launch_mixed<bhalf_t, 64>(a, f, p, few_rows, ws, stream)
+                : launch_mixed<half_t, 64>(a, f, p, few_rows, ws, stream);
+  return bf16 ? launch_mixed<bhalf_t, 128>(a, f, p, few_rows, ws, stream)
+              : launch_mixed<half_t, 128>(a, f, p, few_rows, ws, stream);
 }
 
 }  // namespace kf

@@ -61,6 +61,8 @@ FewPlan few_rows_plan(const AttnArgs& a, int64_t rows, int max_rows, int cu_coun
   const int64_t tile = 16 * p.row_tiles;
   const int64_t items = std::min((int64_t)a.tokens * (a.heads / a.kv_heads) / tile + a.seqs,
                                  a.seqs * ((max_rows + tile - 1) / tile)) * a.kv_heads;
+  // The lengths are on the device, so plans go by what the table has room for.  Tables of 131072 tokens in place of tight
+  // ones, us: 16 requests of up to 450 tokens 8.5 -> 11.2, 128 of 50 .. 900 (8 KV heads of 128) 33 -> 41.
   const int64_t keys = (int64_t)a.table_width << a.log2_block;
   // A CU holds one workgroup of four wavefronts or two of two, one of which then copies while the other begins or ends an
   // item.  That pays where there are an item or more for each CU and they are short; otherwise the second

@@ -946,8 +946,8 @@ def paged_tables(block_table: torch.Tensor, context_lens: torch.Tensor, new_lens
     block_table int32 [B, width] (updated in place); context_lens, new_lens int32 [B]: tokens of each request in
     the cache and tokens that this step adds (0 for a request that pauses). Pages that they need beyond those they
     hold come from the stack free_pages int32 [F] with free_count int32 [1] pages on it, the last first, and are
-    entered into the table; -1 is entered once the stack is empty or where context + new passes the table's width
-    (no slot then). max_tokens: rows of positions and slots (the step's tokens at least). free_pages and
+    entered into the table, -1 once the stack is empty; tokens whose page is -1 or past the table's width have no
+    slot. max_tokens: rows of positions and slots (the step's tokens at least). free_pages and
     free_count are not changed: PagedStep.free_count is the count after the step. Lengths stay on the device, so a
     captured call follows them. No reference counterpart.
     """
@@ -1113,15 +1113,16 @@ def _(qkv, cos, sin, positions, slots, cache_k, cache_v, heads):
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, *,
                      scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-    """Causal attention over whole prompts, packed one after the other, in one launch (kf_prompt_attention).
+    """Causal attention over whole prompts, packed one after the other (kf_prompt_attention): one launch, or two for
+    few row tiles over many keys.
 
     q [T, heads, head_dim], k and v [T, kv_heads, head_dim], fp16 or bf16, any strides of the first two dimensions
-    (views of a fused projection are read in place); cu_seqlens int32 [B + 1] on the device: sequence s is rows
-    cu_seqlens[s] .. cu_seqlens[s + 1] - 1, ascending from 0, empty ones allowed. Query head h reads KV head h //
-    (heads / kv_heads); scale defaults to 1 / sqrt(head_dim). Scores, softmax and sums in 32 bits, probabilities
-    rounded to the inputs' type for their product with v. Rows behind the last sequence are zeros in a new output
-    and left as they are in ``out``, which must not overlap k or v. The form of decode_attention for prompts; no
-    reference counterpart (its models run torch's attention).
+    (views of a fused projection are read in place; tokens of k and v up to 2^26 elements apart); cu_seqlens int32
+    [B + 1] on the device: sequence s is rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1, ascending from 0, empty ones
+    allowed. Query head h reads KV head h // (heads / kv_heads); scale defaults to 1 / sqrt(head_dim). Scores, softmax
+    and sums in 32 bits, probabilities rounded to the inputs' type for their product with v. Rows behind the last
+    sequence are zeros in a new output and left as they are in ``out``, which must not overlap k or v. The form of
+    decode_attention for prompts; no reference counterpart (its models run torch's attention).
     """
     tensors = (q, k, v, cu_seqlens)
     if _direct(q.get_device(), tensors) and out is None and q.dim() == 3 and k.dim() == 3 and v.dim() == 3:
@@ -1212,11 +1213,12 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
     cu_new int32 [B + 1]: request r's new tokens are rows cu_new[r] .. cu_new[r + 1] - 1 of q, the last ones of
     its seq_lens[r] tokens (int32 [B]), whose keys and values the cache holds already (rope_paged_cache). One
     token per request (decode), chunks of prompts and batches of both. max_new: an upper bound of a request's new
-    tokens, if the caller knows one; it chooses kernels and splits only. Tokens whose page is not in the cache
-    (-1) and those behind the table's last page are not attended to; a row with no key gets zeros. Rows behind the
-    last request are zeros in a new output and left as they are in ``out``, which must not overlap the caches.
-    Arithmetic as in prompt_attention; results do not change from run to run. The form of decode_attention for many
-    requests; no reference counterpart.
+    tokens, if the caller knows one; it and the table's width choose kernels and splits only (short requests are
+    faster with a table, or a view of its first columns, that is not much wider than they need). Tokens whose page
+    is not in the cache (-1) and those behind the table's last page are not attended to; a row with no key gets
+    zeros. Rows behind the last request are zeros in a new output and left as they are in ``out``, which must not
+    overlap the caches. Arithmetic as in prompt_attention; results do not change from run to run. The form of
+    decode_attention for many requests; no reference counterpart.
     """
     tensors = (q, cache_k, cache_v, block_table, cu_new, seq_lens)
     if (_direct(q.get_device(), tensors) and out is None and q.dim() == 3 and block_table.dim() == 2
