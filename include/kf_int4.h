@@ -381,6 +381,100 @@ typedef struct {
 size_t kf_paged_attention_workspace_bytes(const kf_paged_attention_args* args);
 int kf_paged_attention(const kf_paged_attention_args* args, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- decoding with drafted tokens -----------------------------------------------------------------
+ * A request's new tokens in a step are the nodes of a tree: node 0 is its pending token, which the cache does not hold
+ * yet, the others are drafted continuations.  parents[t] is the number, in its request, of the parent of row t's node:
+ * smaller than the node's own; another value: a root (its tokens follow what the cache holds).  The new tokens lie in the
+ * cache in the order of their numbers, node i of request r in place seq_lens[r] - (its new tokens) + i.  A request has up
+ * to KF_MAX_NODES nodes; further new tokens are none.  No counterpart in the reference, which drafts nothing.
+ * Indices are bounded as above. */
+#define KF_MAX_NODES 64
+
+/* ancestors[t]: bit j set where node j of the request is row t's node or one of its ancestors; positions[t]: the tokens
+ * before it, the cached ones and its ancestors (the position that RoPE takes).  0 and -1 for rows that are no node.  One
+ * launch. */
+typedef struct {
+  const void* parents;  /* int32 [tokens] */
+  const void* cu_new;   /* int32 [seqs + 1] */
+  const void* seq_lens; /* int32 [seqs] */
+  void* ancestors;      /* int64 [tokens] */
+  void* positions;      /* int64 [tokens] */
+  int tokens, seqs;
+} kf_draft_trees_args;
+int kf_draft_trees(const kf_draft_trees_args* args, void* stream);
+
+/* kf_paged_attention for such trees: row t attends to the tokens of its request before the new ones, and to those new ones
+ * whose bit of ancestors[t] (int64 [tokens], 8-byte aligned) is set, itself included only if its own is.  The words may hold
+ * any bits.  New tokens past the KF_MAX_NODES-th are attended to by none. */
+size_t kf_paged_tree_attention_workspace_bytes(const kf_paged_attention_args* args);
+int kf_paged_tree_attention(const kf_paged_attention_args* args, const void* ancestors, void* ws, size_t ws_bytes,
+                            void* stream);
+
+/* Which drafted tokens stay.  The path of a request begins with its node 0; a node's child of the lowest number that is accepted
+ * follows it, until none is.  Row t of target says what follows row t's node:
+ *   KF_VERIFY_BEST   scores; a child is accepted if its token is the index of the largest (the first of equal ones; NaN above
+ *                    all numbers), which is also the token behind the path.
+ *   KF_VERIFY_GIVEN  probabilities (fp32, summing to 1; NaN and negative ones count as 0).  The children of a node, tokens from
+ *                    anywhere, are tested in order: child c is accepted if accept_u[c] m < p(token), where m is 1 less the
+ *                    probabilities of the children before it; a token that was rejected is not accepted again.  The token behind
+ *                    the path is drawn from what the last node's children leave, f = p without their tokens: the first index at
+ *                    which the running sum of f is above sample_u times its whole.
+ *   KF_VERIFY_DRAWN  the same for children that were drawn, independently, from row t of draft (q, fp32): with a = 0 and m = 1
+ *                    at first, a child is accepted if accept_u[c] m q(token) < f(token), f = max(p - a q, 0), else a grows by
+ *                    m, and m becomes the sum of the new f.  f is also what the token behind the path is drawn from.
+ * Emitted tokens then have the target's distribution, if accept_u and sample_u are independent uniform numbers in [0, 1).
+ * Where f has no mass, the token is drawn from p; where that has none, it is 0; for a sample_u that is not below 1, the last index
+ * with any.  Sums in 64 bits; results do not change from run to run.  A token outside [0, vocab) is never accepted.
+ * Writes counts [seqs] (nodes on the path; 0 where a request has no new tokens), path [seqs, width] (their numbers, then
+ * -1) and emitted [seqs, width] (the accepted drafted tokens and the one behind them, counts[r] in all, then -1).  Only the first
+ * `width` nodes of a request count.  Rows target_row and draft_row elements apart, of their type's alignment.
+ * ws: at least kf_verify_drafts_workspace_bytes(args) bytes, 16-byte aligned, not shared with a call that may run at the
+ * same time. */
+#define KF_VERIFY_BEST 0
+#define KF_VERIFY_GIVEN 1
+#define KF_VERIFY_DRAWN 2
+typedef struct {
+  const void* tokens;   /* int64 [tokens_count] */
+  const void* parents;  /* int32 [tokens_count] */
+  const void* cu_new;   /* int32 [seqs + 1] */
+  const void* target;   /* [tokens_count, vocab] */
+  const void* draft;    /* fp32 [tokens_count, vocab]: KF_VERIFY_DRAWN */
+  const void* accept_u; /* fp32 [tokens_count]: KF_VERIFY_GIVEN and DRAWN */
+  const void* sample_u; /* fp32 [seqs]: the same */
+  void* counts;         /* int32 [seqs] */
+  void* path;           /* int32 [seqs, width] */
+  void* emitted;        /* int64 [seqs, width] */
+  int64_t target_row, draft_row;
+  int mode, tokens_count, seqs, vocab, width;
+  int dtype; /* of target: KF_DTYPE_* for KF_VERIFY_BEST, else KF_DTYPE_F32 */
+} kf_verify_drafts_args;
+size_t kf_verify_drafts_workspace_bytes(const kf_verify_drafts_args* args);
+int kf_verify_drafts(const kf_verify_drafts_args* args, void* ws, size_t ws_bytes, void* stream);
+
+/* What is kept of a step in the cache, one launch.  The first counts[r] nodes of path (ascending) stay: the entry of node
+ * path[r][i] moves to place context_lens[r] + i, in every one of `arrays` caches [num_pages, kv_heads, block_size, head_dim] of
+ * 16-bit values, array_stride apart; kept_lens[r] = context_lens[r] + counts[r] (at most seq_lens[r]).  Pages that held the
+ * others alone go onto the stack free_pages[*free_count ..], requests and pages in order, as far as there is room;
+ * *free_left is the count then.  The table keeps their numbers behind a request's last page, where kf_paged_tables enters
+ * new ones.  free_count NULL: no pages are given back; kept_lens NULL: the lengths are not written (further calls, for caches
+ * that are not one array).  A node without a place in the cache moves nothing.  Pages must not be shared between requests, nor
+ * kept_lens and free_left be arrays that are read. */
+typedef struct {
+  void* caches;
+  const void* block_table;  /* int32 [seqs, table_width], rows table_stride apart */
+  const void* context_lens; /* int32 [seqs]: before the step */
+  const void* seq_lens;     /* int32 [seqs]: with its new tokens */
+  const void* counts;       /* int32 [seqs] */
+  const void* path;         /* int32 [seqs, width], rows path_stride apart */
+  void* free_pages;         /* int32 [free_capacity] */
+  const void* free_count;   /* int32 [1], or NULL */
+  void* kept_lens;          /* int32 [seqs], or NULL */
+  void* free_left;          /* int32 [1], with free_count */
+  int64_t array_stride, page_stride, head_stride, token_stride, table_stride, path_stride;
+  int arrays, num_pages, kv_heads, head_dim, block_size, seqs, table_width, width, free_capacity;
+} kf_keep_drafts_args;
+int kf_keep_drafts(const kf_keep_drafts_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

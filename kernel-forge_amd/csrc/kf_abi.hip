@@ -26,6 +26,8 @@ static_assert(KF_GEMV_MAX_GROUP == kf::kMaxGemvGroup, "header and kernels disagr
 static_assert(KF_PROLOGUE_NONE == kf::kGemvProNone && KF_PROLOGUE_RMSNORM == kf::kGemvProRmsNorm &&
                   KF_PROLOGUE_SWIGLU == kf::kGemvProSwiGLU,
               "prologue codes of the C ABI and the kernels differ");
+static_assert(KF_VERIFY_BEST == kf::kVerifyBest && KF_VERIFY_GIVEN == kf::kVerifyGiven && KF_VERIFY_DRAWN == kf::kVerifyDrawn,
+              "verification modes of the C ABI and the kernels differ");
 static_assert(KF_GEMV_FUSED_MAX_K == kf::kGemvFusedMaxK, "header and kernels disagree on the fused K limit");
 
 namespace {
@@ -222,12 +224,12 @@ int check_strides(const int64_t* s, int count) {
 
 // Which kernels a paged_attention call launches.  few: the one that splits the keys; many: the one that splits the rows.
 struct PagedPlan {
-  bool few, many;
+  bool few, many, tree;
   int64_t rows;  // (token, query head of a group) rows of a request that the first one has to expect
   int max_rows;  // ... and up to which it takes requests
   kf::AttnArgs args;
 };
-int paged_plan(const kf_paged_attention_args& a, PagedPlan* p) {
+int paged_plan(const kf_paged_attention_args& a, bool tree, PagedPlan* p) {
   if (int st = check_attention(a.tokens, a.seqs, a.heads, a.kv_heads, a.head_dim, a.dtype, a.scale)) return st;
   kf::AttnArgs& t = p->args;
   t = {};
@@ -249,6 +251,7 @@ int paged_plan(const kf_paged_attention_args& a, PagedPlan* p) {
                                   (1 << 27);
   p->many = rows > kFewRows && !few_on_average;
   p->few = !p->many || a.seqs > 1;
+  p->tree = tree;
   p->rows = std::min<int64_t>(rows, kFewRows);
   p->max_rows = p->many ? kFewRows : 0x7fffffff;
   t.q = a.q, t.k = a.cache_k, t.v = a.cache_v, t.out = a.out;
@@ -277,7 +280,7 @@ PagedLaunches paged_launches(const PagedPlan& p, int cus) {
   if (p.many) l.many = kf::flash_plan(p.args, true, cus);
   if (p.few) {
     // Where there are many row tiles, and the others are cut; the grid stays below 2^31 work-items.
-    l.together = p.many && !l.many.cut && l.many.groups == 1 && p.args.head_dim <= 128;
+    l.together = p.many && !p.tree && !l.many.cut && l.many.groups == 1 && p.args.head_dim <= 128;
     if (l.together) {
       l.few = kf::few_rows_plan(p.args, p.rows, p.max_rows, cus, true);
       l.together = l.few.cut && ((int64_t)l.many.grid + l.few.grid) * 256 < (int64_t)1 << 31;
@@ -309,6 +312,79 @@ int prompt_args(const kf_prompt_attention_args& a, kf::AttnArgs* p) {
   t.tokens = a.tokens, t.seqs = a.seqs, t.heads = a.heads, t.kv_heads = a.kv_heads, t.head_dim = a.head_dim;
   t.zero_rest = a.zero_rest;
   t.scale = a.scale;
+  return KF_OK;
+}
+
+// a: of a call whose new tokens are chains, or (tree) the nodes of trees whose ancestors are given.
+int paged_attention(const kf_paged_attention_args* a, const void* ancestors, bool tree, void* ws, size_t ws_bytes, void* stream,
+                    const char* what) {
+  if (!a) return fail(KF_ERR_INVALID_ARG, "args must be non-null");
+  PagedPlan p;
+  if (int st = paged_plan(*a, tree, &p)) return st;
+  if (a->tokens == 0) return KF_OK;
+  if (tree && !ancestors) return fail(KF_ERR_INVALID_ARG, "every array must be non-null");
+  p.args.ancestors = static_cast<const uint64_t*>(ancestors);
+  const void* const arrays[] = {a->q, a->cache_k, a->cache_v, a->out};
+  if (int st = check_arrays(arrays, 4)) return st;
+  if (!a->block_table || !a->cu_new || !a->seq_lens) return fail(KF_ERR_INVALID_ARG, "every array must be non-null");
+  const int64_t strides[] = {a->q_token, a->q_head, a->out_token, a->out_head, a->k_page, a->k_head,
+                             a->k_token, a->v_page, a->v_head, a->v_token};
+  if (int st = check_strides(strides, 10)) return st;
+  if (a->k_token > kMaxTokenStride || a->v_token > kMaxTokenStride)
+    return fail(KF_ERR_UNSUPPORTED, "token strides of the caches go up to %d elements", kMaxTokenStride);
+  const bool bf16 = a->dtype == KF_DTYPE_BF16;
+  int cus;
+  if (int st = cu_count(&cus)) return st;
+  const PagedLaunches l = paged_launches(p, cus);
+  if (int st = check_workspace(ws, ws_bytes, l.workspace)) return st;
+  if (p.few && l.few.most_units >= kf::kNoWork)
+    return fail(KF_ERR_UNSUPPORTED, "%d tokens over tables of %d pages are more than one launch takes", a->tokens,
+                a->table_width);
+  hipStream_t const on = static_cast<hipStream_t>(stream);
+  if (l.together) return hip_status(kf::mixed_attention_launch(p.args, bf16, l.few, l.many, kFewRows, ws, on), what);
+  if (p.few)
+    if (int st = hip_status(kf::few_rows_launch(p.args, bf16, l.few, p.max_rows, ws, on), what)) return st;
+  if (p.many) {
+    kf::AttnArgs t = p.args;
+    if (p.few) t.zero_rest = 0;  // done
+    return hip_status(kf::flash_attention_launch(t, true, bf16, l.many, p.few ? kFewRows + 1 : 0, ws, on), what);
+  }
+  return KF_OK;
+}
+
+int check_nodes(int tokens, int seqs) {
+  if (tokens < 0 || seqs < 1) return fail(KF_ERR_INVALID_ARG, "need tokens >= 0 and seqs >= 1, got %d, %d", tokens, seqs);
+  if (seqs > 65535) return fail(KF_ERR_UNSUPPORTED, "one launch takes up to 65535 requests, got %d", seqs);
+  return KF_OK;
+}
+
+int verify_args(const kf_verify_drafts_args& a, kf::VerifyArgs* v) {
+  if (int st = check_nodes(a.tokens_count, a.seqs)) return st;
+  if (a.vocab < 1 || a.vocab > 1 << 30) return fail(KF_ERR_INVALID_ARG, "vocab must be from 1 to 2^30, got %d", a.vocab);
+  if (a.width < 1 || a.width > KF_MAX_NODES)
+    return fail(KF_ERR_INVALID_ARG, "paths have 1 to %d nodes, got %d", KF_MAX_NODES, a.width);
+  if (a.mode != KF_VERIFY_BEST && a.mode != KF_VERIFY_GIVEN && a.mode != KF_VERIFY_DRAWN)
+    return fail(KF_ERR_INVALID_ARG, "mode must be one of KF_VERIFY_*, got %d", a.mode);
+  if (a.dtype != KF_DTYPE_F32 && (a.mode != KF_VERIFY_BEST || (a.dtype != KF_DTYPE_F16 && a.dtype != KF_DTYPE_BF16)))
+    return fail(KF_ERR_INVALID_ARG, "scores are KF_DTYPE_F32, F16 or BF16, probabilities KF_DTYPE_F32, got %d", a.dtype);
+  if (a.target_row < 0 || a.draft_row < 0) return fail(KF_ERR_INVALID_ARG, "strides must not be negative");
+  // Workgroups of a launch: shares of every row, or pieces of every request's last row.
+  if ((int64_t)a.tokens_count * 256 >= (int64_t)1 << 31)
+    return fail(KF_ERR_UNSUPPORTED, "%d tokens are more than one launch takes", a.tokens_count);
+  *v = {};
+  v->tokens = static_cast<const int64_t*>(a.tokens);
+  v->parents = static_cast<const int*>(a.parents);
+  v->cu = static_cast<const int*>(a.cu_new);
+  v->target = a.target;
+  v->draft = static_cast<const float*>(a.draft);
+  v->accept_u = static_cast<const float*>(a.accept_u);
+  v->sample_u = static_cast<const float*>(a.sample_u);
+  v->counts = static_cast<int*>(a.counts);
+  v->path = static_cast<int*>(a.path);
+  v->emitted = static_cast<int64_t*>(a.emitted);
+  v->target_row = a.target_row, v->draft_row = a.draft_row;
+  v->mode = a.mode;
+  v->tokens_count = a.tokens_count, v->seqs = a.seqs, v->vocab = a.vocab, v->width = a.width;
   return KF_OK;
 }
 
@@ -786,47 +862,98 @@ int kf_prompt_attention(const kf_prompt_attention_args* a, void* ws, size_t ws_b
 size_t kf_paged_attention_workspace_bytes(const kf_paged_attention_args* a) {
   PagedPlan p;
   int cus;
-  if (!a || paged_plan(*a, &p) || cu_count(&cus)) return 0;
+  if (!a || paged_plan(*a, false, &p) || cu_count(&cus)) return 0;
   return paged_launches(p, cus).workspace;
 }
 
 int kf_paged_attention(const kf_paged_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
-  if (!a) return fail(KF_ERR_INVALID_ARG, "args must be non-null");
+  return paged_attention(a, nullptr, false, ws, ws_bytes, stream, "paged_attention launch");
+}
+
+size_t kf_paged_tree_attention_workspace_bytes(const kf_paged_attention_args* a) {
   PagedPlan p;
-  if (int st = paged_plan(*a, &p)) return st;
-  if (a->tokens == 0) return KF_OK;
-  const void* const arrays[] = {a->q, a->cache_k, a->cache_v, a->out};
-  if (int st = check_arrays(arrays, 4)) return st;
-  if (!a->block_table || !a->cu_new || !a->seq_lens) return fail(KF_ERR_INVALID_ARG, "every array must be non-null");
-  const int64_t strides[] = {a->q_token, a->q_head, a->out_token, a->out_head, a->k_page, a->k_head,
-                             a->k_token, a->v_page, a->v_head, a->v_token};
-  if (int st = check_strides(strides, 10)) return st;
-  if (a->k_token > kMaxTokenStride || a->v_token > kMaxTokenStride)
-    return fail(KF_ERR_UNSUPPORTED, "token strides of the caches go up to %d elements", kMaxTokenStride);
-  const bool bf16 = a->dtype == KF_DTYPE_BF16;
   int cus;
-  if (int st = cu_count(&cus)) return st;
-  const PagedLaunches l = paged_launches(p, cus);
-  if (int st = check_workspace(ws, ws_bytes, l.workspace)) return st;
-  if (p.few && l.few.most_units >= kf::kNoWork)
-    return fail(KF_ERR_UNSUPPORTED, "%d tokens over tables of %d pages are more than one launch takes", a->tokens,
-                a->table_width);
-  if (l.together)
-    return hip_status(kf::mixed_attention_launch(p.args, bf16, l.few, l.many, kFewRows, ws, static_cast<hipStream_t>(stream)),
-                      "paged_attention launch");
-  if (p.few) {
-    if (int st = hip_status(kf::few_rows_launch(p.args, bf16, l.few, p.max_rows, ws, static_cast<hipStream_t>(stream)),
-                            "paged_attention launch"))
-      return st;
-  }
-  if (p.many) {
-    kf::AttnArgs t = p.args;
-    if (p.few) t.zero_rest = 0;  // done
-    return hip_status(kf::flash_attention_launch(t, true, bf16, l.many, p.few ? kFewRows + 1 : 0, ws,
-                                                 static_cast<hipStream_t>(stream)),
-                      "paged_attention launch");
-  }
-  return KF_OK;
+  if (!a || paged_plan(*a, true, &p) || cu_count(&cus)) return 0;
+  return paged_launches(p, cus).workspace;
+}
+
+int kf_paged_tree_attention(const kf_paged_attention_args* a, const void* ancestors, void* ws, size_t ws_bytes, void* stream) {
+  return paged_attention(a, ancestors, true, ws, ws_bytes, stream, "paged_tree_attention launch");
+}
+
+int kf_draft_trees(const kf_draft_trees_args* a, void* stream) {
+  if (!a) return fail(KF_ERR_INVALID_ARG, "args must be non-null");
+  if (int st = check_nodes(a->tokens, a->seqs)) return st;
+  if (a->tokens == 0) return KF_OK;
+  if (!a->parents || !a->cu_new || !a->seq_lens || !a->ancestors || !a->positions)
+    return fail(KF_ERR_INVALID_ARG, "every array must be non-null");
+  kf::DraftTreesArgs t;
+  t.parents = static_cast<const int*>(a->parents);
+  t.cu = static_cast<const int*>(a->cu_new);
+  t.seq_lens = static_cast<const int*>(a->seq_lens);
+  t.ancestors = static_cast<int64_t*>(a->ancestors);
+  t.positions = static_cast<int64_t*>(a->positions);
+  t.tokens = a->tokens, t.seqs = a->seqs;
+  return hip_status(kf::draft_trees_launch(t, static_cast<hipStream_t>(stream)), "draft_trees launch");
+}
+
+size_t kf_verify_drafts_workspace_bytes(const kf_verify_drafts_args* a) {
+  kf::VerifyArgs v;
+  if (!a || verify_args(*a, &v)) return 0;
+  return kf::verify_workspace_bytes(v);
+}
+
+int kf_verify_drafts(const kf_verify_drafts_args* a, void* ws, size_t ws_bytes, void* stream) {
+  if (!a) return fail(KF_ERR_INVALID_ARG, "args must be non-null");
+  kf::VerifyArgs v;
+  if (int st = verify_args(*a, &v)) return st;
+  if (!v.cu || !v.counts || !v.path || !v.emitted || (v.tokens_count && (!v.tokens || !v.parents || !v.target)) ||
+      (v.mode != KF_VERIFY_BEST && (!v.sample_u || (v.tokens_count && !v.accept_u))) ||
+      (v.mode == KF_VERIFY_DRAWN && v.tokens_count && !v.draft))
+    return fail(KF_ERR_INVALID_ARG, "every array must be non-null");
+  if (int st = check_workspace(ws, ws_bytes, kf::verify_workspace_bytes(v))) return st;
+  v.ws = ws;
+  return hip_status(kf::verify_launch(v, a->dtype, static_cast<hipStream_t>(stream)), "verify_drafts launch");
+}
+
+int kf_keep_drafts(const kf_keep_drafts_args* a, void* stream) {
+  if (!a) return fail(KF_ERR_INVALID_ARG, "args must be non-null");
+  if (a->arrays < 1 || a->num_pages < 1 || a->kv_heads < 1 || a->seqs < 1 || a->table_width < 1 || a->free_capacity < 0)
+    return fail(KF_ERR_INVALID_ARG, "need arrays, num_pages, kv_heads, seqs, table_width >= 1 and free_capacity >= 0, got %d, "
+                "%d, %d, %d, %d, %d", a->arrays, a->num_pages, a->kv_heads, a->seqs, a->table_width, a->free_capacity);
+  if (a->head_dim < 8 || a->head_dim % 8)
+    return fail(KF_ERR_UNSUPPORTED, "head_dim must be a multiple of 8, got %d", a->head_dim);
+  if (a->width < 1 || a->width > KF_MAX_NODES)
+    return fail(KF_ERR_INVALID_ARG, "paths have 1 to %d nodes, got %d", KF_MAX_NODES, a->width);
+  kf::KeepArgs k;
+  if (int st = check_block(a->block_size, &k.log2_block)) return st;
+  if ((int64_t)a->seqs * a->table_width >= (int64_t)1 << 31 || (int64_t)a->table_width << k.log2_block >= (int64_t)1 << 30)
+    return fail(KF_ERR_UNSUPPORTED, "%d tables of %d pages of %d tokens are too long", a->seqs, a->table_width, a->block_size);
+  if (!a->caches || !a->block_table || !a->context_lens || !a->seq_lens || !a->counts || !a->path ||
+      (a->free_count && ((!a->free_pages && a->free_capacity) || !a->free_left)))
+    return fail(KF_ERR_INVALID_ARG, "every array must be non-null");
+  if (!aligned(a->caches, 16)) return fail(KF_ERR_INVALID_ARG, "arrays must be 16-byte aligned");
+  const int64_t strides[] = {a->array_stride, a->page_stride, a->head_stride, a->token_stride};
+  if (int st = check_strides(strides, 4)) return st;
+  // Written while others still read their old values.
+  if ((a->kept_lens && (a->kept_lens == a->context_lens || a->kept_lens == a->seq_lens || a->kept_lens == a->counts)) ||
+      (a->free_count && a->free_left == a->free_count))
+    return fail(KF_ERR_INVALID_ARG, "kept_lens and free_left must be arrays of their own");
+  k.caches = a->caches;
+  k.table = static_cast<const int*>(a->block_table);
+  k.context_lens = static_cast<const int*>(a->context_lens);
+  k.seq_lens = static_cast<const int*>(a->seq_lens);
+  k.counts = static_cast<const int*>(a->counts);
+  k.path = static_cast<const int*>(a->path);
+  k.free_pages = static_cast<int*>(a->free_pages);
+  k.free_count = static_cast<const int*>(a->free_count);
+  k.kept_lens = static_cast<int*>(a->kept_lens);
+  k.free_left = static_cast<int*>(a->free_left);
+  k.array_stride = a->array_stride, k.page_stride = a->page_stride, k.head_stride = a->head_stride;
+  k.token_stride = a->token_stride, k.table_stride = a->table_stride, k.path_stride = a->path_stride;
+  k.arrays = a->arrays, k.num_pages = a->num_pages, k.kv_heads = a->kv_heads, k.head_dim = a->head_dim;
+  k.seqs = a->seqs, k.table_width = a->table_width, k.width = a->width, k.free_capacity = a->free_capacity;
+  return hip_status(kf::keep_drafts_launch(k, static_cast<hipStream_t>(stream)), "keep_drafts launch");
 }
 
 }  // extern "C"

@@ -311,6 +311,23 @@ __device__ __forceinline__ SeqKeys seq_keys(const AttnArgs& a, int s, int len) {
   return SeqKeys{PAGED ? min(n, a.table_width << a.log2_block) : n, n - len};
 }
 
+// The keys that a node of a tree of new tokens attends to: all that were there before them, and of the new ones, of which node j
+// is at key shift + j, those whose bit is set (64 at most).  Only tiles with new tokens' keys, the last of a request, ask.
+struct TreeRow {
+  uint64_t bits;
+  __device__ __forceinline__ bool sees(const SeqKeys& sk, int key) const {
+    const int node = key - sk.shift;
+    return key < sk.keys && (node < 0 || (node < 64 && (bits >> node & 1)));
+  }
+  // Bit e: key + e, e < 4.
+  __device__ __forceinline__ uint32_t four(const SeqKeys& sk, int key) const {
+    const int node = key - sk.shift, there = min(max(sk.keys - key, 0), 4);
+    const uint64_t old = 0xFull << min(max(-node, 0), 4);  // its low four bits: those of the new tokens among them
+    const uint64_t mine = node >= 64 ? 0 : node >= 0 ? bits >> node : bits << min(-node, 4);
+    return ((uint32_t)(mine & old) | ~(uint32_t)old) & ((1u << there) - 1);
+  }
+};
+
 // Tiles of BM rows over the packed sequences, numbered so that a tile finds its sequence without a scan: sequence
 // s owns the numbers from offset(s) * rep / BM + s on, enough for its rows, as
 // floor(a + b) + 1 >= floor(a) + ceil(b).  Returns the largest s <= seqs whose first number is at most t.

@@ -2,6 +2,8 @@
 //
 //   out[t, h] = sum_s softmax_s(scale q[t, h] . k[s, kv]) v[s, kv],   s <= position of t,   kv = h / rep
 //
+// or, where the new tokens are the nodes of a tree (TREE), over the s before them and the node's ancestors.
+//
 // What bounds it: the bytes of K and V, read once.  Three requests of up to 131071 tokens (8 KV heads of 128) take 204 us,
 // 6.3 TB/s of the 7.1 that a plain read of the card reaches; 64 of 100 .. 8191 tokens (2 of 128), 112 MB, take 25 us: 21 the
 // first launch, of which 15.8 at that rate, the rest finding the stretches until the first keys are there, and 4 the second.
@@ -71,7 +73,7 @@ struct FewShared {
 
 // Stretch `me` of `stretches`, by one workgroup.
 // CUT: items may be cut; otherwise every stretch is of whole ones, and nothing is left to join.
-template <class E, class C, bool CUT>
+template <class E, class C, bool CUT, bool TREE>
 __device__ __forceinline__ void few_rows_stretch(const AttnArgs& args, FewShared<C>& sh, int me, int stretches, int rep,
                                                  int max_rows, float scale_log2, float* ws, Piece* pieces) {
   constexpr int HDP = C::HDP, MT = C::MT;
@@ -171,11 +173,13 @@ __device__ __forceinline__ void few_rows_stretch(const AttnArgs& args, FewShared
     const int64_t table_at = (int64_t)seq * a.table_stride;
 
     u32x4 qf[MT][ST];
-    int limit[MT];
+    int limit[MT];     // the row's last key
+    TreeRow node[MT];  // TREE: its keys
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       const int row = min(row0 + 16 * t + l16, rows - 1), tok = row / rep, head = kv * rep + (row - tok * rep);
-      limit[t] = sk.last_key(tok);
+      if constexpr (TREE) node[t].bits = a.ancestors[tok0 + tok];
+      else limit[t] = sk.last_key(tok);
       const E* const qp = (const E*)a.q + (size_t)(tok0 + tok) * a.q_token + (size_t)head * a.q_head;
 #pragma unroll
       for (int s = 0; s < ST; ++s)
@@ -183,8 +187,9 @@ __device__ __forceinline__ void few_rows_stretch(const AttnArgs& args, FewShared
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) arrived(qf[t]);
-    const int kend = sk.last_key(min(row0 + C::ROWS - 1, rows - 1) / rep) + 1;  // keys of the tile's last row
-    const int first_limit = sk.last_key(row0 / rep);
+    // Keys of the tile's last row, the last that all its rows attend to.
+    const int kend = TREE ? sk.keys : sk.last_key(min(row0 + C::ROWS - 1, rows - 1) / rep) + 1;
+    const int first_limit = TREE ? sk.before() - 1 : sk.last_key(row0 / rep);
 
     auto page_of = [&](int key) {  // uniform; -1: not in the cache
       if (kend <= 0) return -1;
@@ -252,10 +257,17 @@ __device__ __forceinline__ void few_rows_stretch(const AttnArgs& args, FewShared
         if (masked) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const int last = keys_at(t, u);
+            if constexpr (TREE) {
+              const uint32_t seen = (u ? bad1 : bad0) ? 0 : node[t].four(sk, key0 + 16 * u + 4 * g);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (e > last) s[u][e] = -__builtin_inff();
+              for (int e = 0; e < 4; ++e)
+                if (!(seen >> e & 1)) s[u][e] = -__builtin_inff();
+            } else {
+              const int last = keys_at(t, u);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (e > last) s[u][e] = -__builtin_inff();
+            }
           }
         }
         float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
@@ -299,7 +311,7 @@ __device__ __forceinline__ void few_rows_stretch(const AttnArgs& args, FewShared
             float4_t add = {0.0f, 0.0f, 0.0f, 0.0f};  // of dims 16 c + 4 g + (0 .. 3)
 #pragma unroll 1
             for (int k = 0; k < 32; ++k)
-              if (key0 + k <= limit[t] && !(k >> 4 ? bad1 : bad0))
+              if ((TREE ? node[t].sees(sk, key0 + k) : key0 + k <= limit[t]) && !(k >> 4 ? bad1 : bad0))
                 add += nonfinite_of<E>(
                     lds_read8(v_tile + k * ROW + 16 * ((2 * c + (g >> 1)) ^ swizzle_v16<HDP>(k)) + 8 * (g & 1)));
             o[t][c] += add;

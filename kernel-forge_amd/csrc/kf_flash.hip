@@ -3,6 +3,8 @@
 //
 //   out[t, h] = sum_s softmax_s(scale q[t, h] . k[s, kv]) v[s, kv],   s <= position of t,   kv = h / rep
 //
+// or, over pages, where the new tokens are the nodes of a tree, over the s before them and the node's ancestors.
+//
 // A workgroup owns 128 rows of one KV head (kf_attn_tiles.h), 32 per wavefront, and walks their keys 64 at a time (32
 // for heads of more than 128, whose outputs fill half the registers) through two LDS buffers.  Scores, maximum, sum
 // and outputs are held in 32 bits; probabilities are rounded to the inputs' type for the second matrix product (half
@@ -35,6 +37,9 @@ constexpr int kFlashRows = 32 * kFlashWaves;
 // The kernel that cuts the work needs some registers more.
 constexpr int flash_waves_per_simd(int hdp, bool cut) { return hdp == 64 ? (cut ? 3 : 4) : hdp == 128 ? 2 : 1; }
 
+// Where the keys are: rows beside the queries' own, or pages of a cache; over pages the new tokens are a chain or a tree.
+enum class Keys { kPacked, kPages, kTree };
+
 // Two groups where their buffers fit.
 constexpr int flash_groups(int hdp) { return hdp == 256 ? 1 : 2; }
 
@@ -59,10 +64,11 @@ struct FlashShared {
 
 // Rows row0 .. + 127 of a sequence over its key tiles tile0 .. tiles - 1 (those that it has of them).
 // part: nullptr, or where the maximum, sum and unscaled outputs of an item that is cut go.
-template <class E, int HDP, bool PAGED, int GROUPS>
+template <class E, int HDP, Keys KEYS_OF, int GROUPS>
 __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, GROUPS>& sh, int rep, float scale_log2, int seq,
                                            int row0, int kv, int tile0, int tiles, float* part) {
   using C = FlashConfig<HDP>;
+  constexpr bool PAGED = KEYS_OF != Keys::kPacked, TREE = KEYS_OF == Keys::kTree;
   constexpr int ROW = C::ROW, KEYS = C::KEYS, KU = KEYS / 32, KK = KEYS / 16, TILE = C::TILE;
   constexpr int MINE = KEYS / kFlashWaves;          // keys of a tile that a wavefront fetches
   constexpr int ST = HDP / 16;                      // k steps of the first product
@@ -86,10 +92,13 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
   // Keys: positions before this lane's row's own, itself included.
   const SeqKeys sk = seq_keys<PAGED>(a, seq, len);
   const int limit = sk.last_key(tok);  // may be negative: no keys
+  TreeRow node;
+  if constexpr (TREE) node.bits = a.ancestors[tok0 + tok];
   const int wave_row = row0 + 32 * wave;
-  const int wave_lo = sk.last_key(min(wave_row, rows - 1) / rep), wave_hi = sk.last_key(min(wave_row + 31, rows - 1) / rep);
-  const int first_limit = sk.last_key(row0 / rep);  // the workgroup's first row's
-  const int kend = sk.last_key(min(row0 + kFlashRows - 1, rows - 1) / rep) + 1;
+  const int wave_lo = TREE ? sk.before() - 1 : sk.last_key(min(wave_row, rows - 1) / rep);
+  const int wave_hi = TREE ? sk.keys - 1 : sk.last_key(min(wave_row + 31, rows - 1) / rep);
+  const int first_limit = TREE ? sk.before() - 1 : sk.last_key(row0 / rep);  // the last key that all rows attend to
+  const int kend = TREE ? sk.keys : sk.last_key(min(row0 + kFlashRows - 1, rows - 1) / rep) + 1;
   tiles = min(tiles, kend <= 0 ? 0 : (kend + KEYS - 1) / KEYS);
   const int mine0 = tile0 + group;  // this group's first tile
 
@@ -227,10 +236,17 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
     if (__builtin_expect(masked, 0)) {
 #pragma unroll
       for (int q = 0; q < 2 * KK; ++q) {
-        const int last = keys_at(q);
+        if constexpr (TREE) {
+          const uint32_t seen = (bad >> (q >> 1)) & 1 ? 0 : node.four(sk, key0 + 8 * q + 4 * half);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e > last) s[q >> 2][4 * (q & 3) + e] = -__builtin_inff();
+          for (int e = 0; e < 4; ++e)
+            if (!(seen >> e & 1)) s[q >> 2][4 * (q & 3) + e] = -__builtin_inff();
+        } else {
+          const int last = keys_at(q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e > last) s[q >> 2][4 * (q & 3) + e] = -__builtin_inff();
+        }
       }
     }
 
@@ -323,7 +339,7 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
       } else {
         v += (int64_t)(tok0 + key) * b.v_token;
       }
-      if (key <= limit) add += nonfinite_of<E>(*reinterpret_cast<const u32x2*>(v));
+      if (TREE ? node.sees(sk, key) : key <= limit) add += nonfinite_of<E>(*reinterpret_cast<const u32x2*>(v));
     }
     return add;
   };
@@ -431,14 +447,14 @@ __device__ __forceinline__ bool longest_tile(const AttnArgs& a, int rep, int min
 }
 
 // One workgroup per row tile and KV head: `block` of `blocks`.
-template <class E, int HDP, bool PAGED, int GROUPS>
+template <class E, int HDP, Keys KEYS_OF, int GROUPS>
 __device__ __forceinline__ void flash_block(const AttnArgs& a, FlashShared<HDP, GROUPS>& sh, unsigned block, unsigned blocks,
                                             int rep, int min_rows, int longest_first, float scale_log2) {
   const int kv = (int)(block % a.kv_heads);
   const int numbers = (int)(blocks / a.kv_heads), number = (int)(block / a.kv_heads);
   int seq, tile, total;
   if (longest_first) {
-    if (!longest_tile<PAGED>(a, rep, min_rows, number, threadIdx.x & 63, &seq, &tile, &total)) {
+    if (!longest_tile<KEYS_OF != Keys::kPacked>(a, rep, min_rows, number, threadIdx.x & 63, &seq, &tile, &total)) {
       if (a.zero_rest && kv == 0)
         zero_rows<E>(a, (int64_t)(number - total) * GROUPS * kFlashThreads + threadIdx.x,
                      (int64_t)(numbers - total) * GROUPS * kFlashThreads);
@@ -461,14 +477,14 @@ __device__ __forceinline__ void flash_block(const AttnArgs& a, FlashShared<HDP, 
     if (tile * kFlashRows >= rows || rows < min_rows) return;
   }
   const int row0 = tile * kFlashRows;
-  flash_item<E, HDP, PAGED, GROUPS>(a, sh, rep, scale_log2, seq, row0, kv, 0, 0x7fffffff / FlashConfig<HDP>::KEYS, nullptr);
+  flash_item<E, HDP, KEYS_OF, GROUPS>(a, sh, rep, scale_log2, seq, row0, kv, 0, 0x7fffffff / FlashConfig<HDP>::KEYS, nullptr);
 }
 
-template <class E, int HDP, bool PAGED, int GROUPS>
+template <class E, int HDP, Keys KEYS_OF, int GROUPS>
 __global__ __launch_bounds__(GROUPS * kFlashThreads, flash_waves_per_simd(HDP, GROUPS > 1)) void flash_attention_kernel(
     AttnArgs a, int rep, int min_rows, int longest_first, float scale_log2) {
   __shared__ FlashShared<HDP, GROUPS> sh;
-  flash_block<E, HDP, PAGED, GROUPS>(a, sh, blockIdx.x, gridDim.x, rep, min_rows, longest_first, scale_log2);
+  flash_block<E, HDP, KEYS_OF, GROUPS>(a, sh, blockIdx.x, gridDim.x, rep, min_rows, longest_first, scale_log2);
 }
 
 // A batch of both kinds of requests in one launch: the first few_grid workgroups, of which two wavefronts work, take the
@@ -488,12 +504,12 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, false)) vo
   __shared__ MixedShared<HDP> sh;
   if ((int)blockIdx.x < few_grid) {  // zeros the rows behind the last request too
     if (threadIdx.x >= MixedFew<HDP>::THREADS) return;
-    few_rows_stretch<E, MixedFew<HDP>, true>(a, sh.few, (int)blockIdx.x, few_grid, rep, few_rows, scale_log2,
+    few_rows_stretch<E, MixedFew<HDP>, true, false>(a, sh.few, (int)blockIdx.x, few_grid, rep, few_rows, scale_log2,
                                          ws, pieces);
   } else {
     AttnArgs b = a;
     b.zero_rest = 0;
-    flash_block<E, HDP, true, 1>(b, sh.many, blockIdx.x - few_grid, gridDim.x - few_grid, rep,
+    flash_block<E, HDP, Keys::kPages, 1>(b, sh.many, blockIdx.x - few_grid, gridDim.x - few_grid, rep,
                                  few_rows + 1, longest_first, scale_log2);
   }
 }
@@ -519,9 +535,10 @@ __device__ __forceinline__ FlashWork flash_work(const AttnArgs& a, int s, int re
   return w;
 }
 
-template <class E, int HDP, bool PAGED>
+template <class E, int HDP, Keys KEYS_OF>
 __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) void flash_cut_kernel(
     AttnArgs args) {
+  constexpr bool PAGED = KEYS_OF != Keys::kPacked;
   __shared__ FlashShared<HDP, 1> sh;
   __shared__ int scan[kFlashWaves], found[2];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -592,7 +609,8 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
     const int item_at = head_at + (int)w.upto(tile), cost = w.base + 2 * (tile + 1);
     const int from = at - item_at, to = min(cost, end - item_at);
     const int row0 = tile * kFlashRows, len = w.rows / rep;
-    const int kend = seq_keys<PAGED>(a, seq, len).last_key(min(row0 + kFlashRows - 1, w.rows - 1) / rep) + 1;
+    const SeqKeys sk = seq_keys<PAGED>(a, seq, len);
+    const int kend = KEYS_OF == Keys::kTree ? sk.keys : sk.last_key(min(row0 + kFlashRows - 1, w.rows - 1) / rep) + 1;
     // The part's tiles: floor(position * tiles / cost), the same for a piece's end and the next one's beginning.
     const double tiles = max((kend + FlashConfig<HDP>::KEYS - 1) / FlashConfig<HDP>::KEYS, 1), each = cost;
     const int t0 = __builtin_amdgcn_readfirstlane((int)(from * tiles / each));
@@ -604,22 +622,22 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
     const bool whole = t0 == 0 && to == cost;
     float* const part = static_cast<float*>(a.ws) + (size_t)(2 * me + (t0 == 0 ? 1 : 0)) * kFlashRows * (HDP + 2);
     if (tid == 0 && t0 == 0 && !whole) static_cast<Piece*>(a.pieces)[me] = Piece{seq, row0, kv, last_stretch(item_at, cost, per)};
-    flash_item<E, HDP, PAGED, 1>(a, sh, rep, a.scale_log2, seq, row0, kv, t0, t1, whole ? nullptr : part);
+    flash_item<E, HDP, KEYS_OF, 1>(a, sh, rep, a.scale_log2, seq, row0, kv, t0, t1, whole ? nullptr : part);
     lds_barrier();  // the tiles have been read: the buffers are free
   }
 }
 
-template <class E, int HDP, bool PAGED>
+template <class E, int HDP, Keys KEYS_OF>
 hipError_t launch(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws, hipStream_t stream) {
   const int rep = a.heads / a.kv_heads;
   const float scale_log2 = a.scale * 1.44269504088896340736f;
   constexpr int GROUPS = flash_groups(HDP);
   if (!p.cut) {
     if (p.groups > 1)
-      flash_attention_kernel<E, HDP, PAGED, GROUPS>
+      flash_attention_kernel<E, HDP, KEYS_OF, GROUPS>
           <<<p.grid, GROUPS * kFlashThreads, 0, stream>>>(a, rep, min_rows, p.longest_first, scale_log2);
     else
-      flash_attention_kernel<E, HDP, PAGED, 1>
+      flash_attention_kernel<E, HDP, KEYS_OF, 1>
           <<<p.grid, kFlashThreads, 0, stream>>>(a, rep, min_rows, p.longest_first, scale_log2);
     return hipGetLastError();
   }
@@ -627,7 +645,7 @@ hipError_t launch(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws,
   Piece* const pieces = reinterpret_cast<Piece*>(parts + (size_t)2 * p.grid * kFlashRows * (HDP + 2));
   AttnArgs c = a;
   c.scale_log2 = scale_log2, c.rep = rep, c.min_rows = min_rows, c.ws = parts, c.pieces = pieces;
-  flash_cut_kernel<E, HDP, PAGED><<<p.grid, kFlashThreads, 0, stream>>>(c);
+  flash_cut_kernel<E, HDP, KEYS_OF><<<p.grid, kFlashThreads, 0, stream>>>(c);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   join_pieces_kernel<E, HDP, kFlashRows>
@@ -649,11 +667,11 @@ hipError_t launch_mixed(const AttnArgs& a, const FewPlan& f, const FlashPlan& p,
   return hipGetLastError();
 }
 
-template <class E, bool PAGED>
+template <class E, Keys KEYS_OF>
 hipError_t launch_dim(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws, hipStream_t stream) {
-  if (a.head_dim <= 64) return launch<E, 64, PAGED>(a, p, min_rows, ws, stream);
-  if (a.head_dim <= 128) return launch<E, 128, PAGED>(a, p, min_rows, ws, stream);
-  return launch<E, 256, PAGED>(a, p, min_rows, ws, stream);
+  if (a.head_dim <= 64) return launch<E, 64, KEYS_OF>(a, p, min_rows, ws, stream);
+  if (a.head_dim <= 128) return launch<E, 128, KEYS_OF>(a, p, min_rows, ws, stream);
+  return launch<E, 256, KEYS_OF>(a, p, min_rows, ws, stream);
 }
 
 }  // namespace
@@ -694,11 +712,14 @@ size_t flash_workspace_bytes(int head_dim, const FlashPlan& p) {
 
 hipError_t flash_attention_launch(const AttnArgs& a, bool paged, bool bf16, const FlashPlan& p, int min_rows, void* ws,
                                   hipStream_t stream) {
+  if (a.ancestors)
+    return bf16 ? launch_dim<bhalf_t, Keys::kTree>(a, p, min_rows, ws, stream)
+                : launch_dim<half_t, Keys::kTree>(a, p, min_rows, ws, stream);
   if (paged)
-    return bf16 ? launch_dim<bhalf_t, true>(a, p, min_rows, ws, stream)
-                : launch_dim<half_t, true>(a, p, min_rows, ws, stream);
-  return bf16 ? launch_dim<bhalf_t, false>(a, p, min_rows, ws, stream)
-              : launch_dim<half_t, false>(a, p, min_rows, ws, stream);
+    return bf16 ? launch_dim<bhalf_t, Keys::kPages>(a, p, min_rows, ws, stream)
+                : launch_dim<half_t, Keys::kPages>(a, p, min_rows, ws, stream);
+  return bf16 ? launch_dim<bhalf_t, Keys::kPacked>(a, p, min_rows, ws, stream)
+              : launch_dim<half_t, Keys::kPacked>(a, p, min_rows, ws, stream);
 }
 
 hipError_t mixed_attention_launch(const AttnArgs& a, bool bf16, const FewPlan& f, const FlashPlan& p, int few_rows, void* ws,

@@ -240,6 +240,7 @@ struct AttnArgs {
   int rep, min_rows;        // heads / kv_heads; sequences of fewer rows are not theirs
   void* ws;
   void* pieces;
+  const uint64_t* ancestors;  // paged, or nullptr: [tokens] bit j: the row attends to its request's new token j
 };
 struct FlashPlan {
   bool cut;    // the work of all row tiles is cut into equal stretches, and a second launch joins what was cut
@@ -249,7 +250,8 @@ struct FlashPlan {
 };
 FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count);
 size_t flash_workspace_bytes(int head_dim, const FlashPlan& p);
-// Requests of fewer than min_rows rows are left to the other kernel.  ws: flash_workspace_bytes, 16-byte aligned.
+// Requests of fewer than min_rows rows are left to the other kernel.  ws: flash_workspace_bytes, 16-byte aligned.  Both
+// launchers take trees of new tokens where a.ancestors is set, chains of them where it is not.
 hipError_t flash_attention_launch(const AttnArgs& a, bool paged, bool bf16, const FlashPlan& p, int min_rows, void* ws,
                                   hipStream_t stream);
 
@@ -303,6 +305,54 @@ struct RopePagedArgs {
   int tokens, heads, kv_heads, head_dim, max_pos, log2_block;
 };
 hipError_t rope_paged_launch(const RopePagedArgs& a, bool bf16, hipStream_t stream);
+
+// ---- decoding with drafted tokens (kf_drafts.hip) -----------------------------
+// cu: [seqs + 1] offsets of the requests' new tokens, the nodes of their trees; parents: [tokens] a node's parent by its number
+// in the request, which is smaller than the node's.
+struct DraftTreesArgs {
+  const int* parents;
+  const int* cu;
+  const int* seq_lens;      // [seqs] tokens of each request, the new ones included
+  int64_t* ancestors;       // [tokens] bit j: node j is the node itself or its ancestor
+  int64_t* positions;       // [tokens]
+  int tokens, seqs;
+};
+hipError_t draft_trees_launch(const DraftTreesArgs& a, hipStream_t stream);
+
+constexpr int kVerifyBest = 0, kVerifyGiven = 1, kVerifyDrawn = 2;  // == KF_VERIFY_* of the C ABI
+struct VerifyArgs {
+  const int64_t* tokens;    // [tokens_count]
+  const int* parents;
+  const int* cu;
+  const void* target;       // [tokens_count, vocab] scores, or fp32 probabilities, of what follows each node
+  const float* draft;       // drawn drafts: [tokens_count, vocab] what each node's children were drawn from
+  const float* accept_u;    // given and drawn drafts: [tokens_count]
+  const float* sample_u;    // ... and [seqs]
+  int* counts;              // [seqs]
+  int* path;                // [seqs, width]
+  int64_t* emitted;         // [seqs, width]
+  void* ws;
+  int64_t target_row, draft_row;
+  int mode, tokens_count, seqs, vocab, width;
+};
+size_t verify_workspace_bytes(const VerifyArgs& a);
+hipError_t verify_launch(const VerifyArgs& a, int dtype, hipStream_t stream);
+
+struct KeepArgs {
+  void* caches;             // [arrays, pages, kv_heads, block, d] of 16-bit values: strides (array, page, head, token)
+  const int* table;         // [seqs, table_width]
+  const int* context_lens;  // [seqs] tokens in the cache before the step
+  const int* seq_lens;      // [seqs] with the step's new ones
+  const int* counts;        // [seqs]
+  const int* path;          // [seqs, width], rows path_stride apart
+  int* free_pages;          // [free_capacity], a stack
+  const int* free_count;    // pages on it after the step's were taken; nullptr: none are given back
+  int* kept_lens;           // [seqs], or nullptr
+  int* free_left;
+  int64_t array_stride, page_stride, head_stride, token_stride, table_stride, path_stride;
+  int arrays, num_pages, kv_heads, head_dim, log2_block, seqs, table_width, width, free_capacity;
+};
+hipError_t keep_drafts_launch(const KeepArgs& a, hipStream_t stream);
 
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 

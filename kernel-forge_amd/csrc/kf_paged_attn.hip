@@ -7,49 +7,49 @@
 namespace kf {
 namespace {
 
-template <class E, class C, bool CUT>
+template <class E, class C, bool CUT, bool TREE>
 __global__ __launch_bounds__(C::THREADS) void few_rows_kernel(AttnArgs a, int rep, int max_rows, float scale_log2, float* ws,
                                                               Piece* pieces) {
   __shared__ FewShared<C> sh;
-  few_rows_stretch<E, C, CUT>(a, sh, (int)blockIdx.x, (int)gridDim.x, rep, max_rows, scale_log2, ws, pieces);
+  few_rows_stretch<E, C, CUT, TREE>(a, sh, (int)blockIdx.x, (int)gridDim.x, rep, max_rows, scale_log2, ws, pieces);
 }
 
-template <class E, int HDP, int MT, int WAVES>
+template <class E, int HDP, int MT, int WAVES, bool TREE>
 hipError_t launch(const AttnArgs& a, const FewPlan& p, int max_rows, void* ws, hipStream_t stream) {
   using C = FewConfig<HDP, MT, WAVES>;
   const int rep = a.heads / a.kv_heads;
   const float scale_log2 = a.scale * 1.44269504088896340736f;
   if (!p.cut) {
-    few_rows_kernel<E, C, false><<<p.grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, nullptr, nullptr);
+    few_rows_kernel<E, C, false, TREE><<<p.grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, nullptr, nullptr);
     return hipGetLastError();
   }
   float* const parts = static_cast<float*>(ws);
   Piece* const pieces = reinterpret_cast<Piece*>(parts + (size_t)2 * p.grid * C::ROWS * (HDP + 2));
-  few_rows_kernel<E, C, true><<<p.grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, parts, pieces);
+  few_rows_kernel<E, C, true, TREE><<<p.grid, C::THREADS, 0, stream>>>(a, rep, max_rows, scale_log2, parts, pieces);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   join_pieces_kernel<E, HDP, C::ROWS><<<join_grid<HDP, C::ROWS>(p.grid), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
   return hipGetLastError();
 }
 
-template <class E, int HDP>
+template <class E, int HDP, bool TREE>
 hipError_t launch_rows(const AttnArgs& a, const FewPlan& p, int max_rows, void* ws, hipStream_t stream) {
   if constexpr (HDP == 256) {  // one row tile of 256 dims fills the registers, two wavefronts the buffers
-    return launch<E, HDP, 1, 2>(a, p, max_rows, ws, stream);
+    return launch<E, HDP, 1, 2, TREE>(a, p, max_rows, ws, stream);
   } else {
     if (p.waves == 2)
-      return p.row_tiles == 2 ? launch<E, HDP, 2, 2>(a, p, max_rows, ws, stream)
-                              : launch<E, HDP, 1, 2>(a, p, max_rows, ws, stream);
-    return p.row_tiles == 2 ? launch<E, HDP, 2, 4>(a, p, max_rows, ws, stream)
-                            : launch<E, HDP, 1, 4>(a, p, max_rows, ws, stream);
+      return p.row_tiles == 2 ? launch<E, HDP, 2, 2, TREE>(a, p, max_rows, ws, stream)
+                              : launch<E, HDP, 1, 2, TREE>(a, p, max_rows, ws, stream);
+    return p.row_tiles == 2 ? launch<E, HDP, 2, 4, TREE>(a, p, max_rows, ws, stream)
+                            : launch<E, HDP, 1, 4, TREE>(a, p, max_rows, ws, stream);
   }
 }
 
-template <class E>
+template <class E, bool TREE>
 hipError_t launch_dim(const AttnArgs& a, const FewPlan& p, int max_rows, void* ws, hipStream_t stream) {
-  if (a.head_dim <= 64) return launch_rows<E, 64>(a, p, max_rows, ws, stream);
-  if (a.head_dim <= 128) return launch_rows<E, 128>(a, p, max_rows, ws, stream);
-  return launch_rows<E, 256>(a, p, max_rows, ws, stream);
+  if (a.head_dim <= 64) return launch_rows<E, 64, TREE>(a, p, max_rows, ws, stream);
+  if (a.head_dim <= 128) return launch_rows<E, 128, TREE>(a, p, max_rows, ws, stream);
+  return launch_rows<E, 256, TREE>(a, p, max_rows, ws, stream);
 }
 
 }  // namespace
@@ -86,7 +86,9 @@ size_t few_rows_workspace_bytes(int head_dim, const FewPlan& p) {
 }
 
 hipError_t few_rows_launch(const AttnArgs& a, bool bf16, const FewPlan& p, int max_rows, void* ws, hipStream_t stream) {
-  return bf16 ? launch_dim<bhalf_t>(a, p, max_rows, ws, stream) : launch_dim<half_t>(a, p, max_rows, ws, stream);
+  if (a.ancestors)
+    return bf16 ? launch_dim<bhalf_t, true>(a, p, max_rows, ws, stream) : launch_dim<half_t, true>(a, p, max_rows, ws, stream);
+  return bf16 ? launch_dim<bhalf_t, false>(a, p, max_rows, ws, stream) : launch_dim<half_t, false>(a, p, max_rows, ws, stream);
 }
 
 }  // namespace kf

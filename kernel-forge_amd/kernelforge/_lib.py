@@ -28,6 +28,8 @@ KF_NOALLOC_SCRATCH_BYTES = 32 << 20
 KF_GEMV_KERNEL_ROWS1, KF_GEMV_KERNEL_ROWS2, KF_GEMV_KERNEL_MIXED, KF_GEMV_KERNEL_SHAPED = 1, 2, 3, 4
 KF_GEMV_DEEP = 8
 KF_GEMV_FLAT = 16
+KF_VERIFY_BEST, KF_VERIFY_GIVEN, KF_VERIFY_DRAWN = 0, 1, 2
+KF_MAX_NODES = 64
 
 GEMV_MAX_GROUP = 8
 
@@ -85,6 +87,29 @@ class PagedAttentionArgs(ctypes.Structure):
         [("scale", ctypes.c_float), ("zero_rest", _I)]
 
 
+class DraftTreesArgs(ctypes.Structure):
+    """kf_draft_trees_args of include/kf_int4.h."""
+    _fields_ = [(n, _VP) for n in ("parents", "cu_new", "seq_lens", "ancestors", "positions")] + \
+        [(n, _I) for n in ("tokens", "seqs")]
+
+
+class VerifyDraftsArgs(ctypes.Structure):
+    """kf_verify_drafts_args of include/kf_int4.h."""
+    _fields_ = [(n, _VP) for n in ("tokens", "parents", "cu_new", "target", "draft", "accept_u", "sample_u", "counts",
+                                   "path", "emitted")] + \
+        [(n, _I64) for n in ("target_row", "draft_row")] + \
+        [(n, _I) for n in ("mode", "tokens_count", "seqs", "vocab", "width", "dtype")]
+
+
+class KeepDraftsArgs(ctypes.Structure):
+    """kf_keep_drafts_args of include/kf_int4.h."""
+    _fields_ = [(n, _VP) for n in ("caches", "block_table", "context_lens", "seq_lens", "counts", "path", "free_pages",
+                                   "free_count", "kept_lens", "free_left")] + \
+        [(n, _I64) for n in ("array_stride", "page_stride", "head_stride", "token_stride", "table_stride", "path_stride")] + \
+        [(n, _I) for n in ("arrays", "num_pages", "kv_heads", "head_dim", "block_size", "seqs", "table_width", "width",
+                           "free_capacity")]
+
+
 def packer(args: type[ctypes.Structure]):
     """A function that packs the fields' values, in order, into the structure's bytes, for a parameter that is a
     pointer to it: in half the time that ctypes takes to fill a structure of 30 fields (1.3 and 2.7 us), and a value that
@@ -105,6 +130,9 @@ pack_paged_tables = packer(PagedTablesArgs)
 pack_rope_paged = packer(RopePagedArgs)
 pack_prompt_attention = packer(PromptAttentionArgs)
 pack_paged_attention = packer(PagedAttentionArgs)
+pack_draft_trees = packer(DraftTreesArgs)
+pack_verify_drafts = packer(VerifyDraftsArgs)
+pack_keep_drafts = packer(KeepDraftsArgs)
 
 # The paged operators take their structure as an address (_VP): packed bytes, or a structure by reference.
 SIGNATURES = {
@@ -138,6 +166,12 @@ SIGNATURES = {
     "kf_prompt_attention": (_I, [_VP, _VP, _SZ, _VP]),
     "kf_paged_attention_workspace_bytes": (_SZ, [_VP]),
     "kf_paged_attention": (_I, [_VP, _VP, _SZ, _VP]),
+    "kf_draft_trees": (_I, [_VP, _VP]),
+    "kf_paged_tree_attention_workspace_bytes": (_SZ, [_VP]),
+    "kf_paged_tree_attention": (_I, [_VP, _VP, _VP, _SZ, _VP]),
+    "kf_verify_drafts_workspace_bytes": (_SZ, [_VP]),
+    "kf_verify_drafts": (_I, [_VP, _VP, _SZ, _VP]),
+    "kf_keep_drafts": (_I, [_VP, _VP]),
     "kf_decode_argmax_step": (_I, [_VP, _I, _VP, _VP, _VP, _I, _VP, _VP]),
 }
 

@@ -1233,7 +1233,17 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
                 and block_table.dtype == i32 and cu_new.dtype == i32 and seq_lens.dtype == i32 and cu_new.shape == (b + 1,)
                 and seq_lens.shape == (b,) and cu_new.is_contiguous() and seq_lens.is_contiguous()
                 and (max_new is None or max_new > 0)):
-            return _run_paged(*tensors, int(max_new or 0), _check_scale(scale, d), q.new_empty((t, heads, d)), True)
+            return _run_paged(*tensors, None, int(max_new or 0), _check_scale(scale, d), q.new_empty((t, heads, d)), True)
+    scale = _check_paged(*tensors, max_new, scale, out, "paged_attention")
+    if _traced(tensors):
+        if out is not None:
+            raise RuntimeError("paged_attention with out updates it in place and has no traceable form")
+        return _paged_attention_op(*tensors, int(max_new or 0), scale)
+    return _launch_paged(*tensors, None, int(max_new or 0), scale, out)
+
+
+def _check_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scale, out, what: str) -> float:
+    """The checks of paged_attention and paged_tree_attention one by one; returns the scale."""
     if q.dim() != 3 or q.dtype not in _HALF_TYPES:
         raise TypeError("q must be a 3-D fp16 or bf16 tensor [T, heads, head_dim]")
     _check_cache(cache_k, cache_v, q.dtype)
@@ -1245,24 +1255,22 @@ def paged_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tenso
     _check_int("cu_new", cu_new, torch.int32, (b + 1,))
     _check_table(block_table, b)
     if b < 1:
-        raise ValueError("paged_attention needs at least one request")
+        raise ValueError(f"{what} needs at least one request")
     if max_new is not None and max_new < 1:
         raise ValueError(f"max_new must be positive, got {max_new}")
     scale = _check_scale(scale, q.shape[2])
     _check_out(out, q)
-    _check_plain("paged_attention", tensors if out is None else (*tensors, out))
-    if _traced(tensors):
-        if out is not None:
-            raise RuntimeError("paged_attention with out updates it in place and has no traceable form")
-        return _paged_attention_op(*tensors, int(max_new or 0), scale)
-    return _launch_paged(*tensors, int(max_new or 0), scale, out)
+    tensors = (q, cache_k, cache_v, block_table, cu_new, seq_lens)
+    _check_plain(what, tensors if out is None else (*tensors, out))
+    return scale
 
 
-def _launch_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scale, out=None):
+def _launch_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, ancestors, max_new, scale, out=None):
     dev = q.device
     for name, t in (("q", q), ("cache_k", cache_k), ("cache_v", cache_v), ("block_table", block_table),
-                    ("cu_new", cu_new), ("seq_lens", seq_lens)):
-        _check_memory(name, t, dev)
+                    ("cu_new", cu_new), ("seq_lens", seq_lens), ("ancestors", ancestors)):
+        if t is not None:
+            _check_memory(name, t, dev)
     if not _rows_ok(q):
         q = q.clone(memory_format=torch.contiguous_format)
     zero_rest = out is None
@@ -1271,11 +1279,11 @@ def _launch_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, s
     if q.shape[0] == 0:
         return out
     with _on(dev):
-        return _run_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scale, out, zero_rest)
+        return _run_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, ancestors, max_new, scale, out, zero_rest)
 
 
-def _run_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scale, out, zero_rest):
-    """kf_paged_attention on checked arguments of the current device."""
+def _run_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, ancestors, max_new, scale, out, zero_rest):
+    """kf_paged_attention (kf_paged_tree_attention with ancestors) on checked arguments of the current device."""
     t, heads, d = q.shape
     pages, kv_heads, block_size, _ = cache_k.shape
     q_token, q_head, _ = q.stride()
@@ -1288,21 +1296,402 @@ def _run_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scal
                                      block_table.stride(0), t, seq_lens.numel(), heads, kv_heads, d, _HALF_TYPES[q.dtype],
                                      block_table.shape[1], pages, block_size, max_new, scale, zero_rest)
     lib = _lib.load()
-    ws_bytes = lib.kf_paged_attention_workspace_bytes(args)
-    ws = q.new_empty((ws_bytes + 1) // 2) if ws_bytes else None  # two bytes a value
-    status = lib.kf_paged_attention(args, ws.data_ptr() if ws is not None else None, ws_bytes,
-                                    torch._C._cuda_getCurrentRawStream(q.get_device()))
+    stream = torch._C._cuda_getCurrentRawStream(q.get_device())
+    if ancestors is None:
+        ws_bytes = lib.kf_paged_attention_workspace_bytes(args)
+        ws = q.new_empty((ws_bytes + 1) // 2) if ws_bytes else None  # two bytes a value
+        status = lib.kf_paged_attention(args, ws.data_ptr() if ws is not None else None, ws_bytes, stream)
+    else:
+        ws_bytes = lib.kf_paged_tree_attention_workspace_bytes(args)
+        ws = q.new_empty((ws_bytes + 1) // 2) if ws_bytes else None
+        status = lib.kf_paged_tree_attention(args, ancestors.data_ptr(), ws.data_ptr() if ws is not None else None, ws_bytes,
+                                             stream)
     if status:
-        _lib.check(status, "paged_attention")
+        _lib.check(status, "paged_attention" if ancestors is None else "paged_tree_attention")
     return out
 
 
 @torch.library.custom_op("kernelforge::paged_attention", mutates_args=())
 def _paged_attention_op(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, block_table: torch.Tensor,
                         cu_new: torch.Tensor, seq_lens: torch.Tensor, max_new: int, scale: float) -> torch.Tensor:
-    return _launch_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scale)
+    return _launch_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, None, max_new, scale)
 
 
 @_paged_attention_op.register_fake
 def _(q, cache_k, cache_v, block_table, cu_new, seq_lens, max_new, scale):
     return q.new_empty(q.shape)
+
+
+# ---- decoding with drafted tokens -----------------------------------------------------------------------
+#
+# A request's new tokens in a step are the nodes of a tree: node 0 is its pending token, which the cache does not hold yet, the
+# others are drafted continuations.  parents int32 [T] names each node's parent by its number in the request, which is smaller than
+# the node's own (another value: a root).  A request has up to MAX_NODES nodes.  One step of a server is paged_tables, draft_trees,
+# per layer rope_paged_cache (with DraftTrees.positions) and paged_tree_attention, then verify_drafts and keep_drafts.  Inference
+# only.
+
+MAX_NODES = _lib.KF_MAX_NODES
+
+
+class DraftTrees(NamedTuple):
+    """What draft_trees makes of a step's parents."""
+
+    ancestors: torch.Tensor  # int64 [T]: bit j: node j of the request is the row's node or its ancestor
+    positions: torch.Tensor  # int64 [T]: tokens before the row's, its ancestors among them; -1 for rows that are no node
+
+
+class VerifiedDrafts(NamedTuple):
+    """What verify_drafts decides for every request."""
+
+    counts: torch.Tensor  # int32 [B]: nodes on the path, node 0 among them, and tokens emitted; 0 without new tokens
+    path: torch.Tensor    # int32 [B, width]: the path's nodes, -1 behind them
+    tokens: torch.Tensor  # int64 [B, width]: the accepted drafted tokens and the one that follows them, -1 behind
+
+
+class KeptDrafts(NamedTuple):
+    """Lengths and pages after keep_drafts."""
+
+    context_lens: torch.Tensor         # int32 [B]: tokens that the cache holds
+    free_count: Optional[torch.Tensor]  # int32 [1]: pages on the stack (None without one)
+
+
+def draft_trees(parents: torch.Tensor, cu_new: torch.Tensor, seq_lens: torch.Tensor) -> DraftTrees:
+    """The ancestors and positions of drafted nodes, from their parents, in one launch (kf_draft_trees).
+
+    parents int32 [T]; cu_new int32 [B + 1] and seq_lens int32 [B] as paged_tables gives them (PagedStep): request r's nodes are
+    rows cu_new[r] .. cu_new[r + 1] - 1, the last of its seq_lens[r] tokens. A node's position is that of the request's first new
+    token plus its depth. Rows behind the last request and nodes past the 64th have no ancestors and position -1, for which
+    rope_paged_cache writes no cache entry. No reference counterpart.
+    """
+    args = (parents, cu_new, seq_lens)
+    i32 = torch.int32
+    if not (_direct(parents.get_device(), args) and parents.dim() == 1 and seq_lens.dim() == 1 and parents.dtype == i32
+            and cu_new.dtype == i32 and seq_lens.dtype == i32 and cu_new.shape == (seq_lens.shape[0] + 1,)
+            and seq_lens.shape[0] > 0 and parents.is_contiguous() and cu_new.is_contiguous() and seq_lens.is_contiguous()):
+        _check_int("parents", parents, i32, (parents.numel(),))
+        _check_int("seq_lens", seq_lens, i32, (seq_lens.numel(),))
+        _check_int("cu_new", cu_new, i32, (seq_lens.numel() + 1,))
+        if seq_lens.numel() < 1:
+            raise ValueError("draft_trees needs at least one request")
+        _check_plain("draft_trees", args)
+        if _traced(args):
+            return DraftTrees(*_draft_trees_op(*args))
+        for name, t in zip(("parents", "cu_new", "seq_lens"), args):
+            _check_memory(name, t, parents.device)
+        with _on(parents.device):
+            return _run_draft_trees(*args)
+    return _run_draft_trees(*args)
+
+
+def _run_draft_trees(parents, cu_new, seq_lens) -> DraftTrees:
+    """kf_draft_trees on checked arguments of the current device."""
+    t = parents.shape[0]
+    odd = t & 1  # both start at 16 bytes, as rope_paged_cache takes positions
+    positions, _, ancestors = parents.new_empty(2 * t + odd, dtype=torch.int64).split_with_sizes((t, odd, t))
+    args = _lib.pack_draft_trees(parents.data_ptr(), cu_new.data_ptr(), seq_lens.data_ptr(), ancestors.data_ptr(),
+                                 positions.data_ptr(), t, seq_lens.shape[0])
+    status = _lib.load().kf_draft_trees(args, torch._C._cuda_getCurrentRawStream(parents.get_device()))
+    if status:
+        _lib.check(status, "draft_trees")
+    return DraftTrees(ancestors, positions)
+
+
+@torch.library.custom_op("kernelforge::draft_trees", mutates_args=())
+def _draft_trees_op(parents: torch.Tensor, cu_new: torch.Tensor, seq_lens: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    return tuple(t.clone() for t in draft_trees(parents, cu_new, seq_lens))  # an op's outputs must not be views of one tensor
+
+
+@_draft_trees_op.register_fake
+def _(parents, cu_new, seq_lens):
+    return (parents.new_empty(parents.shape, dtype=torch.int64), parents.new_empty(parents.shape, dtype=torch.int64))
+
+
+def paged_tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, block_table: torch.Tensor,
+                         cu_new: torch.Tensor, seq_lens: torch.Tensor, ancestors: torch.Tensor, *,
+                         max_new: int | None = None, scale: float | None = None,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted tokens, the nodes of a tree per request, over the request's pages (kf_paged_tree_attention).
+
+    The arguments of paged_attention and ancestors int64 [T] (DraftTrees.ancestors): a row attends to the tokens of its request
+    before the new ones, and to new token j where bit j of its word is set, itself only if its own bit is; any bits are taken. New
+    tokens past the 64th are attended to by none. All else as in paged_attention, whose result this is for words
+    that say a chain. No reference counterpart.
+    """
+    tensors = (q, cache_k, cache_v, block_table, cu_new, seq_lens, ancestors)
+    if (_direct(q.get_device(), tensors) and out is None and q.dim() == 3 and block_table.dim() == 2
+            and _caches_ok(cache_k, cache_v, q.dtype)):
+        t, heads, d = q.shape
+        _, kv_heads, _, kd = cache_k.shape
+        b, width = block_table.shape
+        a, c, one = q.stride()
+        i32 = torch.int32
+        if (d == kd and t > 0 and heads > 0 and heads % kv_heads == 0 and d <= _ATTN_MAX_HEAD_DIM and not d & 7 and one == 1
+                and not (a | c) & 7 and not q.data_ptr() & 15 and b > 0 and width > 0 and block_table.stride(1) == 1
+                and block_table.dtype == i32 and cu_new.dtype == i32 and seq_lens.dtype == i32 and cu_new.shape == (b + 1,)
+                and seq_lens.shape == (b,) and cu_new.is_contiguous() and seq_lens.is_contiguous()
+                and ancestors.shape == (t,) and ancestors.dtype == torch.int64 and ancestors.is_contiguous()
+                and (max_new is None or max_new > 0)):
+            return _run_paged(*tensors, int(max_new or 0), _check_scale(scale, d), q.new_empty((t, heads, d)), True)
+    if q.dim() == 3:
+        _check_int("ancestors", ancestors, torch.int64, (q.shape[0],))
+    scale = _check_paged(*tensors[:6], max_new, scale, out, "paged_tree_attention")
+    _check_plain("paged_tree_attention", (ancestors,))
+    if _traced(tensors):
+        if out is not None:
+            raise RuntimeError("paged_tree_attention with out updates it in place and has no traceable form")
+        return _paged_tree_attention_op(*tensors, int(max_new or 0), scale)
+    return _launch_paged(*tensors, int(max_new or 0), scale, out)
+
+
+@torch.library.custom_op("kernelforge::paged_tree_attention", mutates_args=())
+def _paged_tree_attention_op(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, block_table: torch.Tensor,
+                             cu_new: torch.Tensor, seq_lens: torch.Tensor, ancestors: torch.Tensor, max_new: int,
+                             scale: float) -> torch.Tensor:
+    return _launch_paged(q, cache_k, cache_v, block_table, cu_new, seq_lens, ancestors, max_new, scale)
+
+
+@_paged_tree_attention_op.register_fake
+def _(q, cache_k, cache_v, block_table, cu_new, seq_lens, ancestors, max_new, scale):
+    return q.new_empty(q.shape)
+
+
+def verify_drafts(tokens: torch.Tensor, parents: torch.Tensor, cu_new: torch.Tensor, target: torch.Tensor,
+                  accept_uniforms: torch.Tensor | None = None, sample_uniforms: torch.Tensor | None = None, *,
+                  draft: torch.Tensor | None = None, max_new: int | None = None) -> VerifiedDrafts:
+    """Which drafted tokens stay, and the token behind them, for every request (kf_verify_drafts).
+
+    tokens int64 [T] and parents int32 [T]: the nodes; row t of target [T, vocab] says what follows node t. The path begins with
+    the request's node 0 and goes on with the child of the lowest number that is accepted, until none is:
+
+    * greedy, without uniforms: target holds scores (fp32, fp16 or bf16). A child is accepted if its token is the index of the
+      largest (the first of equal ones, NaN above all numbers); that index follows the path.
+    * sampled: target holds probabilities (fp32, rows summing to 1). accept_uniforms fp32 [T] (one a node) and sample_uniforms fp32
+      [B] are uniform random numbers in [0, 1), independent of each other and of the drafts. Emitted tokens are then distributed
+      as tokens drawn from target one by one. Without ``draft`` a node's children are taken as they are, accepted in turn with what
+      is left of their parent's mass; with draft fp32 [T, vocab] they were drawn, independently of each other, from row t of it, and
+      are accepted with max(p - a q, 0) / (m q). The token behind the path is drawn from what is left: the first index
+      at which the running sum passes the uniform number times the whole. Sums in 64 bits; NaN and negative probabilities count as 0.
+
+    max_new: nodes of a request that are looked at, and the width of the results (64, the most, without it). Tokens outside
+    the vocabulary are never accepted. Rows of target and draft may be strided. Results do not change from run to run. The form
+    of decode_argmax_step for drafts; no reference counterpart.
+    """
+    sampled = accept_uniforms is not None or sample_uniforms is not None
+    tensors = [tokens, parents, cu_new, target]
+    if sampled:
+        if accept_uniforms is None or sample_uniforms is None:
+            raise ValueError("accept_uniforms and sample_uniforms come together")
+        tensors += [accept_uniforms, sample_uniforms]
+    if draft is not None:
+        if not sampled:
+            raise ValueError("draft needs accept_uniforms and sample_uniforms")
+        tensors.append(draft)
+    if max_new is not None and max_new < 1:
+        raise ValueError(f"max_new must be positive, got {max_new}")
+    width = min(max_new or MAX_NODES, MAX_NODES)
+    f32, i32 = torch.float32, torch.int32
+    if _direct(tokens.get_device(), tensors) and target.dim() == 2 and cu_new.dim() == 1:
+        t, vocab = target.shape
+        b = cu_new.shape[0] - 1
+        if (tokens.shape == (t,) and parents.shape == (t,) and b > 0 and t > 0 and vocab > 0 and target.stride(1) == 1
+                and tokens.dtype == torch.int64 and parents.dtype == i32 and cu_new.dtype == i32
+                and tokens.is_contiguous() and parents.is_contiguous() and cu_new.is_contiguous()
+                and (target.dtype == f32 or (not sampled and target.dtype in _QUANT_DTYPES))
+                and (not sampled or (accept_uniforms.dtype == f32 and sample_uniforms.dtype == f32
+                                     and accept_uniforms.shape == (t,) and sample_uniforms.shape == (b,)
+                                     and accept_uniforms.is_contiguous() and sample_uniforms.is_contiguous()))
+                and (draft is None or (draft.dtype == f32 and draft.shape == (t, vocab) and draft.stride(1) == 1))):
+            return _run_verify(tokens, parents, cu_new, target, accept_uniforms, sample_uniforms, draft, width)
+    if target.dim() != 2 or target.dtype not in _QUANT_DTYPES or (sampled and target.dtype != f32):
+        raise TypeError("target must be 2-D [T, vocab]: fp32, fp16 or bf16 scores, or fp32 probabilities, got "
+                        f"{str(target.dtype)[6:]} {list(target.shape)}")
+    t, vocab = target.shape
+    b = cu_new.numel() - 1
+    _check_int("tokens", tokens, torch.int64, (t,))
+    _check_int("parents", parents, i32, (t,))
+    _check_int("cu_new", cu_new, i32, (b + 1,))
+    if b < 1 or vocab < 1:
+        raise ValueError(f"verify_drafts needs at least one request and one token, got {b} and {vocab}")
+    if sampled:
+        _check_int("accept_uniforms", accept_uniforms, f32, (t,))
+        _check_int("sample_uniforms", sample_uniforms, f32, (b,))
+    if draft is not None and (draft.dtype != f32 or draft.shape != target.shape):
+        raise ValueError(f"draft must be float32 {list(target.shape)}, got {str(draft.dtype)[6:]} {list(draft.shape)}")
+    _check_plain("verify_drafts", tensors)
+    args = (tokens, parents, cu_new, target, accept_uniforms, sample_uniforms, draft, width)
+    return VerifiedDrafts(*(_verify_drafts_op(*args) if _traced(tensors) else _launch_verify(*args)))
+
+
+def _launch_verify(tokens, parents, cu_new, target, accept_uniforms, sample_uniforms, draft, width):
+    dev = target.device
+    for name, t in (("target", target), ("tokens", tokens), ("parents", parents), ("cu_new", cu_new),
+                    ("accept_uniforms", accept_uniforms), ("sample_uniforms", sample_uniforms), ("draft", draft)):
+        if t is not None:
+            _check_memory(name, t, dev)
+    target, draft = (x if x is None or x.stride(1) == 1 else x.contiguous() for x in (target, draft))
+    with _on(dev):
+        return _run_verify(tokens, parents, cu_new, target, accept_uniforms, sample_uniforms, draft, width)
+
+
+def _run_verify(tokens, parents, cu_new, target, accept_uniforms, sample_uniforms, draft, width) -> VerifiedDrafts:
+    """kf_verify_drafts on checked arguments of the current device."""
+    t, vocab = target.shape
+    b = cu_new.shape[0] - 1
+    counts, path = parents.new_empty(b * (width + 1)).split_with_sizes((b, b * width))
+    emitted = tokens.new_empty((b, width))
+    sampled = accept_uniforms is not None
+    mode = _lib.KF_VERIFY_BEST if not sampled else _lib.KF_VERIFY_GIVEN if draft is None else _lib.KF_VERIFY_DRAWN
+    args = _lib.pack_verify_drafts(tokens.data_ptr(), parents.data_ptr(), cu_new.data_ptr(), target.data_ptr(),
+                                   draft.data_ptr() if draft is not None else 0,
+                                   accept_uniforms.data_ptr() if sampled else 0, sample_uniforms.data_ptr() if sampled else 0,
+                                   counts.data_ptr(), path.data_ptr(), emitted.data_ptr(), target.stride(0),
+                                   draft.stride(0) if draft is not None else 0, mode, t, b, vocab, width,
+                                   _QUANT_DTYPES[target.dtype])
+    lib = _lib.load()
+    ws_bytes = lib.kf_verify_drafts_workspace_bytes(args)
+    ws = tokens.new_empty((ws_bytes + 7) // 8) if ws_bytes else None
+    status = lib.kf_verify_drafts(args, ws.data_ptr() if ws is not None else None, ws_bytes,
+                                  torch._C._cuda_getCurrentRawStream(tokens.get_device()))
+    if status:
+        _lib.check(status, "verify_drafts")
+    return VerifiedDrafts(counts, path.view(b, width), emitted)
+
+
+@torch.library.custom_op("kernelforge::verify_drafts", mutates_args=())
+def _verify_drafts_op(tokens: torch.Tensor, parents: torch.Tensor, cu_new: torch.Tensor, target: torch.Tensor,
+                      accept_uniforms: Optional[torch.Tensor], sample_uniforms: Optional[torch.Tensor],
+                      draft: Optional[torch.Tensor], width: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    counts, path, emitted = _launch_verify(tokens, parents, cu_new, target, accept_uniforms, sample_uniforms, draft, width)
+    return counts.clone(), path.clone(), emitted
+
+
+@_verify_drafts_op.register_fake
+def _(tokens, parents, cu_new, target, accept_uniforms, sample_uniforms, draft, width):
+    b = cu_new.shape[0] - 1
+    return parents.new_empty(b), parents.new_empty(b, width), tokens.new_empty(b, width)
+
+
+def keep_drafts(caches: torch.Tensor | list[torch.Tensor], block_table: torch.Tensor, context_lens: torch.Tensor,
+                seq_lens: torch.Tensor, counts: torch.Tensor, path: torch.Tensor, free_pages: torch.Tensor | None = None,
+                free_count: torch.Tensor | None = None) -> KeptDrafts:
+    """What is kept of a step's drafts in the cache, in one launch (kf_keep_drafts).
+
+    caches [..., num_pages, kv_heads, block_size, head_dim], fp16 or bf16: all arrays of all layers (TinyLlama.new_paged_cache), or
+    a list of such tensors, a launch each. context_lens, seq_lens int32 [B]: tokens before the step and with its new ones; counts
+    int32 [B] and path int32 [B, width] of verify_drafts. The entry of node path[r, i] moves to place context_lens[r] + i, i <
+    counts[r]; that many tokens are kept. With a stack, free_pages int32 [F] and free_count int32 [1] (PagedStep's), the pages that
+    held other nodes alone go back onto it, as far as it has room: free_pages is written, free_count is not, KeptDrafts has the new
+    one. block_table keeps their numbers, where paged_tables enters new ones. Pages must not be shared between requests.
+    No reference counterpart.
+    """
+    listed = [caches] if isinstance(caches, torch.Tensor) else list(caches)
+    if not listed:
+        raise ValueError("keep_drafts needs at least one cache")
+    if (free_pages is None) != (free_count is None):
+        raise ValueError("free_pages and free_count come together")
+    stack = () if free_pages is None else (free_pages, free_count)
+    tables = (block_table, context_lens, seq_lens, counts, path, *stack)
+    i32 = torch.int32
+    direct = _direct(block_table.get_device(), (*listed, *tables)) and block_table.dim() == 2
+    if direct:
+        b, width = block_table.shape
+        direct = (b > 0 and width > 0 and block_table.stride(1) == 1 and path.dim() == 2 and path.shape[0] == b
+                  and 0 < path.shape[1] <= MAX_NODES and path.stride(1) == 1
+                  and context_lens.shape == (b,) and seq_lens.shape == (b,) and counts.shape == (b,)
+                  and context_lens.is_contiguous() and seq_lens.is_contiguous() and counts.is_contiguous()
+                  and all(t.dtype == i32 for t in tables)
+                  and (not stack or (free_pages.dim() == 1 and free_pages.is_contiguous() and free_count.shape == (1,)))
+                  and all(_kept_cache_ok(c) for c in listed))
+    if not direct:
+        b = block_table.shape[0] if block_table.dim() == 2 else -1
+        _check_table(block_table, b)
+        if b < 1:
+            raise ValueError("keep_drafts needs at least one request")
+        for name, t in (("context_lens", context_lens), ("seq_lens", seq_lens), ("counts", counts)):
+            _check_int(name, t, i32, (b,))
+        if (path.dim() != 2 or path.dtype != i32 or path.shape[0] != b or not 0 < path.shape[1] <= MAX_NODES
+                or path.stride(1) != 1):
+            raise ValueError(f"path must be int32 [{b}, up to {MAX_NODES}] with contiguous rows, got {str(path.dtype)[6:]} "
+                             f"{list(path.shape)}")
+        if stack:
+            _check_int("free_count", free_count, i32, (1,))
+            if free_pages.dtype != i32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
+                raise ValueError("free_pages must be a contiguous 1-D int32 tensor")
+        _check_plain("keep_drafts", (*listed, *tables))
+        for cache in listed:
+            _check_kept_cache(cache)
+    kept = None
+    for i, cache in enumerate(listed):
+        arrays = cache if cache.dim() == 5 else cache.flatten(0, -5) if cache.dim() > 5 else cache[None]
+        args = (arrays, *tables[:5], *((free_pages, free_count) if stack and i == 0 else (None, None)))
+        if direct:
+            lens = _run_keep(*args)
+        else:
+            lens = (_keep_drafts_op if _traced((*listed, *tables)) else _launch_keep)(*args)
+        kept = lens if i == 0 else kept
+    return KeptDrafts(kept[:b], kept[b:] if stack else None)
+
+
+def _one_stride(t: torch.Tensor) -> bool:
+    """Whether all dimensions but the last four are one of constant stride."""
+    return all(t.stride(i) == t.stride(i + 1) * t.shape[i + 1] for i in range(t.dim() - 5))
+
+
+def _kept_cache_ok(t: torch.Tensor) -> bool:
+    return (t.dim() >= 4 and t.dtype in _HALF_TYPES and t.numel() > 0 and _rows_ok(t) and _own_places(t) and _one_stride(t)
+            and 16 <= t.shape[-2] <= 1 << 20 and not t.shape[-2] & (t.shape[-2] - 1) and not t.shape[-1] & 7)
+
+
+def _check_kept_cache(t: torch.Tensor) -> None:
+    if t.dim() < 4 or t.numel() == 0:
+        raise ValueError("caches must be [..., num_pages, kv_heads, block_size, head_dim] and not empty, got "
+                         f"{list(t.shape)}")
+    if t.dtype not in _HALF_TYPES:
+        raise TypeError(f"caches must be fp16 or bf16, got {str(t.dtype)[6:]}")
+    _check_block_size(t.shape[-2])
+    if t.shape[-1] % 8:
+        raise ValueError(f"head_dim must be a multiple of 8, got {t.shape[-1]}")
+    if not _rows_ok(t) or not _own_places(t) or not _one_stride(t):
+        raise ValueError("caches must have a contiguous last dimension, other strides of multiples of 8, none of them 0, leading "
+                         "dimensions that are one, and a 16-byte aligned start")
+
+
+def _launch_keep(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count):
+    dev = caches.device
+    for name, t in (("caches", caches), ("block_table", block_table), ("context_lens", context_lens),
+                    ("seq_lens", seq_lens), ("counts", counts), ("path", path), ("free_pages", free_pages),
+                    ("free_count", free_count)):
+        if t is not None:
+            _check_memory(name, t, dev)
+    with _on(dev):
+        return _run_keep(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count)
+
+
+def _run_keep(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count) -> torch.Tensor:
+    """kf_keep_drafts on checked arguments of the current device; the new lengths and the stack's count in one tensor."""
+    arrays, pages, kv_heads, block_size, d = caches.shape
+    array, page, head, token, _ = caches.stride()
+    b = block_table.shape[0]
+    kept = context_lens.new_empty(b + 1)
+    stack = free_count is not None
+    args = _lib.pack_keep_drafts(caches.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(), seq_lens.data_ptr(),
+                                 counts.data_ptr(), path.data_ptr(), free_pages.data_ptr() if stack else 0,
+                                 free_count.data_ptr() if stack else 0, kept.data_ptr(), kept.data_ptr() + 4 * b, array, page,
+                                 head, token, block_table.stride(0), path.stride(0), arrays, pages, kv_heads, d, block_size, b,
+                                 block_table.shape[1], path.shape[1], free_pages.numel() if stack else 0)
+    status = _lib.load().kf_keep_drafts(args, torch._C._cuda_getCurrentRawStream(caches.get_device()))
+    if status:
+        _lib.check(status, "keep_drafts")
+    return kept
+
+
+@torch.library.custom_op("kernelforge::keep_drafts", mutates_args=("caches", "free_pages"))
+def _keep_drafts_op(caches: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, seq_lens: torch.Tensor,
+                    counts: torch.Tensor, path: torch.Tensor, free_pages: Optional[torch.Tensor],
+                    free_count: Optional[torch.Tensor]) -> torch.Tensor:
+    return _launch_keep(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count)
+
+
+@_keep_drafts_op.register_fake
+def _(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count):
+    return context_lens.new_empty(context_lens.shape[0] + 1)
