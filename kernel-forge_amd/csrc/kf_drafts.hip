@@ -17,7 +17,6 @@ constexpr int kNodes = 64;
 struct Tree {
   int first, len, nodes;  // its first row, its new tokens, those of them that are nodes
   int parent;             // of this lane's node; -1: none, or not a node
-  uint64_t ancestors;     // and the node itself
 };
 __device__ __forceinline__ Tree load_tree(const int* parents, const int* cu, int r, int seqs, int tokens, int most, int lane) {
   Tree t;
@@ -26,14 +25,6 @@ __device__ __forceinline__ Tree load_tree(const int* parents, const int* cu, int
   t.nodes = min(t.len, most);
   const int p = lane < t.nodes ? parents[t.first + lane] : -1;
   t.parent = (unsigned)p < (unsigned)lane ? p : -1;
-  // Pointers doubled: after n rounds a node knows 2^n - 1 ancestors and where the next one is.  A root points to itself.
-  t.ancestors = 1ull << lane;
-  int jump = t.parent < 0 ? lane : t.parent;
-#pragma unroll
-  for (int i = 0; i < 6; ++i) {
-    t.ancestors |= __shfl(t.ancestors, jump);
-    jump = __shfl(jump, jump);
-  }
   return t;
 }
 
@@ -57,9 +48,17 @@ __global__ __launch_bounds__(64 * kTreeWaves) void draft_trees_kernel(DraftTrees
   if (r < a.seqs) {
     const Tree t = load_tree(a.parents, a.cu, r, a.seqs, a.tokens, kNodes, lane);
     const int64_t context = (int64_t)load_const(a.seq_lens, r) - t.len;
+    // Pointers doubled: after n rounds a node knows 2^n - 1 ancestors and where the next one is.  A root points to itself.
+    uint64_t ancestors = 1ull << lane;
+    int jump = t.parent < 0 ? lane : t.parent;
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+      ancestors |= __shfl(ancestors, jump);
+      jump = __shfl(jump, jump);
+    }
     for (int i = lane; i < t.len; i += 64) {  // past the 64th: no node
-      a.ancestors[t.first + i] = i < kNodes ? t.ancestors : 0;
-      a.positions[t.first + i] = i < kNodes ? context + __popcll(t.ancestors) - 1 : -1;
+      a.ancestors[t.first + i] = i < kNodes ? ancestors : 0;
+      a.positions[t.first + i] = i < kNodes ? context + __popcll(ancestors) - 1 : -1;
     }
   }
   // Rows in no request.
@@ -71,26 +70,24 @@ __global__ __launch_bounds__(64 * kTreeWaves) void draft_trees_kernel(DraftTrees
 }
 
 // ---- verification: what all forms share ---------------------------------------------------------------------
-// A node's child is accepted or not by itself and its elder siblings; the path is the nodes all of whose ancestors are the
-// first accepted child of their parents.  So no walk from node to node: every lane judges its own node, and one bit test per node
-// gives the path.
+// Whether a child is accepted depends on itself and its elder siblings only, so every lane judges its own node first; then the path
+// is one ballot a step.
 
-// Of accepted children with one parent the first.
-__device__ __forceinline__ bool first_accepted(bool accepted, int parent, int lane) {
-  bool first = accepted;
-  for (uint64_t m = __ballot(accepted); m; m &= m - 1) {
-    const int e = __builtin_ctzll(m), same = of_lane(parent, e);
-    first &= !(lane > e && parent == same);
+// From node 0 (which is given) along the first accepted children: the path's nodes.
+__device__ __forceinline__ uint64_t path_of(const Tree& t, bool accepted) {
+  if (t.nodes == 0) return 0;
+  uint64_t on = 1;
+  int at = 0;
+  while (const uint64_t next = __ballot(accepted && t.parent == at)) {
+    at = __builtin_ctzll(next);
+    on |= 1ull << at;
   }
-  return first;
+  return on;
 }
-// The nodes on the path, node 0 (which is given) among them; a chain from it.
-__device__ __forceinline__ uint64_t path_of(const Tree& t, bool chosen, int lane) {
-  const uint64_t ok = __ballot(chosen) | 1;
-  return __ballot(lane < t.nodes && (t.ancestors & ~ok) == 0);
-}
+__device__ __forceinline__ int last_of(uint64_t on) { return on ? 63 - __clzll((long long)on) : -1; }
+
 // counts, path and emitted tokens of request r but for the token behind the path; last: the path's last node.
-__device__ __forceinline__ void write_path(const VerifyArgs& a, int r, const Tree& t, uint64_t on, int64_t token, int lane) {
+__device__ __forceinline__ void write_path(const VerifyArgs& a, int r, uint64_t on, int64_t token, int lane) {
   const int count = __popcll(on), rank = __popcll(on & ((1ull << lane) - 1));
   int* const path = a.path + (int64_t)r * a.width;
   int64_t* const emitted = a.emitted + (int64_t)r * a.width;
@@ -197,343 +194,405 @@ __global__ __launch_bounds__(64 * kTreeWaves) void verify_best_kernel(VerifyArgs
   }
   const int64_t wanted = __shfl(best, max(t.parent, 0));
   const bool accepted = t.parent >= 0 && token == wanted;
-  const uint64_t on = path_of(t, first_accepted(accepted, t.parent, lane), lane);
-  write_path(a, r, t, on, token, lane);
-  const int last = on ? 63 - __clzll((long long)on) : -1;
-  if (lane == last) a.emitted[(int64_t)r * a.width + __popcll(on) - 1] = best;
+  const uint64_t on = path_of(t, accepted);
+  write_path(a, r, on, token, lane);
+  if (lane == last_of(on)) a.emitted[(int64_t)r * a.width + __popcll(on) - 1] = best;
 }
 
 // ---- from probabilities and given random numbers -------------------------------------------------------------
 // What is left of row t's mass after its rejected children is f = max(p - a q, 0) where they were drawn from q, f = p without their
-// tokens where they were given.  One launch adds f up over pieces of the path's last row, the next finds the piece and the
-// token at which the running sum passes u times all of it.  In 64 bits, as an index is an integer and 32 bits would move it.
-constexpr int kPickThreads = 256, kPiece = 16 * kPickThreads;  // values of a row
+// tokens where they were given.  The token behind the path is the one at which the running sum of f passes u times all of it: a
+// sum over the row, then the place in it.  In 64 bits, as an index is an integer and 32 bits would move it.
+//
+// One workgroup per request does this, the sum in 16 parts, one a wavefront, then the part, or the part of the part, that the place
+// is in.  Long rows are first added up by a launch of their own, in pieces of 4096 values: which row it is, is known from the first
+// test of every node's first child, unless a later child is accepted.
+constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64, kPiece = 4 * kPickThreads;
+constexpr int kSumThreads = 256;
 
-struct Last {  // of a request's path
-  double a;      // how much of the draft's probabilities is taken off
-  int row;       // of target and draft; -1: the request has no new tokens
-  int node;
+// Nothing for negative values and NaN.
+__device__ __forceinline__ double positive(double x) { return __builtin_fmax(x, 0.0); }
+__device__ __forceinline__ float positive(float x) { return __builtin_fmaxf(x, 0.0f); }
+
+// Sums over a wavefront's lanes up to and including each.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_dpp(double v) {
+  const u32x2 w = bit_cast<u32x2>(v);
+  const u32x2 x = {(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[0], CTRL, ROWS, 0xF, false),
+                   (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[1], CTRL, ROWS, 0xF, false)};
+  return v + bit_cast<double>(x);
+}
+__device__ __forceinline__ double wave_scan(double v) {
+  v = add_dpp<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+  v = add_dpp<0x112, 0xF>(v);
+  v = add_dpp<0x114, 0xF>(v);
+  v = add_dpp<0x118, 0xF>(v);
+  v = add_dpp<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  return add_dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+}
+__device__ __forceinline__ double wave_sum(double v) { return of_lane(wave_scan(v), 63); }
+
+// A request's tree in LDS: the walk along it is one wavefront's, all others go by what it leaves here.
+struct WalkShared {
+  uint64_t children[kNodes];
+  int64_t token[kNodes];
+  double p[kNodes], q[kNodes], u[kNodes];  // of a node's token in its parent's rows, and its random number
+  int again[kNodes];                       // an elder sibling has the same token
+  int64_t gone[kNodes];                    // the tokens of the path's last node's children
+  uint64_t on, under;
+  int first, last;
+  double taken;
 };
-struct VerifySpace {
-  double* sums;       // [seqs, pieces]
-  Last* last;         // [seqs]
-  double* taken;      // drawn: [tokens] a of every row all of whose children are rejected
-  int* chosen;        // drawn: [tokens] 1: the first accepted child of its parent
+
+// The path as far as it is known without a sum, and the row of its last node with what is taken off.
+struct Way {
+  uint64_t on;
+  int first, last;  // last -1: the request has no nodes
+  uint64_t under;   // the last node's children
+  double taken;
 };
-__device__ __host__ inline VerifySpace verify_space(void* ws, int seqs, int pieces, int tokens) {
-  VerifySpace s;
-  s.sums = static_cast<double*>(ws);
-  s.last = reinterpret_cast<Last*>(s.sums + (size_t)seqs * pieces);
-  s.taken = reinterpret_cast<double*>(s.last + seqs);
-  s.chosen = reinterpret_cast<int*>(s.taken + tokens);
-  return s;
-}
 
-__device__ __forceinline__ double positive(double x) { return x > 0.0 ? x : 0.0; }  // of NaN: nothing
-
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off);
-  return v;
-}
-// Of a workgroup, the same in all threads.
-template <int THREADS>
-__device__ __forceinline__ double block_sum(double v, double* parts) {
-  v = wave_sum(v);
-  __syncthreads();  // the last sum's have been read
-  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0.0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) v += parts[w];
-  return v;
-}
-
-// Value i of a row as a double, or 0 for one that is none.
-__device__ __forceinline__ double prob_at(const float* row, int64_t token, int vocab) {
-  return token >= 0 && token < vocab ? (double)row[token] : 0.0;
-}
-
-// Drafts that were drawn from given probabilities, one workgroup per node: which of its children is accepted.  A test after a
-// rejection needs a sum over the node's row, so only nodes that the path may still come to make any: children whose first
-// test fails end the ways through them, those of a second test keep theirs open.
-constexpr int kChooseThreads = 512;
-__global__ __launch_bounds__(kChooseThreads) void choose_child_kernel(VerifyArgs a, int pieces) {
-  __shared__ double parts[kChooseThreads / 64];
-  const int lane = threadIdx.x & 63, node = blockIdx.x, r = blockIdx.y;
+// By one wavefront: the tests that need no sum, and the path that they make.  Children given as tokens: each is accepted with what
+// is left of its parent's mass, of several with one token the first.  Children that were drawn: the first of each node.
+template <bool DRAWN>
+__device__ __forceinline__ void walk(const VerifyArgs& a, WalkShared& sh, int r, int lane) {
   const Tree t = load_tree(a.parents, a.cu, r, a.seqs, a.tokens_count, a.width, lane);
-  if (node >= t.nodes) return;
-  const VerifySpace space = verify_space(a.ws, a.seqs, pieces, a.tokens_count);
-  const int up = t.first + max(t.parent, 0);
-  double p = 0.0, q = 0.0, u = 1.0;
-  if (t.parent >= 0) {
-    const int64_t token = a.tokens[t.first + lane];
-    p = prob_at((const float*)a.target + (int64_t)up * a.target_row, token, a.vocab);
-    q = prob_at(a.draft + (int64_t)up * a.draft_row, token, a.vocab);
-    u = a.accept_u[t.first + lane];
+  sh.children[lane] = 0;
+  if (t.nodes > 0) {  // the same for all lanes
+    const int mine = t.first + min(lane, t.nodes - 1), up = t.first + max(t.parent, 0);
+    const int64_t token = a.tokens[mine], inside = token >= 0 && token < a.vocab ? token : 0;
+    const float u = a.accept_u[mine], p = ((const float*)a.target)[(int64_t)up * a.target_row + inside];
+    const float q = DRAWN ? a.draft[(int64_t)up * a.draft_row + inside] : 0.0f;
+    const bool real = token == inside;  // others have no mass
+    sh.token[lane] = token;
+    sh.p[lane] = real ? positive(p) : 0.0;
+    sh.q[lane] = real ? (double)q : 0.0;
+    sh.u[lane] = u;
+    if (t.parent >= 0)
+      atomicOr((unsigned long long*)&sh.children[t.parent], 1ull << lane);  // by one wavefront, an or: no order to it
   }
-  const bool first_ok = t.parent >= 0 && u * q < positive(p);
-  bool eldest = t.parent >= 0, open = true;
-  for (uint64_t m = __ballot(t.parent >= 0); m; m &= m - 1) {
-    const int e = __builtin_ctzll(m), of = of_lane(t.parent, e), ok = of_lane((int)first_ok, e);
-    if (of == t.parent && e < lane) {
-      if (eldest) open = !ok;  // e is the first child: only if it was not accepted is this one asked
-      eldest = false;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const uint64_t elders = t.parent >= 0 ? sh.children[t.parent] & ((1ull << lane) - 1) : 0;
+  bool accepted = false;
+  if constexpr (DRAWN) {
+    accepted = t.parent >= 0 && elders == 0 && sh.u[lane] * sh.q[lane] < sh.p[lane];
+  } else {
+    bool again = false;
+    if (t.parent >= 0)
+      for (uint64_t m = elders; m; m &= m - 1) again |= sh.token[__builtin_ctzll(m)] == sh.token[lane];
+    sh.again[lane] = again;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (t.parent >= 0) {
+      double left = 1.0;
+      for (uint64_t m = elders; m; m &= m - 1) {
+        const int e = __builtin_ctzll(m);
+        left -= sh.again[e] ? 0.0 : sh.p[e];
+      }
+      accepted = !again && sh.u[lane] * left < sh.p[lane];
     }
   }
-  if (eldest) open = first_ok;
-  const uint64_t way = __ballot(t.parent >= 0 && open) | 1;
-  const uint64_t mine = of_lane(t.ancestors, node), children = __ballot(t.parent == node);
-  int chosen = -1;
-  double taken = 0.0, left = 1.0;
-  if ((mine & ~way) == 0) {
-    const float* const prow = (const float*)a.target + (int64_t)(t.first + node) * a.target_row;
-    const float* const qrow = a.draft + (int64_t)(t.first + node) * a.draft_row;
-    for (uint64_t m = children; m; m &= m - 1) {
-      const int c = __builtin_ctzll(m);
-      const double pc = of_lane(p, c), qc = of_lane(q, c), uc = of_lane(u, c);
-      if (uc * left * qc < positive(pc - taken * qc)) {
-        chosen = c;
-        break;
-      }
-      taken += left;
-      if (m & (m - 1)) {
-        double sum = 0.0;
-        int i = 4 * threadIdx.x;
-        for (; i + 4 <= a.vocab; i += 4 * kChooseThreads) {
-          const row4_t x = *(const row4_t*)(prow + i), y = *(const row4_t*)(qrow + i);
+  const uint64_t on = path_of(t, accepted);
+  const int last = last_of(on);
+  const uint64_t under = __ballot(t.parent == last && last >= 0);
+  if (under >> lane & 1) sh.gone[__popcll(under & ((1ull << lane) - 1))] = sh.token[lane];
+  if (lane == 0) {
+    sh.on = on;
+    sh.under = under;
+    sh.first = t.first;
+    sh.last = last;
+    sh.taken = DRAWN && under ? 1.0 : 0.0;
+  }
+}
+// Of all wavefronts, behind a barrier: the same in all lanes, and known to be.
+__device__ __forceinline__ Way way_of(const WalkShared& sh) {
+  Way w;
+  w.on = of_lane(sh.on, 0);
+  w.under = of_lane(sh.under, 0);
+  w.first = of_lane(sh.first, 0);
+  w.last = of_lane(sh.last, 0);
+  w.taken = of_lane(sh.taken, 0);
+  return w;
+}
+
+// Values of f in a row.
+template <bool DRAWN>
+struct Rest {
+  const float* p;
+  const float* q;
+  const int64_t* gone;  // LDS: tokens that are out of it
+  int gone_count, vocab;
+  double taken;
+
+  // Four values from i on; `from` and the next 4 x LANES values are what the lanes that come here together look at.
+  template <int LANES>
+  __device__ __forceinline__ void four(row4_t x, row4_t y, int i, int from, double (&f)[4]) const {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sum += positive(fma(-taken, (double)y[e], (double)x[e]));
+    for (int e = 0; e < 4; ++e) f[e] = DRAWN ? positive(fma(-taken, (double)y[e], (double)x[e])) : (double)positive(x[e]);
+    if constexpr (!DRAWN) {
+      for (int g = 0; g < gone_count; ++g) {
+        const int64_t token = gone[g];
+        if (token >= from && token < from + 4 * LANES) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i + e == token) f[e] = 0.0;
         }
-        for (; i < a.vocab; ++i) sum += positive(fma(-taken, (double)qrow[i], (double)prow[i]));
-        left = block_sum<kChooseThreads>(sum, parts);
       }
     }
   }
-  if (threadIdx.x < 64) {
-    if (children >> lane & 1) space.chosen[t.first + lane] = lane == chosen;
-    if (lane == 0) space.taken[t.first + node] = taken;
+  __device__ __forceinline__ row4_t load(const float* row, int i, int end) const {  // zeros from `end` on
+    if (i + 4 <= end) return *(const row4_t*)(row + i);
+    row4_t v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = i + e < end ? row[i + e] : 0.0f;
+    return v;
   }
-}
-
-// Children of each node given as tokens: each accepted with what is left of its parent's mass.
-__device__ __forceinline__ bool accept_given(const VerifyArgs& a, const Tree& t, int64_t token, int lane) {
-  double p = 0.0, u = 1.0;
-  if (t.parent >= 0) {
-    p = positive(prob_at((const float*)a.target + (int64_t)(t.first + t.parent) * a.target_row, token, a.vocab));
-    u = a.accept_u[t.first + lane];
-  }
-  double left = 1.0;
-  bool again = false;  // an elder has this token
-  for (uint64_t m = __ballot(t.parent >= 0); m; m &= m - 1) {
-    const int e = __builtin_ctzll(m), of = of_lane(t.parent, e), counted = of_lane((int)again, e);
-    const double mass = of_lane(p, e);
-    const int64_t other = of_lane(token, e);
-    if (of == t.parent && e < lane) {
-      again |= other == token;
-      left -= counted ? 0.0 : mass;
+  // The sum over [begin, end) by one wavefront, the same in all lanes.
+  __device__ __forceinline__ double wave_total(int begin, int end, int lane) const {
+    constexpr int AHEAD = 8;  // loads of each row on their way
+    double sum = 0.0;
+    for (int i0 = begin; i0 < end; i0 += 256 * AHEAD) {
+      row4_t x[AHEAD], y[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        x[j] = load(p, i0 + 256 * j + 4 * lane, end);
+        if (DRAWN) y[j] = load(q, i0 + 256 * j + 4 * lane, end);
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (i0 + 256 * j >= end) break;
+        double f[4];
+        four<64>(x[j], y[j], i0 + 256 * j + 4 * lane, i0 + 256 * j, f);
+        sum += (f[0] + f[1]) + (f[2] + f[3]);
+      }
     }
+    return wave_sum(sum);
   }
-  return t.parent >= 0 && !again && u * left < p;
-}
-
-// A thread's 16 values of a piece: four each of every quarter.
-struct PieceValues {
-  double f[4][4];
 };
 template <bool DRAWN>
-__device__ __forceinline__ PieceValues piece_values(const float* prow, const float* qrow, double taken, const uint32_t* gone,
-                                                    int begin, int vocab) {
-  PieceValues v;
-  row4_t x[4], y[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int at = 4 * (kPickThreads * j + (int)threadIdx.x), i = begin + at;
-    if (i + 4 <= vocab) {
-      x[j] = *(const row4_t*)(prow + i);
-      if (DRAWN) y[j] = *(const row4_t*)(qrow + i);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[j][e] = i + e < vocab ? prow[i + e] : 0.0f;
-        if (DRAWN) y[j][e] = i + e < vocab ? qrow[i + e] : 0.0f;
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int at = 4 * (kPickThreads * j + (int)threadIdx.x);
-    const uint32_t out = DRAWN ? 0 : gone[at >> 5] >> (at & 31);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      v.f[j][e] = DRAWN ? positive(fma(-taken, (double)y[j][e], (double)x[j][e])) : out >> e & 1 ? 0.0 : positive(x[j][e]);
-  }
-  return v;
-}
-// The bits of a piece's values that are no longer there: the tokens of the last node's children.
-__device__ __forceinline__ void mark_gone(uint32_t* gone, bool under, int64_t token, int begin) {
-  __syncthreads();
-  for (int i = threadIdx.x; i < kPiece / 32; i += kPickThreads) gone[i] = 0;
-  __syncthreads();
-  if (threadIdx.x < 64 && under && token >= begin && token < begin + kPiece)
-    atomicOr(&gone[(token - begin) >> 5], 1u << ((token - begin) & 31));
-  __syncthreads();
+__device__ __forceinline__ Rest<DRAWN> rest_of(const VerifyArgs& a, const WalkShared& sh, const Way& w) {
+  const int64_t row = w.first + w.last;
+  return Rest<DRAWN>{(const float*)a.target + row * a.target_row, DRAWN ? a.draft + row * a.draft_row : nullptr, sh.gone,
+                     DRAWN ? 0 : (int)__popcll(w.under), a.vocab, w.taken};
 }
 
-// Workgroup (piece, request).
+// Workgroup (piece, request): the sum over the piece.
 template <bool DRAWN>
-__global__ __launch_bounds__(kPickThreads) void verify_sum_kernel(VerifyArgs a, int pieces) {
-  __shared__ double parts[kPickThreads / 64];
-  __shared__ uint32_t gone[DRAWN ? 1 : kPiece / 32];
+__global__ __launch_bounds__(kSumThreads) void verify_sum_kernel(VerifyArgs a, int pieces) {
+  __shared__ double parts[kSumThreads / 64];
+  __shared__ WalkShared walked;
   const int lane = threadIdx.x & 63, piece = blockIdx.x, r = blockIdx.y;
-  const VerifySpace space = verify_space(a.ws, a.seqs, pieces, a.tokens_count);
-  const Tree t = load_tree(a.parents, a.cu, r, a.seqs, a.tokens_count, a.width, lane);
-  const int64_t token = lane < t.nodes ? a.tokens[t.first + lane] : -1;
-  bool chosen;
-  if constexpr (DRAWN) chosen = t.parent >= 0 && space.chosen[t.first + lane];
-  else chosen = first_accepted(accept_given(a, t, token, lane), t.parent, lane);
-  const uint64_t on = path_of(t, chosen, lane);
-  const int last = on ? 63 - __clzll((long long)on) : -1;
-  const int row = last < 0 ? -1 : t.first + last;
-  const double taken = DRAWN && last >= 0 ? space.taken[row] : 0.0;
-  if (piece == 0 && threadIdx.x < 64) {
-    write_path(a, r, t, on, token, lane);
-    if (lane == 0) space.last[r] = Last{taken, row, last};
-  }
-  if (last < 0) return;
-  if constexpr (!DRAWN) mark_gone(gone, t.parent == last, token, piece * kPiece);
-  const PieceValues v = piece_values<DRAWN>((const float*)a.target + (int64_t)row * a.target_row,
-                                            DRAWN ? a.draft + (int64_t)row * a.draft_row : nullptr, taken, gone, piece * kPiece,
-                                            a.vocab);
-  double sum = 0.0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum += v.f[j][e];
-  sum = block_sum<kPickThreads>(sum, parts);
-  if (threadIdx.x == 0) space.sums[(int64_t)r * pieces + piece] = sum;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (wave == 0) walk<DRAWN>(a, walked, r, lane);
+  __syncthreads();
+  const Way w = way_of(walked);
+  if (w.last < 0) return;
+  const Rest<DRAWN> rest = rest_of<DRAWN>(a, walked, w);
+  constexpr int MINE = kPiece / (kSumThreads / 64);
+  const int begin = piece * kPiece + wave * MINE;
+  const double sum = rest.wave_total(begin, min(begin + MINE, a.vocab), lane);
+  if (lane == 0) parts[wave] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    static_cast<double*>(a.ws)[(int64_t)r * pieces + piece] = (parts[0] + parts[1]) + (parts[2] + parts[3]);
 }
+
+struct PickShared {
+  WalkShared walked;
+  double parts[kPickWaves], scan[kPickWaves];
+  double before;
+  int low[kPickWaves], high[kPickWaves];
+};
 
 // Sums over the threads up to and including each, and of all.
 struct Scan {
   double upto, all;
 };
-__device__ __forceinline__ Scan block_scan(double v, double* parts) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double w = __shfl_up(v, off);
-    if (lane >= off) v += w;
-  }
-  __syncthreads();
-  if (lane == 63) parts[wave] = v;
+__device__ __forceinline__ Scan block_scan(double v, PickShared& sh, int lane, int wave) {
+  v = wave_scan(v);
+  __syncthreads();  // the last scan's have been read
+  if (lane == 63) sh.scan[wave] = v;
   __syncthreads();
   double before = 0.0, all = 0.0;
 #pragma unroll
-  for (int w = 0; w < kPickThreads / 64; ++w) {
-    if (w < wave) before += parts[w];
-    all += parts[w];
+  for (int w = 0; w < kPickWaves; ++w) {
+    if (w < wave) before += sh.scan[w];
+    all += sh.scan[w];
   }
   return Scan{before + v, all};
 }
 
-template <bool DRAWN>
-__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a, int pieces) {
-  __shared__ double parts[kPickThreads / 64];
-  __shared__ uint32_t gone[DRAWN ? 1 : kPiece / 32];
-  __shared__ int found, some;
-  __shared__ double found_at;
-  const int tid = threadIdx.x, r = blockIdx.x;
-  const VerifySpace space = verify_space(a.ws, a.seqs, pieces, a.tokens_count);
-  const Last last = space.last[r];
-  if (last.row < 0) return;
-  const float* const prow = (const float*)a.target + (int64_t)last.row * a.target_row;
-  const float* const qrow = DRAWN ? a.draft + (int64_t)last.row * a.draft_row : nullptr;
-  const int first = last.row - last.node;
-  const int nodes = min(seq_offset(a.cu, r + 1, a.seqs, a.tokens_count) - first, a.width);
-  const bool node = tid < nodes;
-  const int64_t token = node ? a.tokens[first + tid] : -1;
-  bool under = node && tid > last.node && a.parents[first + tid] == last.node;
-  double taken = last.a;
-  const double* sums = space.sums + (int64_t)r * pieces;
-
-  // What is left may be nothing, where the probabilities do not add up: the token is drawn from all of the row then.
-  bool whole = false;
-  auto sum_of = [&](int s) { return s < pieces ? sums[s] : 0.0; };
-  auto values = [&](int s) {
-    if constexpr (!DRAWN) mark_gone(gone, under && !whole, token, s * kPiece);
-    return piece_values<DRAWN>(prow, qrow, taken, gone, s * kPiece, a.vocab);
-  };
-  auto add_up = [&](const PieceValues& v) {
-    double sum = 0.0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum += v.f[j][e];
-    return block_sum<kPickThreads>(sum, parts);
-  };
-  double all = 0.0;
-  for (int s0 = 0; s0 < pieces; s0 += kPickThreads) all += block_sum<kPickThreads>(sum_of(s0 + tid), parts);
-  if (!(all > 0.0)) {
-    whole = true;
-    taken = 0.0;
-    all = 0.0;
-    for (int s = 0; s < pieces; ++s) all += add_up(values(s));
-  }
-  const double mark = (double)a.sample_u[r] * all;
-
-  // The first piece with whose end the sum passes the mark; if none does (a number that is not below 1), the last with any.
-  int piece = -1;
-  double before = 0.0;
-  if (!whole) {
-    if (tid == 0) found = 0x7fffffff, some = -1;
-    double carry = 0.0;
-    for (int s0 = 0; s0 < pieces; s0 += kPickThreads) {
-      const double mine = sum_of(s0 + tid);
-      const Scan scan = block_scan(mine, parts);  // its barriers are behind the store above
-      if (mine > 0.0) {
-        atomicMax(&some, s0 + tid);
-        if (carry + scan.upto > mark) atomicMin(&found, s0 + tid);
-      }
-      __syncthreads();
-      if (found == s0 + tid) found_at = carry + scan.upto - mine;
-      carry += scan.all;
-      if (found != 0x7fffffff) break;
-    }
-    __syncthreads();
-    piece = found != 0x7fffffff ? found : some;
-    before = found != 0x7fffffff ? found_at : 0.0;
-  } else {
-    for (int s = 0; s < pieces; ++s) {
-      const double sum = add_up(values(s));
-      if (sum > 0.0) piece = s;
-      if (sum > 0.0 && before + sum > mark) break;
-      before += sum;
-    }
-  }
-  __syncthreads();  // both have been read
-  if (tid == 0) found = 0x7fffffff, some = piece < 0 ? 0 : -1;
-  if (piece >= 0) {
-    const PieceValues v = values(piece);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const double mine = v.f[j][0] + v.f[j][1] + v.f[j][2] + v.f[j][3];
-      const Scan scan = block_scan(mine, parts);
-      double upto = before + (scan.upto - mine);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        upto += v.f[j][e];
-        const int i = piece * kPiece + 4 * (kPickThreads * j + tid) + e;
-        if (v.f[j][e] > 0.0) {
-          atomicMax(&some, i);
-          if (upto > mark) atomicMin(&found, i);
-        }
-      }
-      before += scan.all;
-    }
+// The lowest and the highest number that any thread has (0x7fffffff and -1: none), where numbers ascend with the threads.
+struct Ends {
+  int low, high;
+};
+__device__ __forceinline__ Ends ends_of(int low, int high, PickShared& sh, int lane, int wave) {
+  const uint64_t lows = __ballot(low != 0x7fffffff), highs = __ballot(high >= 0);
+  const int l = lows ? of_lane(low, __builtin_ctzll(lows)) : 0x7fffffff, h = highs ? of_lane(high, 63 - __clzll((long long)highs)) : -1;
+  __syncthreads();
+  if (lane == 0) {
+    sh.low[wave] = l;
+    sh.high[wave] = h;
   }
   __syncthreads();
-  if (tid == 0) a.emitted[(int64_t)r * a.width + a.counts[r] - 1] = found != 0x7fffffff ? found : some;
+  Ends e = {0x7fffffff, -1};
+#pragma unroll
+  for (int w = 0; w < kPickWaves; ++w) {
+    e.low = min(e.low, sh.low[w]);
+    e.high = max(e.high, sh.high[w]);
+  }
+  return e;
+}
+
+// The same where they do not: rows of more than 2^22 values.
+__device__ __forceinline__ Ends lowest_of(int low, int high, PickShared& sh, int lane, int wave) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    low = min(low, __shfl_xor(low, off));
+    high = max(high, __shfl_xor(high, off));
+  }
+  return ends_of(lane == 0 ? low : 0x7fffffff, lane == 0 ? high : -1, sh, lane, wave);
+}
+
+// The sum over the row, a 16th of it by each wavefront; those stay in sh.parts.
+template <bool DRAWN>
+__device__ __forceinline__ double row_total(PickShared& sh, const Rest<DRAWN>& rest, int begin, int end, int lane, int wave) {
+  const int part = ((end - begin + kPickWaves - 1) / kPickWaves + 3) & ~3;
+  const int64_t at = begin + (int64_t)part * wave;
+  const double mine = rest.wave_total((int)min(at, (int64_t)end), (int)min(at + part, (int64_t)end), lane);
+  __syncthreads();
+  if (lane == 0) sh.parts[wave] = mine;
+  __syncthreads();
+  double all = 0.0;
+#pragma unroll
+  for (int w = 0; w < kPickWaves; ++w) all += sh.parts[w];
+  return all;
+}
+
+// One workgroup per request.  pieces: of the rows, whose sums the launch before has left in a.ws; 0: there was none.
+template <bool DRAWN>
+__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a, int pieces) {
+  __shared__ PickShared sh;
+  WalkShared& walked = sh.walked;
+  const int tid = threadIdx.x, lane = tid & 63, r = blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const double* const sums = static_cast<const double*>(a.ws) + (int64_t)r * pieces;
+  const float sample_u = a.sample_u[r];
+  const double my_sum = tid < pieces ? sums[tid] : 0.0;
+  if (wave == 0) walk<DRAWN>(a, walked, r, lane);
+  __syncthreads();
+  Way w = way_of(walked);
+  if (w.last < 0) {
+    if (wave == 0) write_path(a, r, 0, 0, lane);
+    return;
+  }
+  bool summed = pieces > 0;  // the pieces' sums are those of the present row and what is taken off
+  auto add_pieces = [&] {
+    double sum = my_sum;
+    for (int i = tid + kPickThreads; i < pieces; i += kPickThreads) sum += sums[i];
+    sum = wave_sum(sum);
+    __syncthreads();
+    if (lane == 0) sh.parts[wave] = sum;
+    __syncthreads();
+    double all = 0.0;
+#pragma unroll
+    for (int v = 0; v < kPickWaves; ++v) all += sh.parts[v];
+    return all;
+  };
+  if constexpr (DRAWN) {
+    // Further children: each test needs the sum of what the ones before have left.
+    uint64_t open = w.under & (w.under - 1);  // the first has been rejected
+    while (open) {
+      const double left = summed ? add_pieces() : row_total(sh, rest_of<true>(a, walked, w), 0, a.vocab, lane, wave);
+      const int c = __builtin_ctzll(open);
+      open &= open - 1;
+      summed = false;
+      if (!(walked.u[c] * left * walked.q[c] < positive(walked.p[c] - w.taken * walked.q[c]))) {
+        w.taken += left;
+        continue;
+      }
+      // Accepted: on along first children, as far as they are.
+      w.on |= 1ull << c;
+      w.last = c;
+      while (true) {
+        w.under = of_lane(walked.children[w.last], 0);
+        w.taken = w.under ? 1.0 : 0.0;
+        open = w.under & (w.under - 1);
+        if (!w.under) break;
+        const int e = __builtin_ctzll(w.under);
+        if (!(walked.u[e] * walked.q[e] < walked.p[e])) break;
+        w.on |= 1ull << e;
+        w.last = e;
+      }
+    }
+  }
+  if (wave == 0) write_path(a, r, w.on, walked.token[lane], lane);
+  Rest<DRAWN> rest = rest_of<DRAWN>(a, walked, w);
+  double all = summed ? add_pieces() : row_total(sh, rest, 0, a.vocab, lane, wave);
+  if (!(all > 0.0)) {
+    // Nothing is left, where the probabilities do not add up: the token is drawn from all of the row.
+    rest.taken = 0.0;
+    rest.gone_count = 0;
+    summed = false;
+    all = row_total(sh, rest, 0, a.vocab, lane, wave);
+  }
+  const double mark = (double)sample_u * all;
+
+  // The part of [begin, end) with whose end the sum passes the mark; if none does (a number that is not below 1), the last with any.
+  double before = 0.0;
+  int begin = 0, end = a.vocab;
+  if (summed) {
+    double carry = 0.0, low_at = 0.0;
+    int low = 0x7fffffff, high = -1;
+    for (int i0 = 0; i0 < pieces; i0 += kPickThreads) {
+      const double mine = i0 == 0 ? my_sum : i0 + tid < pieces ? sums[i0 + tid] : 0.0;
+      const Scan scan = block_scan(mine, sh, lane, wave);
+      if (mine > 0.0) {
+        high = i0 + tid;
+        if (low == 0x7fffffff && carry + scan.upto > mark) low = i0 + tid, low_at = carry + (scan.upto - mine);
+      }
+      carry += scan.all;
+    }
+    const Ends e = pieces <= kPickThreads ? ends_of(low, high, sh, lane, wave) : lowest_of(low, high, sh, lane, wave);
+    if (low == e.low && low != 0x7fffffff) sh.before = low_at;
+    __syncthreads();
+    const int piece = e.low != 0x7fffffff ? e.low : max(e.high, 0);
+    before = e.low != 0x7fffffff ? sh.before : 0.0;
+    begin = piece * kPiece;
+    end = min(begin + kPiece, a.vocab);
+  }
+  while (end - begin > kPiece) {
+    if (begin != 0 || end != a.vocab) row_total(sh, rest, begin, end, lane, wave);  // the whole row's parts are there
+    const int part = ((end - begin + kPickWaves - 1) / kPickWaves + 3) & ~3;
+    int at = -1, some = 0;
+    double upto = before, found = before;
+    for (int v = 0; v < kPickWaves; ++v) {
+      const double sum = sh.parts[v];
+      if (sum > 0.0) some = v;
+      if (at < 0 && sum > 0.0 && upto + sum > mark) at = v, found = upto;
+      upto += sum;
+    }
+    before = at >= 0 ? found : 0.0;
+    begin = min(begin + (at >= 0 ? at : some) * part, end);
+    end = min(begin + part, end);
+    __syncthreads();  // the parts have been read
+  }
+  const int i = begin + 4 * tid;
+  double f[4];
+  rest.template four<kPickThreads>(rest.load(rest.p, i, end), DRAWN ? rest.load(rest.q, i, end) : row4_t{}, i, begin, f);
+  const double mine = (f[0] + f[1]) + (f[2] + f[3]);
+  const Scan scan = block_scan(mine, sh, lane, wave);
+  double upto = before + (scan.upto - mine);
+  int low = 0x7fffffff, high = -1;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    upto += f[e];
+    if (f[e] > 0.0) {
+      high = i + e;
+      if (low == 0x7fffffff && upto > mark) low = i + e;
+    }
+  }
+  const Ends e = ends_of(low, high, sh, lane, wave);
+  if (tid == 0) a.emitted[(int64_t)r * a.width + __popcll(w.on) - 1] = e.low != 0x7fffffff ? e.low : max(e.high, 0);
 }
 
 // ---- what is kept -----------------------------------------------------------------------------------------------
@@ -633,7 +692,7 @@ __global__ __launch_bounds__(kKeepThreads) void keep_drafts_kernel(KeepArgs a) {
   }
 }
 
-int row_pieces(int vocab) { return (int)(((int64_t)vocab + kPiece - 1) / kPiece); }
+constexpr int kSumFrom = 32768;
 
 // Workgroups per row of scores, where there are fewer rows than fill the card, of at least four rounds of loads.
 int row_shares(const VerifyArgs& a) {
@@ -647,11 +706,16 @@ void best_launch(const VerifyArgs& a, int shares, hipStream_t stream) {
   best_token_kernel<T><<<a.tokens_count * shares, kBestThreads, 0, stream>>>(a, shares, part);
 }
 
+// Pieces of a row whose sums a launch of their own leaves; 0: one workgroup adds the row up.
+int summed_pieces(const VerifyArgs& a) { return a.vocab <= kSumFrom ? 0 : (a.vocab + kPiece - 1) / kPiece; }
+
 template <bool DRAWN>
 hipError_t sample_launch(const VerifyArgs& a, hipStream_t stream) {
-  const int pieces = row_pieces(a.vocab);
-  if (DRAWN) choose_child_kernel<<<dim3(a.width, a.seqs), kChooseThreads, 0, stream>>>(a, pieces);
-  verify_sum_kernel<DRAWN><<<dim3(pieces, a.seqs), kPickThreads, 0, stream>>>(a, pieces);
+  const int pieces = summed_pieces(a);
+  if (pieces) {
+    verify_sum_kernel<DRAWN><<<dim3(pieces, a.seqs), kSumThreads, 0, stream>>>(a, pieces);
+    if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
+  }
   verify_pick_kernel<DRAWN><<<a.seqs, kPickThreads, 0, stream>>>(a, pieces);
   return hipGetLastError();
 }
@@ -665,8 +729,7 @@ hipError_t draft_trees_launch(const DraftTreesArgs& a, hipStream_t stream) {
 
 size_t verify_workspace_bytes(const VerifyArgs& a) {
   if (a.mode == kVerifyBest) return (size_t)a.tokens_count * row_shares(a) * sizeof(uint64_t);
-  const VerifySpace s = verify_space(nullptr, a.seqs, row_pieces(a.vocab), a.tokens_count);
-  return a.mode == kVerifyDrawn ? (size_t)(s.chosen + a.tokens_count) : (size_t)s.taken;
+  return (size_t)a.seqs * summed_pieces(a) * sizeof(double);
 }
 
 hipError_t verify_launch(const VerifyArgs& a, int dtype, hipStream_t stream) {
