@@ -177,6 +177,12 @@ constexpr int kMaxTokenStride = 1 << 26;  // elements: 16 keys' byte offsets fit
 // 78 / 55; 4 of 64 and 64 rows 27 / 33, 96 rows 33 / 39, 128 rows 34 / 41.
 constexpr int kFewRows = 64;
 
+// The same for trees, whose row tiles the other kernel cuts into pieces (tree_plan) without a stretch's search.  Few rows / many rows,
+// us: 8 requests over 1000 .. 4000 keys (8 KV heads of 128) and 32 rows 34 / 28, 64 rows 45 / 30, 8 of 64 dims and 32 rows 17 / 16, 64 of
+// 32 rows over 100 .. 3000 82 / 69; but 16 rows 57 / 72, 32 of 8 rows over 100 .. 4000 34 / 40, 128 of 12 over 4000 (2 KV heads)
+// 36 / 41.
+constexpr int kTreeFewRows = 16;
+
 int check_block(int block_size, int* log2_block) {
   if (block_size < 16 || block_size > (1 << 20) || (block_size & (block_size - 1)))
     return fail(KF_ERR_INVALID_ARG, "block_size must be a power of two from 16 to 2^20, got %d", block_size);
@@ -254,6 +260,11 @@ int paged_plan(const kf_paged_attention_args& a, bool tree, PagedPlan* p) {
   p->tree = tree;
   p->rows = std::min<int64_t>(rows, kFewRows);
   p->max_rows = p->many ? kFewRows : 0x7fffffff;
+  if (tree) {  // trees of one batch are much alike: one kernel takes them all
+    p->many = rows > kTreeFewRows;
+    p->few = !p->many;
+    p->max_rows = 0x7fffffff;
+  }
   t.q = a.q, t.k = a.cache_k, t.v = a.cache_v, t.out = a.out;
   t.cu = static_cast<const int*>(a.cu_new);
   t.seq_lens = static_cast<const int*>(a.seq_lens);
@@ -277,7 +288,7 @@ struct PagedLaunches {
 };
 PagedLaunches paged_launches(const PagedPlan& p, int cus) {
   PagedLaunches l = {};
-  if (p.many) l.many = kf::flash_plan(p.args, true, cus);
+  if (p.many) l.many = p.tree ? kf::tree_plan(p.args, cus) : kf::flash_plan(p.args, true, cus);
   if (p.few) {
     // Where there are many row tiles, and the others are cut; the grid stays below 2^31 work-items.
     l.together = p.many && !p.tree && !l.many.cut && l.many.groups == 1 && p.args.head_dim <= 128;

@@ -23,6 +23,8 @@
 // take 45 .. 49 us, the longest row tile 23 tiles of keys where the work spread evenly is 14.
 #include <math.h>
 
+#include <algorithm>
+
 #include "kf_few_rows.h"
 #include "kf_launch.h"
 
@@ -102,6 +104,18 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
   tiles = min(tiles, kend <= 0 ? 0 : (kend + KEYS - 1) / KEYS);
   const int mine0 = tile0 + group;  // this group's first tile
 
+  // The pages of the groups' next tiles come by one vector load, lane i's those of 16 keys, a tile ahead of the copies; the first
+  // ones beside the queries.
+  const int* const table = a.table + (PAGED ? (int64_t)seq * a.table_stride : 0);
+  auto load_pages = [&](int kt0) {
+    const int key = kt0 * KEYS + 16 * (lane % (GROUPS * KK));
+    const int p = load_const(table, min(key, kend - 1) >> a.log2_block);
+    return (unsigned)p < (unsigned)a.num_pages ? p : -1;  // -1: not in the cache
+  };
+  int pages = 0;
+  if constexpr (PAGED)
+    if (tile0 < tiles) pages = load_pages(tile0);
+
   u32x4 qf[Q_LDS ? 1 : ST];
   u32x4* const q_lds = reinterpret_cast<u32x4*>(smem + 4 * TILE) + wave * ST * 64 + lane;
   {
@@ -116,13 +130,6 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
   }
 
   // Copies.  A wavefront fetches rows 16 wave .. + 15 of both tiles: one page, as pages hold 16 keys at least.
-  // The pages of the groups' next tiles come by one vector load, lane i's those of 16 keys, a tile ahead of the copies.
-  const int* const table = a.table + (PAGED ? (int64_t)seq * a.table_stride : 0);
-  auto load_pages = [&](int kt0) {
-    const int key = kt0 * KEYS + 16 * (lane % (GROUPS * KK));
-    const int p = load_const(table, min(key, kend - 1) >> a.log2_block);
-    return (unsigned)p < (unsigned)a.num_pages ? p : -1;  // -1: not in the cache
-  };
   const TileCopy<E, HDP, false, MINE> copy(a.k_token, a.v_token, a.head_dim, lane, MINE * wave);
   auto issue = [&](int kt, uint32_t buf, int page) {
     const int key0 = kt * KEYS + MINE * wave;
@@ -158,15 +165,11 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
 
   int patch_from = 0x7fffffff;  // first key of a tile with masks whose infinities and NaN were taken out
   // Which of this wavefront's pages and of all groups' are not there, now and in the next tiles.
-  int pages = 0;
   uint64_t missing = 0, next_missing = 0;
   auto my_page = [&] { return __builtin_amdgcn_readlane(pages, group * KK + MINE * wave / 16); };
   auto none = [&] { return __ballot(pages < 0) & ((1u << (GROUPS * KK)) - 1); };
   if (tile0 < tiles) {
-    if constexpr (PAGED) {
-      pages = load_pages(tile0);
-      next_missing = none();
-    }
+    if constexpr (PAGED) next_missing = none();
     if (mine0 < tiles) issue(mine0, 0, PAGED ? my_page() : 0);
     if constexpr (PAGED) pages = load_pages(tile0 + GROUPS);
   }
@@ -609,8 +612,7 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
     const int item_at = head_at + (int)w.upto(tile), cost = w.base + 2 * (tile + 1);
     const int from = at - item_at, to = min(cost, end - item_at);
     const int row0 = tile * kFlashRows, len = w.rows / rep;
-    const SeqKeys sk = seq_keys<PAGED>(a, seq, len);
-    const int kend = KEYS_OF == Keys::kTree ? sk.keys : sk.last_key(min(row0 + kFlashRows - 1, w.rows - 1) / rep) + 1;
+    const int kend = seq_keys<PAGED>(a, seq, len).last_key(min(row0 + kFlashRows - 1, w.rows - 1) / rep) + 1;
     // The part's tiles: floor(position * tiles / cost), the same for a piece's end and the next one's beginning.
     const double tiles = max((kend + FlashConfig<HDP>::KEYS - 1) / FlashConfig<HDP>::KEYS, 1), each = cost;
     const int t0 = __builtin_amdgcn_readfirstlane((int)(from * tiles / each));
@@ -627,6 +629,205 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
   }
 }
 
+// Trees of new tokens, whose row tiles all see the same keys: each (request, KV head, row tile) is cut into pieces of at most `per`
+// key tiles, one a workgroup, with the smallest per for which there are workgroups enough.  So a workgroup begins once only, which
+// takes as long as four or five tiles of 64 keys, and all pieces end together.  Equal stretches as above, which can hold the end of
+// one item and the beginning of the next, took 59 in place of 41 us for 8 requests of 256 rows over 500 .. 4000 keys, 37 (29) for 16
+// of 30 .. 186 over 100 .. 8000 (2 KV heads), both with their join; the joins 18 .. 24 (6 .. 9) and, of 24 items in 512 stretches, 72 (7).
+constexpr int kTreeLeast = 4;  // key tiles of a piece; with 2 and 8 the same to 1 us
+struct TreeItem {
+  int seq, row0, kv, first, pieces;  // first: the workgroup of its first piece
+};
+struct TreeSpace {
+  float* parts;   // [grid][kFlashRows (HDP + 2)]
+  int* count;     // of items, once they are all in the list; padded to 16 bytes
+  TreeItem* list;
+};
+template <int HDP>
+__device__ __host__ inline TreeSpace tree_space(void* ws, int grid) {
+  TreeSpace s;
+  s.parts = static_cast<float*>(ws);
+  s.count = reinterpret_cast<int*>(s.parts + (size_t)grid * kFlashRows * (HDP + 2));
+  s.list = reinterpret_cast<TreeItem*>(s.count + 4);
+  return s;
+}
+struct TreeWork {
+  int rows, tiles, key_tiles;  // row tiles; tiles of keys of each
+};
+template <int HDP>
+__device__ __forceinline__ TreeWork tree_work(const AttnArgs& a, int s, int rep) {
+  constexpr int KEYS = FlashConfig<HDP>::KEYS;
+  const int len = max(seq_offset(a.cu, s + 1, a.seqs, a.tokens) - seq_offset(a.cu, s, a.seqs, a.tokens), 0);
+  TreeWork w;
+  w.rows = len * rep;
+  w.tiles = (w.rows + kFlashRows - 1) / kFlashRows;
+  w.key_tiles = max((seq_keys<true>(a, s, len).keys + KEYS - 1) / KEYS, 1);
+  return w;
+}
+// Sums that no lengths make wrap: at kNoWork they stay (kf_stretch.h).
+__device__ __forceinline__ int times_work(int a, int b) { return (int)min((int64_t)a * b, (int64_t)kNoWork); }
+__device__ __forceinline__ int all_work(int v) { return __builtin_amdgcn_readlane(work_prefix(v), 63); }
+
+template <class E, int HDP, int GROUPS>
+__global__ __launch_bounds__(GROUPS* kFlashThreads, flash_waves_per_simd(HDP, true)) void tree_cut_kernel(AttnArgs args) {
+  __shared__ FlashShared<HDP, GROUPS> sh;
+  __shared__ struct {
+    int seq, kv, tile, piece, pieces, per, item;
+  } mine;
+  const int tid = threadIdx.x, lane = tid & 63;
+  // Workgroups go to the 8 XCDs in turn: XCD x takes pieces x * grid / 8 and on, so that the row tiles of one KV head, which read
+  // the same keys, share an L2.
+  const int me = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+  {
+    const AttnArgs& a = args;
+    const int rep = a.rep, grid = gridDim.x;
+    if (tid < 64) {
+      // Every lane takes a run of requests: one, as a rule.
+      const int run = (a.seqs + 63) / 64, s0 = min(lane * run, a.seqs), s1 = min(s0 + run, a.seqs);
+      const TreeWork none = {0, 0, 1}, first = s0 < s1 ? tree_work<HDP>(a, s0, rep) : none;
+      auto of_run = [&](auto&& f) {  // f(request, its work) of the lane's requests
+        if (s0 < s1) f(s0, first);
+        for (int s = s0 + 1; s < s1; ++s) f(s, tree_work<HDP>(a, s, rep));
+      };
+      int items = 0, work = 0, longest = 1;
+      of_run([&](int, const TreeWork& w) {
+        const int n = times_work(w.tiles, a.kv_heads);
+        items = add_work(items, n);
+        work = add_work(work, times_work(n, w.key_tiles));
+        longest = max(longest, w.key_tiles);
+      });
+      auto pieces_of = [&](const TreeWork& w, int per) {
+        return times_work(times_work(w.tiles, a.kv_heads), (w.key_tiles + per - 1) / per);
+      };
+      auto all_pieces = [&](int per) {  // of this lane's requests
+        int n = 0;
+        of_run([&](int, const TreeWork& w) { n = add_work(n, pieces_of(w, per)); });
+        return n;
+      };
+      const int total_items = all_work(items), total = all_work(work);
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) longest = max(longest, __shfl_xor(longest, off));
+      // The smallest number of key tiles a piece, kTreeLeast or more, for which there are workgroups enough: more than
+      // total / (grid + 1), at most total / (grid - items) + 1.
+      int low = max(total / (grid + 1), kTreeLeast - 1);  // not enough, or fewer than that
+      int high = total_items < grid ? min(total / (grid - total_items) + 1, longest) : longest;
+      high = max(high, low + 1);
+      while (high - low > 1) {
+        const int per = low + ((high - low) >> 1);
+        if (all_work(all_pieces(per)) <= grid) high = per;
+        else low = per;
+      }
+      const int here = all_pieces(high), upto = work_prefix(here), items_upto = work_prefix(items);
+      if (lane == 0) mine.seq = -1;
+      int at = upto - here, item = items_upto - items;
+      if (upto != kNoWork && me >= at && me < upto) {
+        bool found = false;
+        of_run([&](int s, const TreeWork& w) {
+          const int n = pieces_of(w, high);
+          if (!found && me < at + n) {
+            const int pieces = (w.key_tiles + high - 1) / high;
+            const int i = (me - at) / pieces;  // items in the order KV head, row tile
+            mine.seq = s;
+            mine.kv = i / w.tiles;
+            mine.tile = i - mine.kv * w.tiles;
+            mine.piece = (me - at) - i * pieces;
+            mine.pieces = pieces;
+            mine.per = high;
+            mine.item = item + i;
+            found = true;
+          }
+          at += n;
+          item += times_work(w.tiles, a.kv_heads);
+        });
+      }
+      // Offsets that do not ascend can make more pieces than workgroups: none is joined then.
+      const int all = __builtin_amdgcn_readlane(upto, 63);
+      if (me == 0 && lane == 0) *tree_space<HDP>(a.ws, grid).count = all <= grid ? min(total_items, a.items) : 0;
+    }
+    if (a.zero_rest) zero_rows<E>(a, (int64_t)me * GROUPS * kFlashThreads + tid, (int64_t)gridDim.x * GROUPS * kFlashThreads);
+    __syncthreads();
+  }
+  const int seq = __builtin_amdgcn_readfirstlane(mine.seq);
+  if (seq < 0) return;
+  const AttnArgs a = reload_args();
+  const int kv = __builtin_amdgcn_readfirstlane(mine.kv), tile = __builtin_amdgcn_readfirstlane(mine.tile);
+  const int piece = __builtin_amdgcn_readfirstlane(mine.piece), pieces = __builtin_amdgcn_readfirstlane(mine.pieces);
+  const int per = __builtin_amdgcn_readfirstlane(mine.per), item = __builtin_amdgcn_readfirstlane(mine.item);
+  const TreeSpace space = tree_space<HDP>(a.ws, gridDim.x);
+  if (tid == 0 && piece == 0 && item < a.items) space.list[item] = TreeItem{seq, tile * kFlashRows, kv, me, pieces};
+  flash_item<E, HDP, Keys::kTree, GROUPS>(a, sh, a.rep, a.scale_log2, seq, tile * kFlashRows, kv, piece * per, (piece + 1) * per,
+                                          pieces == 1 ? nullptr : space.parts + (size_t)me * kFlashRows * (HDP + 2));
+}
+
+// Joins the pieces of item blockIdx.x, each wavefront 64 x 4 values, in the order of the keys.
+template <class E, int HDP>
+__global__ __launch_bounds__(64 * kJoinWaves) void join_tree_kernel(AttnArgs a, int grid) {
+  const TreeSpace space = tree_space<HDP>(a.ws, grid);
+  if ((int)blockIdx.x >= *space.count) return;
+  const TreeItem t = space.list[blockIdx.x];
+  const int pieces = __builtin_amdgcn_readfirstlane(t.pieces);
+  if (pieces == 1) return;
+  const int rep = a.rep, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tok0 = seq_offset(a.cu, t.seq, a.seqs, a.tokens);
+  const int rows = (seq_offset(a.cu, t.seq + 1, a.seqs, a.tokens) - tok0) * rep;
+  const int live = min(rows - t.row0, kFlashRows) * (HDP / 4);
+  constexpr int STRIDE = kFlashRows * (HDP + 2);
+  const int i = (blockIdx.y * kJoinWaves + wave) * 64 + lane;
+  if (i >= live) return;
+  const int r = i / (HDP / 4), d = 4 * (i % (HDP / 4));
+  const float* const from = space.parts + (size_t)t.first * STRIDE;
+  float top = -__builtin_inff(), l = 0.0f;
+  float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+  // As in join_pieces_kernel: nothing of a piece without keys, a NaN among scores is in the sum.
+  auto factor = [](float m, float high) { return m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - high); };
+  auto sum = [](float x, float f) { return x != x ? x : f * x; };
+  constexpr int AHEAD = 16;
+  for (int p0 = 0; p0 < pieces; p0 += AHEAD) {
+    float m[AHEAD], s[AHEAD], high = top;
+    float4_t x[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      m[j] = -__builtin_inff();
+      if (p0 + j >= pieces) continue;
+      const float* const p = from + (size_t)(p0 + j) * STRIDE;
+      m[j] = p[kFlashRows * HDP + r];
+      s[j] = p[kFlashRows * HDP + kFlashRows + r];
+      x[j] = *reinterpret_cast<const float4_t*>(p + r * HDP + d);
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) high = fmaxf(high, m[j]);
+    const float old = factor(top, high);
+    l = sum(l, old);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = scaled(v[e], old);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (p0 + j >= pieces) continue;
+      const float f = factor(m[j], high);
+      l += sum(s[j], f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += scaled(x[j][e], f);
+    }
+    top = high;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int row = t.row0 + r, tok = row / rep, head = t.kv * rep + (row - tok * rep);
+  if (d < a.head_dim)
+    store_global((E*)a.out + (size_t)(tok0 + tok) * a.out_token + (size_t)head * a.out_head + d,
+                 u32x2{Elem<E>::pack(v[0] * inv, v[1] * inv), Elem<E>::pack(v[2] * inv, v[3] * inv)});
+}
+
+template <class E, int HDP>
+hipError_t launch_tree(const AttnArgs& a, const FlashPlan& p, void* ws, hipStream_t stream) {
+  AttnArgs c = a;
+  c.scale_log2 = a.scale * 1.44269504088896340736f, c.rep = a.heads / a.kv_heads, c.ws = ws, c.items = p.items;
+  if (p.groups > 1) tree_cut_kernel<E, HDP, flash_groups(HDP)><<<p.grid, flash_groups(HDP) * kFlashThreads, 0, stream>>>(c);
+  else tree_cut_kernel<E, HDP, 1><<<p.grid, kFlashThreads, 0, stream>>>(c);
+  if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
+  join_tree_kernel<E, HDP><<<dim3((unsigned)p.items, kFlashRows * HDP / 4 / 64 / kJoinWaves), 64 * kJoinWaves, 0, stream>>>(c, p.grid);
+  return hipGetLastError();
+}
+
 template <class E, int HDP, Keys KEYS_OF>
 hipError_t launch(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws, hipStream_t stream) {
   const int rep = a.heads / a.kv_heads;
@@ -641,6 +842,7 @@ hipError_t launch(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws,
           <<<p.grid, kFlashThreads, 0, stream>>>(a, rep, min_rows, p.longest_first, scale_log2);
     return hipGetLastError();
   }
+  if constexpr (KEYS_OF == Keys::kTree) return launch_tree<E, HDP>(a, p, ws, stream);
   float* const parts = static_cast<float*>(ws);
   Piece* const pieces = reinterpret_cast<Piece*>(parts + (size_t)2 * p.grid * kFlashRows * (HDP + 2));
   AttnArgs c = a;
@@ -701,12 +903,43 @@ FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count) {
   // One sequence has its longest tiles last in any case, and workgroups that all run at once need no order.
   p.longest_first = a.seqs > 1 && a.seqs <= 64 && items * p.groups > cu_count * flash_waves_per_simd(hdp, false);
   p.grid = p.cut ? cu_count * flash_waves_per_simd(hdp, true) : (int)items;
+  p.items = 0;
+  return p;
+}
+
+// For trees (us over 8 KV heads of 128 as a rule):
+//   cut         as above, into pieces, where there are as many workgroups as items and more than 768 keys: below, the second
+//               launch costs more than the pieces spare (8 requests of 128 rows over 200 .. 500 keys 18 / 24 cut, 400 .. 700
+//               22 / 25; 64 rows over 1000 keys 22 / 18).  8 of 256 rows over 500 .. 4000 57 / 37, 16 of 30 .. 150 over 100 ..
+//               8000 (2 KV heads) 91 / 26, 24 of 96 over 500 .. 4000 61 / 49, 2 of 108 over up to 131071 1880 / 196.
+//   two groups  of wavefronts a workgroup where there are two or more pieces an item: half as many pieces to write and join (2 of
+//               108 rows over up to 131071 keys 200 / 196, 4 of 80 over 40000 118 / 116, one of 320 over 30000, 64 dims, 37 / 32).
+//               With more items two workgroups a CU even them out better (three of up to 64 dims): 128 of 12 rows over 4000 keys
+//               (2 KV heads) 74 two groups / 41 two workgroups, 64 of 100 .. 190 rows of 64 dims 44 / 38.
+FlashPlan tree_plan(const AttnArgs& a, int cu_count) {
+  FlashPlan p = flash_plan(a, true, cu_count);
+  const int64_t rep = a.heads / a.kv_heads, keys = (int64_t)a.table_width << a.log2_block;
+  const int64_t items = (a.tokens * rep / kFlashRows + a.seqs + 1) * a.kv_heads;
+  const int hdp = a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256;
+  const int held = flash_waves_per_simd(hdp, true);  // workgroups of one group that a CU holds
+  p.cut = keys > 768 && items <= (int64_t)held * cu_count;
+  if (!p.cut) {
+    p.grid = (int)items;
+    return p;
+  }
+  p.groups = 2 * items <= cu_count ? flash_groups(hdp) : 1;
+  p.grid = (p.groups > 1 ? 1 : held) * cu_count;
+  p.grid -= p.grid % 8;  // as many on every XCD
+  p.items = (int)items;
+  p.cut = p.grid >= items;
+  if (!p.cut) p.grid = (int)items;
   return p;
 }
 
 size_t flash_workspace_bytes(int head_dim, const FlashPlan& p) {
   if (!p.cut) return 0;
   const int padded = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+  if (p.items) return (size_t)p.grid * sizeof(float) * kFlashRows * (padded + 2) + 4 * sizeof(int) + (size_t)p.items * sizeof(TreeItem);
   return (size_t)p.grid * (2 * sizeof(float) * kFlashRows * (padded + 2) + sizeof(Piece));
 }
 

@@ -240,6 +240,7 @@ struct AttnArgs {
   int rep, min_rows;        // heads / kv_heads; sequences of fewer rows are not theirs
   void* ws;
   void* pieces;
+  int items;                // trees: FlashPlan's
   const uint64_t* ancestors;  // paged, or nullptr: [tokens] bit j: the row attends to its request's new token j
 };
 struct FlashPlan {
@@ -247,8 +248,10 @@ struct FlashPlan {
   int groups;  // of four wavefronts that share a row tile's keys
   bool longest_first;  // row tiles start in the order of their lengths
   int grid;
+  int items;  // trees, cut: an upper bound of (request, row tile, KV head) triples
 };
 FlashPlan flash_plan(const AttnArgs& a, bool paged, int cu_count);
+FlashPlan tree_plan(const AttnArgs& a, int cu_count);  // trees of new tokens over pages
 size_t flash_workspace_bytes(int head_dim, const FlashPlan& p);
 // Requests of fewer than min_rows rows are left to the other kernel.  ws: flash_workspace_bytes, 16-byte aligned.  Both
 // launchers take trees of new tokens where a.ancestors is set, chains of them where it is not.

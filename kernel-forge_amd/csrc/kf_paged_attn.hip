@@ -36,6 +36,9 @@ template <class E, int HDP, bool TREE>
 hipError_t launch_rows(const AttnArgs& a, const FewPlan& p, int max_rows, void* ws, hipStream_t stream) {
   if constexpr (HDP == 256) {  // one row tile of 256 dims fills the registers, two wavefronts the buffers
     return launch<E, HDP, 1, 2, TREE>(a, p, max_rows, ws, stream);
+  } else if constexpr (TREE) {  // more than one row tile goes to the other kernel
+    return p.waves == 2 ? launch<E, HDP, 1, 2, TREE>(a, p, max_rows, ws, stream)
+                        : launch<E, HDP, 1, 4, TREE>(a, p, max_rows, ws, stream);
   } else {
     if (p.waves == 2)
       return p.row_tiles == 2 ? launch<E, HDP, 2, 2, TREE>(a, p, max_rows, ws, stream)
