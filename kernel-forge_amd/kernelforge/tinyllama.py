@@ -146,10 +146,10 @@ class Attention(nn.Module):
             return y[..., :nqk], y[..., nqk:]
         return torch.cat([self.q_proj(x), self.k_proj(x)], dim=-1), self.v_proj(x)
 
-    def paged(self, x, step, rope, cache_k, cache_v, block_table, max_new, whole_prompts, norm=None):
+    def paged(self, x, step, rope, cache_k, cache_v, block_table, max_new, whole_prompts, trees=None, norm=None):
         """Attention of several requests' new tokens, x [1, T, H] packed (normalized unless `norm` is given), over
         a paged cache: [1, T, heads d], before o_proj.  whole_prompts: no request with new tokens has any in the
-        cache yet."""
+        cache yet.  trees (ops.draft_trees): the new tokens are the nodes of trees."""
         cfg = self.cfg
         if self.qkv is None:
             qkv = torch.cat(self.project(x, norm), dim=-1)
@@ -159,9 +159,12 @@ class Attention(nn.Module):
             qkv = self.qkv.forward_concat(x)
         qkv = qkv.view(-1, qkv.shape[-1])
         v = qkv[:, (cfg.heads + cfg.kv_heads) * cfg.head_dim:]
-        q, k = ops.rope_paged_cache(qkv, rope[0], rope[1], step.positions, step.slots, cache_k, cache_v,
-                                    heads=cfg.heads)
-        if whole_prompts:
+        q, k = ops.rope_paged_cache(qkv, rope[0], rope[1], step.positions if trees is None else trees.positions, step.slots,
+                                    cache_k, cache_v, heads=cfg.heads)
+        if trees is not None:
+            out = ops.paged_tree_attention(q, cache_k, cache_v, block_table, step.cu_new, step.seq_lens, trees.ancestors,
+                                           max_new=max_new)
+        elif whole_prompts:
             out = ops.prompt_attention(q, k, v.unflatten(1, (cfg.kv_heads, cfg.head_dim)), step.cu_new)
         else:
             out = ops.paged_attention(q, cache_k, cache_v, block_table, step.cu_new, step.seq_lens, max_new=max_new)
@@ -338,13 +341,16 @@ class TinyLlama(nn.Module):
 
     @torch.no_grad()
     def forward_paged(self, tokens, step: ops.PagedStep, cache, rope, block_table, *, max_new: int,
-                      whole_prompts: bool = False):
+                      whole_prompts: bool = False, trees: ops.DraftTrees | None = None):
         """Several requests at once: tokens int64 [T], packed request by request as `step` (ops.paged_tables) says; cache
         from new_paged_cache; rope: the fp32 tables of _rope_tables.  Returns the logits after each request's last new
-        token, [requests, vocab] (of some other token for requests without new ones)."""
+        token, [requests, vocab] (of some other token for requests without new ones).  With trees (ops.draft_trees) the
+        new tokens are the nodes of a tree per request, and the logits after each of them are returned, [T, vocab]."""
         x = self.embed_tokens(tokens).unsqueeze(0)
         for i, layer in enumerate(self.layers):
-            x = layer.paged(x, step, rope, cache[i, 0], cache[i, 1], block_table, max_new, whole_prompts)
+            x = layer.paged(x, step, rope, cache[i, 0], cache[i, 1], block_table, max_new, whole_prompts, trees)
+        if trees is not None:
+            return self.lm_head(self.norm(x[0]))
         last = (step.cu_new[1:].long() - 1).clamp(0, tokens.numel() - 1)
         return self.lm_head(self.norm(x[0, last]))
 
@@ -501,8 +507,8 @@ class PagedDecoder:
     """Greedy decode of several requests at once over a paged KV cache, one HIP-graph-captured step for all.
 
     Every request has a row.  ``admit`` gives prompts to free rows (whole, or in chunks between which nothing else runs),
-    ``decode`` appends one token per step to every row that holds a request, ``finish`` frees a row and returns its
-    pages.  Lengths, tables and the stack of free pages are on the device, where the step advances them; the host
+    ``decode`` appends one token per step to every row that holds a request, ``decode_drafts`` as many drafted ones as the
+    model agrees with and one more, ``finish`` frees a row and returns its pages.  Lengths, tables and the stack of free pages are on the device, where the step advances them; the host
     keeps its own count of lengths and pages and refuses (ValueError) what would pass max_seq or the pages there are.
     """
 
@@ -660,6 +666,105 @@ class PagedDecoder:
         finally:
             self.host_lens = [n + done if n else 0 for n in self.host_lens]
         return self.history
+
+    def _packed_drafts(self, drafts: dict) -> tuple[list[int], torch.Tensor, torch.Tensor, list]:
+        """(nodes per row, tokens, parents, (first node, parents, probabilities) of drafts that have some), checked."""
+        vocab, dev = self.model.cfg.vocab, self.tokens.device
+        for row in drafts:
+            if not 0 <= row < len(self.host_lens) or not self.host_lens[row]:
+                raise ValueError(f"decode_drafts: row {row} holds no request")
+        new, tokens, parents, drawn, at = [0] * len(self.host_lens), [], [], [], 0
+        for row, held in enumerate(self.host_lens):
+            if not held:
+                continue
+            draft = drafts.get(row, self.tokens[:0])
+            draft, above, probs = (draft, None, None) if isinstance(draft, torch.Tensor) else (*draft, None)[:3]
+            n = draft.numel()
+            if draft.dim() != 1 or draft.dtype not in (torch.int64, torch.int32) or draft.device != dev:
+                raise ValueError(f"decode_drafts: the tokens of row {row} must be 1-D int64 on {dev}, got "
+                                 f"{str(draft.dtype)[6:]} {list(draft.shape)} on {draft.device}")
+            if n >= ops.MAX_NODES:
+                raise ValueError(f"decode_drafts: row {row} has {n} drafted tokens, more than {ops.MAX_NODES - 1}")
+            if above is None:
+                above = torch.arange(-1, n - 1, device=dev)
+            if above.shape != draft.shape or above.dtype not in (torch.int64, torch.int32) or above.device != dev:
+                raise ValueError(f"decode_drafts: the parents of row {row} must be int64 [{n}] on {dev}")
+            if probs is not None:
+                if probs.shape != (n, vocab) or probs.dtype != torch.float32 or probs.device != dev:
+                    raise ValueError(f"decode_drafts: the probabilities of row {row} must be float32 [{n}, {vocab}] on {dev}")
+                drawn.append((at, above, probs))
+            new[row] = n + 1
+            tokens += [self.tokens[row:row + 1], draft.long()]
+            parents += [above.new_full((1,), -1), above + 1]
+            at += n + 1
+        if drawn and len(drawn) != sum(n > 1 for n in new):
+            raise ValueError("decode_drafts: all drafts of a step have probabilities, or none")
+        if not tokens:
+            return new, self.tokens[:0], self.tokens[:0].int(), drawn
+        tokens = torch.cat(tokens)
+        if bool(((tokens < 0) | (tokens >= vocab)).any()):
+            raise ValueError(f"decode_drafts: a drafted token is outside of the vocabulary of {vocab}")
+        return new, tokens, torch.cat([p.int() for p in parents]), drawn
+
+    @torch.no_grad()
+    def decode_drafts(self, drafts: dict, *, temperature: float = 0.0,
+                      generator: torch.Generator | None = None) -> list[int]:
+        """One step that takes drafted tokens: every row that holds a request gets those that the model agrees with and one
+        more token; returns how many each row got.
+
+        drafts: row -> what may follow its last token: int64 tokens [n] one after the other, or (tokens, parents) with
+        parents[i] the number of the drafted token that token i follows, smaller than i (-1: the row's last token), up to 63 tokens.
+        Rows without drafts get one token.  Greedy at temperature 0, and then as ``decode`` to within roundings.  Otherwise
+        tokens are distributed as if drawn one by one at that temperature, with random numbers from `generator`; drafts that
+        were drawn from probabilities come with them, (tokens, parents, float32 [n, vocab]), and all drafts of the step do.
+        Eager: the host waits for the counts."""
+        if not 0.0 <= temperature < float("inf"):
+            raise ValueError(f"decode_drafts: the temperature must be 0 or positive, got {temperature}")
+        new, tokens, parents, drawn = self._packed_drafts(drafts)
+        if drawn and temperature == 0.0:
+            raise ValueError("decode_drafts: probabilities of drafts need a temperature")
+        self._reserve(new, "decode_drafts")
+        if not any(new):
+            return new
+        try:
+            counts = self._verify_step(new, tokens, parents, drawn, temperature, generator)
+        finally:
+            # Pages that a row does not have, or not any longer, leave its table.
+            pages = (self.context_lens + self.block_size - 1) // self.block_size
+            self.block_table.masked_fill_(torch.arange(self.block_table.shape[1], device=self.device) >= pages[:, None], -1)
+        self.host_lens = [n + c for n, c in zip(self.host_lens, counts)]
+        return counts
+
+    def _verify_step(self, new, tokens, parents, drawn, temperature, generator) -> list[int]:
+        """decode_drafts on packed drafts: the step, and what the device keeps of it."""
+        step = ops.paged_tables(self.block_table, self.context_lens, torch.tensor(new, dtype=torch.int32, device=self.device),
+                                self.free_pages, self.free_count, block_size=self.block_size, max_tokens=sum(new))
+        trees = ops.draft_trees(parents, step.cu_new, step.seq_lens)
+        logits = self.model.forward_paged(tokens, step, self.cache, self.rope, self.block_table, max_new=max(new), trees=trees)
+        if temperature == 0.0:
+            done = ops.verify_drafts(tokens, parents, step.cu_new, logits, max_new=max(new))
+        else:
+            target = torch.softmax(logits.float() / temperature, dim=-1)
+            accept = torch.rand(tokens.numel(), generator=generator, device=self.device)
+            sample = torch.rand(len(new), generator=generator, device=self.device)
+            draft = None
+            if drawn:  # what each node's children were drawn from, in the node's row
+                draft = torch.zeros_like(target)
+                for first, above, probs in drawn:
+                    draft[first + 1 + above.long()] = probs
+            done = ops.verify_drafts(tokens, parents, step.cu_new, target, accept, sample, draft=draft, max_new=max(new))
+        counts = done.counts.tolist()
+        kept = ops.keep_drafts(self.cache, self.block_table, self.context_lens, step.seq_lens, done.counts, done.path,
+                               self.free_pages, step.free_count)
+        # Emitted tokens stand behind each row's last one.
+        place = torch.arange(done.tokens.shape[1], device=self.device)
+        row, i = (place < done.counts[:, None]).nonzero(as_tuple=True)
+        self.history[row, self.context_lens.long()[row] + 1 + i] = done.tokens[row, i]
+        last = done.tokens.gather(1, (done.counts.long() - 1).clamp(min=0).unsqueeze(1))[:, 0]
+        self.tokens.copy_(torch.where(done.counts > 0, last, self.tokens))
+        self.context_lens.copy_(kept.context_lens)
+        self.free_count.copy_(kept.free_count)
+        return counts
 
     def generated(self, row: int, prompt_len: int) -> torch.Tensor:
         """The tokens generated so far for a row, the one not yet in the cache included."""
