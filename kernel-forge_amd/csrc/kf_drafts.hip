@@ -133,9 +133,10 @@ __device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
   }
 }
 
-constexpr int kBestThreads = 256, kBestStep = 8 * kBestThreads;
+constexpr int kBestThreads = 256, kBestAhead = 4, kBestStep = 8 * kBestThreads;
 
-// keys[row * shares + share] = the largest of the share's part of the row.
+// keys[row * shares + share] = the largest of the share's part of the row.  Bound by memory: a thread keeps the largest value and the
+// eight that it is among, which it reads again at the end, so that a value costs two vector instructions in place of five.
 template <class T>
 __global__ __launch_bounds__(kBestThreads) void best_token_kernel(VerifyArgs a, int shares, int part) {
   __shared__ uint64_t keys[kBestThreads / 64];
@@ -143,28 +144,45 @@ __global__ __launch_bounds__(kBestThreads) void best_token_kernel(VerifyArgs a, 
   if (row >= seq_offset(a.cu, a.seqs, a.seqs, a.tokens_count)) return;
   const T* const src = (const T*)a.target + (int64_t)row * a.target_row;
   const int begin = share * part, end = min(begin + part, a.vocab), tid = threadIdx.x;
-  float best = -__builtin_inff();
-  int at = 0;
-  bool any = false;  // a row of -inf has its first index as well
-  auto take = [&](float x, int i) {
-    if (!any || x > best || (x != x && best == best)) {
-      best = x;
-      at = i;
-      any = true;
-    }
-  };
   // A row of 16-bit values may begin between two words: its first value is taken alone.
   const int odd = sizeof(T) == 2 ? (int)((uintptr_t)(src + begin) >> 1 & 1) : 0;
-  if (odd && tid == 0 && begin < end) take((float)src[begin], begin);
-  int i = begin + odd + 8 * tid;
-  for (; i + 8 <= end; i += kBestStep) {
-    float x[8];
-    load8(src + i, x);
+  float best = -__builtin_inff();
+  int group = -1;  // of eight values from begin + odd + 8 group on; -1: none above -inf
+  const int groups = (end - begin - odd) / 8;
+  auto above = [](float x, float y) { return !(x <= y) && y == y; };  // NaN above all numbers
+  auto look = [&](const float(&x)[8], int g) {
+    const float m0 = __builtin_elementwise_maximum(__builtin_elementwise_maximum(x[0], x[1]), x[2]);
+    const float m1 = __builtin_elementwise_maximum(__builtin_elementwise_maximum(x[3], x[4]), x[5]);
+    const float m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(__builtin_elementwise_maximum(x[6], x[7]), m0), m1);
+    if (above(m, best)) {
+      best = m;
+      group = g;
+    }
+  };
+  int g = tid;
+  for (; g + (kBestAhead - 1) * kBestThreads < groups; g += kBestAhead * kBestThreads) {
+    float x[kBestAhead][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) take(x[e], i + e);
+    for (int n = 0; n < kBestAhead; ++n) load8(src + begin + odd + 8 * (g + n * kBestThreads), x[n]);
+#pragma unroll
+    for (int n = 0; n < kBestAhead; ++n) look(x[n], g + n * kBestThreads);
   }
-  for (int e = 0; e < 8 && i + e < end; ++e) take((float)src[i + e], i + e);
-  uint64_t key = any ? score_key(best, at) : 0;
+  for (; g < groups; g += kBestThreads) {
+    float x[8];
+    load8(src + begin + odd + 8 * g, x);
+    look(x, g);
+  }
+  uint64_t key = 0;
+  auto offer = [&](float x, int i) {
+    const uint64_t k = score_key(x, i);
+    key = k > key ? k : key;
+  };
+  if (group >= 0)
+    for (int e = 0; e < 8; ++e) offer((float)src[begin + odd + 8 * group + e], begin + odd + 8 * group + e);
+  // The values before and behind the groups, and the first of all, in case they are all -inf.
+  const int rest = begin + odd + 8 * groups;
+  if (tid < 8 && rest + tid < end) offer((float)src[rest + tid], rest + tid);
+  if (tid == 0 && begin < end) offer((float)src[begin], begin);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) {
     const uint64_t other = __shfl_xor(key, off);
@@ -346,24 +364,47 @@ struct Rest {
     for (int e = 0; e < 4; ++e) v[e] = i + e < end ? row[i + e] : 0.0f;
     return v;
   }
-  // The sum over [begin, end) by one wavefront, the same in all lanes.
+  // The sum over [begin, end) by one wavefront, the same in all lanes: in groups of four values, of which the next come while
+  // the present ones are added up, then up to three values alone.
+  struct Batch {
+    static constexpr int N = DRAWN ? 4 : 8;
+    row4_t x[N], y[N];
+  };
+  __device__ __forceinline__ Batch load_batch(int begin, int group, int groups) const {
+    Batch b;
+#pragma unroll
+    for (int j = 0; j < Batch::N; ++j) {
+      const int i = begin + 4 * (group + 64 * j < groups ? group + 64 * j : 0);  // past the last one: the first, for nothing
+      b.x[j] = *(const row4_t*)(p + i);
+      if (DRAWN) b.y[j] = *(const row4_t*)(q + i);
+    }
+    return b;
+  }
   __device__ __forceinline__ double wave_total(int begin, int end, int lane) const {
-    constexpr int AHEAD = 8;  // loads of each row on their way
     double sum = 0.0;
-    for (int i0 = begin; i0 < end; i0 += 256 * AHEAD) {
-      row4_t x[AHEAD], y[AHEAD];
+    const int groups = max(end - begin, 0) / 4;
+    if (groups > 0) {
+      Batch now = load_batch(begin, lane, groups), next;
+      for (int g0 = 0; g0 < groups; g0 += 64 * Batch::N) {
+        if (g0 + 64 * Batch::N < groups) next = load_batch(begin, g0 + 64 * Batch::N + lane, groups);
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        x[j] = load(p, i0 + 256 * j + 4 * lane, end);
-        if (DRAWN) y[j] = load(q, i0 + 256 * j + 4 * lane, end);
+        for (int j = 0; j < Batch::N; ++j) {
+          const int g = g0 + 64 * j + lane;
+          if (g0 + 64 * j < groups) {
+            double f[4];
+            four<64>(now.x[j], now.y[j], begin + 4 * g, begin + 4 * (g0 + 64 * j), f);
+            const double four_of = (f[0] + f[1]) + (f[2] + f[3]);
+            sum += g < groups ? four_of : 0.0;
+          }
+        }
+        now = next;
       }
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        if (i0 + 256 * j >= end) break;
-        double f[4];
-        four<64>(x[j], y[j], i0 + 256 * j + 4 * lane, i0 + 256 * j, f);
-        sum += (f[0] + f[1]) + (f[2] + f[3]);
-      }
+    }
+    const int rest = begin + 4 * groups;
+    if (rest + lane < end) {
+      double f[4];
+      four<64>(row4_t{p[rest + lane], 0.0f, 0.0f, 0.0f}, row4_t{DRAWN ? q[rest + lane] : 0.0f, 0.0f, 0.0f, 0.0f}, rest + lane, rest, f);
+      sum += f[0];
     }
     return wave_sum(sum);
   }
@@ -498,16 +539,25 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a,
     for (int v = 0; v < kPickWaves; ++v) all += sh.parts[v];
     return all;
   };
-  if constexpr (DRAWN) {
-    // Further children: each test needs the sum of what the ones before have left.
-    uint64_t open = w.under & (w.under - 1);  // the first has been rejected
-    while (open) {
-      const double left = summed ? add_pieces() : row_total(sh, rest_of<true>(a, walked, w), 0, a.vocab, lane, wave);
+  // Drawn: the last node's further children, each of whose tests needs the sum of what the ones before have left; the first one has
+  // been rejected.  Then the sum of what is left to draw from.
+  uint64_t open = DRAWN ? w.under & (w.under - 1) : 0;
+  bool whole = false;
+  double all;
+  Rest<DRAWN> rest;
+  while (true) {
+    rest = rest_of<DRAWN>(a, walked, w);
+    if (whole) {
+      rest.taken = 0.0;
+      rest.gone_count = 0;
+    }
+    all = summed ? add_pieces() : row_total(sh, rest, 0, a.vocab, lane, wave);
+    if (open) {
       const int c = __builtin_ctzll(open);
       open &= open - 1;
       summed = false;
-      if (!(walked.u[c] * left * walked.q[c] < positive(walked.p[c] - w.taken * walked.q[c]))) {
-        w.taken += left;
+      if (!(walked.u[c] * all * walked.q[c] < positive(walked.p[c] - w.taken * walked.q[c]))) {
+        w.taken += all;
         continue;
       }
       // Accepted: on along first children, as far as they are.
@@ -523,18 +573,14 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a,
         w.on |= 1ull << e;
         w.last = e;
       }
+    } else if (all > 0.0 || whole) {
+      break;
+    } else {
+      whole = true;  // nothing is left, where the probabilities do not add up: the token is drawn from all of the row
+      summed = false;
     }
   }
   if (wave == 0) write_path(a, r, w.on, walked.token[lane], lane);
-  Rest<DRAWN> rest = rest_of<DRAWN>(a, walked, w);
-  double all = summed ? add_pieces() : row_total(sh, rest, 0, a.vocab, lane, wave);
-  if (!(all > 0.0)) {
-    // Nothing is left, where the probabilities do not add up: the token is drawn from all of the row.
-    rest.taken = 0.0;
-    rest.gone_count = 0;
-    summed = false;
-    all = row_total(sh, rest, 0, a.vocab, lane, wave);
-  }
   const double mark = (double)sample_u * all;
 
   // The part of [begin, end) with whose end the sum passes the mark; if none does (a number that is not below 1), the last with any.
@@ -692,7 +738,10 @@ __global__ __launch_bounds__(kKeepThreads) void keep_drafts_kernel(KeepArgs a) {
   }
 }
 
-constexpr int kSumFrom = 32768;
+// Rows up to which one workgroup adds them up.  One launch / two, us: tokens given, 16 requests of 32000 values 11.5 / 13.1, of 40000
+// 13.4 / 13.0, of 50000 14.4 / 13.0, of 65000 15.8 / 13.1; drawn, 16 of 32000 16.5 / 17.7, of 40000 16.1 / 16.0, of 65000 25.2 / 23.8.  A
+// launch takes some 3 us of the host's time besides.
+constexpr int kSumFrom = 40960;
 
 // Workgroups per row of scores, where there are fewer rows than fill the card, of at least four rounds of loads.
 int row_shares(const VerifyArgs& a) {

@@ -1386,8 +1386,7 @@ def draft_trees(parents: torch.Tensor, cu_new: torch.Tensor, seq_lens: torch.Ten
 def _run_draft_trees(parents, cu_new, seq_lens) -> DraftTrees:
     """kf_draft_trees on checked arguments of the current device."""
     t = parents.shape[0]
-    odd = t & 1  # both start at 16 bytes, as rope_paged_cache takes positions
-    positions, _, ancestors = parents.new_empty(2 * t + odd, dtype=torch.int64).split_with_sizes((t, odd, t))
+    ancestors, positions = parents.new_empty(t, dtype=torch.int64), parents.new_empty(t, dtype=torch.int64)
     args = _lib.pack_draft_trees(parents.data_ptr(), cu_new.data_ptr(), seq_lens.data_ptr(), ancestors.data_ptr(),
                                  positions.data_ptr(), t, seq_lens.shape[0])
     status = _lib.load().kf_draft_trees(args, torch._C._cuda_getCurrentRawStream(parents.get_device()))
@@ -1398,7 +1397,7 @@ def _run_draft_trees(parents, cu_new, seq_lens) -> DraftTrees:
 
 @torch.library.custom_op("kernelforge::draft_trees", mutates_args=())
 def _draft_trees_op(parents: torch.Tensor, cu_new: torch.Tensor, seq_lens: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    return tuple(t.clone() for t in draft_trees(parents, cu_new, seq_lens))  # an op's outputs must not be views of one tensor
+    return tuple(draft_trees(parents, cu_new, seq_lens))
 
 
 @_draft_trees_op.register_fake
@@ -1537,8 +1536,7 @@ def _run_verify(tokens, parents, cu_new, target, accept_uniforms, sample_uniform
     """kf_verify_drafts on checked arguments of the current device."""
     t, vocab = target.shape
     b = cu_new.shape[0] - 1
-    counts, path = parents.new_empty(b * (width + 1)).split_with_sizes((b, b * width))
-    emitted = tokens.new_empty((b, width))
+    counts, path, emitted = parents.new_empty(b), parents.new_empty((b, width)), tokens.new_empty((b, width))
     sampled = accept_uniforms is not None
     mode = _lib.KF_VERIFY_BEST if not sampled else _lib.KF_VERIFY_GIVEN if draft is None else _lib.KF_VERIFY_DRAWN
     args = _lib.pack_verify_drafts(tokens.data_ptr(), parents.data_ptr(), cu_new.data_ptr(), target.data_ptr(),
@@ -1554,15 +1552,14 @@ def _run_verify(tokens, parents, cu_new, target, accept_uniforms, sample_uniform
                                   torch._C._cuda_getCurrentRawStream(tokens.get_device()))
     if status:
         _lib.check(status, "verify_drafts")
-    return VerifiedDrafts(counts, path.view(b, width), emitted)
+    return VerifiedDrafts(counts, path, emitted)
 
 
 @torch.library.custom_op("kernelforge::verify_drafts", mutates_args=())
 def _verify_drafts_op(tokens: torch.Tensor, parents: torch.Tensor, cu_new: torch.Tensor, target: torch.Tensor,
                       accept_uniforms: Optional[torch.Tensor], sample_uniforms: Optional[torch.Tensor],
                       draft: Optional[torch.Tensor], width: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    counts, path, emitted = _launch_verify(tokens, parents, cu_new, target, accept_uniforms, sample_uniforms, draft, width)
-    return counts.clone(), path.clone(), emitted
+    return tuple(_launch_verify(tokens, parents, cu_new, target, accept_uniforms, sample_uniforms, draft, width))
 
 
 @_verify_drafts_op.register_fake
@@ -1584,51 +1581,47 @@ def keep_drafts(caches: torch.Tensor | list[torch.Tensor], block_table: torch.Te
     one. block_table keeps their numbers, where paged_tables enters new ones. Pages must not be shared between requests.
     No reference counterpart.
     """
+    tables = (block_table, context_lens, seq_lens, counts, path)
+    if (free_pages is not None and free_count is not None and isinstance(caches, torch.Tensor)
+            and _direct(block_table.get_device(), (caches, *tables, free_pages, free_count)) and block_table.dim() == 2
+            and path.dim() == 2 and _kept_cache_ok(caches)):
+        b, columns = block_table.shape
+        rows, width = path.shape
+        i32 = torch.int32
+        if (b > 0 and columns > 0 and block_table.stride(1) == 1 and rows == b and 0 < width <= MAX_NODES and path.stride(1) == 1
+                and context_lens.shape == (b,) and seq_lens.shape == (b,) and counts.shape == (b,)
+                and context_lens.is_contiguous() and seq_lens.is_contiguous() and counts.is_contiguous()
+                and block_table.dtype == i32 and context_lens.dtype == i32 and seq_lens.dtype == i32 and counts.dtype == i32
+                and path.dtype == i32 and free_pages.dtype == i32 and free_count.dtype == i32 and free_pages.dim() == 1
+                and free_pages.is_contiguous() and free_count.shape == (1,)):
+            return KeptDrafts(*_run_keep(caches, *tables, free_pages, free_count).split_with_sizes((b, 1)))
     listed = [caches] if isinstance(caches, torch.Tensor) else list(caches)
     if not listed:
         raise ValueError("keep_drafts needs at least one cache")
     if (free_pages is None) != (free_count is None):
         raise ValueError("free_pages and free_count come together")
+    b = block_table.shape[0] if block_table.dim() == 2 else -1
+    _check_table(block_table, b)
+    if b < 1:
+        raise ValueError("keep_drafts needs at least one request")
+    for name, t in (("context_lens", context_lens), ("seq_lens", seq_lens), ("counts", counts)):
+        _check_int(name, t, torch.int32, (b,))
+    if (path.dim() != 2 or path.dtype != torch.int32 or path.shape[0] != b or not 0 < path.shape[1] <= MAX_NODES
+            or path.stride(1) != 1):
+        raise ValueError(f"path must be int32 [{b}, up to {MAX_NODES}] with contiguous rows, got {str(path.dtype)[6:]} "
+                         f"{list(path.shape)}")
     stack = () if free_pages is None else (free_pages, free_count)
-    tables = (block_table, context_lens, seq_lens, counts, path, *stack)
-    i32 = torch.int32
-    direct = _direct(block_table.get_device(), (*listed, *tables)) and block_table.dim() == 2
-    if direct:
-        b, width = block_table.shape
-        direct = (b > 0 and width > 0 and block_table.stride(1) == 1 and path.dim() == 2 and path.shape[0] == b
-                  and 0 < path.shape[1] <= MAX_NODES and path.stride(1) == 1
-                  and context_lens.shape == (b,) and seq_lens.shape == (b,) and counts.shape == (b,)
-                  and context_lens.is_contiguous() and seq_lens.is_contiguous() and counts.is_contiguous()
-                  and all(t.dtype == i32 for t in tables)
-                  and (not stack or (free_pages.dim() == 1 and free_pages.is_contiguous() and free_count.shape == (1,)))
-                  and all(_kept_cache_ok(c) for c in listed))
-    if not direct:
-        b = block_table.shape[0] if block_table.dim() == 2 else -1
-        _check_table(block_table, b)
-        if b < 1:
-            raise ValueError("keep_drafts needs at least one request")
-        for name, t in (("context_lens", context_lens), ("seq_lens", seq_lens), ("counts", counts)):
-            _check_int(name, t, i32, (b,))
-        if (path.dim() != 2 or path.dtype != i32 or path.shape[0] != b or not 0 < path.shape[1] <= MAX_NODES
-                or path.stride(1) != 1):
-            raise ValueError(f"path must be int32 [{b}, up to {MAX_NODES}] with contiguous rows, got {str(path.dtype)[6:]} "
-                             f"{list(path.shape)}")
-        if stack:
-            _check_int("free_count", free_count, i32, (1,))
-            if free_pages.dtype != i32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
-                raise ValueError("free_pages must be a contiguous 1-D int32 tensor")
-        _check_plain("keep_drafts", (*listed, *tables))
-        for cache in listed:
-            _check_kept_cache(cache)
-    kept = None
-    for i, cache in enumerate(listed):
-        arrays = cache if cache.dim() == 5 else cache.flatten(0, -5) if cache.dim() > 5 else cache[None]
-        args = (arrays, *tables[:5], *((free_pages, free_count) if stack and i == 0 else (None, None)))
-        if direct:
-            lens = _run_keep(*args)
-        else:
-            lens = (_keep_drafts_op if _traced((*listed, *tables)) else _launch_keep)(*args)
-        kept = lens if i == 0 else kept
+    if stack:
+        _check_int("free_count", free_count, torch.int32, (1,))
+        if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
+            raise ValueError("free_pages must be a contiguous 1-D int32 tensor")
+    _check_plain("keep_drafts", (*listed, *tables, *stack))
+    for cache in listed:
+        _check_kept_cache(cache)
+    run = _keep_drafts_op if _traced((*listed, *tables, *stack)) else _launch_keep
+    kept = run(listed[0], *tables, free_pages, free_count)
+    for cache in listed[1:]:  # the lengths and the stack are dealt with
+        run(cache, *tables, None, None)
     return KeptDrafts(kept[:b], kept[b:] if stack else None)
 
 
@@ -1638,8 +1631,18 @@ def _one_stride(t: torch.Tensor) -> bool:
 
 
 def _kept_cache_ok(t: torch.Tensor) -> bool:
-    return (t.dim() >= 4 and t.dtype in _HALF_TYPES and t.numel() > 0 and _rows_ok(t) and _own_places(t) and _one_stride(t)
-            and 16 <= t.shape[-2] <= 1 << 20 and not t.shape[-2] & (t.shape[-2] - 1) and not t.shape[-1] & 7)
+    """_check_kept_cache as one test, for plain tensors of five or six dimensions."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 6:
+        if stride[0] != stride[1] * shape[1]:
+            return False
+        shape, stride = shape[1:], stride[1:]
+    if len(shape) != 5 or t.dtype not in _HALF_TYPES:
+        return False
+    a, b, c, d, one = stride
+    block = shape[3]
+    return (one == 1 and not (a | b | c | d) & 7 and a > 0 and b > 0 and c > 0 and d > 0 and not t.data_ptr() & 15
+            and 16 <= block <= 1 << 20 and not block & (block - 1) and not shape[4] & 7 and t.numel() > 0)
 
 
 def _check_kept_cache(t: torch.Tensor) -> None:
@@ -1669,8 +1672,9 @@ def _launch_keep(caches, block_table, context_lens, seq_lens, counts, path, free
 
 def _run_keep(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count) -> torch.Tensor:
     """kf_keep_drafts on checked arguments of the current device; the new lengths and the stack's count in one tensor."""
-    arrays, pages, kv_heads, block_size, d = caches.shape
-    array, page, head, token, _ = caches.stride()
+    pages, kv_heads, block_size, d = caches.shape[-4:]
+    page, head, token, _ = caches.stride()[-4:]
+    arrays, array = caches.numel() // (pages * kv_heads * block_size * d), caches.stride(-5) if caches.dim() > 4 else 0
     b = block_table.shape[0]
     kept = context_lens.new_empty(b + 1)
     stack = free_count is not None

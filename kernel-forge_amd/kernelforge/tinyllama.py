@@ -673,7 +673,7 @@ class PagedDecoder:
         for row in drafts:
             if not 0 <= row < len(self.host_lens) or not self.host_lens[row]:
                 raise ValueError(f"decode_drafts: row {row} holds no request")
-        new, tokens, parents, drawn, at = [0] * len(self.host_lens), [], [], [], 0
+        new, tokens, parents, numbers, drawn, at = [0] * len(self.host_lens), [], [], [], [], 0
         for row, held in enumerate(self.host_lens):
             if not held:
                 continue
@@ -696,15 +696,21 @@ class PagedDecoder:
             new[row] = n + 1
             tokens += [self.tokens[row:row + 1], draft.long()]
             parents += [above.new_full((1,), -1), above + 1]
+            numbers.append(torch.arange(n + 1, device=dev))
             at += n + 1
         if drawn and len(drawn) != sum(n > 1 for n in new):
             raise ValueError("decode_drafts: all drafts of a step have probabilities, or none")
         if not tokens:
             return new, self.tokens[:0], self.tokens[:0].int(), drawn
-        tokens = torch.cat(tokens)
-        if bool(((tokens < 0) | (tokens >= vocab)).any()):
+        tokens, parents, numbers = torch.cat(tokens), torch.cat([p.long() for p in parents]), torch.cat(numbers)
+        outside = ((tokens < 0) | (tokens >= vocab)).any()
+        orphan = ((numbers > 0) & ((parents < 0) | (parents >= numbers))).any()
+        outside, orphan = torch.stack([outside, orphan]).tolist()
+        if outside:
             raise ValueError(f"decode_drafts: a drafted token is outside of the vocabulary of {vocab}")
-        return new, tokens, torch.cat([p.int() for p in parents]), drawn
+        if orphan:
+            raise ValueError("decode_drafts: a drafted token's parent must be one before it, or -1")
+        return new, tokens, parents.int(), drawn
 
     @torch.no_grad()
     def decode_drafts(self, drafts: dict, *, temperature: float = 0.0,

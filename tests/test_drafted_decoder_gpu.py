@@ -177,7 +177,8 @@ def test_refusals(model):
     for drafts, match in (({1: t}, "holds no request"), ({5: t}, "holds no request"), ({0: t.float()}, "1-D int64"),
                           ({0: t[None]}, "1-D int64"), ({0: t.cpu()}, "1-D int64"), ({0: (t, t[:2])}, "the parents"),
                           ({0: (t, t.float())}, "the parents"), ({0: t + 2000}, "outside of the vocabulary"),
-                          ({0: t - 1}, "outside of the vocabulary"), ({0: t.new_zeros(64)}, "more than 63"),
+                          ({0: t - 1}, "outside of the vocabulary"), ({0: (t, t - 2)}, "one before it"),
+                          ({0: (t, t)}, "one before it"), ({0: (t, t + (1 << 40))}, "one before it"), ({0: t.new_zeros(64)}, "more than 63"),
                           ({0: (t, t - 1, torch.zeros(3, 7, device=DEV))}, "the probabilities"),
                           ({0: (t, t - 1, torch.zeros(3, 2000, device=DEV))}, "need a temperature")):
         with pytest.raises(ValueError, match=match):

@@ -197,7 +197,7 @@ def test_verify_drafts_abi(change, match):
 def test_verify_workspaces():
     lib = _lib.load()
     for mode in (0, 1, 2):
-        args = struct(_lib.VerifyDraftsArgs, dtype=0, mode=mode)
+        args = struct(_lib.VerifyDraftsArgs, dtype=0, mode=mode, vocab=100000)
         need = lib.kf_verify_drafts_workspace_bytes(ctypes.byref(args))
         assert need > 0
         _err(lib.kf_verify_drafts(ctypes.byref(args), 0x1000, need - 1, None), "workspace too small")
