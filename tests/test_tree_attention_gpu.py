@@ -68,6 +68,34 @@ def test_lengths(ctx, new, heads, kv_heads, d):
 
 
 @DTYPES
+@pytest.mark.parametrize("heads,kv_heads,d", LAYOUTS)
+def test_wide_tables(dtype, heads, kv_heads, d):
+    """Tables that long requests would fill: row tiles are cut into pieces, most of short requests' into one."""
+    b = Trees([0, 70, 3000, 5, 640, 1], [64, 1, 17, 0, 30, 63], heads, kv_heads, d, dtype, 16, pad=3, extra_width=90)
+    b.check(b(max_new=64))
+    b.check(b())
+    assert torch.equal(b(), b(max_new=64))
+
+
+@pytest.mark.parametrize("requests,new", [(65, 8), (100, 20), (300, 3), (1000, 2)])
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (16, 2, 128), (2, 1, 256)])
+def test_more_requests_than_lanes(requests, new, heads, kv_heads, d):
+    """With and without pieces; the requests' pieces are counted by one wavefront, a run of requests a lane."""
+    rng = random.Random(requests)
+    ctx = [rng.choice([0, 3, 40, 200, 1500 if requests < 300 else 90]) for _ in range(requests)]
+    lens = [rng.randrange(0, new + 1) for _ in range(requests)]
+    b = Trees(ctx, lens, heads, kv_heads, d, torch.float16, 16, pad=2, extra_width=70)
+    out = b(max_new=max(lens))
+    at = 0
+    assert bool((out[sum(lens):] == 0).all())
+    for r, n in enumerate(lens):
+        if n and r % (1 + requests // 60) == 0:  # a sample of them against 64 bits
+            ref, bound = tree64(b.q[at:at + n], b.k[r], b.v[r], b.words[r])
+            check(out[at:at + n], ref, bound, f"request {r}")
+        at += n
+
+
+@DTYPES
 @pytest.mark.parametrize("ctx", [[0, 1, 61, 300], [64, 128, 1000, 4000]])
 def test_any_words(dtype, ctx):
     """Words that are no tree's: later tokens, none at all, bits past the new tokens."""
@@ -109,11 +137,14 @@ def test_a_chain_is_paged_attention(dtype, heads, kv_heads, d):
 
 @DTYPES
 @pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
-@pytest.mark.parametrize("heads,kv_heads,d,ctx", [(8, 2, 64, 40), (32, 2, 128, 300), (32, 2, 64, 20), (4, 2, 256, 90)])
-def test_keys_and_values_that_are_not_finite(dtype, bad, heads, kv_heads, d, ctx):
+@pytest.mark.parametrize("heads,kv_heads,d,ctx,more", [(8, 2, 64, 40, 2), (32, 2, 128, 300, 2), (32, 2, 64, 20, 2), (4, 2, 256, 90, 2),
+                                                       (2, 2, 128, 50, 2), (8, 2, 64, 900, 2), (32, 2, 128, 1400, 2),
+                                                       (4, 2, 256, 800, 2), (32, 2, 64, 30, 80)])
+def test_keys_and_values_that_are_not_finite(dtype, bad, heads, kv_heads, d, ctx, more):
     """In nodes beside a row's own branch they do not reach it; values in its branch do."""
     parents = [-1, 0, 0, 1, 2, 3, 4, 5]
-    b = Trees([ctx, ctx + 7], [8, 8], heads, kv_heads, d, dtype, 16, words=[ancestors_of(parents)] * 2)
+    b = Trees([ctx, ctx + 7], [8, 8], heads, kv_heads, d, dtype, 16, words=[ancestors_of(parents)] * 2,
+              extra_width=more)
     clean = b(max_new=8)
     b.check(clean)
     node = ctx + 3  # seen by nodes 3, 5 and 7
@@ -158,12 +189,19 @@ def test_lengths_that_do_not_fit_stay_inside():
     b.seq_lens.copy_(torch.tensor([1 << 30, -5]))
     out = b(max_new=1)
     assert bool((out[1] == 0).all())
-    b = Trees([50, 20], [40, 40], 4, 2, 64, torch.float16, 16, words=[ancestors_of(chain(40))] * 2)
-    b.seq_lens.copy_(torch.tensor([3, 0]))  # fewer keys than new tokens: the first ones have none
-    out = b()
-    assert bool((out[:37] == 0).all()) and bool(out[37:40].isfinite().all()) and bool((out[40:] == 0).all())
-    b.cu.copy_(torch.tensor([0, 1 << 30, -4]))
-    b()
+    for more in (2, 80):
+        b = Trees([50, 20], [40, 40], 4, 2, 64, torch.float16, 16, words=[ancestors_of(chain(40))] * 2, extra_width=more)
+        b.seq_lens.copy_(torch.tensor([3, 0]))  # fewer keys than new tokens: the first ones have none
+        out = b()
+        assert bool((out[:37] == 0).all()) and bool(out[37:40].isfinite().all()) and bool((out[40:] == 0).all())
+        for cu in ([0, 1 << 30, -4], [70, 3, 80], [80, 80, 80]):
+            b.cu.copy_(torch.tensor(cu))
+            b()
+            b.seq_lens.copy_(torch.tensor([1 << 30, 1 << 29]))
+            b()
+    many = Trees([0] * 60, [1] * 60, 4, 2, 64, torch.float16, 16, extra_width=80)  # offsets that go up and down
+    many.cu.copy_(torch.tensor([0 if i % 2 == 0 else 60 for i in range(61)]))
+    many()
     torch.cuda.synchronize()
 
 
