@@ -635,8 +635,9 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
 // one item and the beginning of the next, took 59 in place of 41 us for 8 requests of 256 rows over 500 .. 4000 keys, 37 (29) for 16
 // of 30 .. 186 over 100 .. 8000 (2 KV heads), both with their join; the joins 18 .. 24 (6 .. 9) and, of 24 items in 512 stretches, 72 (7).
 constexpr int kTreeLeast = 4;  // key tiles of a piece; with 2 and 8 the same to 1 us
-struct TreeItem {
-  int seq, row0, kv, first, pieces;  // first: the workgroup of its first piece
+struct __attribute__((aligned(16))) TreeItem {
+  int tok0, row0, rows, kv;  // its request's first token, its first row, the request's rows
+  int first, pieces;         // the workgroup of its first piece
 };
 struct TreeSpace {
   float* parts;   // [grid][kFlashRows (HDP + 2)]
@@ -754,7 +755,11 @@ __global__ __launch_bounds__(GROUPS* kFlashThreads, flash_waves_per_simd(HDP, tr
   const int piece = __builtin_amdgcn_readfirstlane(mine.piece), pieces = __builtin_amdgcn_readfirstlane(mine.pieces);
   const int per = __builtin_amdgcn_readfirstlane(mine.per), item = __builtin_amdgcn_readfirstlane(mine.item);
   const TreeSpace space = tree_space<HDP>(a.ws, gridDim.x);
-  if (tid == 0 && piece == 0 && item < a.items) space.list[item] = TreeItem{seq, tile * kFlashRows, kv, me, pieces};
+  if (tid == 0 && piece == 0 && item < a.items) {
+    const int tok0 = seq_offset(a.cu, seq, a.seqs, a.tokens);
+    space.list[item] =
+        TreeItem{tok0, tile * kFlashRows, (seq_offset(a.cu, seq + 1, a.seqs, a.tokens) - tok0) * a.rep, kv, me, pieces};
+  }
   flash_item<E, HDP, Keys::kTree, GROUPS>(a, sh, a.rep, a.scale_log2, seq, tile * kFlashRows, kv, piece * per, (piece + 1) * per,
                                           pieces == 1 ? nullptr : space.parts + (size_t)me * kFlashRows * (HDP + 2));
 }
@@ -763,14 +768,12 @@ __global__ __launch_bounds__(GROUPS* kFlashThreads, flash_waves_per_simd(HDP, tr
 template <class E, int HDP>
 __global__ __launch_bounds__(64 * kJoinWaves) void join_tree_kernel(AttnArgs a, int grid) {
   const TreeSpace space = tree_space<HDP>(a.ws, grid);
-  if ((int)blockIdx.x >= *space.count) return;
-  const TreeItem t = space.list[blockIdx.x];
+  const int count = *space.count;
+  const TreeItem t = space.list[blockIdx.x];  // loaded beside the count: the list has room for every workgroup
   const int pieces = __builtin_amdgcn_readfirstlane(t.pieces);
-  if (pieces == 1) return;
+  if ((int)blockIdx.x >= count || pieces == 1) return;
   const int rep = a.rep, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int tok0 = seq_offset(a.cu, t.seq, a.seqs, a.tokens);
-  const int rows = (seq_offset(a.cu, t.seq + 1, a.seqs, a.tokens) - tok0) * rep;
-  const int live = min(rows - t.row0, kFlashRows) * (HDP / 4);
+  const int live = min(t.rows - t.row0, kFlashRows) * (HDP / 4);
   constexpr int STRIDE = kFlashRows * (HDP + 2);
   const int i = (blockIdx.y * kJoinWaves + wave) * 64 + lane;
   if (i >= live) return;
@@ -813,7 +816,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_tree_kernel(AttnArgs a, 
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int row = t.row0 + r, tok = row / rep, head = t.kv * rep + (row - tok * rep);
   if (d < a.head_dim)
-    store_global((E*)a.out + (size_t)(tok0 + tok) * a.out_token + (size_t)head * a.out_head + d,
+    store_global((E*)a.out + (size_t)(t.tok0 + tok) * a.out_token + (size_t)head * a.out_head + d,
                  u32x2{Elem<E>::pack(v[0] * inv, v[1] * inv), Elem<E>::pack(v[2] * inv, v[3] * inv)});
 }
 
