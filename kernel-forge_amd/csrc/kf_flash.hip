@@ -65,10 +65,11 @@ struct FlashShared {
 };
 
 // Rows row0 .. + 127 of a sequence over its key tiles tile0 .. tiles - 1 (those that it has of them).
-// part: nullptr, or where the maximum, sum and unscaled outputs of an item that is cut go.
+// tok0, len, sk: the sequence's new tokens and keys.  part: nullptr, or where the maximum, sum and unscaled outputs of an item that is
+// cut go: rows of values, for trees as the lanes hold them.
 template <class E, int HDP, Keys KEYS_OF, int GROUPS>
 __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, GROUPS>& sh, int rep, float scale_log2, int seq,
-                                           int row0, int kv, int tile0, int tiles, float* part) {
+                                           int tok0, int len, SeqKeys sk, int row0, int kv, int tile0, int tiles, float* part) {
   using C = FlashConfig<HDP>;
   constexpr bool PAGED = KEYS_OF != Keys::kPacked, TREE = KEYS_OF == Keys::kTree;
   constexpr int ROW = C::ROW, KEYS = C::KEYS, KU = KEYS / 32, KK = KEYS / 16, TILE = C::TILE;
@@ -82,8 +83,6 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
   const int group = GROUPS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
   unsigned char* const smem = sh.smem + group * C::LDS;
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
-  const int tok0 = seq_offset(a.cu, seq, a.seqs, a.tokens);
-  const int len = max(seq_offset(a.cu, seq + 1, a.seqs, a.tokens) - tok0, 0);
   const int rows = len * rep;
 
   // This lane's row.  Rows past the end repeat the last one and are not stored.
@@ -92,7 +91,6 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
   const int tok = row / rep;
   const int head = kv * rep + (row - tok * rep);
   // Keys: positions before this lane's row's own, itself included.
-  const SeqKeys sk = seq_keys<PAGED>(a, seq, len);
   const int limit = sk.last_key(tok);  // may be negative: no keys
   TreeRow node;
   if constexpr (TREE) node.bits = a.ancestors[tok0 + tok];
@@ -353,7 +351,7 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
       for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          store_global(part + r * HDP + 32 * t + 8 * i + 4 * half,
+          store_global(TREE ? part + 4 * (256 * (4 * t + i) + 64 * wave + lane) : part + r * HDP + 32 * t + 8 * i + 4 * half,
                        float4_t{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]});
       int first_half = half;
       asm volatile("" : "+v"(first_half));  // compared here, not kept in scalar registers for the whole loop
@@ -364,7 +362,8 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
     }
     if (__builtin_expect(patch_from < kend, 0) && my_row < rows)
       for (int d = 4 * half; d < b.head_dim; d += 8)
-        *reinterpret_cast<float4_t*>(part + (my_row - row0) * HDP + d) += patch_of(d);
+        *reinterpret_cast<float4_t*>(TREE ? part + 4 * (256 * (d / 8) + 64 * wave + lane) : part + (my_row - row0) * HDP + d) +=
+            patch_of(d);
     return;
   }
   const int group_heads = b.heads / b.kv_heads, out_row = min(my_row, rows - 1), out_tok = out_row / group_heads;
@@ -480,7 +479,10 @@ __device__ __forceinline__ void flash_block(const AttnArgs& a, FlashShared<HDP, 
     if (tile * kFlashRows >= rows || rows < min_rows) return;
   }
   const int row0 = tile * kFlashRows;
-  flash_item<E, HDP, KEYS_OF, GROUPS>(a, sh, rep, scale_log2, seq, row0, kv, 0, 0x7fffffff / FlashConfig<HDP>::KEYS, nullptr);
+  const int tok0 = seq_offset(a.cu, seq, a.seqs, a.tokens);
+  const int len = max(seq_offset(a.cu, seq + 1, a.seqs, a.tokens) - tok0, 0);
+  flash_item<E, HDP, KEYS_OF, GROUPS>(a, sh, rep, scale_log2, seq, tok0, len, seq_keys<KEYS_OF != Keys::kPacked>(a, seq, len), row0,
+                                      kv, 0, 0x7fffffff / FlashConfig<HDP>::KEYS, nullptr);
 }
 
 template <class E, int HDP, Keys KEYS_OF, int GROUPS>
@@ -624,7 +626,8 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
     const bool whole = t0 == 0 && to == cost;
     float* const part = static_cast<float*>(a.ws) + (size_t)(2 * me + (t0 == 0 ? 1 : 0)) * kFlashRows * (HDP + 2);
     if (tid == 0 && t0 == 0 && !whole) static_cast<Piece*>(a.pieces)[me] = Piece{seq, row0, kv, last_stretch(item_at, cost, per)};
-    flash_item<E, HDP, KEYS_OF, 1>(a, sh, rep, a.scale_log2, seq, row0, kv, t0, t1, whole ? nullptr : part);
+    flash_item<E, HDP, KEYS_OF, 1>(a, sh, rep, a.scale_log2, seq, seq_offset(a.cu, seq, a.seqs, a.tokens), len,
+                                   seq_keys<PAGED>(a, seq, len), row0, kv, t0, t1, whole ? nullptr : part);
     lds_barrier();  // the tiles have been read: the buffers are free
   }
 }
@@ -653,16 +656,19 @@ __device__ __host__ inline TreeSpace tree_space(void* ws, int grid) {
   return s;
 }
 struct TreeWork {
-  int rows, tiles, key_tiles;  // row tiles; tiles of keys of each
+  int tok0, rows, tiles, key_tiles;  // row tiles; tiles of keys of each
+  SeqKeys sk;
 };
 template <int HDP>
 __device__ __forceinline__ TreeWork tree_work(const AttnArgs& a, int s, int rep) {
   constexpr int KEYS = FlashConfig<HDP>::KEYS;
-  const int len = max(seq_offset(a.cu, s + 1, a.seqs, a.tokens) - seq_offset(a.cu, s, a.seqs, a.tokens), 0);
   TreeWork w;
+  w.tok0 = seq_offset(a.cu, s, a.seqs, a.tokens);
+  const int len = max(seq_offset(a.cu, s + 1, a.seqs, a.tokens) - w.tok0, 0);
+  w.sk = seq_keys<true>(a, s, len);
   w.rows = len * rep;
   w.tiles = (w.rows + kFlashRows - 1) / kFlashRows;
-  w.key_tiles = max((seq_keys<true>(a, s, len).keys + KEYS - 1) / KEYS, 1);
+  w.key_tiles = max((w.sk.keys + KEYS - 1) / KEYS, 1);
   return w;
 }
 // Sums that no lengths make wrap: at kNoWork they stay (kf_stretch.h).
@@ -673,7 +679,7 @@ template <class E, int HDP, int GROUPS>
 __global__ __launch_bounds__(GROUPS* kFlashThreads, flash_waves_per_simd(HDP, true)) void tree_cut_kernel(AttnArgs args) {
   __shared__ FlashShared<HDP, GROUPS> sh;
   __shared__ struct {
-    int seq, kv, tile, piece, pieces, per, item;
+    int seq, tok0, len, keys, shift, kv, tile, piece, pieces, per, item;
   } mine;
   const int tid = threadIdx.x, lane = tid & 63;
   // Workgroups go to the 8 XCDs in turn: XCD x takes pieces x * grid / 8 and on, so that the row tiles of one KV head, which read
@@ -685,7 +691,7 @@ __global__ __launch_bounds__(GROUPS* kFlashThreads, flash_waves_per_simd(HDP, tr
     if (tid < 64) {
       // Every lane takes a run of requests: one, as a rule.
       const int run = (a.seqs + 63) / 64, s0 = min(lane * run, a.seqs), s1 = min(s0 + run, a.seqs);
-      const TreeWork none = {0, 0, 1}, first = s0 < s1 ? tree_work<HDP>(a, s0, rep) : none;
+      const TreeWork none = {0, 0, 0, 1, {0, 0}}, first = s0 < s1 ? tree_work<HDP>(a, s0, rep) : none;
       auto of_run = [&](auto&& f) {  // f(request, its work) of the lane's requests
         if (s0 < s1) f(s0, first);
         for (int s = s0 + 1; s < s1; ++s) f(s, tree_work<HDP>(a, s, rep));
@@ -729,6 +735,10 @@ __global__ __launch_bounds__(GROUPS* kFlashThreads, flash_waves_per_simd(HDP, tr
             const int pieces = (w.key_tiles + high - 1) / high;
             const int i = (me - at) / pieces;  // items in the order KV head, row tile
             mine.seq = s;
+            mine.tok0 = w.tok0;
+            mine.len = w.rows / rep;
+            mine.keys = w.sk.keys;
+            mine.shift = w.sk.shift;
             mine.kv = i / w.tiles;
             mine.tile = i - mine.kv * w.tiles;
             mine.piece = (me - at) - i * pieces;
@@ -755,16 +765,15 @@ __global__ __launch_bounds__(GROUPS* kFlashThreads, flash_waves_per_simd(HDP, tr
   const int piece = __builtin_amdgcn_readfirstlane(mine.piece), pieces = __builtin_amdgcn_readfirstlane(mine.pieces);
   const int per = __builtin_amdgcn_readfirstlane(mine.per), item = __builtin_amdgcn_readfirstlane(mine.item);
   const TreeSpace space = tree_space<HDP>(a.ws, gridDim.x);
-  if (tid == 0 && piece == 0 && item < a.items) {
-    const int tok0 = seq_offset(a.cu, seq, a.seqs, a.tokens);
-    space.list[item] =
-        TreeItem{tok0, tile * kFlashRows, (seq_offset(a.cu, seq + 1, a.seqs, a.tokens) - tok0) * a.rep, kv, me, pieces};
-  }
-  flash_item<E, HDP, Keys::kTree, GROUPS>(a, sh, a.rep, a.scale_log2, seq, tile * kFlashRows, kv, piece * per, (piece + 1) * per,
-                                          pieces == 1 ? nullptr : space.parts + (size_t)me * kFlashRows * (HDP + 2));
+  const int tok0 = __builtin_amdgcn_readfirstlane(mine.tok0), len = __builtin_amdgcn_readfirstlane(mine.len);
+  const SeqKeys sk = {__builtin_amdgcn_readfirstlane(mine.keys), __builtin_amdgcn_readfirstlane(mine.shift)};
+  if (tid == 0 && piece == 0 && item < a.items)
+    space.list[item] = TreeItem{tok0, tile * kFlashRows, len * a.rep, kv, me, pieces};
+  flash_item<E, HDP, Keys::kTree, GROUPS>(a, sh, a.rep, a.scale_log2, seq, tok0, len, sk, tile * kFlashRows, kv, piece * per,
+                                          (piece + 1) * per, pieces == 1 ? nullptr : space.parts + (size_t)me * kFlashRows * (HDP + 2));
 }
 
-// Joins the pieces of item blockIdx.x, each wavefront 64 x 4 values, in the order of the keys.
+// Joins the pieces of item blockIdx.x in the order of the keys.
 template <class E, int HDP>
 __global__ __launch_bounds__(64 * kJoinWaves) void join_tree_kernel(AttnArgs a, int grid) {
   const TreeSpace space = tree_space<HDP>(a.ws, grid);
@@ -773,12 +782,12 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_tree_kernel(AttnArgs a, 
   const int pieces = __builtin_amdgcn_readfirstlane(t.pieces);
   if ((int)blockIdx.x >= count || pieces == 1) return;
   const int rep = a.rep, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int live = min(t.rows - t.row0, kFlashRows) * (HDP / 4);
   constexpr int STRIDE = kFlashRows * (HDP + 2);
-  const int i = (blockIdx.y * kJoinWaves + wave) * 64 + lane;
-  if (i >= live) return;
-  const int r = i / (HDP / 4), d = 4 * (i % (HDP / 4));
+  // As the lanes held them: a workgroup has eight dims of every row, a wavefront 32 rows.
+  const int r = 32 * wave + (lane & 31), d = 8 * blockIdx.y + 4 * (lane >> 5);
+  if (t.row0 + r >= t.rows) return;
   const float* const from = space.parts + (size_t)t.first * STRIDE;
+  const int at = 4 * (256 * blockIdx.y + 64 * wave + lane);
   float top = -__builtin_inff(), l = 0.0f;
   float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
   // As in join_pieces_kernel: nothing of a piece without keys, a NaN among scores is in the sum.
@@ -795,7 +804,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_tree_kernel(AttnArgs a, 
       const float* const p = from + (size_t)(p0 + j) * STRIDE;
       m[j] = p[kFlashRows * HDP + r];
       s[j] = p[kFlashRows * HDP + kFlashRows + r];
-      x[j] = *reinterpret_cast<const float4_t*>(p + r * HDP + d);
+      x[j] = *reinterpret_cast<const float4_t*>(p + at);
     }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) high = fmaxf(high, m[j]);
@@ -827,7 +836,7 @@ hipError_t launch_tree(const AttnArgs& a, const FlashPlan& p, void* ws, hipStrea
   if (p.groups > 1) tree_cut_kernel<E, HDP, flash_groups(HDP)><<<p.grid, flash_groups(HDP) * kFlashThreads, 0, stream>>>(c);
   else tree_cut_kernel<E, HDP, 1><<<p.grid, kFlashThreads, 0, stream>>>(c);
   if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
-  join_tree_kernel<E, HDP><<<dim3((unsigned)p.items, kFlashRows * HDP / 4 / 64 / kJoinWaves), 64 * kJoinWaves, 0, stream>>>(c, p.grid);
+  join_tree_kernel<E, HDP><<<dim3((unsigned)p.items, HDP / 8), 64 * kJoinWaves, 0, stream>>>(c, p.grid);
   return hipGetLastError();
 }
 
@@ -845,17 +854,20 @@ hipError_t launch(const AttnArgs& a, const FlashPlan& p, int min_rows, void* ws,
           <<<p.grid, kFlashThreads, 0, stream>>>(a, rep, min_rows, p.longest_first, scale_log2);
     return hipGetLastError();
   }
-  if constexpr (KEYS_OF == Keys::kTree) return launch_tree<E, HDP>(a, p, ws, stream);
-  float* const parts = static_cast<float*>(ws);
-  Piece* const pieces = reinterpret_cast<Piece*>(parts + (size_t)2 * p.grid * kFlashRows * (HDP + 2));
-  AttnArgs c = a;
-  c.scale_log2 = scale_log2, c.rep = rep, c.min_rows = min_rows, c.ws = parts, c.pieces = pieces;
-  flash_cut_kernel<E, HDP, KEYS_OF><<<p.grid, kFlashThreads, 0, stream>>>(c);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess) return err;
-  join_pieces_kernel<E, HDP, kFlashRows>
-      <<<join_grid<HDP, kFlashRows>(p.grid), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
-  return hipGetLastError();
+  if constexpr (KEYS_OF == Keys::kTree) {
+    return launch_tree<E, HDP>(a, p, ws, stream);
+  } else {
+    float* const parts = static_cast<float*>(ws);
+    Piece* const pieces = reinterpret_cast<Piece*>(parts + (size_t)2 * p.grid * kFlashRows * (HDP + 2));
+    AttnArgs c = a;
+    c.scale_log2 = scale_log2, c.rep = rep, c.min_rows = min_rows, c.ws = parts, c.pieces = pieces;
+    flash_cut_kernel<E, HDP, KEYS_OF><<<p.grid, kFlashThreads, 0, stream>>>(c);
+    hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+    join_pieces_kernel<E, HDP, kFlashRows>
+        <<<join_grid<HDP, kFlashRows>(p.grid), 64 * kJoinWaves, 0, stream>>>(a, rep, parts, pieces);
+    return hipGetLastError();
+  }
 }
 
 template <class E, int HDP>
