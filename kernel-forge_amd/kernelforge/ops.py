@@ -1469,7 +1469,7 @@ def verify_drafts(tokens: torch.Tensor, parents: torch.Tensor, cu_new: torch.Ten
       as tokens drawn from target one by one. Without ``draft`` a node's children are taken as they are, accepted in turn with what
       is left of their parent's mass; with draft fp32 [T, vocab] they were drawn, independently of each other, from row t of it, and
       are accepted with max(p - a q, 0) / (m q). The token behind the path is drawn from what is left: the first index
-      at which the running sum passes the uniform number times the whole. Sums in 64 bits; NaN and negative probabilities count as 0.
+      at which the running sum passes the uniform number times the whole. Sums in 64 bits; NaN and negative ones count as 0.
 
     max_new: nodes of a request that are looked at, and the width of the results (64, the most, without it). Tokens outside
     the vocabulary are never accepted. Rows of target and draft may be strided. Results do not change from run to run. The form
@@ -1616,18 +1616,15 @@ def keep_drafts(caches: torch.Tensor | list[torch.Tensor], block_table: torch.Te
         if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
             raise ValueError("free_pages must be a contiguous 1-D int32 tensor")
     _check_plain("keep_drafts", (*listed, *tables, *stack))
-    for cache in listed:
-        _check_kept_cache(cache)
-    run = _keep_drafts_op if _traced((*listed, *tables, *stack)) else _launch_keep
+    listed = [_check_kept_cache(cache) for cache in listed]
+    traced = _traced((*listed, *tables, *stack))
+    if not traced and len({cache.data_ptr() for cache in listed}) < len(listed):
+        raise ValueError("caches must be different arrays")
+    run = _keep_drafts_op if traced else _launch_keep
     kept = run(listed[0], *tables, free_pages, free_count)
     for cache in listed[1:]:  # the lengths and the stack are dealt with
         run(cache, *tables, None, None)
     return KeptDrafts(kept[:b], kept[b:] if stack else None)
-
-
-def _one_stride(t: torch.Tensor) -> bool:
-    """Whether all dimensions but the last four are one of constant stride."""
-    return all(t.stride(i) == t.stride(i + 1) * t.shape[i + 1] for i in range(t.dim() - 5))
 
 
 def _kept_cache_ok(t: torch.Tensor) -> bool:
@@ -1645,7 +1642,8 @@ def _kept_cache_ok(t: torch.Tensor) -> bool:
             and 16 <= block <= 1 << 20 and not block & (block - 1) and not shape[4] & 7 and t.numel() > 0)
 
 
-def _check_kept_cache(t: torch.Tensor) -> None:
+def _check_kept_cache(t: torch.Tensor) -> torch.Tensor:
+    """t [arrays, num_pages, kv_heads, block_size, head_dim]."""
     if t.dim() < 4 or t.numel() == 0:
         raise ValueError("caches must be [..., num_pages, kv_heads, block_size, head_dim] and not empty, got "
                          f"{list(t.shape)}")
@@ -1654,9 +1652,14 @@ def _check_kept_cache(t: torch.Tensor) -> None:
     _check_block_size(t.shape[-2])
     if t.shape[-1] % 8:
         raise ValueError(f"head_dim must be a multiple of 8, got {t.shape[-1]}")
-    if not _rows_ok(t) or not _own_places(t) or not _one_stride(t):
+    try:
+        flat = t.view(-1, *t.shape[-4:])
+    except RuntimeError:
+        flat = None
+    if flat is None or not _rows_ok(t) or not _own_places(t):
         raise ValueError("caches must have a contiguous last dimension, other strides of multiples of 8, none of them 0, leading "
                          "dimensions that are one, and a 16-byte aligned start")
+    return flat
 
 
 def _launch_keep(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count):

@@ -104,6 +104,7 @@ def keep_args(caches=None):
 
 
 H = dict(dtype=torch.float16)
+CACHE = torch.zeros(4, 5, 2, 16, 64, **H)
 
 
 @pytest.mark.parametrize("change,error,match", [
@@ -115,6 +116,7 @@ H = dict(dtype=torch.float16)
     (dict(caches=torch.zeros(4, 1, 2, 16, 64, **H).expand(4, 5, 2, 16, 64)), ValueError, "none of them 0"),
     (dict(caches=torch.zeros(3, 4, 5, 2, 16, 64, **H)[:, :2]), ValueError, "leading dimensions"),
     (dict(caches=[torch.zeros(5, 2, 16, 64, **H), torch.zeros(5, 2, 16, 64)]), TypeError, "fp16 or bf16"),
+    (dict(caches=[CACHE, CACHE]), ValueError, "different arrays"), (dict(caches=[CACHE, CACHE[0]]), ValueError, "different arrays"),
     (dict(block_table=zeros(2, 3, dtype=torch.int64)), ValueError, "block_table"), (dict(block_table=zeros(0, 3)), ValueError, "at least one"),
     (dict(context_lens=zeros(3)), ValueError, "context_lens"), (dict(seq_lens=zeros(2, dtype=torch.int64)), ValueError, "seq_lens"),
     (dict(counts=zeros(1)), ValueError, "counts"), (dict(path=zeros(2, 65)), ValueError, "path"), (dict(path=zeros(2, 0)), ValueError, "path"),

@@ -112,6 +112,14 @@ def test_layouts():
     assert torch.equal(torch.stack(parts).cpu(), want[0]) and got.context_lens.tolist() == want[2] and got.free_count is None
 
 
+def test_leading_dimensions_of_one():
+    """Their strides say nothing."""
+    step = Step([30, 5], [40, 64], arrays=6)
+    whole = torch.zeros(6, 2, 1, *step.caches.shape[1:], dtype=torch.float16, device=DEV)
+    step.check(whole[:, :1].copy_(step.caches[:, None, None]))
+    step.check(whole[:, 1].copy_(step.caches[:, None]))
+
+
 def test_counts_that_do_not_fit():
     step = Step([30, 5, 9], [4, 64, 2], width=4)
     step.counts = [1 << 30, 3, -2]
