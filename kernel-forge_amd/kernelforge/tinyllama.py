@@ -146,7 +146,7 @@ class Attention(nn.Module):
             return y[..., :nqk], y[..., nqk:]
         return torch.cat([self.q_proj(x), self.k_proj(x)], dim=-1), self.v_proj(x)
 
-    def paged(self, x, step, rope, cache_k, cache_v, block_table, max_new, whole_prompts, trees=None, norm=None):
+    def paged(self, x, step, rope, cache_k, cache_v, block_table, max_new, whole_prompts, norm=None, trees=None):
         """Attention of several requests' new tokens, x [1, T, H] packed (normalized unless `norm` is given), over
         a paged cache: [1, T, heads d], before o_proj.  whole_prompts: no request with new tokens has any in the
         cache yet.  trees (ops.draft_trees): the new tokens are the nodes of trees."""
@@ -295,14 +295,14 @@ class DecoderLayer(nn.Module):
         return x + m(self.post_attention_layernorm(x))
 
 
-    def paged(self, x, *args):
+    def paged(self, x, *args, trees=None):
         """The layer on several requests' packed new tokens (Attention.paged's arguments after x)."""
         a, m = self.self_attn, self.mlp
         if self.int4_fusable():
-            x = _int4_fused(a.o_proj, a.paged(x, *args, norm=self.input_layernorm), residual=x)
+            x = _int4_fused(a.o_proj, a.paged(x, *args, norm=self.input_layernorm, trees=trees), residual=x)
             g, u = m.project(x, self.post_attention_layernorm)
             return _int4_fused(m.down_proj, g, up=u, residual=x)
-        x = x + a.o_proj(a.paged(self.input_layernorm(x), *args))
+        x = x + a.o_proj(a.paged(self.input_layernorm(x), *args, trees=trees))
         return x + m(self.post_attention_layernorm(x))
 
 
@@ -348,7 +348,7 @@ class TinyLlama(nn.Module):
         new tokens are the nodes of a tree per request, and the logits after each of them are returned, [T, vocab]."""
         x = self.embed_tokens(tokens).unsqueeze(0)
         for i, layer in enumerate(self.layers):
-            x = layer.paged(x, step, rope, cache[i, 0], cache[i, 1], block_table, max_new, whole_prompts, trees)
+            x = layer.paged(x, step, rope, cache[i, 0], cache[i, 1], block_table, max_new, whole_prompts, trees=trees)
         if trees is not None:
             return self.lm_head(self.norm(x[0]))
         last = (step.cu_new[1:].long() - 1).clamp(0, tokens.numel() - 1)
@@ -508,8 +508,9 @@ class PagedDecoder:
 
     Every request has a row.  ``admit`` gives prompts to free rows (whole, or in chunks between which nothing else runs),
     ``decode`` appends one token per step to every row that holds a request, ``decode_drafts`` as many drafted ones as the
-    model agrees with and one more, ``finish`` frees a row and returns its pages.  Lengths, tables and the stack of free pages are on the device, where the step advances them; the host
-    keeps its own count of lengths and pages and refuses (ValueError) what would pass max_seq or the pages there are.
+    model agrees with and one more, ``finish`` frees a row and returns its pages.  Lengths, tables and the stack of free
+    pages are on the device, where the step advances them; the host keeps its own count of lengths and pages and refuses
+    (ValueError) what would pass max_seq or the pages there are.
     """
 
     def __init__(self, model: TinyLlama, device, requests: int, num_pages: int, block_size: int = 16):
@@ -692,7 +693,8 @@ class PagedDecoder:
             if probs is not None:
                 if probs.shape != (n, vocab) or probs.dtype != torch.float32 or probs.device != dev:
                     raise ValueError(f"decode_drafts: the probabilities of row {row} must be float32 [{n}, {vocab}] on {dev}")
-                drawn.append((at, above, probs))
+                if n:
+                    drawn.append((at, above, probs))
             new[row] = n + 1
             tokens += [self.tokens[row:row + 1], draft.long()]
             parents += [above.new_full((1,), -1), above + 1]
@@ -722,7 +724,8 @@ class PagedDecoder:
         parents[i] the number of the drafted token that token i follows, smaller than i (-1: the row's last token), up to 63 tokens.
         Rows without drafts get one token.  Greedy at temperature 0, and then as ``decode`` to within roundings.  Otherwise
         tokens are distributed as if drawn one by one at that temperature, with random numbers from `generator`; drafts that
-        were drawn from probabilities come with them, (tokens, parents, float32 [n, vocab]), and all drafts of the step do.
+        were drawn from probabilities come with them, (tokens, parents, float32 [n, vocab]; the same for tokens with one parent),
+        and all drafts of the step do.
         Eager: the host waits for the counts."""
         if not 0.0 <= temperature < float("inf"):
             raise ValueError(f"decode_drafts: the temperature must be 0 or positive, got {temperature}")
@@ -750,7 +753,9 @@ class PagedDecoder:
         if temperature == 0.0:
             done = ops.verify_drafts(tokens, parents, step.cu_new, logits, max_new=max(new))
         else:
-            target = torch.softmax(logits.float() / temperature, dim=-1)
+            # Above the largest score first, and by no less than this: no quotient passes the type's range.
+            logits = logits.float()
+            target = torch.softmax((logits - logits.amax(-1, keepdim=True)) / max(temperature, 1e-30), dim=-1)
             accept = torch.rand(tokens.numel(), generator=generator, device=self.device)
             sample = torch.rand(len(new), generator=generator, device=self.device)
             draft = None

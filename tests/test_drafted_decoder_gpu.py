@@ -145,6 +145,20 @@ def test_sampled(model):
     choices_are_good(cold, 0, ps[0])
 
 
+def test_lowest_temperatures_and_drafts_of_no_tokens(model):
+    """At temperatures whose quotients no float holds the choices are the greedy ones'; a draft with probabilities may be empty."""
+    ps = prompts(30, 50)
+    dec = tl.PagedDecoder(model, DEV, requests=2, num_pages=30)
+    dec.admit(dict(enumerate(ps)))
+    none, q = dec.tokens[:0], torch.full((1, 2000), 1 / 2000, device=DEV)
+    for temperature in (1e-45, 1e-300, 1e-38):
+        assert dec.decode_drafts({0: (none, none, q[:0])}, temperature=temperature) == [1, 1]
+        dec.decode_drafts({0: (none, none, q[:0]), 1: (dec.tokens[:1], None, q)}, temperature=temperature)
+    no_page_is_lost(dec)
+    for row, p in enumerate(ps):
+        choices_are_good(dec, row, p)
+
+
 def test_a_step_that_fails(model, monkeypatch):
     """The rows are as before it, and go on."""
     p, = prompts(47)
