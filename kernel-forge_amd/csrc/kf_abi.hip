@@ -177,10 +177,10 @@ constexpr int kMaxTokenStride = 1 << 26;  // elements: 16 keys' byte offsets fit
 // 78 / 55; 4 of 64 and 64 rows 27 / 33, 96 rows 33 / 39, 128 rows 34 / 41.
 constexpr int kFewRows = 64;
 
-// The same for trees, whose row tiles the other kernel cuts into pieces (tree_plan) without a stretch's search.  Few rows / many rows,
-// us: 8 requests over 1000 .. 4000 keys (8 KV heads of 128) and 32 rows 34 / 28, 64 rows 45 / 30, 8 of 64 dims and 32 rows 17 / 16, 64 of
-// 32 rows over 100 .. 3000 82 / 69; but 16 rows 57 / 72, 32 of 8 rows over 100 .. 4000 34 / 40, 128 of 12 over 4000 (2 KV heads)
-// 36 / 41.
+// The same for trees, whose row tiles the other kernel cuts into pieces (tree_plan) without a stretch's search.  Few rows /
+// many rows, us: 8 requests over 1000 .. 4000 keys (8 KV heads of 128) and 32 rows 34 / 28, 64 rows 45 / 30, 8 of 64 dims and
+// 32 rows 17 / 16, 64 of 32 rows over 100 .. 3000 82 / 69; but 16 rows 57 / 72, 32 of 8 rows over 100 .. 4000 34 / 40, 128 of
+// 12 over 4000 (2 KV heads) 36 / 41.
 constexpr int kTreeFewRows = 16;
 
 int check_block(int block_size, int* log2_block) {

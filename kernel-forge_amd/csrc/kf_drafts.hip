@@ -39,7 +39,8 @@ __device__ __forceinline__ T of_lane(T v, int lane) {
 }
 
 // ---- tables ---------------------------------------------------------------------------------------------
-// A wavefront per request.  Bound by latency: the offsets, then the parents, then six rounds of lane exchange.
+// A wavefront per request.  Bound by latency: the offsets, then the parents, then six rounds of lane exchange: 1.6 us for one
+// tree of 16 nodes, 2.7 for 500 of up to 64.
 constexpr int kTreeWaves = 4;
 
 __global__ __launch_bounds__(64 * kTreeWaves) void draft_trees_kernel(DraftTreesArgs a) {
@@ -135,8 +136,9 @@ __device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
 
 constexpr int kBestThreads = 256, kBestAhead = 4, kBestStep = 8 * kBestThreads;
 
-// keys[row * shares + share] = the largest of the share's part of the row.  Bound by memory: a thread keeps the largest value and the
-// eight that it is among, which it reads again at the end, so that a value costs two vector instructions in place of five.
+// keys[row * shares + share] = the largest of the share's part of the row.  Bound by memory: a thread keeps the largest value
+// and the eight that it is among, which it reads again at the end, so that a value costs two vector instructions in place of
+// five.  464 rows of 100003 bf16 values, 93 MB, take 19.0 us, 4.9 TB/s (with a key for every value 30); 16 of 32000 3.8.
 template <class T>
 __global__ __launch_bounds__(kBestThreads) void best_token_kernel(VerifyArgs a, int shares, int part) {
   __shared__ uint64_t keys[kBestThreads / 64];
@@ -197,6 +199,8 @@ __global__ __launch_bounds__(kBestThreads) void best_token_kernel(VerifyArgs a, 
   }
 }
 
+// A wavefront per request.  Latency, 2.3 us for one, 3.9 for 16: the tree, a node's keys, a round of exchange for every node of the
+// path.
 __global__ __launch_bounds__(64 * kTreeWaves) void verify_best_kernel(VerifyArgs a, int shares) {
   const int lane = threadIdx.x & 63;
   const int r = blockIdx.x * kTreeWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -403,7 +407,8 @@ struct Rest {
     const int rest = begin + 4 * groups;
     if (rest + lane < end) {
       double f[4];
-      four<64>(row4_t{p[rest + lane], 0.0f, 0.0f, 0.0f}, row4_t{DRAWN ? q[rest + lane] : 0.0f, 0.0f, 0.0f, 0.0f}, rest + lane, rest, f);
+      four<64>(row4_t{p[rest + lane], 0.0f, 0.0f, 0.0f}, row4_t{DRAWN ? q[rest + lane] : 0.0f, 0.0f, 0.0f, 0.0f},
+               rest + lane, rest, f);
       sum += f[0];
     }
     return wave_sum(sum);
@@ -416,7 +421,8 @@ __device__ __forceinline__ Rest<DRAWN> rest_of(const VerifyArgs& a, const WalkSh
                      DRAWN ? 0 : (int)__popcll(w.under), a.vocab, w.taken};
 }
 
-// Workgroup (piece, request): the sum over the piece.
+// Workgroup (piece, request): the sum over the piece.  16 rows of 150001 values of p and of q, 19 MB, take 6.7 us, the walk before
+// them included.
 template <bool DRAWN>
 __global__ __launch_bounds__(kSumThreads) void verify_sum_kernel(VerifyArgs a, int pieces) {
   __shared__ double parts[kSumThreads / 64];
@@ -468,7 +474,8 @@ struct Ends {
 };
 __device__ __forceinline__ Ends ends_of(int low, int high, PickShared& sh, int lane, int wave) {
   const uint64_t lows = __ballot(low != 0x7fffffff), highs = __ballot(high >= 0);
-  const int l = lows ? of_lane(low, __builtin_ctzll(lows)) : 0x7fffffff, h = highs ? of_lane(high, 63 - __clzll((long long)highs)) : -1;
+  const int l = lows ? of_lane(low, __builtin_ctzll(lows)) : 0x7fffffff;
+  const int h = highs ? of_lane(high, 63 - __clzll((long long)highs)) : -1;
   __syncthreads();
   if (lane == 0) {
     sh.low[wave] = l;
@@ -509,7 +516,11 @@ __device__ __forceinline__ double row_total(PickShared& sh, const Rest<DRAWN>& r
   return all;
 }
 
-// One workgroup per request.  pieces: of the rows, whose sums the launch before has left in a.ws; 0: there was none.
+// One workgroup per request.  pieces: of the rows, whose sums the launch before has left in a.ws; 0: there was none.  64 requests
+// over 32000 values, tokens given, 12.2 us (with an LDS atomic for every value that may be the place 60).  Drawn, bound by what one
+// CU reads: every rejected child behind a node's first costs a sum over the row, 1.2 MB of 150001 values in 12 us; 25 to 38 for
+// trees with up to three of them.  (Such sums by a further launch of all CUs made those calls 30 % shorter, and ones without
+// such children 25 % longer.)
 template <bool DRAWN>
 __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a, int pieces) {
   __shared__ PickShared sh;
@@ -583,7 +594,8 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a,
   if (wave == 0) write_path(a, r, w.on, walked.token[lane], lane);
   const double mark = (double)sample_u * all;
 
-  // The part of [begin, end) with whose end the sum passes the mark; if none does (a number that is not below 1), the last with any.
+  // The part of [begin, end) with whose end the sum passes the mark; if none does (a number that is not below 1), the last
+  // with any.
   double before = 0.0;
   int begin = 0, end = a.vocab;
   if (summed) {
@@ -645,7 +657,8 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a,
 // Node path[i] of the tree goes to place context + i, in all arrays of the cache.  Nodes have larger numbers than their
 // ancestors, so path[i] >= i, and a place is read before it is written if every thread takes the moves of its 16 bytes in
 // order.  Bound by latency: the offsets of the moves by way of the table, then a read and a write.  Workgroup (r, y): share y of
-// the arrays of request r; r = seqs: the lengths, and the pages behind them back onto the stack.
+// the arrays of request r; r = seqs: the lengths, and the pages behind them back onto the stack.  3.3 us for one request in 44
+// arrays, 3.7 for 64 in 56 (3 MB).
 constexpr int kKeepThreads = 256, kKeepAhead = 4;
 
 __device__ __forceinline__ int kept_tokens(const KeepArgs& a, int r) {
@@ -738,9 +751,9 @@ __global__ __launch_bounds__(kKeepThreads) void keep_drafts_kernel(KeepArgs a) {
   }
 }
 
-// Rows up to which one workgroup adds them up.  One launch / two, us: tokens given, 16 requests of 32000 values 11.5 / 13.1, of 40000
-// 13.4 / 13.0, of 50000 14.4 / 13.0, of 65000 15.8 / 13.1; drawn, 16 of 32000 16.5 / 17.7, of 40000 16.1 / 16.0, of 65000 25.2 / 23.8.  A
-// launch takes some 3 us of the host's time besides.
+// Rows up to which one workgroup adds them up.  One launch / two, us: tokens given, 16 requests of 32000 values 11.5 / 13.1,
+// of 40000 13.4 / 13.0, of 50000 14.4 / 13.0, of 65000 15.8 / 13.1; drawn, 16 of 32000 16.5 / 17.7, of 40000 16.1 / 16.0, of
+// 65000 25.2 / 23.8.  A launch takes some 3 us of the host's time besides.
 constexpr int kSumFrom = 40960;
 
 // Workgroups per row of scores, where there are fewer rows than fill the card, of at least four rounds of loads.

@@ -65,8 +65,8 @@ struct FlashShared {
 };
 
 // Rows row0 .. + 127 of a sequence over its key tiles tile0 .. tiles - 1 (those that it has of them).
-// tok0, len, sk: the sequence's new tokens and keys.  part: nullptr, or where the maximum, sum and unscaled outputs of an item that is
-// cut go: rows of values, for trees as the lanes hold them.
+// tok0, len, sk: the sequence's new tokens and keys.  part: nullptr, or where the maximum, sum and unscaled outputs of an
+// item that is cut go: rows of values, for trees as the lanes hold them.
 template <class E, int HDP, Keys KEYS_OF, int GROUPS>
 __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, GROUPS>& sh, int rep, float scale_log2, int seq,
                                            int tok0, int len, SeqKeys sk, int row0, int kv, int tile0, int tiles, float* part) {
@@ -633,10 +633,15 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
 }
 
 // Trees of new tokens, whose row tiles all see the same keys: each (request, KV head, row tile) is cut into pieces of at most `per`
-// key tiles, one a workgroup, with the smallest per for which there are workgroups enough.  So a workgroup begins once only, which
-// takes as long as four or five tiles of 64 keys, and all pieces end together.  Equal stretches as above, which can hold the end of
-// one item and the beginning of the next, took 59 in place of 41 us for 8 requests of 256 rows over 500 .. 4000 keys, 37 (29) for 16
-// of 30 .. 186 over 100 .. 8000 (2 KV heads), both with their join; the joins 18 .. 24 (6 .. 9) and, of 24 items in 512 stretches, 72 (7).
+// key tiles, one a workgroup, with the smallest per for which there are workgroups enough.  So a workgroup begins once
+// only, which takes as long as four or five tiles of 64 keys, and all pieces end together.  Equal stretches as above, which
+// can hold the end of one item and the beginning of the next, took 59 in place of 41 us for 8 requests of 256 rows over 500
+// .. 4000 keys, 37 (29) for 16 of 30 .. 186 over 100 .. 8000 (2 KV heads), both with their join; the joins 18 .. 24 (6 .. 9)
+// and, of 24 items in 512 stretches, 72 (7).
+//   What bounds it: long requests the bytes of K and V (two of 108 rows over up to 131071 keys, 8 KV heads of 128: 179 us,
+// 5.8 TB/s, and 7 the join); others latency: 16 of 30 .. 186 rows over 100 .. 8000 keys, 24 MB, take 19.2 us, of which 2.0
+// finding the piece, 2.0 until the queries and pages are there, 1.6 until the first tiles are, 2.3 two tiles of 64 keys, 3.3
+// joining the groups and writing the piece; the join 5.4.
 constexpr int kTreeLeast = 4;  // key tiles of a piece; with 2 and 8 the same to 1 us
 struct __attribute__((aligned(16))) TreeItem {
   int tok0, row0, rows, kv;  // its request's first token, its first row, the request's rows
@@ -770,7 +775,8 @@ __global__ __launch_bounds__(GROUPS* kFlashThreads, flash_waves_per_simd(HDP, tr
   if (tid == 0 && piece == 0 && item < a.items)
     space.list[item] = TreeItem{tok0, tile * kFlashRows, len * a.rep, kv, me, pieces};
   flash_item<E, HDP, Keys::kTree, GROUPS>(a, sh, a.rep, a.scale_log2, seq, tok0, len, sk, tile * kFlashRows, kv, piece * per,
-                                          (piece + 1) * per, pieces == 1 ? nullptr : space.parts + (size_t)me * kFlashRows * (HDP + 2));
+                                          (piece + 1) * per,
+                                          pieces == 1 ? nullptr : space.parts + (size_t)me * kFlashRows * (HDP + 2));
 }
 
 // Joins the pieces of item blockIdx.x in the order of the keys.
@@ -937,7 +943,8 @@ FlashPlan tree_plan(const AttnArgs& a, int cu_count) {
   const int64_t items = (a.tokens * rep / kFlashRows + a.seqs + 1) * a.kv_heads;
   const int hdp = a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256;
   const int held = flash_waves_per_simd(hdp, true);  // workgroups of one group that a CU holds
-  p.cut = keys > 768 && items <= (int64_t)held * cu_count;
+  const int64_t most_work = items * (keys / (hdp == 256 ? 32 : 64) + 1);
+  p.cut = keys > 768 && items <= (int64_t)held * cu_count && most_work < kNoWork;
   if (!p.cut) {
     p.grid = (int)items;
     return p;
@@ -954,7 +961,8 @@ FlashPlan tree_plan(const AttnArgs& a, int cu_count) {
 size_t flash_workspace_bytes(int head_dim, const FlashPlan& p) {
   if (!p.cut) return 0;
   const int padded = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
-  if (p.items) return (size_t)p.grid * sizeof(float) * kFlashRows * (padded + 2) + 4 * sizeof(int) + (size_t)p.items * sizeof(TreeItem);
+  if (p.items)
+    return (size_t)p.grid * sizeof(float) * kFlashRows * (padded + 2) + 4 * sizeof(int) + (size_t)p.items * sizeof(TreeItem);
   return (size_t)p.grid * (2 * sizeof(float) * kFlashRows * (padded + 2) + sizeof(Piece));
 }
 
