@@ -138,7 +138,7 @@ constexpr int kBestThreads = 256, kBestAhead = 4, kBestStep = 8 * kBestThreads;
 
 // keys[row * shares + share] = the largest of the share's part of the row.  Bound by memory: a thread keeps the largest value
 // and the eight that it is among, which it reads again at the end, so that a value costs two vector instructions in place of
-// five.  464 rows of 100003 bf16 values, 93 MB, take 19.0 us, 4.9 TB/s (with a key for every value 30); 16 of 32000 3.8.
+// five.  464 rows of 100003 bf16 values, 93 MB, take 17.7 us, 5.2 TB/s (with a key for every value 30); 16 of 32000 3.8.
 template <class T>
 __global__ __launch_bounds__(kBestThreads) void best_token_kernel(VerifyArgs a, int shares, int part) {
   __shared__ uint64_t keys[kBestThreads / 64];
@@ -756,10 +756,12 @@ __global__ __launch_bounds__(kKeepThreads) void keep_drafts_kernel(KeepArgs a) {
 // 65000 25.2 / 23.8.  A launch takes some 3 us of the host's time besides.
 constexpr int kSumFrom = 40960;
 
-// Workgroups per row of scores, where there are fewer rows than fill the card, of at least four rounds of loads.
+// Workgroups per row of scores, where there are fewer rows than fill the card, of at least four rounds of loads.  In all up to 512 /
+// 768 / 1024, us of both launches over rows of 100003 bf16 values: 100 rows 7.6 / 7.9 / 8.1, 150 9.7 / 8.9 / 9.2, 464 19.7 / 19.6 /
+// 21.0, 512 21.1 / 21.3 / 22.9; 300 rows of 32000 fp16 ones 8.6 / 7.3 / 7.5.
 int row_shares(const VerifyArgs& a) {
   const int64_t most = ((int64_t)a.vocab + 4 * kBestStep - 1) / (4 * kBestStep);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(most, 1024 / std::max(a.tokens_count, 1)));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(most, 768 / std::max(a.tokens_count, 1)));
 }
 
 template <class T>
