@@ -230,6 +230,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) void verify_best_kernel(VerifyArgs
 // is in.  Long rows are first added up by a launch of their own, in pieces of 4096 values: which row it is, is known from the first
 // test of every node's first child, unless a later child is accepted.
 constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64, kPiece = 4 * kPickThreads;
+constexpr int kSubs = 4;  // pieces of a 16th whose sums are kept: rows of up to 2^18 values are searched at once
 constexpr int kSumThreads = 256;
 
 // Nothing for negative values and NaN.
@@ -369,41 +370,43 @@ struct Rest {
     return v;
   }
   // The sum over [begin, end) by one wavefront, the same in all lanes: in groups of four values, of which the next come while
-  // the present ones are added up, then up to three values alone.
-  struct Batch {
-    static constexpr int N = DRAWN ? 4 : 8;
-    row4_t x[N], y[N];
-  };
-  __device__ __forceinline__ Batch load_batch(int begin, int group, int groups) const {
-    Batch b;
-#pragma unroll
-    for (int j = 0; j < Batch::N; ++j) {
-      const int i = begin + 4 * (group + 64 * j < groups ? group + 64 * j : 0);  // past the last one: the first, for nothing
-      b.x[j] = *(const row4_t*)(p + i);
-      if (DRAWN) b.y[j] = *(const row4_t*)(q + i);
-    }
-    return b;
-  }
-  __device__ __forceinline__ double wave_total(int begin, int end, int lane) const {
-    double sum = 0.0;
+  // the present ones are added up, then up to three values alone.  KEEP: subs has those of each 4096 values, the first kSubs.
+  template <bool KEEP>
+  __device__ __forceinline__ double wave_total(int begin, int end, int lane, double* subs) const {
+    constexpr int AHEAD = 4;
+    static_assert(kPiece % (4 * 64 * AHEAD) == 0, "a piece ends with a round of loads");
+    double all = 0.0, sum = 0.0;
     const int groups = max(end - begin, 0) / 4;
+    auto next_piece = [&](int at) {  // of the values from `begin` on
+      if (!KEEP || at == 0 || at % kPiece != 0) return;
+      const double one = wave_sum(sum);
+      if (lane == 0 && at <= kSubs * kPiece) subs[at / kPiece - 1] = one;
+      all += one;
+      sum = 0.0;
+    };
     if (groups > 0) {
-      Batch now = load_batch(begin, lane, groups), next;
-      for (int g0 = 0; g0 < groups; g0 += 64 * Batch::N) {
-        if (g0 + 64 * Batch::N < groups) next = load_batch(begin, g0 + 64 * Batch::N + lane, groups);
+      row4_t x[AHEAD], y[AHEAD];
+      auto load_group = [&](int j, int g) {
+        const int i = begin + 4 * (g < groups ? g : 0);  // past the last one: the first, for nothing
+        x[j] = *(const row4_t*)(p + i);
+        if (DRAWN) y[j] = *(const row4_t*)(q + i);
+      };
 #pragma unroll
-        for (int j = 0; j < Batch::N; ++j) {
+      for (int j = 0; j < AHEAD; ++j) load_group(j, 64 * j + lane);
+      for (int g0 = 0; g0 < groups; g0 += 64 * AHEAD) {
+        next_piece(4 * g0);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
           const int g = g0 + 64 * j + lane;
-          if (g0 + 64 * j < groups) {
-            double f[4];
-            four<64>(now.x[j], now.y[j], begin + 4 * g, begin + 4 * (g0 + 64 * j), f);
-            const double four_of = (f[0] + f[1]) + (f[2] + f[3]);
-            sum += g < groups ? four_of : 0.0;
-          }
+          double f[4];
+          four<64>(x[j], y[j], begin + 4 * g, begin + 4 * (g0 + 64 * j), f);
+          const double four_of = (f[0] + f[1]) + (f[2] + f[3]);
+          sum += g < groups ? four_of : 0.0;
+          load_group(j, g + 64 * AHEAD);
         }
-        now = next;
       }
     }
+    next_piece(4 * groups);
     const int rest = begin + 4 * groups;
     if (rest + lane < end) {
       double f[4];
@@ -411,7 +414,10 @@ struct Rest {
                rest + lane, rest, f);
       sum += f[0];
     }
-    return wave_sum(sum);
+    const double one = wave_sum(sum);
+    if (KEEP && lane == 0)
+      for (int i = 4 * groups / kPiece, first = i; i < kSubs; ++i) subs[i] = i == first ? one : 0.0;
+    return all + one;
   }
 };
 template <bool DRAWN>
@@ -421,7 +427,7 @@ __device__ __forceinline__ Rest<DRAWN> rest_of(const VerifyArgs& a, const WalkSh
                      DRAWN ? 0 : (int)__popcll(w.under), a.vocab, w.taken};
 }
 
-// Workgroup (piece, request): the sum over the piece.  16 rows of 150001 values of p and of q, 19 MB, take 6.7 us, the walk before
+// Workgroup (piece, request): the sum over the piece.  16 rows of 150001 values of p and of q, 19 MB, take 6.3 us, the walk before
 // them included.
 template <bool DRAWN>
 __global__ __launch_bounds__(kSumThreads) void verify_sum_kernel(VerifyArgs a, int pieces) {
@@ -436,7 +442,7 @@ __global__ __launch_bounds__(kSumThreads) void verify_sum_kernel(VerifyArgs a, i
   const Rest<DRAWN> rest = rest_of<DRAWN>(a, walked, w);
   constexpr int MINE = kPiece / (kSumThreads / 64);
   const int begin = piece * kPiece + wave * MINE;
-  const double sum = rest.wave_total(begin, min(begin + MINE, a.vocab), lane);
+  const double sum = rest.template wave_total<false>(begin, min(begin + MINE, a.vocab), lane, nullptr);
   if (lane == 0) parts[wave] = sum;
   __syncthreads();
   if (threadIdx.x == 0)
@@ -445,7 +451,7 @@ __global__ __launch_bounds__(kSumThreads) void verify_sum_kernel(VerifyArgs a, i
 
 struct PickShared {
   WalkShared walked;
-  double parts[kPickWaves], scan[kPickWaves];
+  double parts[kPickWaves], subs[kPickWaves][kSubs], scan[kPickWaves];
   double before;
   int low[kPickWaves], high[kPickWaves];
 };
@@ -501,12 +507,14 @@ __device__ __forceinline__ Ends lowest_of(int low, int high, PickShared& sh, int
   return ends_of(lane == 0 ? low : 0x7fffffff, lane == 0 ? high : -1, sh, lane, wave);
 }
 
-// The sum over the row, a 16th of it by each wavefront; those stay in sh.parts.
+// The sum over the row, a 16th of it by each wavefront; those stay in sh.parts, and (DRAWN: others add up short rows only) their
+// pieces' in sh.subs.
 template <bool DRAWN>
 __device__ __forceinline__ double row_total(PickShared& sh, const Rest<DRAWN>& rest, int begin, int end, int lane, int wave) {
   const int part = ((end - begin + kPickWaves - 1) / kPickWaves + 3) & ~3;
   const int64_t at = begin + (int64_t)part * wave;
-  const double mine = rest.wave_total((int)min(at, (int64_t)end), (int)min(at + part, (int64_t)end), lane);
+  const double mine =
+      rest.template wave_total<DRAWN>((int)min(at, (int64_t)end), (int)min(at + part, (int64_t)end), lane, sh.subs[wave]);
   __syncthreads();
   if (lane == 0) sh.parts[wave] = mine;
   __syncthreads();
@@ -517,10 +525,10 @@ __device__ __forceinline__ double row_total(PickShared& sh, const Rest<DRAWN>& r
 }
 
 // One workgroup per request.  pieces: of the rows, whose sums the launch before has left in a.ws; 0: there was none.  64 requests
-// over 32000 values, tokens given, 12.2 us (with an LDS atomic for every value that may be the place 60).  Drawn, bound by what one
-// CU reads: every rejected child behind a node's first costs a sum over the row, 1.2 MB of 150001 values in 12 us; 25 to 38 for
-// trees with up to three of them.  (Such sums by a further launch of all CUs made those calls 30 % shorter, and ones without
-// such children 25 % longer.)
+// over 32000 values, tokens given, 12.1 us (with an LDS atomic for every value that may be the place 60).  Drawn, bound by what one
+// CU reads: every rejected child behind a node's first costs a sum over the row, 1.2 MB of 150001 values in 11 us (10.5 with 32-bit
+// products); 6 us without such children, 22 to 33 with one to three.  (Such sums by a further launch of all CUs: both launches
+// 30 in place of 37 us, but 15.5 in place of 12.5 without such children, and 3 more of the host's time.)
 template <bool DRAWN>
 __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a, int pieces) {
   __shared__ PickShared sh;
@@ -618,20 +626,28 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a,
     begin = piece * kPiece;
     end = min(begin + kPiece, a.vocab);
   }
-  while (end - begin > kPiece) {
-    if (begin != 0 || end != a.vocab) row_total(sh, rest, begin, end, lane, wave);  // the whole row's parts are there
-    const int part = ((end - begin + kPickWaves - 1) / kPickWaves + 3) & ~3;
+  // The one of some sums.
+  auto find = [&](const double* parts, int count) {
     int at = -1, some = 0;
-    double upto = before, found = before;
-    for (int v = 0; v < kPickWaves; ++v) {
-      const double sum = sh.parts[v];
+    double upto = before, found = 0.0;
+    for (int v = 0; v < count; ++v) {
+      const double sum = parts[v];
       if (sum > 0.0) some = v;
       if (at < 0 && sum > 0.0 && upto + sum > mark) at = v, found = upto;
       upto += sum;
     }
-    before = at >= 0 ? found : 0.0;
-    begin = min(begin + (at >= 0 ? at : some) * part, end);
+    before = found;
+    return at >= 0 ? at : some;
+  };
+  while (end - begin > kPiece) {
+    if (begin != 0 || end != a.vocab) row_total(sh, rest, begin, end, lane, wave);  // the whole row's parts are there
+    const int part = ((end - begin + kPickWaves - 1) / kPickWaves + 3) & ~3, at = find(sh.parts, kPickWaves);
+    begin = min(begin + at * part, end);
     end = min(begin + part, end);
+    if (DRAWN && part > kPiece && part <= kSubs * kPiece) {
+      begin = min(begin + find(sh.subs[at], kSubs) * kPiece, end);
+      end = min(begin + kPiece, end);
+    }
     __syncthreads();  // the parts have been read
   }
   const int i = begin + 4 * tid;
@@ -751,9 +767,9 @@ __global__ __launch_bounds__(kKeepThreads) void keep_drafts_kernel(KeepArgs a) {
   }
 }
 
-// Rows up to which one workgroup adds them up.  One launch / two, us: tokens given, 16 requests of 32000 values 11.5 / 13.1,
-// of 40000 13.4 / 13.0, of 50000 14.4 / 13.0, of 65000 15.8 / 13.1; drawn, 16 of 32000 16.5 / 17.7, of 40000 16.1 / 16.0, of
-// 65000 25.2 / 23.8.  A launch takes some 3 us of the host's time besides.
+// Rows up to which one workgroup adds them up.  One launch / two, us: tokens given, 16 requests of 32000 values 11.5 / 12.8,
+// of 40000 13.2 / 12.8, of 50000 15.2 / 12.8, of 65000 15.1 / 12.8; drawn, 16 of 32000 15.1 / 16.5, of 40000 14.8 / 15.2, of
+// 65000 16.8 / 16.2, of 100000 32.6 / 29.6.  A launch takes some 3 us of the host's time besides.
 constexpr int kSumFrom = 40960;
 
 // Workgroups per row of scores, where there are fewer rows than fill the card, of at least four rounds of loads.  In all up to 512 /

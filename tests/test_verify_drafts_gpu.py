@@ -106,6 +106,25 @@ def test_a_large_vocabulary(mode):
     Case([7, 3], 256 * 4096 + 4097, mode, seed=2).check()
 
 
+@pytest.mark.parametrize("vocab", [41000, 65537, 131075, 262143, 262150, 400001])
+def test_rows_added_up_again(vocab):
+    """Rejected siblings, so that the sums of the present row's pieces are not those of the first launch; and rows of which the draft
+    leaves nothing. Places all over the row."""
+    g = torch.Generator().manual_seed(vocab)
+    lens, ends = [4] * 12, [0.0, 1.0 - 2.0 ** -24]
+    case = Case(lens, vocab, "drawn", trees=[[-1, 0, 0, 0]] * 12)
+    case.sample = torch.cat([torch.tensor(ends), torch.rand(10, generator=g)])
+    case.accept[:] = 1.0 - 2.0 ** -24
+    for r in range(12):
+        p, q = case.target[4 * r], case.draft[4 * r]
+        if r % 4 == 3:
+            p.copy_(0.5 * q)
+        worse = (q > 4 * p).nonzero()[:, 0] if r % 4 != 3 else (q > 0).nonzero()[:, 0]
+        case.tokens[4 * r + 1:4 * r + 4] = worse[torch.randperm(len(worse), generator=g)[:3]].tolist()
+    counts = case.check()
+    assert max(counts) == 1
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("vocab", [9, 2049, 20001])
 def test_scores_of_every_type_and_stride(dtype, vocab):
