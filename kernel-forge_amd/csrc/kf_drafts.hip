@@ -772,9 +772,9 @@ __global__ __launch_bounds__(kKeepThreads) void keep_drafts_kernel(KeepArgs a) {
 // 65000 16.8 / 16.2, of 100000 32.6 / 29.6.  A launch takes some 3 us of the host's time besides.
 constexpr int kSumFrom = 40960;
 
-// Workgroups per row of scores, where there are fewer rows than fill the card, of at least four rounds of loads.  In all up to 512 /
-// 768 / 1024, us of both launches over rows of 100003 bf16 values: 100 rows 7.6 / 7.9 / 8.1, 150 9.7 / 8.9 / 9.2, 464 19.7 / 19.6 /
-// 21.0, 512 21.1 / 21.3 / 22.9; 300 rows of 32000 fp16 ones 8.6 / 7.3 / 7.5.
+// Workgroups per row of scores, where there are fewer rows than fill the card, of at least four rounds of loads.  Of up to
+// 512 / 768 / 1024 in all, us of both launches over rows of 100003 bf16 values: 100 rows 7.6 / 7.9 / 8.1, 150 9.7 / 8.9 / 9.2,
+// 464 19.7 / 19.6 / 21.0, 512 21.1 / 21.3 / 22.9; 300 rows of 32000 fp16 ones 8.6 / 7.3 / 7.5.
 int row_shares(const VerifyArgs& a) {
   const int64_t most = ((int64_t)a.vocab + 4 * kBestStep - 1) / (4 * kBestStep);
   return (int)std::max<int64_t>(1, std::min<int64_t>(most, 768 / std::max(a.tokens_count, 1)));
