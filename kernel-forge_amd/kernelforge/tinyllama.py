@@ -679,7 +679,11 @@ class PagedDecoder:
             if not held:
                 continue
             draft = drafts.get(row, self.tokens[:0])
-            draft, above, probs = (draft, None, None) if isinstance(draft, torch.Tensor) else (*draft, None)[:3]
+            draft = (draft,) if isinstance(draft, torch.Tensor) else tuple(draft)
+            if not 1 <= len(draft) <= 3 or not all(isinstance(t, torch.Tensor) or (i and t is None) for i, t in enumerate(draft)):
+                raise TypeError(f"decode_drafts: the draft of row {row} must be tokens, (tokens, parents) or (tokens, parents, "
+                                "probabilities), all of them tensors")
+            draft, above, probs = (*draft, None, None)[:3]
             n = draft.numel()
             if draft.dim() != 1 or draft.dtype not in (torch.int64, torch.int32) or draft.device != dev:
                 raise ValueError(f"decode_drafts: the tokens of row {row} must be 1-D int64 on {dev}, got "
@@ -765,16 +769,18 @@ class PagedDecoder:
                     draft[first + 1 + above.long()] = probs
             done = ops.verify_drafts(tokens, parents, step.cu_new, target, accept, sample, draft=draft, max_new=max(new))
         counts = done.counts.tolist()
-        kept = ops.keep_drafts(self.cache, self.block_table, self.context_lens, step.seq_lens, done.counts, done.path,
-                               self.free_pages, step.free_count)
-        # Emitted tokens stand behind each row's last one.
+        # Emitted tokens stand behind each row's last one.  All that can fail comes before the pages are given back.
         place = torch.arange(done.tokens.shape[1], device=self.device)
         row, i = (place < done.counts[:, None]).nonzero(as_tuple=True)
-        self.history[row, self.context_lens.long()[row] + 1 + i] = done.tokens[row, i]
+        column, emitted = self.context_lens.long()[row] + 1 + i, done.tokens[row, i]
         last = done.tokens.gather(1, (done.counts.long() - 1).clamp(min=0).unsqueeze(1))[:, 0]
-        self.tokens.copy_(torch.where(done.counts > 0, last, self.tokens))
+        last = torch.where(done.counts > 0, last, self.tokens)
+        kept = ops.keep_drafts(self.cache, self.block_table, self.context_lens, step.seq_lens, done.counts, done.path,
+                               self.free_pages, step.free_count)
         self.context_lens.copy_(kept.context_lens)
         self.free_count.copy_(kept.free_count)
+        self.tokens.copy_(last)
+        self.history[row, column] = emitted
         return counts
 
     def generated(self, row: int, prompt_len: int) -> torch.Tensor:

@@ -197,6 +197,9 @@ def test_refusals(model):
                           ({0: (t, t - 1, torch.zeros(3, 2000, device=DEV))}, "need a temperature")):
         with pytest.raises(ValueError, match=match):
             dec.decode_drafts(drafts)
+    for draft in ([1, 2], (t, t, t, t), (), (None, t), (t, [-1, 0, 1]), {1: t}):
+        with pytest.raises(TypeError, match="must be tokens"):
+            dec.decode_drafts({0: draft})
     for temperature in (-1.0, float("nan"), float("inf")):
         with pytest.raises(ValueError, match="temperature"):
             dec.decode_drafts({}, temperature=temperature)
