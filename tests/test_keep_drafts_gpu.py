@@ -246,3 +246,92 @@ def test_steps_in_a_row():
                 assert torch.equal(caches[0, page, :, i % block], kk) and torch.equal(caches[1, page, :, i % block], vv)
         assert sorted(held + free[:int(free_count)].tolist()) == list(range(pages))
     assert max(context.tolist()) > 4
+
+
+@pytest.mark.parametrize("heads,kv,dtype", [(8, 4, torch.float16), (12, 2, torch.bfloat16)])
+@pytest.mark.parametrize("mode", ["greedy", "drawn"])
+def test_a_captured_step(heads, kv, dtype, mode):
+    """A whole step in one graph, replayed over other lengths, trees and drafts, beside the same eager calls on a state of their own:
+    all that it writes is bit for bit the same."""
+    d, block, vocab, rows, pages, b = 64, 16, 211, 150, 100, 4
+    g = torch.Generator(device=DEV).manual_seed(9)
+    rng = random.Random(9)
+    ang = torch.arange(600, dtype=torch.float64, device=DEV)[:, None] * 10000.0 ** (
+        -torch.arange(0, d, 2, dtype=torch.float64, device=DEV) / d)
+    cos, sin = torch.cat([ang.cos()] * 2, 1).float(), torch.cat([-ang.sin(), ang.sin()], 1).float()
+
+    def state():
+        return dict(caches=torch.zeros(2, pages, kv, block, d, dtype=dtype, device=DEV), table=torch.full_like(i32([[0] * 70] * b), -1),
+                    context=i32([0] * b), free=i32(list(range(pages))), count=i32([pages]))
+
+    inputs = dict(new=i32([0] * b), parents=i32([0] * rows), tokens=torch.zeros(rows, dtype=torch.int64, device=DEV),
+                  qkv=torch.zeros(rows, (heads + 2 * kv) * d, dtype=dtype, device=DEV), target=torch.zeros(rows, vocab, device=DEV),
+                  accept=torch.zeros(rows, device=DEV), sample=torch.zeros(b, device=DEV), draft=torch.zeros(rows, vocab, device=DEV))
+
+    def run(s, x):
+        step = ops.paged_tables(s["table"], s["context"], x["new"], s["free"], s["count"], block_size=block, max_tokens=rows)
+        trees = ops.draft_trees(x["parents"], step.cu_new, step.seq_lens)
+        q, _ = ops.rope_paged_cache(x["qkv"], cos, sin, trees.positions, step.slots, s["caches"][0], s["caches"][1], heads=heads)
+        out = ops.paged_tree_attention(q, s["caches"][0], s["caches"][1], s["table"], step.cu_new, step.seq_lens, trees.ancestors)
+        if mode == "greedy":
+            done = ops.verify_drafts(x["tokens"], x["parents"], step.cu_new, x["target"])
+        else:
+            done = ops.verify_drafts(x["tokens"], x["parents"], step.cu_new, x["target"], x["accept"], x["sample"], draft=x["draft"])
+        kept = ops.keep_drafts(s["caches"], s["table"], s["context"], step.seq_lens, done.counts, done.path, s["free"],
+                               step.free_count)
+        s["context"].copy_(kept.context_lens)
+        s["count"].copy_(kept.free_count)
+        return (*trees, out, *done)
+
+    eager, captured = state(), state()
+    run(state(), inputs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = run(captured, inputs)
+    for lens in ([64, 1, 30, 17], [5, 64, 0, 64], [0, 0, 0, 0], [1, 1, 1, 1], [33, 9, 64, 2], [16, 64, 3, 60]):
+        trees = random_trees(lens, sum(lens), 3)
+        inputs["new"].copy_(i32(lens))
+        inputs["parents"].copy_(i32([p for t in trees for p in t] + [0] * (rows - sum(lens))))
+        inputs["qkv"].normal_(generator=g)
+        for name in ("target", "draft"):
+            inputs[name].copy_(torch.softmax(3 * torch.randn(rows, vocab, generator=g, device=DEV), -1))
+        for name in ("accept", "sample"):
+            inputs[name].uniform_(generator=g)
+        inputs["tokens"].copy_(torch.randint(0, vocab, (rows,), generator=g, device=DEV))
+        at = 0
+        for t in trees:
+            for i, p in enumerate(t):
+                if i and rng.random() < 0.8:
+                    inputs["tokens"][at + i] = inputs["target"][at + p].argmax()
+            at += len(t)
+        graph.replay()
+        want = run(eager, inputs)
+        torch.cuda.synchronize()
+        for x, y in zip((*static, *captured.values()), (*want, *eager.values())):
+            assert torch.equal(x, y)
+    assert int(eager["context"].max()) > 10
+
+
+def test_a_cache_whose_offsets_pass_32_bits():
+    """Attention and moves over the last pages of a large cache, against those pages alone."""
+    kv, block, d, pages, few, heads = 4, 64, 128, 70000, 12, 8
+    g = torch.Generator(device=DEV).manual_seed(2)
+    small = torch.randn(2, few, kv, block, d, generator=g, device=DEV).half()
+    large = torch.empty(2, pages, kv, block, d, dtype=torch.float16, device=DEV)
+    assert large[0].numel() > 1 << 31
+    large[:, -few:] = small
+    lens, ctx = [40, 3], [500, 90]
+    trees = random_trees(lens, 4, 2)
+    table = i32([[3, 0, 5, 7, 1, 11, 2, 9, 4], [10, 6, -1, -1, -1, -1, -1, -1, -1]])
+    far = torch.where(table >= 0, table + (pages - few), -1)
+    cu, seq = i32([0, 40, 43]), i32([c + n for c, n in zip(ctx, lens)])
+    words = torch.tensor([w for t in trees for w in ancestors_of(t)], dtype=torch.int64, device=DEV)
+    q = torch.randn(43, heads, d, generator=g, device=DEV).half()
+    for max_new in (None, 2):  # both kernels' plans
+        rows = q if max_new is None else q[:, :4].repeat(1, 2, 1)
+        near = ops.paged_tree_attention(rows, small[0], small[1], table, cu, seq, words, max_new=max_new)
+        assert torch.equal(ops.paged_tree_attention(rows, large[0], large[1], far, cu, seq, words, max_new=max_new), near)
+    path = i32([[0, 7, 20, 39] + [-1] * 60, [0, 2] + [-1] * 62])
+    for cache, t in ((small, table), (large, far)):
+        assert ops.keep_drafts(cache, t, i32(ctx), seq, i32([4, 2]), path).context_lens.tolist() == [504, 92]
+    assert torch.equal(large[:, -few:], small)
