@@ -319,12 +319,13 @@ struct TreeRow {
     const int node = key - sk.shift;
     return key < sk.keys && (node < 0 || (node < 64 && (bits >> node & 1)));
   }
-  // Bit e: key + e, e < 4.
-  __device__ __forceinline__ uint32_t four(const SeqKeys& sk, int key) const {
-    const int node = key - sk.shift, there = min(max(sk.keys - key, 0), 4);
-    const uint64_t old = 0xFull << min(max(-node, 0), 4);  // its low four bits: those of the new tokens among them
-    const uint64_t mine = node >= 64 ? 0 : node >= 0 ? bits >> node : bits << min(-node, 4);
-    return ((uint32_t)(mine & old) | ~(uint32_t)old) & ((1u << there) - 1);
+  // Bit e: key + e, of a key that is the same in all lanes; so are the shifts.
+  __device__ __forceinline__ uint64_t from(const SeqKeys& sk, int key) const {
+    const int node = key - sk.shift, there = sk.keys - key;
+    const uint64_t mine = node >= 64 || node <= -64 ? 0 : node >= 0 ? bits >> node : bits << -node;
+    const uint64_t old = node >= 0 ? 0 : node <= -64 ? ~0ull : (1ull << -node) - 1;
+    const uint64_t in = there >= 64 ? ~0ull : there <= 0 ? 0 : (1ull << there) - 1;
+    return (mine | old) & in;
   }
 };
 

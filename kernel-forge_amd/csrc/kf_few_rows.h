@@ -255,13 +255,15 @@ __device__ __forceinline__ void few_rows_stretch(const AttnArgs& args, FewShared
             s[u] = Elem<E>::mfma16(lds_read16(((buf + k_at) ^ (uint32_t)(64 * st)) + u * 16 * ROW), qf[t][st], s[u]);
         }
         if (masked) {
+          uint32_t seen = 0;  // this lane's keys: bits 16 u + e
+          if constexpr (TREE)
+            seen = ((uint32_t)node[t].from(sk, key0) & ((bad0 ? 0 : 0xFFFF) | (bad1 ? 0 : 0xFFFF0000u))) >> (4 * g);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             if constexpr (TREE) {
-              const uint32_t seen = (u ? bad1 : bad0) ? 0 : node[t].four(sk, key0 + 16 * u + 4 * g);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (!(seen >> e & 1)) s[u][e] = -__builtin_inff();
+                if (!(seen >> (16 * u + e) & 1)) s[u][e] = -__builtin_inff();
             } else {
               const int last = keys_at(t, u);
 #pragma unroll

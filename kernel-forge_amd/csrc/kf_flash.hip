@@ -235,13 +235,19 @@ __device__ __forceinline__ void flash_item(const AttnArgs& a, FlashShared<HDP, G
       return u32x4{v0[0], v0[1], v1[0], v1[1]};
     };
     if (__builtin_expect(masked, 0)) {
+      uint64_t seen = 0;  // this lane's keys: bits 8 q + e
+      if constexpr (TREE) {
+        uint64_t there = 0;
+#pragma unroll
+        for (int i = 0; i < KK; ++i) there |= (bad >> i) & 1 ? 0 : 0xFFFFull << (16 * i);
+        seen = (node.from(sk, key0) & there) >> (4 * half);
+      }
 #pragma unroll
       for (int q = 0; q < 2 * KK; ++q) {
         if constexpr (TREE) {
-          const uint32_t seen = (bad >> (q >> 1)) & 1 ? 0 : node.four(sk, key0 + 8 * q + 4 * half);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (!(seen >> e & 1)) s[q >> 2][4 * (q & 3) + e] = -__builtin_inff();
+            if (!((uint32_t)(seen >> (32 * (q >> 2))) >> (8 * (q & 3) + e) & 1)) s[q >> 2][4 * (q & 3) + e] = -__builtin_inff();
         } else {
           const int last = keys_at(q);
 #pragma unroll
