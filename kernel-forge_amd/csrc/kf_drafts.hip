@@ -226,7 +226,7 @@ __global__ __launch_bounds__(64 * kTreeWaves) void verify_best_kernel(VerifyArgs
 // tokens where they were given.  The token behind the path is the one at which the running sum of f passes u times all of it: a
 // sum over the row, then the place in it.  In 64 bits, as an index is an integer and 32 bits would move it.
 //
-// One workgroup per request does this, the sum in 16 parts, one a wavefront, then the part, or the part of the part, that the place
+// A workgroup per request does this, the sum in 16 parts, one a wavefront, then the part, or the part of the part, that the place
 // is in.  Long rows are first added up by a launch of their own, in pieces of 4096 values: which row it is, is known from the first
 // test of every node's first child, unless a later child is accepted.
 constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64, kPiece = 4 * kPickThreads;
@@ -427,6 +427,18 @@ __device__ __forceinline__ Rest<DRAWN> rest_of(const VerifyArgs& a, const WalkSh
                      DRAWN ? 0 : (int)__popcll(w.under), a.vocab, w.taken};
 }
 
+// The workspace where rows are summed by a launch of their own; again and come: DRAWN.
+struct PickSpace {
+  double* sums;    // [seqs][pieces]
+  double* again;   // the same with more taken off
+  uint32_t* come;  // [seqs] workgroups whose pieces are in `again`
+};
+__device__ __host__ __forceinline__ PickSpace pick_space(const VerifyArgs& a, int pieces) {
+  double* const sums = static_cast<double*>(a.ws);
+  double* const again = sums + (int64_t)a.seqs * pieces;
+  return PickSpace{sums, again, reinterpret_cast<uint32_t*>(again + (int64_t)a.seqs * pieces)};
+}
+
 // Workgroup (piece, request): the sum over the piece.  16 rows of 150001 values of p and of q, 19 MB, take 6.3 us, the walk before
 // them included.
 template <bool DRAWN>
@@ -435,6 +447,7 @@ __global__ __launch_bounds__(kSumThreads) void verify_sum_kernel(VerifyArgs a, i
   __shared__ WalkShared walked;
   const int lane = threadIdx.x & 63, piece = blockIdx.x, r = blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (DRAWN && piece == 0 && threadIdx.x == 0) pick_space(a, pieces).come[r] = 0;
   if (wave == 0) walk<DRAWN>(a, walked, r, lane);
   __syncthreads();
   const Way w = way_of(walked);
@@ -446,7 +459,7 @@ __global__ __launch_bounds__(kSumThreads) void verify_sum_kernel(VerifyArgs a, i
   if (lane == 0) parts[wave] = sum;
   __syncthreads();
   if (threadIdx.x == 0)
-    static_cast<double*>(a.ws)[(int64_t)r * pieces + piece] = (parts[0] + parts[1]) + (parts[2] + parts[3]);
+    pick_space(a, pieces).sums[(int64_t)r * pieces + piece] = (parts[0] + parts[1]) + (parts[2] + parts[3]);
 }
 
 struct PickShared {
@@ -454,6 +467,7 @@ struct PickShared {
   double parts[kPickWaves], subs[kPickWaves][kSubs], scan[kPickWaves];
   double before;
   int low[kPickWaves], high[kPickWaves];
+  int goes_on;
 };
 
 // Sums over the threads up to and including each, and of all.
@@ -524,25 +538,51 @@ __device__ __forceinline__ double row_total(PickShared& sh, const Rest<DRAWN>& r
   return all;
 }
 
-// One workgroup per request.  pieces: of the rows, whose sums the launch before has left in a.ws; 0: there was none.  64 requests
-// over 32000 values, tokens given, 12.1 us (with an LDS atomic for every value that may be the place 60).  Drawn, bound by what one
-// CU reads: every rejected child behind a node's first costs a sum over the row, 1.2 MB of 150001 values in 11 us (10.5 with 32-bit
-// products); 6 us without such children, 22 to 33 with one to three.  (Such sums by a further launch of all CUs: both launches
-// 30 in place of 37 us, but 15.5 in place of 12.5 without such children, and 3 more of the host's time.)
+// By all workgroups of a request: the sums over the pieces once more, to `again`.  True in the one that is last done.
+template <bool DRAWN>
+__device__ __forceinline__ bool add_together(const VerifyArgs& a, PickShared& sh, const Rest<DRAWN>& rest, double* again,
+                                             int pieces, int lane, int wave) {
+  for (int p0 = 4 * blockIdx.y; p0 < pieces; p0 += 4 * gridDim.y) {
+    const int piece = p0 + wave / 4, begin = piece * kPiece + wave % 4 * (kPiece / 4);
+    const double sum = rest.template wave_total<false>(min(begin, a.vocab), min(begin + kPiece / 4, a.vocab), lane, nullptr);
+    __syncthreads();
+    if (lane == 0) sh.parts[wave] = sum;
+    __syncthreads();
+    const double* const four = sh.parts + wave;  // as verify_sum_kernel adds them
+    if (lane == 0 && wave % 4 == 0 && piece < pieces)
+      __hip_atomic_store(again + piece, (four[0] + four[1]) + (four[2] + four[3]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  // The sums are atomics of the whole device's scope, which go past the caches that XCDs have of their own: there once they are
+  // acknowledged, before the barrier, and so before the count.  (Fences of that scope write back and empty the caches: 10 us.)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0)
+    sh.goes_on = __hip_atomic_fetch_add(pick_space(a, pieces).come + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                 gridDim.y - 1;
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(sh.goes_on) != 0;
+}
+
+// One workgroup per request, or (DRAWN) several of which one goes on.  pieces: of the rows, whose sums the launch before has
+// left in a.ws; 0: there was none.  64 requests over 32000 values, tokens given, 12.1 us (with an LDS atomic for every value
+// that may be the place 60).  Drawn, bound by what CUs read: each child that is tested behind a node's first costs a sum over the
+// row that is left then, 1.2 MB of 150001 values, 11 us by one CU (10.5 with 32-bit products), 3 by ten.  Both launches of 16 such
+// requests: 12.5 us without such children, 15.7 with one, 28 with two (one workgroup each 26 and 37.5; a launch of all CUs for
+// these sums 30 for two, but 15.5 for none).
 template <bool DRAWN>
 __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a, int pieces) {
   __shared__ PickShared sh;
   WalkShared& walked = sh.walked;
   const int tid = threadIdx.x, lane = tid & 63, r = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const double* const sums = static_cast<const double*>(a.ws) + (int64_t)r * pieces;
+  const double* sums = pick_space(a, pieces).sums + (int64_t)r * pieces;
   const float sample_u = a.sample_u[r];
-  const double my_sum = tid < pieces ? sums[tid] : 0.0;
+  double my_sum = tid < pieces ? sums[tid] : 0.0;
   if (wave == 0) walk<DRAWN>(a, walked, r, lane);
   __syncthreads();
   Way w = way_of(walked);
   if (w.last < 0) {
-    if (wave == 0) write_path(a, r, 0, 0, lane);
+    if (wave == 0 && blockIdx.y == 0) write_path(a, r, 0, 0, lane);
     return;
   }
   bool summed = pieces > 0;  // the pieces' sums are those of the present row and what is taken off
@@ -561,6 +601,39 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a,
   // Drawn: the last node's further children, each of whose tests needs the sum of what the ones before have left; the first one has
   // been rejected.  Then the sum of what is left to draw from.
   uint64_t open = DRAWN ? w.under & (w.under - 1) : 0;
+  auto test = [&](double all) {  // of the first open child
+    const int c = __builtin_ctzll(open);
+    open &= open - 1;
+    if (!(walked.u[c] * all * walked.q[c] < positive(walked.p[c] - w.taken * walked.q[c]))) {
+      w.taken += all;
+      return;
+    }
+    // Accepted: on along first children, as far as they are.
+    w.on |= 1ull << c;
+    w.last = c;
+    while (true) {
+      w.under = of_lane(walked.children[w.last], 0);
+      w.taken = w.under ? 1.0 : 0.0;
+      open = w.under & (w.under - 1);
+      if (!w.under) break;
+      const int e = __builtin_ctzll(w.under);
+      if (!(walked.u[e] * walked.q[e] < walked.p[e])) break;
+      w.on |= 1ull << e;
+      w.last = e;
+    }
+  };
+  // The workgroups of a request make the first of these tests all together.  If there is none, the first one goes on alone.  If
+  // there is, each adds up some of the pieces of what is left then, and the one that is last done goes on: none waits for another.
+  if (DRAWN && gridDim.y > 1) {  // a thread has all of the sums that it reads: pick_team
+    bool on = blockIdx.y == 0;
+    if (open) {
+      test(add_pieces());
+      sums += (int64_t)a.seqs * pieces;
+      on = add_together<DRAWN>(a, sh, rest_of<DRAWN>(a, walked, w), const_cast<double*>(sums), pieces, lane, wave);
+      if (on) my_sum = tid < pieces ? __hip_atomic_load(sums + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    }
+    if (!on) return;
+  }
   bool whole = false;
   double all;
   Rest<DRAWN> rest;
@@ -572,26 +645,8 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a,
     }
     all = summed ? add_pieces() : row_total(sh, rest, 0, a.vocab, lane, wave);
     if (open) {
-      const int c = __builtin_ctzll(open);
-      open &= open - 1;
+      test(all);
       summed = false;
-      if (!(walked.u[c] * all * walked.q[c] < positive(walked.p[c] - w.taken * walked.q[c]))) {
-        w.taken += all;
-        continue;
-      }
-      // Accepted: on along first children, as far as they are.
-      w.on |= 1ull << c;
-      w.last = c;
-      while (true) {
-        w.under = of_lane(walked.children[w.last], 0);
-        w.taken = w.under ? 1.0 : 0.0;
-        open = w.under & (w.under - 1);
-        if (!w.under) break;
-        const int e = __builtin_ctzll(w.under);
-        if (!(walked.u[e] * walked.q[e] < walked.p[e])) break;
-        w.on |= 1ull << e;
-        w.last = e;
-      }
     } else if (all > 0.0 || whole) {
       break;
     } else {
@@ -768,8 +823,9 @@ __global__ __launch_bounds__(kKeepThreads) void keep_drafts_kernel(KeepArgs a) {
 }
 
 // Rows up to which one workgroup adds them up.  One launch / two, us: tokens given, 16 requests of 32000 values 11.5 / 12.8,
-// of 40000 13.2 / 12.8, of 50000 15.2 / 12.8, of 65000 15.1 / 12.8; drawn, 16 of 32000 15.1 / 16.5, of 40000 14.8 / 15.2, of
-// 65000 16.8 / 16.2, of 100000 32.6 / 29.6.  A launch takes some 3 us of the host's time besides.
+// of 40000 13.2 / 12.8, of 50000 15.2 / 12.8, of 65000 15.1 / 12.8; drawn, 16 of 32000 10.0 / 11.9 without further sums and
+// 15.3 / 17.3 with one, of 40000 11.1 / 11.8 and 15.4 / 14.8, of 65000 12.3 / 11.6 and 17.6 / 14.9.  A launch takes some 3 us of
+// the host's time besides.
 constexpr int kSumFrom = 40960;
 
 // Workgroups per row of scores, where there are fewer rows than fill the card, of at least four rounds of loads.  Of up to
@@ -789,6 +845,13 @@ void best_launch(const VerifyArgs& a, int shares, hipStream_t stream) {
 // Pieces of a row whose sums a launch of their own leaves; 0: one workgroup adds the row up.
 int summed_pieces(const VerifyArgs& a) { return a.vocab <= kSumFrom ? 0 : (a.vocab + kPiece - 1) / kPiece; }
 
+// Workgroups that add up a request's row again together, four pieces at a time; no more in all than the card has CUs, one for
+// each.  In all up to 128 / 256 / 512, us of both launches over rows of 150001 values: 16 requests 17.5 / 15.3 / 15.4, 32
+// 24.4 / 22.4 / 24.9, 64 49.6 / 45.6 / 45.8; without such sums the same to 0.2.
+int pick_team(const VerifyArgs& a, int pieces) {
+  return pieces > kPickThreads ? 1 : std::max(1, std::min((pieces + 3) / 4, 256 / a.seqs));
+}
+
 template <bool DRAWN>
 hipError_t sample_launch(const VerifyArgs& a, hipStream_t stream) {
   const int pieces = summed_pieces(a);
@@ -796,7 +859,7 @@ hipError_t sample_launch(const VerifyArgs& a, hipStream_t stream) {
     verify_sum_kernel<DRAWN><<<dim3(pieces, a.seqs), kSumThreads, 0, stream>>>(a, pieces);
     if (hipError_t err = hipGetLastError(); err != hipSuccess) return err;
   }
-  verify_pick_kernel<DRAWN><<<a.seqs, kPickThreads, 0, stream>>>(a, pieces);
+  verify_pick_kernel<DRAWN><<<dim3(a.seqs, DRAWN ? pick_team(a, pieces) : 1), kPickThreads, 0, stream>>>(a, pieces);
   return hipGetLastError();
 }
 
@@ -809,7 +872,8 @@ hipError_t draft_trees_launch(const DraftTreesArgs& a, hipStream_t stream) {
 
 size_t verify_workspace_bytes(const VerifyArgs& a) {
   if (a.mode == kVerifyBest) return (size_t)a.tokens_count * row_shares(a) * sizeof(uint64_t);
-  return (size_t)a.seqs * summed_pieces(a) * sizeof(double);
+  const size_t sums = (size_t)a.seqs * summed_pieces(a) * sizeof(double);
+  return a.mode == kVerifyDrawn && sums ? 2 * sums + a.seqs * sizeof(uint32_t) : sums;
 }
 
 hipError_t verify_launch(const VerifyArgs& a, int dtype, hipStream_t stream) {

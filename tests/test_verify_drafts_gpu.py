@@ -125,6 +125,25 @@ def test_rows_added_up_again(vocab):
     assert max(counts) == 1
 
 
+def test_rows_added_up_by_several_workgroups():
+    """Requests with and without further sums side by side, on several streams at once and again and again: always the same."""
+    case = Case([1, 9, 0, 20, 3, 16, 2, 30] * 3, 90001, "drawn", seed=5, width=4, pad=1)
+    case.check()
+    args, draft = case.args()
+    want = ops.verify_drafts(*args, draft=draft)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for side in streams:
+        side.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(40):
+        for side in streams:
+            with torch.cuda.stream(side):
+                got.append(ops.verify_drafts(*args, draft=draft))
+    torch.cuda.synchronize()
+    for done in got:
+        assert all(torch.equal(x, y) for x, y in zip(done, want))
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("vocab", [9, 2049, 20001])
 def test_scores_of_every_type_and_stride(dtype, vocab):
