@@ -419,9 +419,10 @@ int kf_paged_tree_attention(const kf_paged_attention_args* args, const void* anc
  *                    probabilities of the children before it; a token that was rejected is not accepted again.  The token behind
  *                    the path is drawn from what the last node's children leave, f = p without their tokens: the first index at
  *                    which the running sum of f is above sample_u times its whole.
- *   KF_VERIFY_DRAWN  the same for children that were drawn, independently, from row t of draft (q, fp32): with a = 0 and m = 1
- *                    at first, a child is accepted if accept_u[c] m q(token) < f(token), f = max(p - a q, 0), else a grows by
- *                    m, and m becomes the sum of the new f.  f is also what the token behind the path is drawn from.
+ *   KF_VERIFY_DRAWN  the same for children that were drawn, independently, from row t of draft (q, fp32; NaN and negative ones
+ *                    count as 0, others above 1 as 1): with a = 0 and m = 1 at first, a child is accepted if accept_u[c] m
+ *                    q(token) < f(token), f = max(p - a q, 0), else a grows by m, and m becomes the sum of the new f.  f is
+ *                    also what the token behind the path is drawn from.  Rows of nodes without children may hold anything.
  * Emitted tokens then have the target's distribution, if accept_u and sample_u are independent uniform numbers in [0, 1).
  * Where f has no mass, the token is drawn from p; where that has none, it is 0; for a sample_u that is not below 1, the last index
  * with any.  Sums in 64 bits; results do not change from run to run.  A token outside [0, vocab) is never accepted.

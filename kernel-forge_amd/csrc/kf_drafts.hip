@@ -237,6 +237,10 @@ constexpr int kSumThreads = 256;
 __device__ __forceinline__ double positive(double x) { return __builtin_fmax(x, 0.0); }
 __device__ __forceinline__ float positive(float x) { return __builtin_fmaxf(x, 0.0f); }
 
+// A draft's probability: from 0, which is also NaN's, to 1.  Infinity or NaN times an `a` of 0 (a node without children) would be
+// none, and the target's mass there lost.  Costs nothing: the conversion to 64 bits clamps.
+__device__ __forceinline__ double drawn_from(float q) { return __builtin_fmin(__builtin_fmax((double)q, 0.0), 1.0); }
+
 // Sums over a wavefront's lanes up to and including each.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double add_dpp(double v) {
@@ -285,11 +289,11 @@ __device__ __forceinline__ void walk(const VerifyArgs& a, WalkShared& sh, int r,
     const int mine = t.first + min(lane, t.nodes - 1), up = t.first + max(t.parent, 0);
     const int64_t token = a.tokens[mine], inside = token >= 0 && token < a.vocab ? token : 0;
     const float u = a.accept_u[mine], p = ((const float*)a.target)[(int64_t)up * a.target_row + inside];
-    const float q = DRAWN ? a.draft[(int64_t)up * a.draft_row + inside] : 0.0f;
+    const double q = DRAWN ? drawn_from(a.draft[(int64_t)up * a.draft_row + inside]) : 0.0;
     const bool real = token == inside;  // others have no mass
     sh.token[lane] = token;
     sh.p[lane] = real ? positive(p) : 0.0;
-    sh.q[lane] = real ? (double)q : 0.0;
+    sh.q[lane] = real ? q : 0.0;
     sh.u[lane] = u;
     if (t.parent >= 0)
       atomicOr((unsigned long long*)&sh.children[t.parent], 1ull << lane);  // by one wavefront, an or: no order to it
@@ -350,7 +354,7 @@ struct Rest {
   template <int LANES>
   __device__ __forceinline__ void four(row4_t x, row4_t y, int i, int from, double (&f)[4]) const {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = DRAWN ? positive(fma(-taken, (double)y[e], (double)x[e])) : (double)positive(x[e]);
+    for (int e = 0; e < 4; ++e) f[e] = DRAWN ? positive(fma(-taken, drawn_from(y[e]), (double)x[e])) : (double)positive(x[e]);
     if constexpr (!DRAWN) {
       for (int g = 0; g < gone_count; ++g) {
         const int64_t token = gone[g];

@@ -1469,7 +1469,8 @@ def verify_drafts(tokens: torch.Tensor, parents: torch.Tensor, cu_new: torch.Ten
       as tokens drawn from target one by one. Without ``draft`` a node's children are taken as they are, accepted in turn with what
       is left of their parent's mass; with draft fp32 [T, vocab] they were drawn, independently of each other, from row t of it, and
       are accepted with max(p - a q, 0) / (m q). The token behind the path is drawn from what is left: the first index
-      at which the running sum passes the uniform number times the whole. Sums in 64 bits; NaN and negative ones count as 0.
+      at which the running sum passes the uniform number times the whole. Sums in 64 bits; NaN and negative ones count as 0,
+      draft's above 1 as 1; its rows of nodes without children may hold anything.
 
     max_new: nodes of a request that are looked at, and the width of the results (64, the most, without it). Tokens outside
     the vocabulary are never accepted. Rows of target and draft may be strided. Results do not change from run to run. The form

@@ -339,3 +339,22 @@ def test_captured(mode):
         torch.cuda.synchronize()
         for out in outs:
             case.check(out)
+
+
+@pytest.mark.parametrize("vocab", [4500, 90001])
+@pytest.mark.parametrize("bad,counts_as", [(float("nan"), 0.0), (float("-inf"), 0.0), (-3.0, 0.0), (float("inf"), 1.0), (7.0, 1.0)],
+                         ids=["nan", "-inf", "negative", "inf", "seven"])
+def test_draft_probabilities_that_are_none(vocab, bad, counts_as):
+    """What a draft row holds beside numbers from 0 to 1 counts as the nearer end, NaN as 0: the target's mass there stays, and
+    drafted tokens that the target does not have are not accepted. Rows of nodes without children may hold anything."""
+    case = Case([6, 9, 2], vocab, "drawn", seed=11, trees=[[-1, 0, 0, 0, 1, 1], [-1, 0, 0, 0, 0, 1, 2, 3, 3], [-1, 0]])
+    case.draft[:, ::7] = counts_as
+    case.target[:, ::14] = 0.0
+    for i in range(1, 17, 3):
+        case.tokens[i] = 14 * (i + 1)  # neither has any
+    case.accept[3::2] = 1.0 - 2.0 ** -24
+    raw = case.draft.clone()
+    raw[:, ::7] = bad
+    for leaf in (2, 3, 4, 5, 10, 11, 12, 13, 14, 16):
+        raw[leaf] = bad
+    case.check(case.call(draft=raw.to(DEV)))
