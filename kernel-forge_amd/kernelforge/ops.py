@@ -1575,11 +1575,12 @@ def keep_drafts(caches: torch.Tensor | list[torch.Tensor], block_table: torch.Te
     """What is kept of a step's drafts in the cache, in one launch (kf_keep_drafts).
 
     caches [..., num_pages, kv_heads, block_size, head_dim], fp16 or bf16: all arrays of all layers (TinyLlama.new_paged_cache), or
-    a list of such tensors, a launch each. context_lens, seq_lens int32 [B]: tokens before the step and with its new ones; counts
-    int32 [B] and path int32 [B, width] of verify_drafts. The entry of node path[r, i] moves to place context_lens[r] + i, i <
-    counts[r]; that many tokens are kept. With a stack, free_pages int32 [F] and free_count int32 [1] (PagedStep's), the pages that
-    held other nodes alone go back onto it, as far as it has room: free_pages is written, free_count is not, KeptDrafts has the new
-    one. block_table keeps their numbers, where paged_tables enters new ones. Pages must not be shared between requests.
+    a list of such tensors without places in common, a launch each. context_lens, seq_lens int32 [B]: tokens before the step and
+    with its new ones; counts int32 [B] and path int32 [B, width] of verify_drafts. The entry of node path[r, i] moves to place
+    context_lens[r] + i, i < counts[r]; that many tokens are kept. With a stack, free_pages int32 [F] and free_count int32 [1]
+    (PagedStep's), the pages that held other nodes alone go back onto it, as far as it has room: free_pages is written, free_count
+    is not, KeptDrafts has the new one. block_table keeps their numbers, where paged_tables enters new ones. Pages must not be
+    shared between requests.
     No reference counterpart.
     """
     tables = (block_table, context_lens, seq_lens, counts, path)
@@ -1619,8 +1620,8 @@ def keep_drafts(caches: torch.Tensor | list[torch.Tensor], block_table: torch.Te
     _check_plain("keep_drafts", (*listed, *tables, *stack))
     listed = [_check_kept_cache(cache) for cache in listed]
     traced = _traced((*listed, *tables, *stack))
-    if not traced and len({cache.data_ptr() for cache in listed}) < len(listed):
-        raise ValueError("caches must be different arrays")
+    if not traced and len(listed) > 1:
+        _check_apart(listed)
     run = _keep_drafts_op if traced else _launch_keep
     kept = run(listed[0], *tables, free_pages, free_count)
     for cache in listed[1:]:  # the lengths and the stack are dealt with
@@ -1661,6 +1662,56 @@ def _check_kept_cache(t: torch.Tensor) -> torch.Tensor:
         raise ValueError("caches must have a contiguous last dimension, other strides of multiples of 8, none of them 0, leading "
                          "dimensions that are one, and a 16-byte aligned start")
     return flat
+
+
+def _check_apart(caches: list[torch.Tensor]) -> None:
+    """Refuses caches (16-bit values) that have places in common: their entries would move twice."""
+    known, spans = {}, []  # layout -> its number, and the values from its first to its last
+    for cache in caches:
+        layout = cache.shape, cache.stride()
+        if layout not in known:
+            known[layout] = len(known), sum((n - 1) * s for n, s in zip(*layout))
+        number, extent = known[layout]
+        start = cache.data_ptr() // 2
+        spans.append((start, start + extent, number))
+    spans.sort()
+    apart, before = set(), []  # two layouts, and how far the second one begins behind the first
+    for start, end, number in spans:
+        before = [span for span in before if span[1] >= start]  # those that reach this one's first value
+        apart.update([(other, number, start - first) for first, _, other in before])
+        before.append((start, end, number))
+    layouts = list(known)
+    if any(_layouts_meet(layouts[a], layouts[b], distance) for a, b, distance in apart):
+        raise ValueError("caches must be different arrays, with no places in common")
+
+
+def _layouts_meet(a: tuple, b: tuple, apart: int, most_steps: int = 20000) -> bool:
+    """Whether an array of the shape and strides `a` and one of `b` that begins `apart` values behind it have a value in common: whether
+    sum(i_k stride_a[k]) - sum(j_k stride_b[k]) is `apart` for indices i, j inside the shapes.  Stride by stride, the largest
+    first, with the multiples from which the smaller ones still reach; True if most_steps do not tell."""
+    reach = {}  # stride -> the lowest and the highest multiple of it
+    for layout, sign in ((a, 1), (b, -1)):
+        for n, s in zip(*layout):
+            if n > 1:
+                low, high = reach.get(s, (0, 0))
+                reach[s] = (low, high + n - 1) if sign > 0 else (low - n + 1, high)
+    strides = sorted(reach, reverse=True)
+    ends = [(0, 0)]  # the lowest and the highest sum of the strides behind each, itself included
+    for s in reversed(strides):
+        ends.append((ends[-1][0] + s * reach[s][0], ends[-1][1] + s * reach[s][1]))
+    ends.reverse()
+    open_sums, steps = {apart}, 0  # what is left to reach, for every choice so far
+    for s, (low_end, high_end) in zip(strides, ends[1:]):
+        left = set()
+        for value in open_sums:
+            low = max(reach[s][0], -((high_end - value) // s))
+            high = min(reach[s][1], (value - low_end) // s)
+            steps += max(high - low + 1, 0) + 1
+            if steps > most_steps:
+                return True
+            left.update(value - s * m for m in range(low, high + 1))
+        open_sums = left
+    return 0 in open_sums
 
 
 def _launch_keep(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count):

@@ -4,6 +4,8 @@ their registered ops under a tracer, and the host's own oracle against the defin
 from __future__ import annotations
 
 import ctypes
+import itertools
+import random
 import re
 
 import pytest
@@ -259,3 +261,43 @@ def test_the_walk_on_the_host():
     q = torch.tensor([[0.0, 0.5, 0.5]] * 3)
     assert verify_on_host(accept=torch.tensor([0, 0.49, 0.0]), draft=q, **call)[1] == [[0, 1, -1]]
     assert verify_on_host(accept=torch.tensor([0, 0.51, 0.0]), draft=q, **call)[2] == [[0, -1, -1]]
+
+
+def test_layouts_that_meet():
+    """Against all places of small arrays, one by one; and a search that is given up counts as a meeting."""
+    rng, hits = random.Random(0), 0
+
+    def places(shape, stride):
+        return {sum(i * s for i, s in zip(index, stride)) for index in itertools.product(*map(range, shape))}
+
+    for _ in range(3000):
+        a, b = (tuple(zip(*[(rng.randrange(1, 4), rng.choice(strides)) for _ in range(rng.randrange(1, 5))]))
+                for strides in ((1, 2, 3, 4, 6, 8, 12, 24, 5), (1, 2, 3, 4, 6, 8, 12, 24, 7)))
+        apart = rng.randrange(-10, 60)
+        want = bool(places(*a) & {p + apart for p in places(*b)})
+        assert ops._layouts_meet(a, b, apart) == want, (a, b, apart)
+        hits += want
+    assert 300 < hits < 2700
+    wide = ((5000, 22, 4, 16, 64), (22 * 8192, 8192, 1024, 64, 1))
+    assert not ops._layouts_meet(wide, wide, 4096) and ops._layouts_meet(wide, wide, 8192)
+    assert ops._layouts_meet(wide, wide, 4096, most_steps=1)
+
+
+@pytest.mark.parametrize("views", [
+    lambda c: [c, c[1:]], lambda c: [c[3], c[1:]], lambda c: [c[:3], c[2:]], lambda c: [c[:, :4], c[:, 3:]],
+    lambda c: [c[0], c.view(-1)[64:64 + c[0].numel()].view(c[0].shape)], lambda c: [c[..., :64], c[2:3, ..., 32:]],
+    lambda c: [c[0], c[2], c[3], c[2:3]],
+])
+def test_caches_that_share_places(views):
+    with pytest.raises(ValueError, match="different arrays"):
+        ops.keep_drafts(**keep_args(views(torch.zeros(4, 5, 2, 16, 64, dtype=torch.float16))))
+
+
+@pytest.mark.parametrize("views", [
+    lambda c: list(c), lambda c: [c[:1], c[1], c[2:]], lambda c: [c[::2], c[1::2]], lambda c: [c[:, :3], c[:, 3:]],
+    lambda c: [c[..., :32], c[..., 32:]], lambda c: [c[:, :, :1], c[:, :, 1:]], lambda c: list(c.transpose(0, 1)),
+])
+def test_views_of_one_tensor_that_share_no_place(views):
+    """Past the checks, as far as the device."""
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        ops.keep_drafts(**keep_args(views(torch.zeros(4, 5, 2, 16, 64, dtype=torch.float16))))

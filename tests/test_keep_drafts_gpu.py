@@ -335,3 +335,25 @@ def test_a_cache_whose_offsets_pass_32_bits():
     for cache, t in ((small, table), (large, far)):
         assert ops.keep_drafts(cache, t, i32(ctx), seq, i32([4, 2]), path).context_lens.tolist() == [504, 92]
     assert torch.equal(large[:, -few:], small)
+
+
+def test_lists_of_arrays_that_share_places():
+    """Views that meet are refused before anything moves; views of one tensor that do not are taken."""
+    step = Step([30, 5], [40, 64], arrays=6)
+    args, want = step.args(), step.host()
+    caches, stack = step.caches.to(DEV), i32(step.stack)
+    before = caches.clone()
+    flat = caches.view(-1)
+    shifted = flat[64:64 + 5 * caches[0].numel()].view(5, *caches.shape[1:])  # begins one token later
+    for listed in ([caches, caches[1:]], [caches[5], caches[1:]], [caches[:4], caches[3:]], [caches[:, :9], caches[:, 8:]],
+                   [caches[0], shifted], [caches[..., :64], caches[2:3, ..., 32:]]):
+        with pytest.raises(ValueError, match="different arrays"):
+            ops.keep_drafts(listed, *args, stack, i32([step.free]))
+    assert torch.equal(caches, before) and stack.tolist() == step.stack
+    turned = torch.empty(step.caches.shape[1], 6, 16, 2, 64, dtype=torch.float16, device=DEV).permute(1, 0, 3, 2, 4)
+    for whole in (caches, turned):
+        for parts in ([whole[i] for i in range(6)], [whole[:2], whole[2], whole[3:]], [whole[::2], whole[1::2]]):
+            whole.copy_(step.caches)
+            stack = i32(step.stack)
+            got = ops.keep_drafts(parts, *args, stack, i32([step.free]))
+            assert torch.equal(whole.cpu(), want[0]) and stack.tolist() == want[1] and got.context_lens.tolist() == want[2]
