@@ -1623,6 +1623,9 @@ def keep_drafts(caches: torch.Tensor | list[torch.Tensor], block_table: torch.Te
     if not traced and len(listed) > 1:
         _check_apart(listed)
     run = _keep_drafts_op if traced else _launch_keep
+    if not traced:  # of all arrays, before anything is moved
+        for cache in listed[1:]:
+            _check_memory("caches", cache, listed[0].device)
     kept = run(listed[0], *tables, free_pages, free_count)
     for cache in listed[1:]:  # the lengths and the stack are dealt with
         run(cache, *tables, None, None)

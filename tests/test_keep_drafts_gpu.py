@@ -357,3 +357,12 @@ def test_lists_of_arrays_that_share_places():
             stack = i32(step.stack)
             got = ops.keep_drafts(parts, *args, stack, i32([step.free]))
             assert torch.equal(whole.cpu(), want[0]) and stack.tolist() == want[1] and got.context_lens.tolist() == want[2]
+
+
+def test_a_list_with_an_array_elsewhere():
+    """Nothing is moved before all arrays have been looked at."""
+    step = Step([30, 5], [40, 64], arrays=2)
+    caches, stack = step.caches.to(DEV), i32(step.stack)
+    with pytest.raises(RuntimeError, match="must be on cuda"):
+        ops.keep_drafts([caches[0], step.caches[1]], *step.args(), stack, i32([step.free]))
+    assert torch.equal(caches.cpu(), step.caches) and stack.tolist() == step.stack
