@@ -1619,6 +1619,8 @@ def keep_drafts(caches: torch.Tensor | list[torch.Tensor], block_table: torch.Te
             raise ValueError("free_pages must be a contiguous 1-D int32 tensor")
     _check_plain("keep_drafts", (*listed, *tables, *stack))
     listed = [_check_kept_cache(cache) for cache in listed]
+    if any(cache.shape[3] != listed[0].shape[3] for cache in listed):
+        raise ValueError(f"caches must have one block size, got {[cache.shape[3] for cache in listed]}")
     traced = _traced((*listed, *tables, *stack))
     if not traced and len(listed) > 1:
         _check_apart(listed)

@@ -301,3 +301,9 @@ def test_views_of_one_tensor_that_share_no_place(views):
     """Past the checks, as far as the device."""
     with pytest.raises(RuntimeError, match="CUDA device"):
         ops.keep_drafts(**keep_args(views(torch.zeros(4, 5, 2, 16, 64, dtype=torch.float16))))
+
+
+def test_caches_of_several_block_sizes():
+    """One table cannot be of pages of 16 and of 32 tokens."""
+    with pytest.raises(ValueError, match="one block size"):
+        ops.keep_drafts(**keep_args([CACHE, torch.zeros(4, 5, 2, 32, 64, **H)]))
