@@ -1621,16 +1621,11 @@ def keep_drafts(caches: torch.Tensor | list[torch.Tensor], block_table: torch.Te
     listed = [_check_kept_cache(cache) for cache in listed]
     if any(cache.shape[3] != listed[0].shape[3] for cache in listed):
         raise ValueError(f"caches must have one block size, got {[cache.shape[3] for cache in listed]}")
-    traced = _traced((*listed, *tables, *stack))
-    if not traced and len(listed) > 1:
-        _check_apart(listed)
-    run = _keep_drafts_op if traced else _launch_keep
-    if not traced:  # of all arrays, before anything is moved
-        for cache in listed[1:]:
-            _check_memory("caches", cache, listed[0].device)
-    kept = run(listed[0], *tables, free_pages, free_count)
-    for cache in listed[1:]:  # the lengths and the stack are dealt with
-        run(cache, *tables, None, None)
+    args = (*tables, free_pages, free_count)
+    if len(listed) > 1:
+        kept = (_keep_listed_op if _traced((*listed, *tables, *stack)) else _launch_keep_listed)(listed, *args)
+    else:
+        kept = (_keep_drafts_op if _traced((*listed, *tables, *stack)) else _launch_keep)(listed[0], *args)
     return KeptDrafts(kept[:b], kept[b:] if stack else None)
 
 
@@ -1730,6 +1725,17 @@ def _launch_keep(caches, block_table, context_lens, seq_lens, counts, path, free
         return _run_keep(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count)
 
 
+def _launch_keep_listed(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count):
+    _check_apart(caches)
+    for cache in caches[1:]:  # of all arrays, before anything is moved
+        _check_memory("caches", cache, caches[0].device)
+    tables = (block_table, context_lens, seq_lens, counts, path)
+    kept = _launch_keep(caches[0], *tables, free_pages, free_count)
+    for cache in caches[1:]:  # the lengths and the stack are dealt with
+        _launch_keep(cache, *tables, None, None)
+    return kept
+
+
 def _run_keep(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count) -> torch.Tensor:
     """kf_keep_drafts on checked arguments of the current device; the new lengths and the stack's count in one tensor."""
     pages, kv_heads, block_size, d = caches.shape[-4:]
@@ -1757,5 +1763,17 @@ def _keep_drafts_op(caches: torch.Tensor, block_table: torch.Tensor, context_len
 
 
 @_keep_drafts_op.register_fake
+def _(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count):
+    return context_lens.new_empty(context_lens.shape[0] + 1)
+
+
+@torch.library.custom_op("kernelforge::keep_listed_drafts", mutates_args=("caches", "free_pages"))
+def _keep_listed_op(caches: list[torch.Tensor], block_table: torch.Tensor, context_lens: torch.Tensor, seq_lens: torch.Tensor,
+                    counts: torch.Tensor, path: torch.Tensor, free_pages: Optional[torch.Tensor],
+                    free_count: Optional[torch.Tensor]) -> torch.Tensor:
+    return _launch_keep_listed(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count)
+
+
+@_keep_listed_op.register_fake
 def _(caches, block_table, context_lens, seq_lens, counts, path, free_pages, free_count):
     return context_lens.new_empty(context_lens.shape[0] + 1)

@@ -307,3 +307,15 @@ def test_caches_of_several_block_sizes():
     """One table cannot be of pages of 16 and of 32 tokens."""
     with pytest.raises(ValueError, match="one block size"):
         ops.keep_drafts(**keep_args([CACHE, torch.zeros(4, 5, 2, 32, 64, **H)]))
+
+
+def test_a_list_under_a_tracer():
+    """One registered op, whose shapes are those of the lengths; what shares places is refused where it runs."""
+    with FakeTensorMode(), torch.no_grad():
+        args = {k: v.cuda() for k, v in keep_args().items()}
+        args["caches"] = [args["caches"], torch.zeros(5, 2, 16, 64, **H).cuda()]
+        kept = ops.keep_drafts(**args)
+        assert kept.context_lens.shape == (2,) and kept.free_count.shape == (1,)
+    cache, rest = CACHE.clone(), list(keep_args().values())[1:]
+    with pytest.raises(ValueError, match="different arrays"):
+        torch.ops.kernelforge.keep_listed_drafts([cache, cache[1:]], *rest)

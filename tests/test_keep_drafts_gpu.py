@@ -7,6 +7,8 @@ import random
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from kernelforge import ops
 
@@ -366,3 +368,26 @@ def test_a_list_with_an_array_elsewhere():
     with pytest.raises(RuntimeError, match="must be on cuda"):
         ops.keep_drafts([caches[0], step.caches[1]], *step.args(), stack, i32([step.free]))
     assert torch.equal(caches.cpu(), step.caches) and stack.tolist() == step.stack
+
+
+def test_a_list_in_a_traced_call():
+    """Through the registered op: the same results, and views that meet are refused when it runs."""
+    step = Step([30, 5], [40, 64], arrays=4)
+    args, want = step.args(), step.host()
+    caches, stack, free = step.caches.to(DEV), i32(step.stack), i32([step.free])
+
+    def call(a, b, *rest):
+        return ops.keep_drafts([a, b], *rest)
+
+    mode = FakeTensorMode()
+    fake = [mode.from_tensor(t) for t in (caches[:2], caches[2:], *args, stack, free)]
+    with torch.no_grad(), mode:
+        graph = make_fx(call)(*fake)
+    got = graph(caches[:2], caches[2:], *args, stack, free)
+    assert torch.equal(caches.cpu(), want[0]) and stack.tolist() == want[1]
+    assert got.context_lens.tolist() == want[2] and got.free_count.tolist() == [want[3]]
+    before = caches.clone()
+    for a, b in ((caches, caches[1:]), (caches[1:3], caches[:2]), (caches[1:2], caches[1:2])):
+        with pytest.raises(ValueError, match="different arrays"):
+            graph(a, b, *args, stack, free)
+    assert torch.equal(caches, before) and stack.tolist() == want[1]
