@@ -711,11 +711,17 @@ class PagedDecoder:
         tokens, parents, numbers = torch.cat(tokens), torch.cat([p.long() for p in parents]), torch.cat(numbers)
         outside = ((tokens < 0) | (tokens >= vocab)).any()
         orphan = ((numbers > 0) & ((parents < 0) | (parents >= numbers))).any()
-        outside, orphan = torch.stack([outside, orphan]).tolist()
+        torn = torch.zeros_like(orphan)
+        for _, above, probs in drawn:  # each row beside that of the first token with its parent
+            first = (above[:, None] == above).int().argmax(1)
+            torn |= ((probs != probs[first]).any(1) & (first < torch.arange(len(first), device=dev))).any()
+        outside, orphan, torn = torch.stack([outside, orphan, torn]).tolist()
         if outside:
             raise ValueError(f"decode_drafts: a drafted token is outside of the vocabulary of {vocab}")
         if orphan:
             raise ValueError("decode_drafts: a drafted token's parent must be one before it, or -1")
+        if torn:
+            raise ValueError("decode_drafts: tokens behind one parent must come with the same probabilities")
         return new, tokens, parents.int(), drawn
 
     @torch.no_grad()
@@ -728,8 +734,8 @@ class PagedDecoder:
         parents[i] the number of the drafted token that token i follows, smaller than i (-1: the row's last token), up to 63 tokens.
         Rows without drafts get one token.  Greedy at temperature 0, and then as ``decode`` to within roundings.  Otherwise
         tokens are distributed as if drawn one by one at that temperature, with random numbers from `generator`; drafts that
-        were drawn from probabilities come with them, (tokens, parents, float32 [n, vocab]; the same for tokens with one parent),
-        and all drafts of the step do.
+        were drawn from probabilities come with them, (tokens, parents, float32 [n, vocab]; tokens with one parent with the same
+        ones), and all drafts of the step do.
         Eager: the host waits for the counts."""
         if not 0.0 <= temperature < float("inf"):
             raise ValueError(f"decode_drafts: the temperature must be 0 or positive, got {temperature}")

@@ -218,3 +218,26 @@ def test_refusals(model):
     for x, y in zip(before, (dec.history, dec.context_lens, dec.free_count, dec.block_table)):
         assert torch.equal(x[0], y[0])
     assert dec.host_lens == [60, 0]
+
+
+def test_drafts_of_one_parent_come_with_one_row(model):
+    """Tokens behind one parent whose probabilities differ were not drawn as the rule of acceptance takes them to be: refused, and
+    nothing is changed."""
+    ps = prompts(30, 50)
+    dec = tl.PagedDecoder(model, DEV, requests=2, num_pages=30)
+    dec.admit(dict(enumerate(ps)))
+    before = (dec.history.clone(), dec.context_lens.clone(), dec.free_count.clone(), dec.block_table.clone(), dec.tokens.clone())
+    g = torch.Generator(device=DEV).manual_seed(4)
+    probs = torch.softmax(torch.randn(5, 2000, generator=g, device=DEV), -1)
+    tokens = torch.multinomial(probs, 1, generator=g)[:, 0]
+    chain = (tokens[:2], None, probs[:2])
+    for above in ([-1, -1, 0, 1, 2], [-1, 0, 1, 1, 3], [-1, 0, 1, 2, -1]):
+        above = torch.tensor(above, device=DEV)
+        for drafts in ({0: (tokens, above, probs), 1: chain}, {0: chain, 1: (tokens, above, probs)}):
+            with pytest.raises(ValueError, match="one parent"):
+                dec.decode_drafts(drafts, temperature=1.0, generator=g)
+    for x, y in zip(before, (dec.history, dec.context_lens, dec.free_count, dec.block_table, dec.tokens)):
+        assert torch.equal(x, y)
+    probs[4], probs[2] = probs[0], probs[1]
+    dec.decode_drafts({0: (tokens, torch.tensor([-1, 0, 0, 1, -1], device=DEV), probs), 1: chain}, temperature=1.0, generator=g)
+    no_page_is_lost(dec)
