@@ -764,8 +764,10 @@ class PagedDecoder:
             done = ops.verify_drafts(tokens, parents, step.cu_new, logits, max_new=max(new))
         else:
             # Above the largest score first, and by no less than this: no quotient passes the type's range.
+            # The largest is at 0 by itself: infinity less infinity is no number.
             logits = logits.float()
-            target = torch.softmax((logits - logits.amax(-1, keepdim=True)) / max(temperature, 1e-30), dim=-1)
+            top = logits.amax(-1, keepdim=True)
+            target = torch.softmax((logits - top).masked_fill_(logits == top, 0.0) / max(temperature, 1e-30), dim=-1)
             accept = torch.rand(tokens.numel(), generator=generator, device=self.device)
             sample = torch.rand(len(new), generator=generator, device=self.device)
             draft = None

@@ -241,3 +241,29 @@ def test_drafts_of_one_parent_come_with_one_row(model):
     probs[4], probs[2] = probs[0], probs[1]
     dec.decode_drafts({0: (tokens, torch.tensor([-1, 0, 0, 1, -1], device=DEV), probs), 1: chain}, temperature=1.0, generator=g)
     no_page_is_lost(dec)
+
+
+def test_sampled_from_scores_that_are_infinite(model, monkeypatch):
+    """A score of infinity has all of the probability, as it is the largest for greedy steps; scores that are all -inf are equal."""
+    p, = prompts(30)
+    forward = model.forward_paged
+
+    def infinite(*args, **kw):
+        logits = forward(*args, **kw)
+        if kw.get("trees") is not None:
+            logits[:] = -float("inf")
+            logits[:, 7] = high
+        return logits
+
+    monkeypatch.setattr(model, "forward_paged", infinite)
+    dec = tl.PagedDecoder(model, DEV, requests=1, num_pages=30)
+    dec.admit({0: p})
+    t = torch.tensor([7, 7, 8], device=DEV)
+    for high in (float("inf"), 3.0):
+        for temperature in (0.0, 1e-20, 0.8, 1e30):
+            assert dec.decode_drafts({0: t}, temperature=temperature) == [3]
+            assert dec.generated(0, 30)[-3:].tolist() == [7, 7, 7]
+    high = -float("inf")
+    g = torch.Generator(device=DEV).manual_seed(6)
+    assert len({dec.decode_drafts({}, temperature=1.0, generator=g)[0] * int(dec.tokens[0]) for _ in range(8)}) > 4
+    no_page_is_lost(dec)
