@@ -267,3 +267,51 @@ def test_sampled_from_scores_that_are_infinite(model, monkeypatch):
     g = torch.Generator(device=DEV).manual_seed(6)
     assert len({dec.decode_drafts({}, temperature=1.0, generator=g)[0] * int(dec.tokens[0]) for _ in range(8)}) > 4
     no_page_is_lost(dec)
+
+
+def test_rows_of_probabilities_stand_at_the_parents(model, monkeypatch):
+    """What verify_drafts is given: each node's row of the draft is what its children were drawn from, zeros without children."""
+    ps = prompts(30, 50, 20)
+    dec = tl.PagedDecoder(model, DEV, requests=3, num_pages=30)
+    dec.admit(dict(enumerate(ps)))
+    seen, verify = [], ops.verify_drafts
+
+    def spy(*args, **kw):
+        seen.append(kw["draft"].clone())
+        return verify(*args, **kw)
+
+    monkeypatch.setattr(ops, "verify_drafts", spy)
+    rows = torch.softmax(torch.randn(7, 2000, generator=torch.Generator(device=DEV).manual_seed(5), device=DEV), -1)
+    tokens = torch.arange(8, device=DEV)
+    # Row 0: two tokens behind the last one, one behind each of them, two behind token 2.  Row 2: a chain of two.
+    dec.decode_drafts({0: (tokens[:6], torch.tensor([-1, -1, 0, 1, 2, 2], device=DEV), rows[[0, 0, 1, 2, 3, 3]]),
+                       2: (tokens[:2], None, rows[4:6])}, temperature=0.9)
+    want = torch.zeros(7 + 1 + 3, 2000, device=DEV)
+    want[0], want[1], want[2], want[3] = rows[0], rows[1], rows[2], rows[3]
+    want[8], want[9] = rows[4], rows[5]
+    assert len(seen) == 1 and torch.equal(seen[0], want)
+    no_page_is_lost(dec)
+
+
+def test_tokens_that_only_the_draft_has_are_rejected(model, monkeypatch):
+    """A draft that is sure of tokens that the model never takes: none stays, in a chain and behind an accepted token."""
+    ps = prompts(30)
+    forward = model.forward_paged
+
+    def without(*args, **kw):  # token 5 has no probability, token 6 nearly all
+        logits = forward(*args, **kw)
+        if kw.get("trees") is not None:
+            logits[:, 5], logits[:, 6] = float("-inf"), logits.amax(-1) + 60
+        return logits
+
+    monkeypatch.setattr(model, "forward_paged", without)
+    sure = torch.zeros(2, 2000, device=DEV)
+    sure[0, 6] = sure[1, 5] = 1.0
+    dec = tl.PagedDecoder(model, DEV, requests=1, num_pages=30)
+    dec.admit({0: ps[0]})
+    t = torch.tensor([6, 5], device=DEV)
+    for _ in range(5):
+        assert dec.decode_drafts({0: (t, None, sure)}, temperature=1.0) == [2]
+        assert dec.generated(0, 30)[-2:].tolist() == [6, 6]
+        assert dec.decode_drafts({0: (t[[1, 1]], t.new_full((2,), -1), sure[[1, 1]])}, temperature=1.0) == [1]
+        assert dec.generated(0, 30)[-1].item() == 6
