@@ -358,3 +358,38 @@ def test_draft_probabilities_that_are_none(vocab, bad, counts_as):
     for leaf in (2, 3, 4, 5, 10, 11, 12, 13, 14, 16):
         raw[leaf] = bad
     case.check(case.call(draft=raw.to(DEV)))
+
+
+@pytest.mark.parametrize("mode", ["given", "drawn"])
+def test_more_pieces_than_threads(mode):
+    """Rows of more than 2^22 values, whose pieces' sums (4096 values each) the 1024 threads of a workgroup take in two rounds, and
+    whose further sums one workgroup makes. Half of the mass is behind the first round's; places in both rounds and at the end."""
+    first, vocab = 1024 * 4096, 1024 * 4096 + 4097
+    g = torch.Generator().manual_seed(3)
+    trees = [[-1, 0, 0], [-1, 0], [-1, 0, 0], [-1], [-1]]
+    lens = [len(t) for t in trees]
+    rows = sum(lens)
+
+    def halves(x):
+        x[:, :first] /= 2 * x[:, :first].double().sum(1, keepdim=True)
+        x[:, first:] /= 2 * x[:, first:].double().sum(1, keepdim=True)
+        return x
+
+    case = Case(lens, 8, mode, trees=trees)
+    case.target = halves(torch.rand(rows, vocab, generator=g))
+    case.accept[:] = 1.0 - 2.0 ** -24
+    case.sample = torch.tensor([0.21, 0.93, 2.0, 0.93, 0.0])
+    case.tokens = [int(t) for t in torch.randint(0, first, (rows,), generator=g)]
+    if mode == "drawn":
+        case.draft = halves(case.target * (0.25 + 4 * torch.rand(rows, vocab, generator=g)))
+        at = 0
+        for tree in trees:  # tokens that the draft has more often are rejected
+            worse = (case.draft[at] > 1.5 * case.target[at]).nonzero()[:, 0]
+            for i in range(1, len(tree)):
+                case.tokens[at + i] = int(worse[5 * i])
+            at += len(tree)
+    got = case.call()
+    case.check(got)
+    assert got.counts.tolist() == [1] * 5
+    places = got.tokens[:, 0].tolist()
+    assert places[0] < first <= min(places[1], places[2], places[3]) and places[4] < 100
