@@ -247,3 +247,30 @@ def test_captured(ctx, new):
         torch.cuda.synchronize()
         want = b(max_new=64)
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+@DTYPES
+@pytest.mark.parametrize("ctx", [[64, 128, 300, 0], [64, 128, 1000, 0]], ids=["whole", "cut"])
+def test_a_single_node_whose_word_lacks_its_own_bit(dtype, ctx):
+    """All bits but its own, and no token in the cache: nothing is left to attend to."""
+    new = [64, 9, 40, 1]
+    words = [ancestors_of(t) for t in random_trees(new[:3], 7)] + [[-2]]
+    for heads, kv_heads, d in ((8, 2, 64), (6, 2, 128), (2, 1, 256)):
+        for max_new in (64, 1):
+            b = Trees(ctx, new, heads, kv_heads, d, dtype, 16, words=words)
+            out = b(max_new=max_new)
+            b.check(out)
+            assert bool((out[-1] == 0).all())
+
+
+@DTYPES
+def test_many_requests_beside_a_long_one(dtype):
+    """More row tiles than workgroups that the card holds, of very different lengths."""
+    rng = random.Random(8)
+    ctx = [rng.choice([0, 17, 100, 400]) for _ in range(63)] + [20000]
+    rng.shuffle(ctx)
+    new = [rng.randrange(1, 17) for _ in ctx]
+    b = Trees(ctx, new, 32, 8, 128, dtype, 16, pad=2)
+    out = b(max_new=16)
+    assert torch.equal(b(max_new=16), out)
+    b.check(out)
