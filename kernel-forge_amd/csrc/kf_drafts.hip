@@ -558,6 +558,11 @@ __device__ __forceinline__ bool add_together(const VerifyArgs& a, PickShared& sh
   }
   // The sums are atomics of the whole device's scope, which go past the caches that XCDs have of their own: there once they are
   // acknowledged, before the barrier, and so before the count.  (Fences of that scope write back and empty the caches: 10 us.)
+  // The language would have those fences: without them this holds for the processors named here, whose stores are counted with
+  // the loads (vmcnt) and acknowledged where the whole device sees them.
+#if defined(__HIP_DEVICE_COMPILE__) && !defined(__gfx950__)
+#error "add_together: sums are handed on as gfx950 orders them; other processors need a release and an acquire here"
+#endif
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0)

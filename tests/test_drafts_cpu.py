@@ -5,14 +5,16 @@ from __future__ import annotations
 
 import ctypes
 import itertools
+import os
 import random
 import re
+import subprocess
 
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-from kernelforge import _lib, ops
+from kernelforge import _lib, build, ops
 
 from draft_cases import ancestors_of, positions_of, verify_on_host
 from test_paged_cpu import _struct, attention_args
@@ -319,3 +321,13 @@ def test_a_list_under_a_tracer():
     cache, rest = CACHE.clone(), list(keep_args().values())[1:]
     with pytest.raises(ValueError, match="different arrays"):
         torch.ops.kernelforge.keep_listed_drafts([cache, cache[1:]], *rest)
+
+
+def test_sums_are_handed_on_as_one_processor_orders_them():
+    """The hand-over between workgroups leaves out fences that the language asks for: a build for another processor fails."""
+    source = build.SRC_DIR / "kf_drafts.hip"
+    for arch, fails in (("gfx90a", True), (build.ARCH, False)):
+        done = subprocess.run([build.hipcc(), "-E", "--cuda-device-only", f"--offload-arch={arch}", "-std=c++17", "-I",
+                               str(build.INCLUDE_DIR), "-I", str(build.SRC_DIR), str(source), "-o", os.devnull],
+                              capture_output=True, text=True)
+        assert (done.returncode != 0) == fails == ("need a release and an acquire" in done.stderr), done.stderr[-2000:]
