@@ -315,7 +315,7 @@ __device__ __forceinline__ void walk(const VerifyArgs& a, WalkShared& sh, int r,
         const int e = __builtin_ctzll(m);
         left -= sh.again[e] ? 0.0 : sh.p[e];
       }
-      accepted = !again && sh.u[lane] * left < sh.p[lane];
+      accepted = !again && sh.p[lane] > 0.0 && sh.u[lane] * left < sh.p[lane];  // `left` may be negative, and numbers too
     }
   }
   const uint64_t on = path_of(t, accepted);

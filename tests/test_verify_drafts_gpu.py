@@ -393,3 +393,18 @@ def test_more_pieces_than_threads(mode):
     assert got.counts.tolist() == [1] * 5
     places = got.tokens[:, 0].tolist()
     assert places[0] < first <= min(places[1], places[2], places[3]) and places[4] < 100
+
+
+@pytest.mark.parametrize("vocab", [50, 41000])
+def test_tokens_without_probability_are_never_accepted(vocab):
+    """Whatever the random numbers: behind siblings that leave less than nothing of their parent's mass, as numbers that are not
+    below 1 and rows that sum to more can, and with negative numbers."""
+    tree = [-1, 0, 0, 0, 0, 0]
+    for u in (2.0, 1.5, 0.9, -1.0):
+        target = torch.zeros(6, vocab)
+        target[:, 1], target[:, 2], target[:, 3] = 0.6, 0.5, 0.7
+        tokens = [0, 1, 2, vocab, -3, 7] if u > 0 else [0, vocab, -1, 7, 8, 1]
+        got = ops.verify_drafts(torch.tensor(tokens, device=DEV), i32(tree), i32([0, 6]), target.to(DEV),
+                                torch.full((6,), u, device=DEV), torch.full((1,), 0.5, device=DEV))
+        emitted = got.tokens[0, :int(got.counts[0])].tolist()
+        assert set(emitted) <= {1, 2, 3}, (u, emitted)
