@@ -668,8 +668,9 @@ class PagedDecoder:
             self.host_lens = [n + done if n else 0 for n in self.host_lens]
         return self.history
 
-    def _packed_drafts(self, drafts: dict) -> tuple[list[int], torch.Tensor, torch.Tensor, list]:
-        """(nodes per row, tokens, parents, (first node, parents, probabilities) of drafts that have some), checked."""
+    def _packed_drafts(self, drafts: dict) -> tuple[list[int], torch.Tensor, torch.Tensor, torch.Tensor | None]:
+        """(nodes per row, tokens, parents, probabilities in the rows of the nodes that children were drawn from, or None),
+        checked."""
         vocab, dev = self.model.cfg.vocab, self.tokens.device
         for row in drafts:
             if not 0 <= row < len(self.host_lens) or not self.host_lens[row]:
@@ -698,7 +699,7 @@ class PagedDecoder:
                 if probs.shape != (n, vocab) or probs.dtype != torch.float32 or probs.device != dev:
                     raise ValueError(f"decode_drafts: the probabilities of row {row} must be float32 [{n}, {vocab}] on {dev}")
                 if n:
-                    drawn.append((at, above, probs))
+                    drawn.append((above.long() + (at + 1), probs))  # the nodes that they follow
             new[row] = n + 1
             tokens += [self.tokens[row:row + 1], draft.long()]
             parents += [above.new_full((1,), -1), above + 1]
@@ -707,14 +708,17 @@ class PagedDecoder:
         if drawn and len(drawn) != sum(n > 1 for n in new):
             raise ValueError("decode_drafts: all drafts of a step have probabilities, or none")
         if not tokens:
-            return new, self.tokens[:0], self.tokens[:0].int(), drawn
+            return new, self.tokens[:0], self.tokens[:0].int(), None
         tokens, parents, numbers = torch.cat(tokens), torch.cat([p.long() for p in parents]), torch.cat(numbers)
         outside = ((tokens < 0) | (tokens >= vocab)).any()
         orphan = ((numbers > 0) & ((parents < 0) | (parents >= numbers))).any()
-        torn = torch.zeros_like(orphan)
-        for _, above, probs in drawn:  # each row beside that of the first token with its parent
-            first = (above[:, None] == above).int().argmax(1)
-            torn |= ((probs != probs[first]).any(1) & (first < torch.arange(len(first), device=dev))).any()
+        draft, torn = None, torch.zeros_like(orphan)
+        if drawn:
+            rows, probs = (torch.cat(parts) for parts in zip(*drawn))
+            rows = rows.clamp(0, at - 1)
+            draft = torch.zeros(at, vocab, device=dev)
+            draft[rows] = probs  # of several rows for a node any: they have to be the same, bit for bit
+            torn = (draft.view(torch.int32)[rows] != probs.view(torch.int32)).any()
         outside, orphan, torn = torch.stack([outside, orphan, torn]).tolist()
         if outside:
             raise ValueError(f"decode_drafts: a drafted token is outside of the vocabulary of {vocab}")
@@ -722,7 +726,7 @@ class PagedDecoder:
             raise ValueError("decode_drafts: a drafted token's parent must be one before it, or -1")
         if torn:
             raise ValueError("decode_drafts: tokens behind one parent must come with the same probabilities")
-        return new, tokens, parents.int(), drawn
+        return new, tokens, parents.int(), draft
 
     @torch.no_grad()
     def decode_drafts(self, drafts: dict, *, temperature: float = 0.0,
@@ -739,14 +743,14 @@ class PagedDecoder:
         Eager: the host waits for the counts."""
         if not 0.0 <= temperature < float("inf"):
             raise ValueError(f"decode_drafts: the temperature must be 0 or positive, got {temperature}")
-        new, tokens, parents, drawn = self._packed_drafts(drafts)
-        if drawn and temperature == 0.0:
+        new, tokens, parents, draft = self._packed_drafts(drafts)
+        if draft is not None and temperature == 0.0:
             raise ValueError("decode_drafts: probabilities of drafts need a temperature")
         self._reserve(new, "decode_drafts")
         if not any(new):
             return new
         try:
-            counts = self._verify_step(new, tokens, parents, drawn, temperature, generator)
+            counts = self._verify_step(new, tokens, parents, draft, temperature, generator)
         finally:
             # Pages that a row does not have, or not any longer, leave its table.
             pages = (self.context_lens + self.block_size - 1) // self.block_size
@@ -754,7 +758,7 @@ class PagedDecoder:
         self.host_lens = [n + c for n, c in zip(self.host_lens, counts)]
         return counts
 
-    def _verify_step(self, new, tokens, parents, drawn, temperature, generator) -> list[int]:
+    def _verify_step(self, new, tokens, parents, draft, temperature, generator) -> list[int]:
         """decode_drafts on packed drafts: the step, and what the device keeps of it."""
         step = ops.paged_tables(self.block_table, self.context_lens, torch.tensor(new, dtype=torch.int32, device=self.device),
                                 self.free_pages, self.free_count, block_size=self.block_size, max_tokens=sum(new))
@@ -770,11 +774,6 @@ class PagedDecoder:
             target = torch.softmax((logits - top).masked_fill_(logits == top, 0.0) / max(temperature, 1e-30), dim=-1)
             accept = torch.rand(tokens.numel(), generator=generator, device=self.device)
             sample = torch.rand(len(new), generator=generator, device=self.device)
-            draft = None
-            if drawn:  # what each node's children were drawn from, in the node's row
-                draft = torch.zeros_like(target)
-                for first, above, probs in drawn:
-                    draft[first + 1 + above.long()] = probs
             done = ops.verify_drafts(tokens, parents, step.cu_new, target, accept, sample, draft=draft, max_new=max(new))
         counts = done.counts.tolist()
         # Emitted tokens stand behind each row's last one.  All that can fail comes before the pages are given back.
