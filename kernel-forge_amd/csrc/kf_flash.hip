@@ -644,10 +644,10 @@ __global__ __launch_bounds__(kFlashThreads, flash_waves_per_simd(HDP, true)) voi
 // can hold the end of one item and the beginning of the next, took 59 in place of 41 us for 8 requests of 256 rows over 500
 // .. 4000 keys, 37 (29) for 16 of 30 .. 186 over 100 .. 8000 (2 KV heads), both with their join; the joins 18 .. 24 (6 .. 9)
 // and, of 24 items in 512 stretches, 72 (7).
-//   What bounds it: long requests the bytes of K and V (two of 108 rows over up to 131071 keys, 8 KV heads of 128: 179 us,
-// 5.8 TB/s, and 7 the join); others latency: 16 of 30 .. 186 rows over 100 .. 8000 keys, 24 MB, take 19.2 us, of which 2.0
+//   What bounds it: long requests the bytes of K and V (two of 108 rows over up to 131071 keys, 8 KV heads of 128: 182 us,
+// 5.7 TB/s, and 7 the join); others latency: 16 of 30 .. 186 rows over 100 .. 8000 keys, 24 MB, take 19.9 us, of which 2.0
 // finding the piece, 2.0 until the queries and pages are there, 1.6 until the first tiles are, 2.3 two tiles of 64 keys, 3.3
-// joining the groups and writing the piece; the join 5.4.
+// joining the groups and writing the piece; the join 5.5.
 constexpr int kTreeLeast = 4;  // key tiles of a piece; with 2 and 8 the same to 1 us
 struct __attribute__((aligned(16))) TreeItem {
   int tok0, row0, rows, kv;  // its request's first token, its first row, the request's rows
